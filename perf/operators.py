@@ -1,0 +1,522 @@
+"""Performance cases of the matrix operators: FP8 products with block scales, and Muon.
+
+The listed cases are the calls of a program that trains or serves linear
+layers in FP8 and updates their weights by Muon: quantizing a matrix with a
+scale for each block of 128 (``block_cast``), the product of two such matrices
+(``block_matmul``), a linear layer's three products in one training step
+(``block_linear``), orthogonalising updates by Newton-Schulz products
+(``orthogonalize``) and the whole parameter update (``hip_muon_step_``,
+``MuonHip``).  Sizes are those of the benchmark's workloads (GPT-2's and
+Llama 3.2 1B's weights) and generic odd ones; ``draw`` spreads over the
+ranges between them.
+
+``run`` computes either the plain form of an operator, in elementary FP32
+torch operations, or (``own``) calls the framework's entry point.
+"""
+
+from __future__ import annotations
+
+import math
+import os
+import sys
+
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+DEVICE = "cuda"
+own = False
+
+DTYPES = {
+    "fp32": torch.float32,
+    "bf16": torch.bfloat16,
+    "fp16": torch.float16,
+    "e4m3": torch.float8_e4m3fn,
+    "e5m2": torch.float8_e5m2,
+}
+SIZES = {"fp32": 4, "bf16": 2, "fp16": 2, "e4m3": 1, "e5m2": 1}
+# Mantissa bits, smallest normal exponent, exponent and value of the largest finite magnitude (1.75 * 2^top).
+FP8 = {"e4m3": (3, -6, 8), "e5m2": (2, -14, 15)}
+BLOCK = 128
+SEED = 7
+STEPS, COEFFICIENTS, EPS = 5, (3.4445, -4.7750, 2.0315), 1e-7
+MOMENTUM, WEIGHT_DECAY = 0.95, 0.01
+
+
+def _states():
+    path = os.path.join(ROOT, "stochastic-rounding-pytorch_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import sr_states
+
+    return sr_states
+
+
+# --------------------------------------------------------------------------------------
+# Cases
+# --------------------------------------------------------------------------------------
+def listed():
+    return [
+        # Activations of 16 sequences, one token each, before an FP8 projection: latency.
+        dict(name="cast_rows_16x2048", kind="cast", rows=16, cols=2048, x="bf16", to="e4m3", rule="nearest",
+             square=False, axes="1"),
+        # A training batch's output gradient in both orientations, stochastically rounded: one read for the
+        # input's and the weight's gradient.
+        dict(name="cast_both_8192x2048", kind="cast", rows=8192, cols=2048, x="bf16", to="e5m2", rule="stochastic",
+             square=False, axes="10"),
+        # One token through an MLP projection of Llama 3.2 1B: the weight's bytes.
+        dict(name="matmul_token_8192x2048", kind="matmul", m=1, n=8192, k=2048, a="e4m3", b="e4m3", scale="e8m0",
+             b_square=True, out="bf16"),
+        # A prompt batch of 8192 tokens through the same projection.
+        dict(name="matmul_8192x8192x2048", kind="matmul", m=8192, n=8192, k=2048, a="e4m3", b="e4m3", scale="e8m0",
+             b_square=True, out="bf16"),
+        # Odd sizes, mixed formats and scales as FP32 checkpoints hold them; FP32 result.
+        dict(name="matmul_1001x2305x1000_f32", kind="matmul", m=1001, n=2305, k=1000, a="e5m2", b="e4m3", scale="fp32",
+             b_square=True, out="fp32"),
+        # Forward and backward of GPT-2's attention projection over half a sequence of odd length.
+        dict(name="linear_501x768x2304", kind="linear", tokens=501, k=768, n=2304),
+        # Forward and backward of a square projection of Llama 3.2 1B over 8192 tokens.
+        dict(name="linear_8192x2048x2048", kind="linear", tokens=8192, k=2048, n=2048),
+        # The update of a small convolution (64 x 64 x 3 x 3): latency.
+        dict(name="orthogonalize_64x576", kind="orthogonalize", batch=1, rows=64, cols=576, x="fp32"),
+        # The update of GPT-2's attention projection.
+        dict(name="orthogonalize_768x2304", kind="orthogonalize", batch=1, rows=768, cols=2304, x="bf16"),
+        # The updates of an MLP projection of Llama 3.2 1B, tall.
+        dict(name="orthogonalize_8192x2048", kind="orthogonalize", batch=1, rows=8192, cols=2048, x="bf16"),
+        # One functional update of an FP32 weight at a decayed learning rate.
+        dict(name="muon_tensor_1023x767", kind="muon_function", rows=1023, cols=767, p="fp32", g="fp32",
+             m="bf16/stochastic", lr=2e-4),
+        # An optimizer step over the attention weights of four Llama 3.2 1B layers, pure BF16 training.
+        dict(name="muon_attention_4_layers", kind="muon", layers=4, width=2048, narrow=512, p="bf16", g="bf16",
+             m="bf16/stochastic", lr=2e-2),
+    ]
+
+
+def _log_uniform(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def draw(rng):
+    kind = rng.choice(("cast", "matmul", "matmul", "matmul", "linear", "orthogonalize", "orthogonalize",
+                       "muon_function", "muon"))
+    if kind == "cast":
+        return dict(kind=kind, rows=_log_uniform(rng, 1, 8192), cols=_log_uniform(rng, 64, 4096),
+                    x=rng.choice(("bf16", "bf16", "fp32", "fp16")), to=rng.choice(("e4m3", "e5m2")),
+                    rule=rng.choice(("nearest", "stochastic")), square=rng.random() < 0.3,
+                    axes=rng.choice(("1", "0", "10")))
+    if kind == "matmul":
+        return dict(kind=kind, m=_log_uniform(rng, 1, 8192), n=_log_uniform(rng, 64, 8192),
+                    k=_log_uniform(rng, 64, 2048), a=rng.choice(("e4m3", "e5m2")), b="e4m3",
+                    scale=rng.choice(("e8m0", "e8m0", "fp32")), b_square=rng.random() < 0.7,
+                    out=rng.choice(("bf16", "bf16", "fp32")))
+    if kind == "linear":
+        return dict(kind=kind, tokens=_log_uniform(rng, 16, 8192), k=_log_uniform(rng, 64, 2048),
+                    n=_log_uniform(rng, 64, 2048))
+    if kind == "orthogonalize":
+        rows, cols = _log_uniform(rng, 16, 2048), _log_uniform(rng, 16, 8192)
+        if rng.random() < 0.5:
+            rows, cols = cols, rows
+        return dict(kind=kind, batch=rng.choice((1, 1, 3)) if rows * cols < 1 << 21 else 1, rows=rows, cols=cols,
+                    x=rng.choice(("bf16", "fp32")))
+    types = rng.choice((dict(p="bf16", g="bf16", lr=2e-2), dict(p="fp32", g="fp32", lr=2e-4),
+                        dict(p="fp32", g="bf16", lr=2e-4)))
+    types["m"] = rng.choice(("bf16/stochastic", "bf16/stochastic", "bf16/nearest", "fp16/stochastic"))
+    if kind == "muon_function":
+        return dict(kind=kind, rows=_log_uniform(rng, 48, 2304), cols=_log_uniform(rng, 48, 2304), **types)
+    return dict(kind=kind, layers=rng.randint(1, 8), width=_log_uniform(rng, 128, 1024),
+                narrow=_log_uniform(rng, 64, 512), **types)
+
+
+def _muon_shapes(case):
+    """Groups of equal shapes: the query and output projections, the narrower key and value ones."""
+    if case["kind"] == "muon_function":
+        return [(1, case["rows"], case["cols"])]
+    d, n = case["width"], 2 * case["layers"]
+    return [(n, d, d), (n, case["narrow"], d)]
+
+
+# --------------------------------------------------------------------------------------
+# Inputs
+# --------------------------------------------------------------------------------------
+def _normal(shape, std, dtype, generator):
+    return torch.empty(shape, dtype=torch.float32, device=DEVICE).normal_(0.0, std, generator=generator).to(dtype)
+
+
+def _activations(shape, std, dtype, generator):
+    """Normal values whose columns differ in scale, a few of them by much, as activations and gradients have it."""
+    spread = torch.empty(shape[-1], device=DEVICE).normal_(0.0, 1.0, generator=generator).exp_()
+    return (_normal(shape, std, torch.float32, generator) * spread).to(dtype)
+
+
+def _gradients(shape, std, dtype, generator):
+    """A gradient's spectrum: a few strong directions over noise."""
+    *batch, rows, cols = shape
+    rank = max(1, min(rows, cols) // 16)
+    strong = torch.matmul(_normal((*batch, rows, rank), 1.0, torch.float32, generator),
+                          _normal((*batch, rank, cols), 1.0, torch.float32, generator))
+    return ((strong * rank ** -0.5 + _normal(shape, 1.0, torch.float32, generator)) * std).to(dtype)
+
+
+def _operand(rows, k, fmt, scale, square, generator):
+    """An FP8 matrix with values over its format's range and a scale for each block of 128."""
+    data = _normal((rows, k), FP8[fmt][2] * 8.0, torch.float32, generator).to(DTYPES[fmt])
+    grid = (-(-rows // BLOCK) if square else rows, -(-k // BLOCK))
+    if scale == "e8m0":
+        codes = torch.randint(127 - 14, 127 - 8, grid, device=DEVICE, generator=generator, dtype=torch.uint8)
+        return data, codes.view(torch.float8_e8m0fnu)
+    return data, torch.empty(grid, device=DEVICE).uniform_(0.2, 2.0, generator=generator).mul_(2.0 ** -10)
+
+
+def prepare(case, seed):
+    generator = torch.Generator(device=DEVICE).manual_seed(seed)
+    kind, state = case["kind"], dict(case=case)
+    if kind == "cast":
+        state["x"] = _activations((case["rows"], case["cols"]), 1.0, DTYPES[case["x"]], generator)
+    elif kind == "matmul":
+        state["a"] = _operand(case["m"], case["k"], case["a"], case["scale"], False, generator)
+        state["b"] = _operand(case["n"], case["k"], case["b"], case["scale"], case["b_square"], generator)
+    elif kind == "linear":
+        state["x"] = _activations((case["tokens"], case["k"]), 1.0, torch.bfloat16, generator).requires_grad_()
+        state["w"] = _normal((case["n"], case["k"]), 0.02, torch.bfloat16, generator).requires_grad_()
+        state["dy"] = _activations((case["tokens"], case["n"]), 1e-3, torch.bfloat16, generator)
+    elif kind == "orthogonalize":
+        shape = (case["rows"], case["cols"]) if case["batch"] == 1 else (case["batch"], case["rows"], case["cols"])
+        state["x"] = _gradients(shape, 1e-3, DTYPES[case["x"]], generator)
+    else:
+        state["step"] = 0
+        dtype = DTYPES[case["m"].split("/")[0]]
+        tensors = {"p": [], "g": [], "m": []}
+        for n, rows, cols in _muon_shapes(case):
+            tensors["p"] += _normal((n, rows, cols), cols ** -0.5, DTYPES[case["p"]], generator).unbind(0)
+            tensors["g"] += _gradients((n, rows, cols), 1e-3, DTYPES[case["g"]], generator).unbind(0)
+            tensors["m"] += _gradients((n, rows, cols), 1e-2, dtype, generator).unbind(0)
+        # A parameter, its gradient and its momentum are allocations of their own in a program.
+        state.update({name: [t.clone() for t in views] for name, views in tensors.items()})
+    return state
+
+
+# --------------------------------------------------------------------------------------
+# Plain forms
+# --------------------------------------------------------------------------------------
+def _h32(x):
+    x &= 0xFFFFFFFF
+    x ^= x >> 16
+    x = (x * 0x7FEB352D) & 0xFFFFFFFF
+    x ^= x >> 15
+    x = (x * 0x846CA68B) & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def _update_key(seed, step, index):
+    key = _h32((seed & 0xFFFFFFFF) ^ 0x9E3779B9)
+    key = _h32(key ^ (seed >> 32))
+    key = _h32(key ^ (step & 0xFFFFFFFF))
+    key = _h32(key ^ (step >> 32))
+    return _h32(key ^ index)
+
+
+def _state_key(key, index):
+    return _h32(key ^ index)
+
+
+def _hashes(shape, seed):
+    """The random word of each element: the hash of its flat index plus the seed."""
+    return _h32(torch.arange(math.prod(shape), device=DEVICE, dtype=torch.int64).view(shape) + seed)
+
+
+def _power(exponent):
+    """2^exponent in FP32 for exponents of normal numbers."""
+    return ((exponent.to(torch.int32) + 127) << 23).view(torch.float32)
+
+
+def _round_fp8(x, fmt, rule, seed):
+    mantissa, lowest, top = FP8[fmt]
+    magnitude = x.abs().clamp(max=1.75 * 2.0 ** top)
+    exponent = ((magnitude.view(torch.int32) >> 23) - 127).clamp(min=lowest)
+    scaled = magnitude * _power(mantissa - exponent)
+    if rule == "nearest":
+        grid = scaled.round()
+    else:
+        grid = scaled.floor()
+        threshold = ((scaled - grid) * 2.0 ** 24).floor().to(torch.int64)
+        grid = grid + ((_hashes(x.shape, seed) >> 8) < threshold).float()
+    value = torch.copysign(grid * _power(exponent - mantissa), x)
+    return torch.where(x.isnan(), x, value).to(DTYPES[fmt])
+
+
+def _blocks(x, rows, cols):
+    """x padded with zeros to whole blocks, as (row blocks, rows, column blocks, cols)."""
+    r, c = x.shape
+    x = torch.nn.functional.pad(x, (0, -c % cols, 0, -r % rows))
+    return x.view(x.shape[0] // rows, rows, x.shape[1] // cols, cols)
+
+
+def _spread(scale, rows, cols, shape):
+    """One factor per block as one per element of ``shape``."""
+    return scale.repeat_interleave(rows, 0)[:shape[0]].repeat_interleave(cols, 1)[:, :shape[1]]
+
+
+def _plain_block_cast(x, fmt, rule, square, axis, seed):
+    x = x.float()
+    rows, cols = (BLOCK, BLOCK) if square else (1, BLOCK) if axis == 1 else (BLOCK, 1)
+    amax = torch.where(x.isfinite(), x.abs(), 0.0)
+    amax = _blocks(amax, rows, cols).amax((1, 3))
+    fraction, exponent = torch.frexp(amax)
+    exponent = exponent - 1 - FP8[fmt][2] + (fraction > 0.875).int()
+    exponent = torch.where(amax > 0, exponent, 0).clamp(min=-127)
+    data = _round_fp8(x * _spread(_power(-exponent), rows, cols, x.shape), fmt, rule, seed)
+    scale = (exponent + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+    return (data, scale) if axis == 1 else (data.view(torch.uint8).t().contiguous().view(data.dtype),
+                                            scale.view(torch.uint8).t().contiguous().view(scale.dtype))
+
+
+def _dequantized(operand):
+    data, scale = operand
+    rows = BLOCK if scale.shape[0] != data.shape[0] else 1
+    return data.float() * _spread(scale.float(), rows, BLOCK, data.shape)
+
+
+def _plain_block_matmul(a, b, dtype):
+    return torch.matmul(_dequantized(a), _dequantized(b).t()).to(dtype)
+
+
+def _plain_linear(x, w, dy, seed):
+    with torch.no_grad():
+        sx, sw, sg = (_state_key(seed, k) for k in range(3))
+        y = _plain_block_matmul(_plain_block_cast(x, "e4m3", "nearest", False, 1, sx),
+                                _plain_block_cast(w, "e4m3", "nearest", True, 1, sw), x.dtype)
+        dx = _plain_block_matmul(_plain_block_cast(dy, "e4m3", "stochastic", False, 1, sg),
+                                 _plain_block_cast(w, "e4m3", "nearest", True, 0, sw), x.dtype)
+        dw = _plain_block_matmul(_plain_block_cast(dy, "e4m3", "stochastic", False, 0, sg),
+                                 _plain_block_cast(x, "e4m3", "nearest", False, 0, sx), w.dtype)
+    return y, dx, dw
+
+
+def _plain_orthogonalize(x):
+    """X (..., rows, cols) in FP32, orthogonalised by the quintic iteration on its smaller side."""
+    a, b, c = COEFFICIENTS
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.float()
+    x = x.transpose(-1, -2).contiguous() if tall else x
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + EPS)
+    for _ in range(STEPS):
+        gram = torch.matmul(x, x.transpose(-1, -2).contiguous())
+        x = a * x + torch.matmul(b * gram + c * torch.matmul(gram, gram), x)
+    return x.transpose(-1, -2).contiguous() if tall else x
+
+
+def _round_state(x, fmt, seed):
+    dtype, rule = fmt.split("/")
+    if rule == "nearest" or dtype == "fp32":
+        return x.to(DTYPES[dtype])
+    if dtype == "bf16":
+        bits = x.view(torch.int32).to(torch.int64) + (_hashes(x.shape, seed) & 0xFFFF)
+        return ((bits >> 16) << 16).to(torch.int32).view(torch.float32).to(torch.bfloat16)
+    # FP16: 10 mantissa bits, smallest normal exponent -14.
+    magnitude = x.abs()
+    exponent = ((magnitude.view(torch.int32) >> 23) - 127).clamp(min=-14)
+    scaled = magnitude * _power(10 - exponent)
+    grid = scaled.floor()
+    threshold = ((scaled - grid) * 2.0 ** 24).floor().to(torch.int64)
+    grid = grid + ((_hashes(x.shape, seed) >> 8) < threshold).float()
+    return torch.copysign(grid * _power(exponent - 10), x).to(torch.float16)
+
+
+def _plain_muon(p, g, m, fmt, lr, keys):
+    """One update of equal-shaped parameters, given as lists: p and m change in place."""
+    g32 = torch.stack(g).float()
+    u = torch.stack(m).float() * MOMENTUM + g32
+    update = _plain_orthogonalize(u * MOMENTUM + g32)
+    scale = math.sqrt(max(1.0, p[0].shape[0] / p[0].shape[1]))
+    stored = torch.stack(p).float() * (1 - lr * WEIGHT_DECAY) - lr * scale * update
+    for k, key in enumerate(keys):
+        m[k].copy_(_round_state(u[k], fmt, key))
+        p[k].copy_(stored[k])
+
+
+def _run_plain(state):
+    case, kind = state["case"], state["case"]["kind"]
+    if kind == "cast":
+        return [_plain_block_cast(state["x"], case["to"], case["rule"], case["square"], int(axis), SEED)
+                for axis in case["axes"]]
+    if kind == "matmul":
+        return _plain_block_matmul(state["a"], state["b"], DTYPES[case["out"]])
+    if kind == "linear":
+        return _plain_linear(state["x"], state["w"], state["dy"], SEED)
+    if kind == "orthogonalize":
+        return _plain_orthogonalize(state["x"]).to(torch.bfloat16)
+    state["step"] += 1
+    at = 0
+    for n, _, _ in _muon_shapes(case):
+        if kind == "muon_function":
+            keys = [_state_key(SEED + state["step"], 0)]
+        else:
+            keys = [_state_key(_update_key(SEED, state["step"], k), 0) for k in range(at, at + n)]
+        _plain_muon(state["p"][at:at + n], state["g"][at:at + n], state["m"][at:at + n], case["m"], case["lr"], keys)
+        at += n
+    return dict(p=state["p"], m=state["m"])
+
+
+# --------------------------------------------------------------------------------------
+# The framework's entry points
+# --------------------------------------------------------------------------------------
+def _run_own(state):
+    sr_states = _states()
+    case, kind = state["case"], state["case"]["kind"]
+    if kind == "cast":
+        axes = tuple(int(axis) for axis in case["axes"])
+        out = sr_states.block_cast(state["x"], dtype=DTYPES[case["to"]], rounding=case["rule"],
+                                   block=(BLOCK, BLOCK) if case["square"] else (1, BLOCK),
+                                   axis=axes if len(axes) > 1 else axes[0], seed=SEED)
+        return [(q.data, q.scale) for q in (out if len(axes) > 1 else [out])]
+    if kind == "matmul":
+        return sr_states.block_matmul(sr_states.BlockScaled(*state["a"]), sr_states.BlockScaled(*state["b"]),
+                                      out_dtype=DTYPES[case["out"]])
+    if kind == "linear":
+        y = sr_states.block_linear(state["x"], state["w"], seed=SEED)
+        dx, dw = torch.autograd.grad(y, (state["x"], state["w"]), state["dy"])
+        return y, dx, dw
+    if kind == "orthogonalize":
+        return sr_states.orthogonalize(state["x"])
+    dtype, rule = case["m"].split("/")
+    fmt = sr_states.StateFormat(DTYPES[dtype], rule)
+    if kind == "muon_function":
+        state["step"] += 1
+        sr_states.hip_muon_step_(state["p"][0], state["g"][0], state["m"][0], lr=case["lr"], momentum_factor=MOMENTUM,
+                                 weight_decay=WEIGHT_DECAY, seed=SEED + state["step"], formats=(fmt,))
+        return dict(p=state["p"], m=state["m"])
+    if "optimizer" not in state:
+        state["parameters"] = [torch.nn.Parameter(p) for p in state["p"]]
+        state["optimizer"] = sr_states.MuonHip(state["parameters"], lr=case["lr"], momentum=MOMENTUM,
+                                               weight_decay=WEIGHT_DECAY, state_format=fmt, seed=SEED)
+        for parameter, g, m in zip(state["parameters"], state["g"], state["m"]):
+            parameter.grad = g
+            state["optimizer"].state[parameter]["momentum_buffer"] = m
+    state["optimizer"].step()
+    return dict(p=state["p"], m=state["m"])
+
+
+def run(state):
+    return _run_own(state) if own else _run_plain(state)
+
+
+# --------------------------------------------------------------------------------------
+# Work
+# --------------------------------------------------------------------------------------
+def _newton_schulz_flops(rows, cols):
+    """Per step: half of a symmetric Gram matrix, half of its square, and one full product."""
+    m, n = min(rows, cols), max(rows, cols)
+    return STEPS * (3 * m * m * n + m ** 3)
+
+
+def work(case):
+    kind = case["kind"]
+    if kind == "cast":
+        elements = case["rows"] * case["cols"]
+        out = len(case["axes"]) * (elements + elements / (BLOCK * BLOCK if case["square"] else BLOCK))
+        return dict(bytes=elements * SIZES[case["x"]] + out, flops=0)
+    if kind == "matmul":
+        m, n, k = case["m"], case["n"], case["k"]
+        scales = (m + n / (BLOCK if case["b_square"] else 1)) * k / BLOCK * (1 if case["scale"] == "e8m0" else 4)
+        return dict(bytes=m * k + n * k + scales + m * n * SIZES[case["out"]], flops=2 * m * n * k)
+    if kind == "linear":
+        t, k, n = case["tokens"], case["k"], case["n"]
+        # x, w and dy read; y, dx and dw written.
+        return dict(bytes=2 * 2 * (t * k + n * k + t * n), flops=6 * t * n * k)
+    if kind == "orthogonalize":
+        elements = case["batch"] * case["rows"] * case["cols"]
+        return dict(bytes=elements * (SIZES[case["x"]] + 2),
+                    flops=case["batch"] * _newton_schulz_flops(case["rows"], case["cols"]))
+    elements = sum(math.prod(shape) for shape in _muon_shapes(case))
+    return dict(bytes=elements * (2 * SIZES[case["p"]] + SIZES[case["g"]] + 2 * SIZES[case["m"].split("/")[0]]),
+                flops=sum(n * _newton_schulz_flops(rows, cols) for n, rows, cols in _muon_shapes(case)))
+
+
+# --------------------------------------------------------------------------------------
+# The definitions in 64 bits
+# --------------------------------------------------------------------------------------
+def _exact_exponents(x, top):
+    """The smallest e with max|x| <= 1.75 * 2^(top + e), for the last axis of x."""
+    amax = x.abs().amax(-1)
+    e = torch.ceil(torch.log2(amax / 1.75).clamp(min=-1000.0)) - top
+    e = torch.where(amax > torch.exp2(e + top) * 1.75, e + 1, e)
+    e = torch.where(amax <= torch.exp2(e + top - 1) * 1.75, e - 1, e)
+    return torch.where(amax > 0, e, 0.0).clamp(min=-127.0)
+
+
+def _exact_cast(x, fmt, rule, square, axis, seed):
+    """(values before the scale, scale) per element of x, in 64 bits: the FP8 values rounded as defined."""
+    mantissa, lowest, top = FP8[fmt]
+    x = x.detach().double()
+    r, c = x.shape
+    index = torch.arange(r * c, device=DEVICE).view(r, c)
+    if axis == 0:
+        x, index = x.t(), index.t()
+    rows, cols = x.shape
+    padded = torch.zeros(-(-rows // BLOCK) * BLOCK, -(-cols // BLOCK) * BLOCK, dtype=torch.float64, device=DEVICE)
+    padded[:rows, :cols] = x
+    if square:
+        tiles = padded.view(-1, BLOCK, padded.shape[1] // BLOCK, BLOCK).transpose(1, 2)
+        e = _exact_exponents(tiles.reshape(*tiles.shape[:2], -1), top)
+        full = e.repeat_interleave(BLOCK, 0)[:rows]
+    else:
+        full = e = _exact_exponents(padded.view(padded.shape[0], -1, BLOCK), top)[:rows]
+    y = x / torch.exp2(full.repeat_interleave(BLOCK, 1)[:, :cols])
+    spacing = torch.exp2(torch.floor(torch.log2(y.abs().clamp(min=2.0 ** lowest))) - mantissa)
+    steps = y.abs() / spacing
+    below = torch.floor(steps)
+    if rule == "nearest":
+        up = (steps - below > 0.5) | ((steps - below == 0.5) & (below % 2 == 1))
+    else:
+        up = torch.div(_h32(index + seed), 256, rounding_mode="floor").double() < torch.floor((steps - below) * 2 ** 24)
+    value = (below + up) * spacing
+    return torch.sign(y) * value, torch.exp2(e)
+
+
+def _exact_product(a, b):
+    """a b^T of two (values, scale) pairs."""
+    full = []
+    for value, scale in (a, b):
+        if scale.shape[0] != value.shape[0]:
+            scale = scale.repeat_interleave(BLOCK, 0)[:value.shape[0]]
+        full.append(value.double() * scale.double().repeat_interleave(BLOCK, 1)[:, :value.shape[1]])
+    return full[0] @ full[1].mT
+
+
+def _exact_orthogonal(x):
+    a, b, c = COEFFICIENTS
+    if x.shape[-1] < x.shape[-2]:
+        return _exact_orthogonal(x.mT.contiguous()).mT.contiguous()
+    x = x / (torch.linalg.vector_norm(x, dim=(-2, -1), keepdim=True) + EPS)
+    for _ in range(STEPS):
+        product = x @ x.mT.contiguous() @ x
+        x = a * x + b * product + c * (x @ x.mT.contiguous() @ product)
+    return x
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    kind = case["kind"]
+    if kind == "cast":
+        return [_exact_cast(state["x"], case["to"], case["rule"], case["square"], int(axis), SEED)
+                for axis in case["axes"]]
+    if kind == "matmul":
+        return _exact_product(state["a"], state["b"])
+    if kind == "linear":
+        keys = [_state_key(SEED, k) for k in range(3)]
+        x, w, dy = state["x"], state["w"], state["dy"]
+        return (_exact_product(_exact_cast(x, "e4m3", "nearest", False, 1, keys[0]),
+                               _exact_cast(w, "e4m3", "nearest", True, 1, keys[1])),
+                _exact_product(_exact_cast(dy, "e4m3", "stochastic", False, 1, keys[2]),
+                               _exact_cast(w, "e4m3", "nearest", True, 0, keys[1])),
+                _exact_product(_exact_cast(dy, "e4m3", "stochastic", False, 0, keys[2]),
+                               _exact_cast(x, "e4m3", "nearest", False, 0, keys[0])))
+    if kind == "orthogonalize":
+        return _exact_orthogonal(state["x"].double())
+    p_out, m_out = [], []
+    for p, g, m in zip(state["p"], state["g"], state["m"]):
+        u = m.double() * MOMENTUM + g.double()
+        update = _exact_orthogonal(g.double() + MOMENTUM * u)
+        scale = math.sqrt(max(1.0, p.shape[0] / p.shape[1]))
+        p_out.append(p.double() * (1 - case["lr"] * WEIGHT_DECAY) - case["lr"] * scale * update)
+        m_out.append(u)  # before its rounding to the stored format
+    return dict(p=p_out, m=m_out)
