@@ -389,6 +389,7 @@ def _run_own(state):
         state["optimizer"] = sr_states.MuonHip(state["parameters"], lr=case["lr"], momentum=MOMENTUM,
                                                weight_decay=WEIGHT_DECAY, state_format=fmt, seed=SEED)
         for parameter, g, m in zip(state["parameters"], state["g"], state["m"]):
+            parameter.grad_dtype = g.dtype  # BF16 gradients of FP32 parameters
             parameter.grad = g
             state["optimizer"].state[parameter]["momentum_buffer"] = m
     state["optimizer"].step()
