@@ -13,12 +13,15 @@
 #include <string>
 
 #include "../../include/sr_states_hip.h"
+#include "sr_error.h"
 #include "sr_kernels.h"
 #include "sr_launch_cap.h"
 
 namespace {
-
 thread_local std::string g_error;
+}  // namespace
+
+namespace sr {
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -33,6 +36,13 @@ int fail(int code, const char* fmt, ...) {
 int hip_fail(hipError_t err, const char* what) {
   return fail(SR_ERR_HIP, "%s failed: %s (%d)", what, hipGetErrorString(err), static_cast<int>(err));
 }
+
+}  // namespace sr
+
+namespace {
+
+using sr::fail;
+using sr::hip_fail;
 
 struct Tables {
   sr::KernelTableAdamW adamw{};

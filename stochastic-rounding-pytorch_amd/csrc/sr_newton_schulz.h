@@ -1,0 +1,376 @@
+// sr_newton_schulz.h -- kernels of the Newton-Schulz orthogonalisation and of the Muon update around it.
+//
+// The iteration.  X0 = V / (|V|_F + eps), then X <- a X + (b G + c G^2) X with
+// G = X X^T, on the orientation with at most as many rows (m) as columns (n).
+// G and P = b G + c G^2 are symmetric, so only the tiles of their lower
+// triangle are computed and each is stored twice.
+//
+// Numbers.  The products take FP16 operands and sum in FP32.  Every operand
+// is held times 2^13: singular values stay near 1, so entries are at most a
+// few units and typical ones 1/sqrt(mn), and 2^13 puts both inside FP16's
+// normal range.  X itself is carried in FP32 beside its FP16 copy H:
+//
+//   X' = a X + P H
+//
+// A rounding error of X that lies in the space of small singular values
+// grows by a (about 3.4) in every step; with a X exact to FP32, the error of
+// H meets P instead, which is near 0 there.  (On a rank-16 matrix with noise
+// of 1e-3, the result's error in the Frobenius norm is 4e-4; with X held in
+// FP16 alone it is 4e-2.)  P is stored as P + s I with s = 1.5, and s H is
+// subtracted in FP32: on the large singular values P lies between -3 and 0,
+// and half the magnitude halves the rounding of its diagonal.
+//
+// Workspace.  Rows and columns are padded to multiples of 64 with zeros, which
+// every step keeps, so the products have no edges along their contracted
+// axis.  Per padded element: X in FP32, H, and two buffers of H^T, which one
+// step reads while it writes the other.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../../include/sr_matrix_hip.h"
+#include "sr_kernels.h"
+#include "sr_tile_product.h"
+
+namespace sr {
+
+constexpr float kNsScale = 8192.0f, kNsInverse = 1.0f / 8192.0f;  // 2^13
+constexpr float kNsProduct = kNsInverse * kNsInverse;             // of a product of two scaled operands
+constexpr float kNsShift = 1.5f;
+constexpr int kNsPad = 64;        // rows and columns of the workspace are padded to it
+constexpr int kNsPartials = 512;  // partial sums of squares per matrix
+constexpr int kNsThreads = 256;
+
+// The matrices of one launch.
+struct MatrixTable {
+  uint64_t p[SR_MATRIX_BATCH];  // parameters, or results
+  uint64_t g[SR_MATRIX_BATCH];  // gradients, or inputs
+  uint64_t u[SR_MATRIX_BATCH];  // momenta
+  uint32_t counter[SR_MATRIX_BATCH];
+};
+
+struct NsArgs {
+  int rows, cols;  // of the matrices
+  int m, n;        // padded: m <= n, X is m x n, transposed where rows > cols
+  int tall;
+  int partials;    // partial sums per matrix in use
+  float a, b, c, eps;
+  float* x;
+  _Float16* h;
+  const _Float16* ht;
+  _Float16* ht_next;
+  _Float16* g;
+  _Float16* p;
+  float* partial;
+  float momentum, decay, neg_lr;  // Muon
+  int nesterov;
+  int muon, out_dtype;  // last step: update p in out_dtype, or store the result
+};
+
+// Sum over the workgroup's 256 threads, in a fixed order; valid in thread 0.
+__device__ __forceinline__ float group_sum(float v, float* scratch) {
+#pragma unroll
+  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+  if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+}
+
+// Reads the gradients (GE) and, with UE >= 0, updates the momenta; leaves V in
+// FP32, in the workspace's orientation, and partial sums of its squares.
+// 64 x 64 tiles, of which a workgroup takes every gridDim.x-th.
+template <int GE, int UE>
+__global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTable t) {
+  __shared__ float turned[kNsPad][kNsPad + 1];
+  __shared__ float scratch[4];
+  const int matrix = blockIdx.y;
+  const void* g = reinterpret_cast<const void*>(t.g[matrix]);
+  void* u = reinterpret_cast<void*>(t.u[matrix]);
+  float* x = a.x + static_cast<int64_t>(matrix) * a.m * a.n;
+  const int tiles_c = (a.tall ? a.m : a.n) / kNsPad, tiles = (a.m / kNsPad) * (a.n / kNsPad);
+  const int tr = threadIdx.x >> 4, tc = 4 * (threadIdx.x & 15);
+  float sum = 0.0f;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int r0 = tile / tiles_c * kNsPad, c = tile % tiles_c * kNsPad + tc;
+    const int live = c >= a.cols ? 0 : (a.cols - c < 4 ? a.cols - c : 4);
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+      const int r = r0 + 16 * pass + tr;
+      const int64_t i = static_cast<int64_t>(r) * a.cols + c;
+      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (r < a.rows && live) {
+        float gv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const bool full = live == 4;
+        if (full) {
+          uint32_t w[group_words(GE)];
+          load_group<GE>(g, i, w);
+          decode_group<GE>(w, gv);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < live) gv[j] = decode<GE>(load1<GE>(g, i + j));
+        }
+        if constexpr (UE < 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = gv[j];
+        } else {
+          float uv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+          const uint32_t counter = t.counter[matrix] + static_cast<uint32_t>(i);
+          uint32_t w[group_words(UE)];
+          if (full) {
+            load_group<UE>(u, i, w);
+            decode_group<UE>(w, uv);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < live) uv[j] = decode<UE>(load1<UE>(u, i + j));
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uv[j] = uv[j] * a.momentum + gv[j];
+            v[j] = a.nesterov ? uv[j] * a.momentum + gv[j] : uv[j];
+          }
+          if (full) {
+            encode_group<UE>(uv, counter, w);
+            store_group<UE>(u, i, w);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (j < live) store1<UE>(u, i + j, encode<UE>(uv[j], counter + static_cast<uint32_t>(j)));
+              else v[j] = 0.0f;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum = fmaf(v[j], v[j], sum);
+      if (a.tall) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) turned[tc + j][16 * pass + tr] = v[j];
+      } else {
+        *reinterpret_cast<f32x4*>(x + static_cast<int64_t>(r) * a.n + c) = f32x4{v[0], v[1], v[2], v[3]};
+      }
+    }
+    if (a.tall) {
+      __syncthreads();
+#pragma unroll
+      for (int pass = 0; pass < 4; ++pass) {
+        const int row = 16 * pass + tr;
+        *reinterpret_cast<f32x4*>(x + static_cast<int64_t>(c - tc + row) * a.n + r0 + tc) =
+            f32x4{turned[row][tc], turned[row][tc + 1], turned[row][tc + 2], turned[row][tc + 3]};
+      }
+      __syncthreads();
+    }
+  }
+  sum = group_sum(sum, scratch);
+  if (threadIdx.x == 0) a.partial[matrix * kNsPartials + blockIdx.x] = sum;
+}
+
+// X = V / (|V|_F + eps) and its FP16 copies H and H^T, one 64 x 64 tile per workgroup.
+__global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a) {
+  __shared__ _Float16 turned[kNsPad][kNsPad + 8];
+  __shared__ float scratch[4];
+  const int matrix = blockIdx.y;
+  const float* partial = a.partial + matrix * kNsPartials;
+  float sum = 0.0f;
+  for (int i = threadIdx.x; i < a.partials; i += kNsThreads) sum += partial[i];
+  const float norm = sqrtf(group_sum(sum, scratch)) + a.eps;
+  const int64_t base = static_cast<int64_t>(matrix) * a.m * a.n;
+  float* x = a.x + base;
+  _Float16* h = a.h + base;
+  _Float16* ht = a.ht_next + base;
+  const int tiles_n = a.n / kNsPad;
+  const int r0 = blockIdx.x / tiles_n * kNsPad, c0 = blockIdx.x % tiles_n * kNsPad;
+  const int tr = threadIdx.x >> 4, tc = 4 * (threadIdx.x & 15);
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int64_t i = static_cast<int64_t>(r0 + 16 * pass + tr) * a.n + c0 + tc;
+    f32x4 v = *reinterpret_cast<const f32x4*>(x + i);
+    f16x4 w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = v[j] / norm;
+      w[j] = static_cast<_Float16>(v[j] * kNsScale);
+      turned[tc + j][16 * pass + tr] = w[j];
+    }
+    *reinterpret_cast<f32x4*>(x + i) = v;
+    *reinterpret_cast<f16x4*>(h + i) = w;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int row = 16 * pass + tr;
+    *reinterpret_cast<f16x4*>(ht + static_cast<int64_t>(c0 + row) * a.m + r0 + tc) =
+        *reinterpret_cast<const f16x4*>(&turned[row][tc]);
+  }
+}
+
+// Four consecutive values of row `row` of the result, in the caller's
+// orientation: stored, or applied to the parameter.
+__device__ __forceinline__ void finish(const NsArgs& a, const MatrixTable& t, int matrix, int row, int col,
+                                       const float (&y)[4]) {
+  if (row >= a.rows || col >= a.cols) return;
+  const int live = a.cols - col < 4 ? a.cols - col : 4;
+  const int64_t i = static_cast<int64_t>(row) * a.cols + col;
+  void* out = reinterpret_cast<void*>(t.p[matrix]);
+  auto at = [&](auto encoding) {
+    constexpr int E = decltype(encoding)::value;
+    if (live == 4) {
+      uint32_t w[group_words(E)];
+      float r[4];
+      if (a.muon) {
+        load_group<E>(out, i, w);
+        decode_group<E>(w, r);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = a.muon ? fmaf(y[j], a.neg_lr, r[j] * a.decay) : y[j];
+      encode_group<E>(r, 0u, w);
+      store_group<E>(out, i, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < live) {
+          const float r = a.muon ? fmaf(y[j], a.neg_lr, decode<E>(load1<E>(out, i + j)) * a.decay) : y[j];
+          store1<E>(out, i + j, encode<E>(r, 0u));
+        }
+    }
+  };
+  if (a.out_dtype == SR_F32) at(std::integral_constant<int, ENC_F32>{});
+  else if (a.out_dtype == SR_BF16) at(std::integral_constant<int, ENC_BF16_RN>{});
+  else at(std::integral_constant<int, ENC_F16_RN>{});
+}
+
+enum NsOp { kNsGram, kNsPolynomial, kNsStep, kNsLast };
+
+// One launch of products: S-shaped tiles of every matrix.
+//   kNsGram        G = H H^T, the lower triangle's tiles
+//   kNsPolynomial  P + s I = b G + c G^2 + s I, the same tiles
+//   kNsStep        X <- a X - s H + (P + s I) H, and the new H and H^T
+//   kNsLast        the same into the results or the parameters; TURNED where
+//                  these are the transpose of the workspace's orientation
+template <int OP, class S, bool TURNED>
+__global__ __launch_bounds__(S::kThreads, 2) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
+                                                                    uint32_t tiles, uint32_t matrices, MatrixTable t) {
+  constexpr bool kSymmetric = OP == kNsGram || OP == kNsPolynomial;
+  __shared__ __align__(1024) char lds[2 * S::kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t id = xcd_run(blockIdx.x, tiles * matrices);
+  const int matrix = id / tiles;
+  uint32_t tile_m, tile_n;
+  if constexpr (kSymmetric) {
+    triangle_tile(id % tiles, tile_m, tile_n);
+  } else {
+    band_tile(id % tiles, tiles_m, tiles_n, tile_m, tile_n);
+  }
+  const int row0 = tile_m * S::BM, col0 = tile_n * S::BN;
+  const int wave_m = wave / S::WN * S::kRowsM, wave_n = wave % S::WN * S::kRowsN;
+  const int64_t base = static_cast<int64_t>(matrix) * a.m * a.n, square = static_cast<int64_t>(matrix) * a.m * a.m;
+
+  Operand oa, ob;
+  int stages;
+  if constexpr (OP == kNsGram) {
+    oa = ob = {reinterpret_cast<const char*>(a.h + base), 2 * static_cast<int64_t>(a.n), a.m};
+    stages = a.n / (kStageBytes / 2);
+  } else {
+    oa = {reinterpret_cast<const char*>((OP == kNsPolynomial ? a.g : a.p) + square), 2 * static_cast<int64_t>(a.m), a.m};
+    ob = oa;
+    if constexpr (!kSymmetric) ob = {reinterpret_cast<const char*>(a.ht + base), 2 * static_cast<int64_t>(a.m), a.n};
+    stages = a.m / (kStageBytes / 2);
+  }
+  Stager<S> stager;
+  stager.init(oa, ob, row0, col0, wave, lane);
+
+  f32x4 acc[S::MI][S::NI] = {};
+  const uint32_t fragment = fragment_offset(lane);
+  stager.load_async(lds, 0, wave);
+  for (int kt = 0; kt < stages; ++kt) {
+    // Stage kt has landed for every wave, and every wave is done with the other buffer.
+    stage_barrier();
+    if (kt + 1 < stages)
+      stager.load_async(lds + (~kt & 1) * S::kStage, static_cast<int64_t>(kt + 1) * kStageBytes, wave);
+    const char* stage = lds + (kt & 1) * S::kStage;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const char* sa = stage + wave_m * kStageBytes + (fragment ^ (64 * ks));
+      const char* sb = stage + (S::BM + wave_n) * kStageBytes + (fragment ^ (64 * ks));
+      f16x8 fb[S::NI];
+#pragma unroll
+      for (int ni = 0; ni < S::NI; ++ni)
+        fb[ni] = __builtin_bit_cast(f16x8, read_chunk(sb + ni * 16 * kStageBytes));
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
+        const f16x8 fa = __builtin_bit_cast(f16x8, read_chunk(sa + mi * 16 * kStageBytes));
+#pragma unroll
+        for (int ni = 0; ni < S::NI; ++ni)
+          acc[mi][ni] = TURNED ? __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, fb[ni], acc[mi][ni], 0, 0, 0)
+                               : __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[ni], fa, acc[mi][ni], 0, 0, 0);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int mi = 0; mi < S::MI; ++mi) {
+#pragma unroll
+    for (int ni = 0; ni < S::NI; ++ni) {
+      const f32x4 v = acc[mi][ni];
+      if constexpr (TURNED) {
+        // Row `row` .. + 3 of the workspace's orientation, column `col`.
+        const int row = row0 + wave_m + mi * 16 + 4 * (lane >> 4), col = col0 + wave_n + ni * 16 + (lane & 15);
+        if (row >= a.m || col >= a.n) continue;
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float x = a.x[base + static_cast<int64_t>(row + j) * a.n + col];
+          const float h = static_cast<float>(static_cast<_Float16>(x * kNsScale)) * kNsInverse;
+          y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x));
+        }
+        finish(a, t, matrix, col, row, y);
+      } else {
+        const int row = row0 + wave_m + mi * 16 + (lane & 15), col = col0 + wave_n + ni * 16 + 4 * (lane >> 4);
+        if (row >= a.m || col >= (kSymmetric ? a.m : a.n)) continue;
+        if constexpr (kSymmetric) {
+          f16x4 w;
+          if constexpr (OP == kNsGram) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = static_cast<_Float16>(v[j] * kNsInverse);
+          } else {
+            const f16x4 g = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float p = fmaf(a.c * kNsInverse, v[j], a.b * static_cast<float>(g[j]));
+              w[j] = static_cast<_Float16>(row == col + j ? p + kNsShift * kNsScale : p);
+            }
+          }
+          _Float16* out = (OP == kNsGram ? a.g : a.p) + square;
+          *reinterpret_cast<f16x4*>(out + static_cast<int64_t>(row) * a.m + col) = w;
+          if (tile_m != tile_n) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) out[static_cast<int64_t>(col + j) * a.m + row] = w[j];
+          }
+        } else {
+          const int64_t i = base + static_cast<int64_t>(row) * a.n + col;
+          const f32x4 x = *reinterpret_cast<const f32x4*>(a.x + i);
+          float y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float h = static_cast<float>(static_cast<_Float16>(x[j] * kNsScale)) * kNsInverse;
+            y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x[j]));
+          }
+          if constexpr (OP == kNsStep) {
+            f16x4 w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              w[j] = static_cast<_Float16>(y[j] * kNsScale);
+              a.ht_next[base + static_cast<int64_t>(col + j) * a.m + row] = w[j];
+            }
+            *reinterpret_cast<f32x4*>(a.x + i) = f32x4{y[0], y[1], y[2], y[3]};
+            *reinterpret_cast<f16x4*>(a.h + i) = w;
+          } else {
+            finish(a, t, matrix, row, col, y);
+          }
+        }
+      }
+    }
+  }
+}
+
+}  // namespace sr

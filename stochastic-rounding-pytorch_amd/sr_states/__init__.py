@@ -6,7 +6,9 @@ optimizers ``AdamWReferenceSR/RN`` and ``SGDMReferenceSR/RN`` (the fused
 launch for the groups it takes, one parameter at a time otherwise) at the
 top level, the functional updates in ``sr_states.reference``, and the
 fused multi-tensor optimizers and casts in ``sr_states.hip`` (the
-counterpart of ``sr_states.triton``).  All arithmetic runs in the HIP
+counterpart of ``sr_states.triton``).  Beyond the reference: FP8 matrices with block scales
+and their products (``block_cast``, ``block_matmul``, ``block_linear``), and
+orthogonalised updates (``orthogonalize``, ``MuonHip``).  All arithmetic runs in the HIP
 library ``libsr_states_hip.so``; there is no CPU execution path.
 """
 
@@ -15,11 +17,19 @@ from .formats import StateFormat
 from .hip import (
     AdamWHip,
     AdamWHipRN,
+    BlockScaled,
+    MuonHip,
+    MuonHipRN,
     SGDMHip,
     SGDMHipRN,
+    block_cast,
+    block_linear,
+    block_matmul,
     hip_adamw_step_,
+    hip_muon_step_,
     hip_sgdm_step_,
     is_hip_available,
+    orthogonalize,
     rn_cast_bf16,
     sr_cast_bf16,
 )
@@ -32,16 +42,24 @@ __all__ = [
     "AdamWHipRN",
     "AdamWReferenceRN",
     "AdamWReferenceSR",
+    "BlockScaled",
+    "MuonHip",
+    "MuonHipRN",
     "SGDMHip",
     "SGDMHipRN",
     "SGDMReferenceRN",
     "SGDMReferenceSR",
     "StateFormat",
     "StateOptimizer",
+    "block_cast",
+    "block_linear",
+    "block_matmul",
     "cast",
     "hip_adamw_step_",
+    "hip_muon_step_",
     "hip_sgdm_step_",
     "is_hip_available",
+    "orthogonalize",
     "register_rounding",
     "rn_cast_bf16",
     "sr_cast_bf16",

@@ -73,6 +73,65 @@ class SgdmHparams(ctypes.Structure):
     _fields_ = [("momentum", ctypes.c_float), ("neg_lr", ctypes.c_float)]
 
 
+# The matrix operators (include/sr_matrix_hip.h).
+MATRIX_ABI_VERSION = 1
+BLOCK = 128  # values that share a scale along the contracted axis
+SCALE_E8M0, SCALE_F32 = range(2)
+MATRIX_BATCH = 64  # matrices one launch takes
+
+
+class BlockMatrix(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("ld", ctypes.c_int64),
+        ("ld_scale", ctypes.c_int64),
+        ("rows", ctypes.c_int64),
+        ("dtype", ctypes.c_int),
+        ("scale_type", ctypes.c_int),
+        ("block_rows", ctypes.c_int),
+        ("reserved", ctypes.c_int),
+    ]
+
+
+class BlockOutput(ctypes.Structure):
+    _fields_ = [
+        ("data", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("ld", ctypes.c_int64),
+        ("ld_scale", ctypes.c_int64),
+    ]
+
+
+class NewtonSchulz(ctypes.Structure):
+    _fields_ = [
+        ("a", ctypes.c_float),
+        ("b", ctypes.c_float),
+        ("c", ctypes.c_float),
+        ("eps", ctypes.c_float),
+        ("steps", ctypes.c_int),
+    ]
+
+
+class MuonRow(ctypes.Structure):
+    _fields_ = [
+        ("p", ctypes.c_void_p),
+        ("g", ctypes.c_void_p),
+        ("u", ctypes.c_void_p),
+        ("key", ctypes.c_uint32),
+        ("offset", ctypes.c_uint32),
+    ]
+
+
+class MuonHparams(ctypes.Structure):
+    _fields_ = [
+        ("momentum", ctypes.c_float),
+        ("decay", ctypes.c_float),
+        ("neg_lr", ctypes.c_float),
+        ("nesterov", ctypes.c_int),
+    ]
+
+
 _vp, _i64, _u32, _u64, _int = (
     ctypes.c_void_p,
     ctypes.c_int64,
@@ -117,6 +176,31 @@ SIGNATURES = {
     ),
 }
 
+# The complete exported surface of sr_matrix_hip.h.
+MATRIX_SIGNATURES = {
+    "sr_matrix_abi_version": (_int, []),
+    "sr_block_cast": (
+        _int,
+        [_vp, _i64, _i64, _i64, _int, _int, _int, _int, _u32, _u32, ctypes.POINTER(BlockOutput),
+         ctypes.POINTER(BlockOutput), _vp],
+    ),
+    "sr_block_matmul": (
+        _int,
+        [ctypes.POINTER(BlockMatrix), ctypes.POINTER(BlockMatrix), _i64, _vp, _i64, _int, _vp, _vp],
+    ),
+    "sr_block_matmul_workspace": (_i64, [_i64, _i64, _i64]),
+    "sr_orthogonalize_workspace": (_i64, [_i64, _i64, _i64]),
+    "sr_orthogonalize": (
+        _int,
+        [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _int, _int, ctypes.POINTER(NewtonSchulz), _vp, _vp],
+    ),
+    "sr_muon_multi": (
+        _int,
+        [ctypes.POINTER(MuonRow), _int, _i64, _i64, _int, _int, _int, _int, ctypes.POINTER(MuonHparams),
+         ctypes.POINTER(NewtonSchulz), _vp, _vp],
+    ),
+}
+
 _lock = threading.Lock()
 _handle: ctypes.CDLL | None = None
 
@@ -134,13 +218,16 @@ def library() -> ctypes.CDLL:
                     "(run stochastic-rounding-pytorch_amd/build.py)"
                 )
             handle = ctypes.CDLL(str(LIBRARY_PATH))
-            for name, (restype, argtypes) in SIGNATURES.items():
+            for name, (restype, argtypes) in {**SIGNATURES, **MATRIX_SIGNATURES}.items():
                 function = getattr(handle, name)
                 function.restype = restype
                 function.argtypes = argtypes
             version = handle.sr_abi_version()
             if version != ABI_VERSION:
                 raise RuntimeError(f"library ABI {version} does not match binding ABI {ABI_VERSION}")
+            version = handle.sr_matrix_abi_version()
+            if version != MATRIX_ABI_VERSION:
+                raise RuntimeError(f"library matrix ABI {version} does not match binding ABI {MATRIX_ABI_VERSION}")
             _handle = handle
     return _handle
 
