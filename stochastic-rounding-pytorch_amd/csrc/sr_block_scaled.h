@@ -12,12 +12,13 @@ namespace sr {
 // ---------------------------------------------------------------------------
 // Cast to FP8 with a power of two for each block of 128.
 //
-// A workgroup takes a 128 x 128 tile of x into registers, each thread 4 x 4
-// values of each of four 32-row bands, so that one read serves both
-// orientations: row blocks reduce over half a wave, column blocks over
-// the bands and, through LDS, over the eight half-waves.  Encoded bytes of
-// the transposed orientation are turned 4 x 4 in registers and cross LDS
-// once; both outputs leave as whole 128-byte runs.
+// A workgroup takes a 128 x 128 tile of x into registers, so that one read
+// serves both orientations.  Sixteen lanes share a row, eight values each (one
+// 16-byte load of BF16): a row's maximum is four rotations inside them.  A
+// thread holds four neighbouring rows of each 64-row band; the columns' maxima
+// cross LDS once, and the encoded bytes of the transposed orientation are
+// turned 4 x 4 in registers and cross it once.  Rows leave as 128 bytes of
+// sixteen lanes, columns as 128 bytes of 32.
 // ---------------------------------------------------------------------------
 constexpr int kCastTile = 128, kCastThreads = 256;
 
@@ -59,107 +60,140 @@ __device__ __forceinline__ void transpose_bytes(uint32_t (&w)[4]) {
   w[3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
 }
 
+// The largest of the 16 lanes of a row, in all of them.
+__device__ __forceinline__ uint32_t max_of_16(uint32_t m) {
+  m = umax(m, __builtin_amdgcn_update_dpp(0u, m, 0x128, 0xF, 0xF, true));  // rotations by 8, 4, 2, 1 lanes
+  m = umax(m, __builtin_amdgcn_update_dpp(0u, m, 0x124, 0xF, 0xF, true));
+  m = umax(m, __builtin_amdgcn_update_dpp(0u, m, 0x122, 0xF, 0xF, true));
+  return umax(m, __builtin_amdgcn_update_dpp(0u, m, 0x121, 0xF, 0xF, true));
+}
+
 template <int XE, int QE, bool SQUARE>
 __global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs a) {
   constexpr int TOP = (QE == ENC_E4M3_RN || QE == ENC_E4M3_SR) ? 8 : 15;
   constexpr int XB = enc_bytes(XE);
   __shared__ uint32_t turned[kCastTile * 32];
-  __shared__ uint32_t partial[8][kCastTile];
-  __shared__ uint32_t whole[8];
-  const int t = threadIdx.x, half = t >> 5, lane = t & 31;
+  __shared__ __align__(16) uint32_t partial[SQUARE ? 1 : 16][kCastTile];
+  __shared__ __align__(16) int exponents[kCastTile];
+  __shared__ uint32_t whole[4];
+  const int t = threadIdx.x, group = t >> 4, lane = t & 15;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x / a.tiles_n) * kCastTile;
   const int64_t col0 = static_cast<int64_t>(blockIdx.x % a.tiles_n) * kCastTile;
-  const int64_t c = col0 + 4 * lane;
-  const int live = c >= a.cols ? 0 : (a.cols - c < 4 ? static_cast<int>(a.cols - c) : 4);
+  const int64_t c = col0 + 8 * lane;
+  const int live = c >= a.cols ? 0 : (a.cols - c < 8 ? static_cast<int>(a.cols - c) : 8);
 
-  // Rows of this thread: band k, row 32 k + 4 half + i.
-  float x[4][4][4];
+  // Rows of this thread: band k, row 64 k + 4 group + i.
+  float x[2][4][8];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < 2; ++k) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t r = row0 + 32 * k + 4 * half + i;
+      const int64_t r = row0 + 64 * k + 4 * group + i;
       const char* p = a.x + (r * a.ldx + c) * XB;
-      if (r < a.rows && live == 4) {
-        uint32_t w[group_words(XE)];
-        load_words<4 * XB, true>(p, w);
-        decode_group<XE>(w, x[k][i]);
+      if (r < a.rows && live == 8) {
+        uint32_t w[2 * group_words(XE)];
+        if constexpr (XB == 4) {
+          load_words<16, true>(p, w);
+          load_words<16, true>(p + 16, w + 4);
+        } else {
+          load_words<16, true>(p, w);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t words[group_words(XE)];
+          float v[4];
+#pragma unroll
+          for (int j = 0; j < group_words(XE); ++j) words[j] = w[h * group_words(XE) + j];
+          decode_group<XE>(words, v);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[k][i][4 * h + j] = v[j];
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          x[k][i][j] = r < a.rows && j < live ? decode<XE>(load1<XE>(p, j)) : 0.0f;
+        for (int j = 0; j < 8; ++j) x[k][i][j] = r < a.rows && j < live ? decode<XE>(load1<XE>(p, j)) : 0.0f;
       }
     }
   }
 
   const bool want_rows = a.by_rows.data != nullptr, want_cols = a.by_cols.data != nullptr;
-  uint32_t tile_max = 0;  // SQUARE
-  int col_exp[4];         // of this thread's four columns
+  int tile_exp = 0;  // SQUARE
+  int col_exp[8];    // of this thread's columns
   if (SQUARE || want_cols) {
-    uint32_t m[4] = {0, 0, 0, 0};
+    uint32_t m[8] = {};
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m[j] = umax(m[j], finite_magnitude(x[k][i][j]));
+        for (int j = 0; j < 8; ++j) m[j] = umax(m[j], finite_magnitude(x[k][i][j]));
     if constexpr (SQUARE) {
-      tile_max = umax(umax(m[0], m[1]), umax(m[2], m[3]));
+      uint32_t tile = 0;
 #pragma unroll
-      for (int d = 16; d; d >>= 1) tile_max = umax(tile_max, __shfl_xor(tile_max, d, 32));
-      if (lane == 0) whole[half] = tile_max;
+      for (int j = 0; j < 8; ++j) tile = umax(tile, m[j]);
+      tile = max_of_16(tile);
+      tile = umax(tile, __shfl_xor(tile, 16));
+      tile = umax(tile, __shfl_xor(tile, 32));
+      if ((t & 63) == 0) whole[t >> 6] = tile;
       __syncthreads();
+      tile_exp = block_exponent<TOP>(umax(umax(whole[0], whole[1]), umax(whole[2], whole[3])));
 #pragma unroll
-      for (int h = 0; h < 8; ++h) tile_max = umax(tile_max, whole[h]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) col_exp[j] = block_exponent<TOP>(tile_max);
+      for (int j = 0; j < 8; ++j) col_exp[j] = tile_exp;
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) partial[half][4 * lane + j] = m[j];
+      for (int j = 0; j < 8; ++j) partial[group][8 * lane + j] = m[j];
+      __syncthreads();
+      if (t < kCastTile) {
+        uint32_t col = 0;
+#pragma unroll
+        for (int h = 0; h < 16; ++h) col = umax(col, partial[h][t]);
+        const int e = block_exponent<TOP>(col);
+        exponents[t] = e;
+        if (col0 + t < a.cols)
+          *gptr_mut<uint8_t>(static_cast<char*>(a.by_cols.scale) + (col0 + t) * a.by_cols.ld_scale + row0 / kCastTile) =
+              static_cast<uint8_t>(e + 127);
+      }
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int h = 0; h < 8; ++h) m[j] = umax(m[j], partial[h][4 * lane + j]);
-        col_exp[j] = block_exponent<TOP>(m[j]);
-      }
+      for (int j = 0; j < 8; ++j) col_exp[j] = exponents[8 * lane + j];
     }
   }
 
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    uint32_t hash[4][4], by_col[4];
+  for (int k = 0; k < 2; ++k) {
+    if (row0 + 64 * k >= a.rows && !want_cols) break;
+    uint32_t by_col[2][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t r = row0 + 32 * k + 4 * half + i;
+      const int64_t r = row0 + 64 * k + 4 * group + i;
       const uint32_t counter = a.counter_base + static_cast<uint32_t>(r) * static_cast<uint32_t>(a.cols) + static_cast<uint32_t>(c);
+      uint32_t hash[2][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) hash[i][j] = enc_stochastic(QE) ? h32(counter + static_cast<uint32_t>(j)) : 0u;
-      uint32_t bits[4], word[1];
+      for (int j = 0; j < 8; ++j) hash[j >> 2][j & 3] = enc_stochastic(QE) ? h32(counter + static_cast<uint32_t>(j)) : 0u;
+      uint32_t bits[4], word[1], words[2];
       if (want_rows) {
-        int e;
-        if constexpr (SQUARE) {
-          e = col_exp[0];
-        } else {
+        int e = tile_exp;
+        if constexpr (!SQUARE) {
           uint32_t m = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) m = umax(m, finite_magnitude(x[k][i][j]));
-#pragma unroll
-          for (int d = 16; d; d >>= 1) m = umax(m, __shfl_xor(m, d, 32));
-          e = block_exponent<TOP>(m);
+          for (int j = 0; j < 8; ++j) m = umax(m, finite_magnitude(x[k][i][j]));
+          e = block_exponent<TOP>(max_of_16(m));
         }
         const float inv = inverse_scale(e);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bits[j] = f32_bits(x[k][i][j] * inv);
-        encode_group_with<QE>(bits, hash[i], word);
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) bits[j] = f32_bits(x[k][i][4 * h + j] * inv);
+          encode_group_with<QE>(bits, hash[h], word);
+          words[h] = word[0];
+        }
         if (r < a.rows) {
           char* q = static_cast<char*>(a.by_rows.data) + r * a.by_rows.ld + c;
-          if (live == 4) {
-            store_words<4>(q, word);
+          if (live == 8) {
+            *(SR_GLOBAL group8*)(q) = group8{words[0], words[1]};
           } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j < live) *gptr_mut<uint8_t>(q + j) = static_cast<uint8_t>(word[0] >> (8 * j));
+            for (int j = 0; j < 8; ++j)
+              if (j < live) *gptr_mut<uint8_t>(q + j) = static_cast<uint8_t>(words[j >> 2] >> (8 * (j & 3)));
           }
           if constexpr (!SQUARE)
             if (lane == 0)
@@ -168,52 +202,55 @@ __global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs 
         }
       }
       if (want_cols) {
+        if (SQUARE && want_rows) {  // the same bytes
+          by_col[0][i] = words[0];
+          by_col[1][i] = words[1];
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) bits[j] = f32_bits(x[k][i][j] * inverse_scale(col_exp[j]));
-        encode_group_with<QE>(bits, hash[i], word);
-        by_col[i] = word[0];
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) bits[j] = f32_bits(x[k][i][4 * h + j] * inverse_scale(col_exp[4 * h + j]));
+            encode_group_with<QE>(bits, hash[h], word);
+            by_col[h][i] = word[0];
+          }
+        }
       }
     }
     if (want_cols) {
-      transpose_bytes(by_col);
-      // Column 4 lane + j, rows 32 k + 4 half .. + 3, at word (row / 4) ^ lane of its column: the lanes of a
-      // half-wave meet in different banks here, and those that read a column below do too.
+      // Column 8 lane + j, rows 64 k + 4 group .. + 3, at word (row / 4) ^ (2 lane) of its column's 32: the lanes
+      // of a wave then meet in a bank two at a time, and those that read a column below do not.
 #pragma unroll
-      for (int j = 0; j < 4; ++j) turned[(4 * lane + j) * 32 + ((8 * k + half) ^ lane)] = by_col[j];
+      for (int h = 0; h < 2; ++h) {
+        transpose_bytes(by_col[h]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) turned[(8 * lane + 4 * h + j) * 32 + ((16 * k + group) ^ (2 * lane))] = by_col[h][j];
+      }
     }
   }
 
   if (SQUARE && t == 0) {
-    const uint8_t byte = static_cast<uint8_t>(block_exponent<TOP>(tile_max) + 127);
+    const uint8_t byte = static_cast<uint8_t>(tile_exp + 127);
     const int64_t rb = row0 / kCastTile, cb = col0 / kCastTile;
     if (want_rows) *gptr_mut<uint8_t>(static_cast<char*>(a.by_rows.scale) + rb * a.by_rows.ld_scale + cb) = byte;
     if (want_cols) *gptr_mut<uint8_t>(static_cast<char*>(a.by_cols.scale) + cb * a.by_cols.ld_scale + rb) = byte;
   }
   if (!want_cols) return;
-  if constexpr (!SQUARE) {
-    if (half == 0) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < live)
-          *gptr_mut<uint8_t>(static_cast<char*>(a.by_cols.scale) + (c + j) * a.by_cols.ld_scale + row0 / kCastTile) =
-              static_cast<uint8_t>(col_exp[j] + 127);
-    }
-  }
   __syncthreads();
-  const int64_t r = row0 + 4 * lane;
+  const int word_at = t & 31, half = t >> 5;
+  const int64_t r = row0 + 4 * word_at;
   const int live_r = r >= a.rows ? 0 : (a.rows - r < 4 ? static_cast<int>(a.rows - r) : 4);
 #pragma unroll
   for (int k = 0; k < kCastTile / 8; ++k) {
     const int col = 8 * k + half;
     if (col0 + col >= a.cols) break;
-    const uint32_t word[1] = {turned[col * 32 + (lane ^ (col >> 2))]};
+    const uint32_t word = turned[col * 32 + (word_at ^ (2 * (col >> 3)))];
     char* q = static_cast<char*>(a.by_cols.data) + (col0 + col) * a.by_cols.ld + r;
     if (live_r == 4) {
-      store_words<4>(q, word);
+      *(SR_GLOBAL group4*)(q) = word;
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (j < live_r) *gptr_mut<uint8_t>(q + j) = static_cast<uint8_t>(word[0] >> (8 * j));
+        if (j < live_r) *gptr_mut<uint8_t>(q + j) = static_cast<uint8_t>(word >> (8 * j));
     }
   }
 }
@@ -239,12 +276,13 @@ struct BlockProductArgs {
 template <int DT>
 constexpr int kFormatCode = DT == SR_E4M3 ? 0 : 1;
 
-// Four consecutive results of row `row`.
+// Four consecutive results of row `row`, as OUT.  EDGE: they may lie outside the result, wholly or in part.
+template <int OUT, bool EDGE>
 __device__ __forceinline__ void store_results(const BlockProductArgs& g, int row, int col, const f32x4& v) {
-  if (row >= g.m || col >= g.n) return;
-  const int live = g.n - col < 4 ? g.n - col : 4;
+  if (EDGE && (row >= g.m || col >= g.n)) return;
+  const int live = EDGE && g.n - col < 4 ? g.n - col : 4;
   const int64_t at = row * g.ldo + col;
-  if (g.out_dtype == SR_F32) {
+  if constexpr (OUT == SR_F32) {
     float* p = reinterpret_cast<float*>(g.out) + at;
     if (live == 4) {
       uint32_t w[4];
@@ -255,20 +293,53 @@ __device__ __forceinline__ void store_results(const BlockProductArgs& g, int row
       for (int j = 0; j < 4; ++j)
         if (j < live) *gptr_mut<float>(p + j) = v[j];
     }
-    return;
-  }
-  uint32_t code[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    code[j] = g.out_dtype == SR_BF16 ? bf16_rn(f32_bits(v[j])) : minifloat_encode<F16, false>(f32_bits(v[j]), 0u);
-  uint16_t* p = reinterpret_cast<uint16_t*>(g.out) + at;
-  if (live == 4) {
-    *(SR_GLOBAL group8*)(p) = group8{code[0] | code[1] << 16, code[2] | code[3] << 16};
   } else {
+    const float x[4] = {v[0], v[1], v[2], v[3]};
+    uint32_t w[2];
+    encode_group<OUT == SR_BF16 ? ENC_BF16_RN : ENC_F16_RN>(x, 0u, w);
+    uint16_t* p = reinterpret_cast<uint16_t*>(g.out) + at;
+    if (live == 4) {
+      *(SR_GLOBAL group8*)(p) = group8{w[0], w[1]};
+    } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < live) *gptr_mut<uint16_t>(p + j) = static_cast<uint16_t>(code[j]);
+      for (int j = 0; j < 4; ++j)
+        if (j < live) *gptr_mut<uint16_t>(p + j) = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+    }
   }
+}
+
+// Calls store(OUT, EDGE) for the result's type and whether the rows x cols from (row0, col0) pass its edges.
+template <class F>
+__device__ __forceinline__ void with_output(const BlockProductArgs& g, int row0, int col0, int rows, int cols, F&& store) {
+  auto typed = [&](auto out) {
+    if (row0 + rows <= g.m && col0 + cols <= g.n) store(out, std::false_type{});
+    else store(out, std::true_type{});
+  };
+  if (g.out_dtype == SR_F32) typed(std::integral_constant<int, SR_F32>{});
+  else if (g.out_dtype == SR_BF16) typed(std::integral_constant<int, SR_BF16>{});
+  else typed(std::integral_constant<int, SR_F16>{});
+}
+
+// Stores a workgroup's results through its LDS, which every wave is done with.
+template <int LDS, class S, class Acc>
+__device__ __forceinline__ void store_chunks(const BlockProductArgs& g, char* lds, int row0, int col0, int wave, int lane,
+                                             const Acc& acc) {
+  using Chunk = ResultChunk<S::kRowsN>;
+  static_assert(S::kWaves * Chunk::kBytes <= LDS, "a chunk per wave");
+  const int wave_row = row0 + wave / S::WN * S::kRowsM, wave_col = col0 + wave % S::WN * S::kRowsN;
+  float* chunk = reinterpret_cast<float*>(lds + wave * Chunk::kBytes);
+  with_output(g, row0, col0, S::BM, S::BN, [&](auto out, auto edge) {
+    for_each_chunk<S>(chunk, lane, acc, [&](int first, const float* from) {
+#pragma unroll
+      for (int i = 0; i < Chunk::kBlocks; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = Chunk::block_row(i, lane) + k, col = Chunk::block_col(lane);
+          store_results<decltype(out)::value, decltype(edge)::value>(g, wave_row + first + row, wave_col + col,
+                                                                     Chunk::get(from, row, col));
+        }
+    });
+  });
 }
 
 // How a product multiplies and scales.
@@ -288,10 +359,42 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
   return bits_f32(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7FC00000u : byte << 23));
 }
 
+// The scales of a workgroup's rows, 32 bytes of each at a time (32 exponent
+// bytes or 8 FP32 factors), in LDS beside the stages.  Read from memory stage
+// by stage they would cost more than they weigh: the scales of one stage lie in a
+// cache line of their own for every row, and an access to 64 lines takes
+// 64 cycles (measured at 8192 x 8192 x 2048 on 128 x 128 tiles: 202 us with a
+// load per fragment and stage, 144 so).
+// Rows are 36 bytes apart: 32 rows' same bytes then lie in different banks.
+template <class S>
+struct ScaleArea {
+  static constexpr int kRow = 36, kFill = 32, kBytes = (S::BM + S::BN) * kRow;
+
+  static __device__ __forceinline__ int period(const BlockProductArgs& g) { return g.scale_f32 ? kFill / 4 : kFill; }
+
+  // Blocks [first, first + period) of every row; rows past the end repeat the last one.
+  static __device__ void fill(char* area, const BlockProductArgs& g, int row0, int col0, int first, int total) {
+    const int size = g.scale_f32 ? 4 : 1;
+    for (int r = threadIdx.x; r < S::BM + S::BN; r += S::kThreads) {
+      const bool of_a = r < S::BM;
+      const int at = of_a ? row0 + r : col0 + r - S::BM, rows = of_a ? g.m : g.n;
+      const char* from = (of_a ? g.scale_a : g.scale_b) +
+                         (((at < rows ? at : rows - 1) >> (of_a ? g.shift_a : g.shift_b)) * (of_a ? g.ld_scale_a : g.ld_scale_b) + first) * size;
+      const int64_t end = static_cast<int64_t>(total - first) * size;
+      const i32x4 lo = load_chunk(from, 0, end), hi = load_chunk(from, 16, end);
+      int* to = reinterpret_cast<int*>(area + r * kRow);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        to[j] = lo[j];
+        to[4 + j] = hi[j];
+      }
+    }
+  }
+};
+
 // The scales one lane needs for one block of the contracted axis.  kExponents:
 // the exponent byte of its row of each fragment.  Otherwise: the factor of its
-// row of A and of each of the four rows of B whose results it holds.  Rows
-// past the end repeat the last one.
+// row of A and of each of the four rows of B whose results it holds.
 template <int MODE, int MI, int NI>
 struct Scales {
   static constexpr bool kExp = MODE == kExponents;
@@ -299,52 +402,24 @@ struct Scales {
   using Value = std::conditional_t<kExp, int, float>;
   Value a[MI], b[NI][kPerB];
 
-  struct Places {
-    const char* a;  // of the first scale row of this workgroup's tile
-    const char* b;
-    uint32_t offset_a[MI], offset_b[NI][kPerB];  // bytes; a tile spans at most 2^8 rows of at most 2^20 scales
-    uint32_t size;                               // of one scale
-    bool shared_b;
+  static __device__ __forceinline__ Value read(const char* p, bool f32) {
+    if constexpr (kExp) return *reinterpret_cast<const uint8_t*>(p);
+    else if constexpr (MODE == kFactors) return *reinterpret_cast<const float*>(p);
+    else return f32 ? *reinterpret_cast<const float*>(p) : e8m0_value(*reinterpret_cast<const uint8_t*>(p));
+  }
 
-    __device__ void init(const BlockProductArgs& g, int tile_row, int tile_col, int wave_row, int wave_col, int lane) {
-      size = kExp ? 1 : (MODE == kFactors || g.scale_f32 ? 4 : 1);
-      const int first_a = tile_row >> g.shift_a, first_b = tile_col >> g.shift_b;
-      a = g.scale_a + first_a * g.ld_scale_a * size;
-      b = g.scale_b + first_b * g.ld_scale_b * size;
-      shared_b = g.shift_b != 0;
+  // `wave_m`, `wave_n`: this wave's first rows of A and B in the area; `slot`: the block's place in a row.
+  template <class S>
+  __device__ __forceinline__ void load(const char* area, int wave_m, int wave_n, int slot, bool f32, int lane) {
+    const char* at = area + (f32 ? 4 * slot : slot);
+    const char* pa = at + (wave_m + (lane & 15)) * ScaleArea<S>::kRow;
+    const char* pb = at + (S::BM + wave_n + (kExp ? lane & 15 : 4 * (lane >> 4))) * ScaleArea<S>::kRow;
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int r = wave_row + i * 16 + (lane & 15);
-        offset_a[i] = static_cast<uint32_t>(((r < g.m ? r : g.m - 1) >> g.shift_a) - first_a) *
-                      static_cast<uint32_t>(g.ld_scale_a) * size;
-      }
+    for (int i = 0; i < MI; ++i) a[i] = read(pa + i * 16 * ScaleArea<S>::kRow, f32);
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-        for (int j = 0; j < kPerB; ++j) {
-          const int r = wave_col + i * 16 + (kExp ? lane & 15 : 4 * (lane >> 4) + j);
-          offset_b[i][j] = static_cast<uint32_t>(((r < g.n ? r : g.n - 1) >> g.shift_b) - first_b) *
-                           static_cast<uint32_t>(g.ld_scale_b) * size;
-        }
-    }
-
-    __device__ Value read(const char* p) const {
-      if constexpr (kExp) return *gptr<uint8_t>(p);
-      else if constexpr (MODE == kFactors) return *gptr<float>(p);
-      else return size == 4 ? *gptr<float>(p) : e8m0_value(*gptr<uint8_t>(p));
-    }
-  };
-
-  __device__ void load(const Places& at, int64_t kb) {
-    const char* pa = at.a + kb * at.size;
-    const char* pb = at.b + kb * at.size;
-#pragma unroll
-    for (int i = 0; i < MI; ++i) a[i] = at.read(pa + at.offset_a[i]);
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-#pragma unroll
-      for (int j = 0; j < kPerB; ++j) b[i][j] = j && at.shared_b ? b[i][0] : at.read(pb + at.offset_b[i][j]);
-    }
+      for (int j = 0; j < kPerB; ++j) b[i][j] = read(pb + (i * 16 + j) * ScaleArea<S>::kRow, f32);
   }
 };
 
@@ -402,7 +477,9 @@ __device__ __forceinline__ void block_mma(f32x4& acc, const Fragment<MODE, FA>& 
 
 template <int MODE, int FA, int FB, class S, bool ASYNC>
 __global__ __launch_bounds__(S::kThreads, 2) void block_product_kernel(BlockProductArgs g) {
-  __shared__ __align__(1024) char lds[2 * S::kStage];
+  constexpr int kStages = 2 * S::kStage + ScaleArea<S>::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
+  constexpr int kLds = kStages > kChunks ? kStages : kChunks;
+  __shared__ __align__(1024) char lds[kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   uint32_t tile_m, tile_n;
   band_tile(xcd_run(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tile_m, tile_n);
@@ -411,13 +488,15 @@ __global__ __launch_bounds__(S::kThreads, 2) void block_product_kernel(BlockProd
 
   Stager<S> stager;
   stager.init(g.a, g.b, row0, col0, wave, lane);
-  Scales<MODE, S::MI, S::NI> scales, next;
-  typename Scales<MODE, S::MI, S::NI>::Places places;
-  places.init(g, row0, col0, row0 + wave_m, col0 + wave_n, lane);
+  char* area = lds + 2 * S::kStage;
+  const int period = ScaleArea<S>::period(g);
 
   f32x4 acc[S::MI][S::NI] = {};
   const uint32_t fragment = fragment_offset(lane);
-  auto multiply = [&](const char* stage) {
+  const int stages = static_cast<int>((g.k + kStageBytes - 1) / kStageBytes);
+  auto multiply = [&](const char* stage, int kt) {
+    Scales<MODE, S::MI, S::NI> scales;
+    scales.template load<S>(area, wave_m, wave_n, kt & (period - 1), g.scale_f32, lane);
     const char* sa = stage + wave_m * kStageBytes + fragment;
     const char* sb = stage + (S::BM + wave_n) * kStageBytes + fragment;
     const char* sa2 = stage + wave_m * kStageBytes + (fragment ^ 64);
@@ -436,57 +515,47 @@ __global__ __launch_bounds__(S::kThreads, 2) void block_product_kernel(BlockProd
   };
 
   // Stage kt lies in buffer kt % 2.  At its barrier it has landed for every
-  // wave, and every wave is done with the other buffer.
-  const int stages = static_cast<int>((g.k + kStageBytes - 1) / kStageBytes);
+  // wave, and every wave is done with the other buffer and the scales before.
+  auto refill = [&](int kt) {
+    if ((kt & (period - 1)) == 0) {
+      ScaleArea<S>::fill(area, g, row0, col0, kt, stages);
+      stage_barrier();
+    }
+  };
   if constexpr (ASYNC) {
     const int whole = static_cast<int>(g.k / kStageBytes);
-    if (whole > 0) {
-      scales.load(places, 0);
-      stager.load_async(lds, 0, wave);
-    }
+    if (whole > 0) stager.load_async(lds, 0, wave);
     for (int kt = 0; kt < whole; ++kt) {
       stage_barrier();
-      if (kt + 1 < whole) {
-        next.load(places, kt + 1);
-        stager.load_async(lds + (~kt & 1) * S::kStage, static_cast<int64_t>(kt + 1) * kStageBytes, wave);
-      }
-      multiply(lds + (kt & 1) * S::kStage);
-      scales = next;
+      refill(kt);
+      if (kt + 1 < whole) stager.load_async(lds + (~kt & 1) * S::kStage, (kt + 1) * kStageBytes, wave);
+      multiply(lds + (kt & 1) * S::kStage, kt);
     }
     if (whole < stages) {  // the contracted axis ends inside a stage
-      char* stage = lds + (whole & 1) * S::kStage;
-      i32x4 regs[S::kLoads];
-      scales.load(places, whole);
-      stager.load(regs, static_cast<int64_t>(whole) * kStageBytes, g.k, wave, lane);
-      stager.store(stage, regs, wave, lane);
       stage_barrier();
-      multiply(stage);
+      refill(whole);
+      char* stage = lds + (whole & 1) * S::kStage;
+      stager.load_through(stage, static_cast<int64_t>(whole) * kStageBytes, g.k, wave, lane);
+      stage_barrier();
+      multiply(stage, whole);
     }
   } else {
     i32x4 regs[S::kLoads];
     if (stages > 0) {
-      scales.load(places, 0);
       stager.load(regs, 0, g.k, wave, lane);
       stager.store(lds, regs, wave, lane);
     }
     for (int kt = 0; kt < stages; ++kt) {
       stage_barrier();
+      refill(kt);
       const bool more = kt + 1 < stages;
-      if (more) {
-        next.load(places, kt + 1);
-        stager.load(regs, static_cast<int64_t>(kt + 1) * kStageBytes, g.k, wave, lane);
-      }
-      multiply(lds + (kt & 1) * S::kStage);
+      if (more) stager.load(regs, static_cast<int64_t>(kt + 1) * kStageBytes, g.k, wave, lane);
+      multiply(lds + (kt & 1) * S::kStage, kt);
       if (more) stager.store(lds + (~kt & 1) * S::kStage, regs, wave, lane);
-      scales = next;
     }
   }
-
-#pragma unroll
-  for (int mi = 0; mi < S::MI; ++mi)
-#pragma unroll
-    for (int ni = 0; ni < S::NI; ++ni)
-      store_results(g, row0 + wave_m + mi * 16 + (lane & 15), col0 + wave_n + ni * 16 + 4 * (lane >> 4), acc[mi][ni]);
+  stage_barrier();
+  store_chunks<kLds, S>(g, lds, row0, col0, wave, lane, acc);
 }
 
 // Few rows of A (at most 16): one 16-column tile of the result per workgroup,
@@ -504,13 +573,21 @@ __global__ __launch_bounds__(64 * kRowWaves) void block_product_rows_kernel(Bloc
   const int row_b = col0 + (lane & 15) < g.n ? col0 + (lane & 15) : g.n - 1;
   const char* pa = g.a.base + row_a * g.a.ld;
   const char* pb = g.b.base + row_b * g.b.ld;
-  typename Scales<MODE, 1, 1>::Places places;
-  places.init(g, 0, col0, 0, col0, lane);
+  const int size = g.scale_f32 ? 4 : 1;
+  const char* scale_a = g.scale_a + (row_a >> g.shift_a) * g.ld_scale_a * size;
+  const char* scale_b[Scales<MODE, 1, 1>::kPerB];
+#pragma unroll
+  for (int j = 0; j < Scales<MODE, 1, 1>::kPerB; ++j) {
+    const int r = col0 + (MODE == kExponents ? lane & 15 : 4 * (lane >> 4) + j);
+    scale_b[j] = g.scale_b + ((r < g.n ? r : g.n - 1) >> g.shift_b) * g.ld_scale_b * size;
+  }
   f32x4 acc{};
   const int stages = static_cast<int>((g.k + kStageBytes - 1) / kStageBytes);
   for (int kb = wave; kb < stages; kb += kRowWaves) {
     Scales<MODE, 1, 1> s;
-    s.load(places, kb);
+    s.a[0] = Scales<MODE, 1, 1>::read(scale_a + kb * size, g.scale_f32);
+#pragma unroll
+    for (int j = 0; j < Scales<MODE, 1, 1>::kPerB; ++j) s.b[0][j] = Scales<MODE, 1, 1>::read(scale_b[j] + kb * size, g.scale_f32);
     const int64_t at = static_cast<int64_t>(kb) * kStageBytes + (lane >> 4) * kChunk;
     Fragment<MODE, FA> a;
     Fragment<MODE, FB> b;
@@ -523,7 +600,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void block_product_rows_kernel(Bloc
   if (wave) return;
 #pragma unroll
   for (int w = 1; w < kRowWaves; ++w) acc += sums[w][lane];
-  store_results(g, lane & 15, col0 + 4 * (lane >> 4), acc);
+  with_output(g, 0, col0, 16, 16, [&](auto out, auto edge) {
+    store_results<decltype(out)::value, decltype(edge)::value>(g, lane & 15, col0 + 4 * (lane >> 4), acc);
+  });
 }
 
 }  // namespace sr

@@ -132,14 +132,17 @@ int sr_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t 
     g.tiles_n = (g.n + 15) / 16;
     return launch(fn.rows, g.tiles_n, 64 * sr::kRowWaves, &g, stream);
   }
-  const uint64_t big = static_cast<uint64_t>((g.m + 127) / 128) * ((g.n + 127) / 128);
-  const bool small = big < 256;
-  const int tile = small ? 64 : 128;
-  g.tiles_m = (g.m + tile - 1) / tile;
-  g.tiles_n = (g.n + tile - 1) / tile;
+  auto tiles = [&](int64_t side) { return ((g.m + side - 1) / side) * ((g.n + side - 1) / side); };
   const bool async = aligned_rows(a) && aligned_rows(b);
-  return launch(fn.tile[small ? sr::kTile64 : sr::kTile128][async],
-                static_cast<uint64_t>(g.tiles_m) * g.tiles_n, 256, &g, stream);
+  auto launch_tiles = [&](const void* kernel, auto shape) {
+    using S = decltype(shape);
+    g.tiles_m = (g.m + S::BM - 1) / S::BM;
+    g.tiles_n = (g.n + S::BN - 1) / S::BN;
+    return launch(kernel, static_cast<uint64_t>(g.tiles_m) * g.tiles_n, S::kThreads, &g, stream);
+  };
+  // The larger tile where it still gives the chip's 256 CUs work.
+  if (tiles(128) >= 256) return launch_tiles(fn.tile[sr::kTile128][async], sr::Tile128{});
+  return launch_tiles(fn.tile[sr::kTile64][async], sr::Tile64{});
 }
 
 }  // extern "C"

@@ -205,41 +205,187 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a) {
 }
 
 // Four consecutive values of row `row` of the result, in the caller's
-// orientation: stored, or applied to the parameter.
+// orientation: stored with encoding E, or (MUON) applied to the parameter.
+template <int E, bool MUON>
 __device__ __forceinline__ void finish(const NsArgs& a, const MatrixTable& t, int matrix, int row, int col,
-                                       const float (&y)[4]) {
+                                       const f32x4& y) {
   if (row >= a.rows || col >= a.cols) return;
   const int live = a.cols - col < 4 ? a.cols - col : 4;
   const int64_t i = static_cast<int64_t>(row) * a.cols + col;
   void* out = reinterpret_cast<void*>(t.p[matrix]);
-  auto at = [&](auto encoding) {
-    constexpr int E = decltype(encoding)::value;
-    if (live == 4) {
-      uint32_t w[group_words(E)];
-      float r[4];
-      if (a.muon) {
-        load_group<E>(out, i, w);
-        decode_group<E>(w, r);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = a.muon ? fmaf(y[j], a.neg_lr, r[j] * a.decay) : y[j];
-      encode_group<E>(r, 0u, w);
-      store_group<E>(out, i, w);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j < live) {
-          const float r = a.muon ? fmaf(y[j], a.neg_lr, decode<E>(load1<E>(out, i + j)) * a.decay) : y[j];
-          store1<E>(out, i + j, encode<E>(r, 0u));
-        }
+  if (live == 4) {
+    uint32_t w[group_words(E)];
+    float r[4];
+    if constexpr (MUON) {
+      load_group<E>(out, i, w);
+      decode_group<E>(w, r);
     }
-  };
-  if (a.out_dtype == SR_F32) at(std::integral_constant<int, ENC_F32>{});
-  else if (a.out_dtype == SR_BF16) at(std::integral_constant<int, ENC_BF16_RN>{});
-  else at(std::integral_constant<int, ENC_F16_RN>{});
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = MUON ? fmaf(y[j], a.neg_lr, r[j] * a.decay) : y[j];
+    encode_group<E>(r, 0u, w);
+    store_group<E>(out, i, w);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < live) {
+        const float r = MUON ? fmaf(y[j], a.neg_lr, decode<E>(load1<E>(out, i + j)) * a.decay) : y[j];
+        store1<E>(out, i + j, encode<E>(r, 0u));
+      }
+  }
 }
 
 enum NsOp { kNsGram, kNsPolynomial, kNsStep, kNsLast };
+
+// A workgroup's tile and operands.
+struct NsTile {
+  Operand a, b;
+  int matrix, row0, col0, stages;
+  bool mirrored;  // a tile below the diagonal, to be stored twice
+};
+
+template <int OP, class S>
+__device__ __forceinline__ NsTile ns_tile(const NsArgs& a, uint32_t tiles_m, uint32_t tiles_n, uint32_t tiles,
+                                          uint32_t matrices) {
+  constexpr bool kSymmetric = OP == kNsGram || OP == kNsPolynomial;
+  NsTile r;
+  const uint32_t id = xcd_run(blockIdx.x, tiles * matrices);
+  r.matrix = id / tiles;
+  uint32_t tile_m, tile_n;
+  if constexpr (kSymmetric) {
+    triangle_tile(id % tiles, S::BM / S::BN, tile_m, tile_n);
+  } else {
+    band_tile(id % tiles, tiles_m, tiles_n, tile_m, tile_n);
+  }
+  r.row0 = tile_m * S::BM;
+  r.col0 = tile_n * S::BN;
+  r.mirrored = tile_n * S::BN < tile_m * S::BM;  // left of the diagonal blocks, which are computed whole
+  const int64_t base = static_cast<int64_t>(r.matrix) * a.m * a.n, square = static_cast<int64_t>(r.matrix) * a.m * a.m;
+  if constexpr (OP == kNsGram) {
+    r.a = r.b = {reinterpret_cast<const char*>(a.h + base), 2 * static_cast<int64_t>(a.n), a.m};
+    r.stages = a.n / (kStageBytes / 2);
+  } else {
+    r.a = {reinterpret_cast<const char*>((OP == kNsPolynomial ? a.g : a.p) + square), 2 * static_cast<int64_t>(a.m), a.m};
+    r.b = r.a;
+    if constexpr (!kSymmetric) r.b = {reinterpret_cast<const char*>(a.ht + base), 2 * static_cast<int64_t>(a.m), a.n};
+    r.stages = a.m / (kStageBytes / 2);
+  }
+  return r;
+}
+
+// Stores a workgroup's sums through its LDS, which every wave is done with.
+//   kNsGram, kNsPolynomial  the FP16 matrix, and its transpose where `mirrored`
+//   kNsStep                 X, H and H^T
+//   kNsLast                 the results (E, MUON), transposed where TURNED
+template <int OP, bool TURNED, int E, bool MUON, int LDS, class S, class Acc>
+__device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, const NsTile& tile, char* lds, int wave,
+                                         int lane, const Acc& acc) {
+  constexpr bool kSymmetric = OP == kNsGram || OP == kNsPolynomial;
+  using Chunk = ResultChunk<S::kRowsN>;
+  using T = std::conditional_t<OP == kNsLast, float, _Float16>;
+  using T4 = std::conditional_t<OP == kNsLast, f32x4, f16x4>;
+  constexpr bool kTurns = OP != kNsLast || TURNED;
+  constexpr int kWaveBytes = Chunk::kBytes + (kTurns ? Chunk::template turned_bytes<T>() : 0);
+  static_assert(S::kWaves * kWaveBytes <= LDS, "a chunk and its transpose per wave");
+  const int width = kSymmetric ? a.m : a.n;
+  const int64_t base = static_cast<int64_t>(tile.matrix) * a.m * a.n, square = static_cast<int64_t>(tile.matrix) * a.m * a.m;
+  const int wave_row = tile.row0 + wave / S::WN * S::kRowsM, wave_col = tile.col0 + wave % S::WN * S::kRowsN;
+  float* chunk = reinterpret_cast<float*>(lds + wave * kWaveBytes);
+  T* turned = reinterpret_cast<T*>(lds + wave * kWaveBytes + Chunk::kBytes);
+  _Float16* out = (OP == kNsGram ? a.g : a.p) + square;  // kSymmetric
+
+  auto use = [&](int first, const float* from) {
+    // The workspace's sizes are multiples of 64, so a chunk of 32 x 32 or 32 x 64 is inside or outside as a whole.
+    const int row0 = wave_row + first;
+    if (row0 >= a.m || wave_col >= width) return;
+    const int col = wave_col + Chunk::block_col(lane);
+#pragma unroll
+    for (int i = 0; i < Chunk::kBlocks; ++i) {
+      const int r0 = Chunk::block_row(i, lane);
+      T4 block[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = row0 + r0 + k;
+        const f32x4 v = Chunk::get(from, r0 + k, Chunk::block_col(lane));
+        if constexpr (OP == kNsGram) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) block[k][j] = static_cast<_Float16>(v[j] * kNsInverse);
+          *reinterpret_cast<f16x4*>(out + static_cast<int64_t>(row) * a.m + col) = block[k];
+        } else if constexpr (OP == kNsPolynomial) {
+          const f16x4 g = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float p = fmaf(a.c * kNsInverse, v[j], a.b * static_cast<float>(g[j]));
+            block[k][j] = static_cast<_Float16>(row == col + j ? p + kNsShift * kNsScale : p);
+          }
+          *reinterpret_cast<f16x4*>(out + static_cast<int64_t>(row) * a.m + col) = block[k];
+        } else {
+          const int64_t at = base + static_cast<int64_t>(row) * a.n + col;
+          const f32x4 x = *reinterpret_cast<const f32x4*>(a.x + at);
+          f32x4 y;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float h = static_cast<float>(static_cast<_Float16>(x[j] * kNsScale)) * kNsInverse;
+            y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x[j]));
+          }
+          if constexpr (OP == kNsStep) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) block[k][j] = static_cast<_Float16>(y[j] * kNsScale);
+            *reinterpret_cast<f32x4*>(a.x + at) = y;
+            *reinterpret_cast<f16x4*>(a.h + at) = block[k];
+          } else {
+            block[k] = y;
+            if constexpr (!TURNED) finish<E, MUON>(a, t, tile.matrix, row, col, y);
+          }
+        }
+      }
+      if constexpr (kTurns) {
+        if (!kSymmetric || tile.mirrored) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            Chunk::template put_turned<T, T4>(turned, Chunk::block_col(lane) + j, r0,
+                                              T4{block[0][j], block[1][j], block[2][j], block[3][j]});
+        }
+      }
+    }
+    if constexpr (kTurns) {
+      if (!kSymmetric || tile.mirrored)
+        Chunk::template store_turned<T, T4>(turned, lane, [&](int c, int r, const T4& v) {
+          if constexpr (OP == kNsLast) {
+            finish<E, MUON>(a, t, tile.matrix, wave_col + c, row0 + r, v);
+          } else {
+            _Float16* to = kSymmetric ? out : a.ht_next + base;
+            *reinterpret_cast<f16x4*>(to + static_cast<int64_t>(wave_col + c) * a.m + row0 + r) = v;
+          }
+        });
+    }
+  };
+  for_each_chunk<S>(chunk, lane, acc, use);
+}
+
+// Bytes of LDS of a kernel that has `stages` bytes of stages.
+template <int OP, bool TURNED, class S>
+constexpr int ns_lds(int stages) {
+  const int turned = OP == kNsLast ? (TURNED ? ResultChunk<S::kRowsN>::template turned_bytes<float>() : 0)
+                                   : ResultChunk<S::kRowsN>::template turned_bytes<_Float16>();
+  const int chunks = S::kWaves * (ResultChunk<S::kRowsN>::kBytes + turned);
+  return stages > chunks ? stages : chunks;
+}
+
+// Calls store(E, MUON) with the last step's encoding and kind; other steps have neither.
+template <int OP, class F>
+__device__ __forceinline__ void with_result(const NsArgs& a, F&& store) {
+  using std::integral_constant;
+  if constexpr (OP != kNsLast) {
+    store(integral_constant<int, ENC_F32>{}, std::false_type{});
+  } else if (a.muon) {
+    if (a.out_dtype == SR_F32) store(integral_constant<int, ENC_F32>{}, std::true_type{});
+    else store(integral_constant<int, ENC_BF16_RN>{}, std::true_type{});
+  } else {
+    if (a.out_dtype == SR_F32) store(integral_constant<int, ENC_F32>{}, std::false_type{});
+    else if (a.out_dtype == SR_BF16) store(integral_constant<int, ENC_BF16_RN>{}, std::false_type{});
+    else store(integral_constant<int, ENC_F16_RN>{}, std::false_type{});
+  }
+}
 
 // One launch of products: S-shaped tiles of every matrix.
 //   kNsGram        G = H H^T, the lower triangle's tiles
@@ -250,34 +396,14 @@ enum NsOp { kNsGram, kNsPolynomial, kNsStep, kNsLast };
 template <int OP, class S, bool TURNED>
 __global__ __launch_bounds__(S::kThreads, 2) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
                                                                     uint32_t tiles, uint32_t matrices, MatrixTable t) {
-  constexpr bool kSymmetric = OP == kNsGram || OP == kNsPolynomial;
-  __shared__ __align__(1024) char lds[2 * S::kStage];
+  constexpr int kLds = ns_lds<OP, TURNED, S>(2 * S::kStage);
+  __shared__ __align__(1024) char lds[kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t id = xcd_run(blockIdx.x, tiles * matrices);
-  const int matrix = id / tiles;
-  uint32_t tile_m, tile_n;
-  if constexpr (kSymmetric) {
-    triangle_tile(id % tiles, tile_m, tile_n);
-  } else {
-    band_tile(id % tiles, tiles_m, tiles_n, tile_m, tile_n);
-  }
-  const int row0 = tile_m * S::BM, col0 = tile_n * S::BN;
+  const NsTile tile = ns_tile<OP, S>(a, tiles_m, tiles_n, tiles, matrices);
   const int wave_m = wave / S::WN * S::kRowsM, wave_n = wave % S::WN * S::kRowsN;
-  const int64_t base = static_cast<int64_t>(matrix) * a.m * a.n, square = static_cast<int64_t>(matrix) * a.m * a.m;
-
-  Operand oa, ob;
-  int stages;
-  if constexpr (OP == kNsGram) {
-    oa = ob = {reinterpret_cast<const char*>(a.h + base), 2 * static_cast<int64_t>(a.n), a.m};
-    stages = a.n / (kStageBytes / 2);
-  } else {
-    oa = {reinterpret_cast<const char*>((OP == kNsPolynomial ? a.g : a.p) + square), 2 * static_cast<int64_t>(a.m), a.m};
-    ob = oa;
-    if constexpr (!kSymmetric) ob = {reinterpret_cast<const char*>(a.ht + base), 2 * static_cast<int64_t>(a.m), a.n};
-    stages = a.m / (kStageBytes / 2);
-  }
+  const int stages = tile.stages;
   Stager<S> stager;
-  stager.init(oa, ob, row0, col0, wave, lane);
+  stager.init(tile.a, tile.b, tile.row0, tile.col0, wave, lane);
 
   f32x4 acc[S::MI][S::NI] = {};
   const uint32_t fragment = fragment_offset(lane);
@@ -285,8 +411,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void ns_product_kernel(NsArgs a, ui
   for (int kt = 0; kt < stages; ++kt) {
     // Stage kt has landed for every wave, and every wave is done with the other buffer.
     stage_barrier();
-    if (kt + 1 < stages)
-      stager.load_async(lds + (~kt & 1) * S::kStage, static_cast<int64_t>(kt + 1) * kStageBytes, wave);
+    if (kt + 1 < stages) stager.load_async(lds + (~kt & 1) * S::kStage, (kt + 1) * kStageBytes, wave);
     const char* stage = lds + (kt & 1) * S::kStage;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
@@ -301,76 +426,31 @@ __global__ __launch_bounds__(S::kThreads, 2) void ns_product_kernel(NsArgs a, ui
         const f16x8 fa = __builtin_bit_cast(f16x8, read_chunk(sa + mi * 16 * kStageBytes));
 #pragma unroll
         for (int ni = 0; ni < S::NI; ++ni)
-          acc[mi][ni] = TURNED ? __builtin_amdgcn_mfma_f32_16x16x32_f16(fa, fb[ni], acc[mi][ni], 0, 0, 0)
-                               : __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[ni], fa, acc[mi][ni], 0, 0, 0);
+          acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[ni], fa, acc[mi][ni], 0, 0, 0);
       }
     }
   }
+  stage_barrier();
+  with_result<OP>(a, [&](auto encoding, auto muon) {
+    ns_store<OP, TURNED, decltype(encoding)::value, decltype(muon)::value, kLds, S>(a, t, tile, lds, wave, lane, acc);
+  });
+}
 
-#pragma unroll
-  for (int mi = 0; mi < S::MI; ++mi) {
-#pragma unroll
-    for (int ni = 0; ni < S::NI; ++ni) {
-      const f32x4 v = acc[mi][ni];
-      if constexpr (TURNED) {
-        // Row `row` .. + 3 of the workspace's orientation, column `col`.
-        const int row = row0 + wave_m + mi * 16 + 4 * (lane >> 4), col = col0 + wave_n + ni * 16 + (lane & 15);
-        if (row >= a.m || col >= a.n) continue;
-        float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = a.x[base + static_cast<int64_t>(row + j) * a.n + col];
-          const float h = static_cast<float>(static_cast<_Float16>(x * kNsScale)) * kNsInverse;
-          y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x));
-        }
-        finish(a, t, matrix, col, row, y);
-      } else {
-        const int row = row0 + wave_m + mi * 16 + (lane & 15), col = col0 + wave_n + ni * 16 + 4 * (lane >> 4);
-        if (row >= a.m || col >= (kSymmetric ? a.m : a.n)) continue;
-        if constexpr (kSymmetric) {
-          f16x4 w;
-          if constexpr (OP == kNsGram) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = static_cast<_Float16>(v[j] * kNsInverse);
-          } else {
-            const f16x4 g = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float p = fmaf(a.c * kNsInverse, v[j], a.b * static_cast<float>(g[j]));
-              w[j] = static_cast<_Float16>(row == col + j ? p + kNsShift * kNsScale : p);
-            }
-          }
-          _Float16* out = (OP == kNsGram ? a.g : a.p) + square;
-          *reinterpret_cast<f16x4*>(out + static_cast<int64_t>(row) * a.m + col) = w;
-          if (tile_m != tile_n) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) out[static_cast<int64_t>(col + j) * a.m + row] = w[j];
-          }
-        } else {
-          const int64_t i = base + static_cast<int64_t>(row) * a.n + col;
-          const f32x4 x = *reinterpret_cast<const f32x4*>(a.x + i);
-          float y[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float h = static_cast<float>(static_cast<_Float16>(x[j] * kNsScale)) * kNsInverse;
-            y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x[j]));
-          }
-          if constexpr (OP == kNsStep) {
-            f16x4 w;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              w[j] = static_cast<_Float16>(y[j] * kNsScale);
-              a.ht_next[base + static_cast<int64_t>(col + j) * a.m + row] = w[j];
-            }
-            *reinterpret_cast<f32x4*>(a.x + i) = f32x4{y[0], y[1], y[2], y[3]};
-            *reinterpret_cast<f16x4*>(a.h + i) = w;
-          } else {
-            finish(a, t, matrix, row, col, y);
-          }
-        }
-      }
-    }
-  }
+// The same launches on wide tiles.
+template <int OP, bool TURNED>
+__global__ __launch_bounds__(TileWide::kThreads, 2) void ns_wide_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
+                                                                        uint32_t tiles, uint32_t matrices, MatrixTable t) {
+  constexpr int kLds = ns_lds<OP, TURNED, TileWide>(2 * TileWide::kStage);
+  __shared__ __align__(1024) char lds[kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const NsTile tile = ns_tile<OP, TileWide>(a, tiles_m, tiles_n, tiles, matrices);
+  Stager<TileWide> stager;
+  stager.init(tile.a, tile.b, tile.row0, tile.col0, wave, lane);
+  f32x16 acc[WideTile::MI][WideTile::NI] = {};
+  WideTile::run(lds, stager, tile.stages, wave, lane, acc);
+  with_result<OP>(a, [&](auto encoding, auto muon) {
+    ns_store<OP, TURNED, decltype(encoding)::value, decltype(muon)::value, kLds, TileWide>(a, t, tile, lds, wave, lane, acc);
+  });
 }
 
 }  // namespace sr

@@ -59,22 +59,44 @@ template <int OP, class S, bool TURNED = false>
 int product(const NsArgs& a, int matrices, const sr::MatrixTable& t, hipStream_t s) {
   constexpr bool kSymmetric = OP == sr::kNsGram || OP == sr::kNsPolynomial;
   const uint32_t tm = (a.m + S::BM - 1) / S::BM, tn = ((kSymmetric ? a.m : a.n) + S::BN - 1) / S::BN;
-  const uint32_t tiles = kSymmetric ? tm * (tm + 1) / 2 : tm * tn;
-  if (static_cast<uint64_t>(tiles) * matrices > 0x7FFFFFu) return fail(SR_ERR_ARGUMENT, "%u tiles exceed a launch", tiles);
-  sr::ns_product_kernel<OP, S, TURNED><<<tiles * matrices, S::kThreads, 0, s>>>(a, tm, tn, tiles, matrices, t);
-  return launched("ns_product_kernel launch");
+  const uint32_t tiles = kSymmetric ? S::BM / S::BN * (tm * (tm + 1) / 2) : tm * tn;
+  if (static_cast<uint64_t>(tiles) * matrices > 0x3FFFFFu) return fail(SR_ERR_ARGUMENT, "%u tiles exceed a launch", tiles);
+  if constexpr (std::is_same_v<S, sr::TileWide>) {
+    sr::ns_wide_kernel<OP, TURNED><<<tiles * matrices, S::kThreads, 0, s>>>(a, tm, tn, tiles, matrices, t);
+  } else {
+    sr::ns_product_kernel<OP, S, TURNED><<<tiles * matrices, S::kThreads, 0, s>>>(a, tm, tn, tiles, matrices, t);
+  }
+  return launched("Newton-Schulz product launch");
 }
 
-// The larger tile where it still gives most of the chip's 256 CUs work.
+// Tiles of a launch of S.
+template <int OP, class S>
+int64_t tile_count(const NsArgs& a, int matrices) {
+  const int64_t tm = (a.m + S::BM - 1) / S::BM, tn = (a.n + S::BN - 1) / S::BN;
+  return (OP == sr::kNsGram || OP == sr::kNsPolynomial ? S::BM / S::BN * (tm * (tm + 1) / 2) : tm * tn) * matrices;
+}
+
+// The largest tile that still gives the chip's 256 CUs work.  The symmetric
+// launches stop at 128 x 128: their triangles have few large tiles (8
+// matrices of 2048 x 2048: G 122 us on 256 x 256 tiles and 102 on 128 x 128,
+// the step 200 and 244).
 template <int OP>
 int product_by_size(const NsArgs& a, int matrices, const sr::MatrixTable& t, hipStream_t s) {
   constexpr bool kSymmetric = OP == sr::kNsGram || OP == sr::kNsPolynomial;
-  const int64_t tm = (a.m + 127) / 128, tn = (a.n + 127) / 128;
-  const bool big = (kSymmetric ? tm * (tm + 1) / 2 : tm * tn) * matrices >= 256;
+  const int tile = !kSymmetric && tile_count<OP, sr::TileWide>(a, matrices) >= 256 ? 256
+                   : tile_count<OP, sr::Tile128>(a, matrices) >= 256              ? 128
+                                                                                   : 64;
   if constexpr (OP == sr::kNsLast) {
-    if (a.tall) return big ? product<OP, sr::Tile128, true>(a, matrices, t, s) : product<OP, sr::Tile64, true>(a, matrices, t, s);
+    if (a.tall)
+      return tile == 256 ? product<OP, sr::TileWide, true>(a, matrices, t, s)
+             : tile == 128 ? product<OP, sr::Tile128, true>(a, matrices, t, s)
+                           : product<OP, sr::Tile64, true>(a, matrices, t, s);
   }
-  return big ? product<OP, sr::Tile128>(a, matrices, t, s) : product<OP, sr::Tile64>(a, matrices, t, s);
+  if constexpr (!kSymmetric) {
+    if (tile == 256) return product<OP, sr::TileWide>(a, matrices, t, s);
+  }
+  return tile == 128 ? product<OP, sr::Tile128>(a, matrices, t, s)
+                     : product<OP, sr::Tile64>(a, matrices, t, s);
 }
 
 // The whole update of up to SR_MATRIX_BATCH matrices.  `ue` is the momentum's

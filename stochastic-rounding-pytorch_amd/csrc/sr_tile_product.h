@@ -27,6 +27,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
+#include <utility>
 
 namespace sr {
 
@@ -87,13 +89,16 @@ __device__ __forceinline__ void band_tile(uint32_t id, uint32_t tm, uint32_t tn,
   col = within / height;
 }
 
-// The lower triangle's tile of index id: row >= col, counted row by row.
-__device__ __forceinline__ void triangle_tile(uint32_t id, uint32_t& row, uint32_t& col) {
-  uint32_t r = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(id) + 1.0f) - 1.0f) * 0.5f);
-  while (r * (r + 1) / 2 > id) --r;
-  while ((r + 1) * (r + 2) / 2 <= id) ++r;
+// The lower triangle's tile of index id, counted row by row, of tiles that are
+// `wide` (1 or 2) times as high as wide: row r has wide * (r + 1) tiles, up to
+// those on its diagonal block.
+__device__ __forceinline__ void triangle_tile(uint32_t id, uint32_t wide, uint32_t& row, uint32_t& col) {
+  const uint32_t half = id / wide;
+  uint32_t r = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(half) + 1.0f) - 1.0f) * 0.5f);
+  while (r * (r + 1) / 2 > half) --r;
+  while ((r + 1) * (r + 2) / 2 <= half) ++r;
   row = r;
-  col = id - r * (r + 1) / 2;
+  col = id - wide * (r * (r + 1) / 2);
 }
 
 // The 16 bytes at `at` of a row that ends at `end`; zeros from there on.
@@ -110,45 +115,57 @@ __device__ __forceinline__ i32x4 load_chunk(const char* row, int64_t at, int64_t
   return i32x4{(int)words[0], (int)words[1], (int)words[2], (int)words[3]};
 }
 
+// A buffer over all that follows `base`: its loads take a 32-bit offset per
+// lane and a uniform one, and need no address arithmetic.  (The host's pass
+// over the kernels knows neither the type nor the builtins.)
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer_of(const char* base) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, -1, 0x00020000);
+}
+// 16 bytes of every lane to consecutive places of LDS from `to` on, which is uniform.
+__device__ __forceinline__ void chunks_to_lds(Buffer from, char* to, uint32_t offset, uint32_t uniform) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void*)to, 16, offset, uniform, 0, 0);
+}
+#else
+typedef const char* Buffer;
+__device__ inline Buffer buffer_of(const char* base) { return base; }
+__device__ inline void chunks_to_lds(Buffer, char*, uint32_t, uint32_t) {}
+#endif
+
 // Stages of both operands' rows for one workgroup.
 template <class S>
 struct Stager {
+  static constexpr int kLoadsA = S::BM / 8 / S::kWaves;  // the others are B's
+  static_assert(S::BM / 8 % S::kWaves == 0, "a load's rows are of one operand");
   const char* a;  // this workgroup's first row of either operand
   const char* b;
-  int64_t lda, ldb;
-  int rows_a, rows_b;  // valid rows from there (at least 1)
+  Buffer buffer_a, buffer_b;
   uint32_t offset[S::kLoads];  // this lane's chunk in each of its loads, from a or b
 
   // `wave` is uniform.  Rows past the operand's end repeat its last row: the
   // results they give are not stored.
   __device__ void init(const Operand& opa, const Operand& opb, int row_a, int row_b, int wave, int lane) {
-    lda = opa.ld;
-    ldb = opb.ld;
-    a = opa.base + row_a * lda;
-    b = opb.base + row_b * ldb;
-    rows_a = opa.rows - row_a;
-    rows_b = opb.rows - row_b;
+    a = opa.base + row_a * opa.ld;
+    b = opb.base + row_b * opb.ld;
+    buffer_a = buffer_of(a);
+    buffer_b = buffer_of(b);
     const uint32_t chunk = static_cast<uint32_t>((lane & 7) ^ (lane >> 3)) * kChunk;
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const int r = (i * S::kWaves + wave) * 8 + (lane >> 3);
-      const bool of_a = r < S::BM;
-      const int valid = of_a ? rows_a : rows_b, at = of_a ? r : r - S::BM;
-      offset[i] = static_cast<uint32_t>(at < valid ? at : valid - 1) * static_cast<uint32_t>(of_a ? lda : ldb) + chunk;
+      const bool of_a = i < kLoadsA;
+      const int at = ((of_a ? i : i - kLoadsA) * S::kWaves + wave) * 8 + (lane >> 3);
+      const int valid = of_a ? opa.rows - row_a : opb.rows - row_b;
+      offset[i] = static_cast<uint32_t>(at < valid ? at : valid - 1) * static_cast<uint32_t>(of_a ? opa.ld : opb.ld) + chunk;
     }
   }
 
   // Asynchronous loads of the stage whose bytes start at k, straight into LDS.
   // Every row has 128 bytes from k, 16-byte aligned.
-  __device__ void load_async(char* stage, int64_t k, int wave) const {
+  __device__ void load_async(char* stage, uint32_t k, int wave) const {
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      const int r0 = (i * S::kWaves + wave) * 8;  // uniform; a load's rows are of one operand
-      const char* base = (r0 < S::BM ? a : b) + k;
-      __builtin_amdgcn_global_load_lds(
-          (const __attribute__((address_space(1))) void*)(base + offset[i]),
-          (__attribute__((address_space(3))) void*)(stage + r0 * kStageBytes), kChunk, 0, 0);
-    }
+    for (int i = 0; i < S::kLoads; ++i)
+      chunks_to_lds(i < kLoadsA ? buffer_a : buffer_b, stage + (i * S::kWaves + wave) * 8 * kStageBytes, offset[i], k);
   }
 
   // The same stage through registers, for rows of any alignment and for a
@@ -157,9 +174,18 @@ struct Stager {
     const int64_t chunk = ((lane & 7) ^ (lane >> 3)) * kChunk;
 #pragma unroll
     for (int i = 0; i < S::kLoads; ++i) {
-      const char* row = ((i * S::kWaves + wave) * 8 < S::BM ? a : b) + (offset[i] - chunk);
+      const char* row = (i < kLoadsA ? a : b) + (offset[i] - chunk);
       regs[i] = load_chunk(row, k + chunk, end);
     }
+  }
+
+  // The two together, chunk by chunk.
+  __device__ void load_through(char* stage, int64_t k, int64_t end, int wave, int lane) const {
+    const int64_t chunk = ((lane & 7) ^ (lane >> 3)) * kChunk;
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i)
+      *reinterpret_cast<i32x4*>(stage + (i * S::kWaves + wave) * 8 * kStageBytes + lane * kChunk) =
+          load_chunk((i < kLoadsA ? a : b) + (offset[i] - chunk), k + chunk, end);
   }
 
   __device__ static void store(char* stage, const i32x4 (&regs)[S::kLoads], int wave, int lane) {
@@ -176,5 +202,182 @@ __device__ __forceinline__ uint32_t fragment_offset(int lane) {
 }
 
 __device__ __forceinline__ i32x4 read_chunk(const char* p) { return *reinterpret_cast<const i32x4*>(p); }
+
+// ---------------------------------------------------------------------------
+// FP16 products on 256 x 256 tiles by eight waves, for launches that fill the
+// chip with them: what a CU reads per product is half of a 128 x 128 tile's.
+//
+// A wave computes 128 x 64 results as 4 x 2 tiles of 32 x 32.  Each stage is
+// two halves of 64 bytes per row.  A half's fragments are read while the
+// products of the half before run.  The one barrier per stage stands between
+// the halves: by then every wave holds the second half in registers, so the
+// buffer is free for the loads of two stages later, and the next stage has had
+// a whole stage's time to arrive.
+// ---------------------------------------------------------------------------
+using TileWide = TileShape<256, 256, 2, 4>;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct WideTile {
+  static constexpr int MI = TileWide::kRowsM / 32, NI = TileWide::kRowsN / 32;
+
+  // One wave's fragments of a half stage: two chunks of its row of each 32-row tile.
+  struct Fragments {
+    f16x8 a[MI][2], b[NI][2];
+    // `a_at`, `b_at`: this lane's first chunk among the stage's bytes, for half 0.
+    __device__ __forceinline__ void read(const char* stage, uint32_t a_at, uint32_t b_at, int half) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          b[i][j] = __builtin_bit_cast(f16x8, read_chunk(stage + (b_at ^ (64 * half + 32 * j)) + i * 32 * kStageBytes));
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+          a[i][j] = __builtin_bit_cast(f16x8, read_chunk(stage + (a_at ^ (64 * half + 32 * j)) + i * 32 * kStageBytes));
+    }
+    __device__ __forceinline__ void multiply(f32x16 (&acc)[MI][NI]) const {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+          for (int ni = 0; ni < NI; ++ni)
+            acc[mi][ni] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[ni][j], a[mi][j], acc[mi][ni], 0, 0, 0);
+    }
+  };
+
+  // Asks the scheduler to issue a half's LDS reads between the first three
+  // quarters of the products that run meanwhile: left alone it gathers them at
+  // the end, to reuse registers, and then waits for them.
+  template <int I = 0>
+  static __device__ __forceinline__ void interleave() {
+    constexpr int kProducts = 2 * MI * NI, kReads = 2 * (MI + NI), kSlots = 3 * kProducts / 4;
+    if constexpr (I == kProducts) {
+      __builtin_amdgcn_sched_barrier(0);
+    } else {
+      constexpr int kNow = I < kSlots ? (I + 1) * kReads / kSlots - I * kReads / kSlots : 0;
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // one matrix instruction
+      if constexpr (kNow > 0) __builtin_amdgcn_sched_group_barrier(0x100, kNow, 0);
+      interleave<I + 1>();
+    }
+  }
+
+  // acc += the products of `stages` whole stages (at least 1).  On return every wave is done with the LDS.
+  static __device__ __forceinline__ void run(char* lds, const Stager<TileWide>& stager, int stages, int wave, int lane,
+                                             f32x16 (&acc)[MI][NI]) {
+    const uint32_t at = (lane & 31) * kStageBytes + (((lane >> 5) ^ (lane & 7)) * kChunk);
+    const uint32_t at_a = wave / TileWide::WN * TileWide::kRowsM * kStageBytes + at;
+    const uint32_t at_b = (TileWide::BM + wave % TileWide::WN * TileWide::kRowsN) * kStageBytes + at;
+    auto load = [&](int kt) { stager.load_async(lds + (kt & 1) * TileWide::kStage, kt * kStageBytes, wave); };
+    Fragments first, second;
+    load(0);
+    stage_barrier();
+    if (stages > 1) load(1);
+    first.read(lds, at_a, at_b, 0);
+    auto step = [&](int kt, auto more) {
+      second.read(lds + (kt & 1) * TileWide::kStage, at_a, at_b, 1);
+      first.multiply(acc);
+      interleave();
+      stage_barrier();
+      if constexpr (decltype(more)::value) load(kt + 2);
+      // Past the last stage this reads what the buffer held two stages ago; nothing uses it.
+      first.read(lds + (~kt & 1) * TileWide::kStage, at_a, at_b, 0);
+      second.multiply(acc);
+      interleave();
+    };
+    int kt = 0;
+    for (; kt + 2 < stages; ++kt) step(kt, std::true_type{});
+    for (; kt < stages; ++kt) step(kt, std::false_type{});
+    stage_barrier();
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Results on their way out.
+//
+// A matrix instruction leaves a lane four neighbours of one row, and the
+// lanes beside it other rows: stored from there, every access would scatter
+// over 16 or 32 rows, 8 to 32 bytes each.  So a wave passes 32 rows by CN
+// columns at a time through LDS of its own and takes them up as blocks of
+// 4 x 4, CN / 4 lanes to a row: a row's lanes then cover whole cache lines, and a
+// block turns in registers where the transpose is stored as well.  The rows
+// are padded so that neither side's accesses meet in the same banks.  Only
+// one wave uses a chunk, so it needs no barrier.
+// ---------------------------------------------------------------------------
+template <int CN>
+struct ResultChunk {
+  static constexpr int kRows = 32, kStride = CN + 4, kTurnedStride = kRows + 4;
+  static constexpr int kLanes = CN / 4, kBlocks = kRows * CN / 16 / 64;  // lanes of a row; blocks of a lane
+  static constexpr int kBytes = kRows * kStride * 4;
+  static constexpr int kTurnedLanes = kRows / 4;  // lanes of a turned row
+  template <class T>
+  static constexpr int turned_bytes() { return CN * kTurnedStride * static_cast<int>(sizeof(T)); }
+
+  // Block `i` of this lane: rows block_row(i) .. + 3, columns block_col() .. + 3.
+  static __device__ __forceinline__ int block_row(int i, int lane) { return 4 * (i * (64 / kLanes) + lane / kLanes); }
+  static __device__ __forceinline__ int block_col(int lane) { return 4 * (lane % kLanes); }
+
+  static __device__ __forceinline__ void put(float* chunk, int row, int col, const f32x4& v) {
+    *reinterpret_cast<f32x4*>(chunk + row * kStride + col) = v;
+  }
+  static __device__ __forceinline__ f32x4 get(const float* chunk, int row, int col) {
+    return *reinterpret_cast<const f32x4*>(chunk + row * kStride + col);
+  }
+
+  // The transpose: columns become rows of 32 values of T.
+  template <class T, class T4>
+  static __device__ __forceinline__ void put_turned(T* turned, int col, int row, const T4& v) {
+    *reinterpret_cast<T4*>(turned + col * kTurnedStride + row) = v;
+  }
+  // Calls store(column, row, four values from that row on) for all of it.
+  template <class T, class T4, class F>
+  static __device__ __forceinline__ void store_turned(const T* turned, int lane, F&& store) {
+#pragma unroll
+    for (int i = 0; i < CN * kTurnedLanes / 64; ++i) {
+      const int col = i * (64 / kTurnedLanes) + lane / kTurnedLanes, row = 4 * (lane % kTurnedLanes);
+      store(col, row, *reinterpret_cast<const T4*>(turned + col * kTurnedStride + row));
+    }
+  }
+};
+
+// The 32-row chunks of a wave of S's results: for each, fills it from the
+// accumulators and calls use(first row, chunk) with the rows counted from the
+// wave's first.  16 x 16 tiles acc[MI][NI] of f32x4, or 32 x 32 ones of f32x16.
+// (Folds, not loops: accumulators live in registers only where every index is
+// known, and the unroller gives up on bodies this long.)
+template <class S, class F, int... C>
+__device__ __forceinline__ void chunks_of(float* chunk, int lane, const f32x4 (&acc)[S::MI][S::NI], F&& use,
+                                          std::integer_sequence<int, C...>) {
+  using Chunk = ResultChunk<S::kRowsN>;
+  ([&] {
+#pragma unroll
+    for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+      for (int ni = 0; ni < S::NI; ++ni)
+        Chunk::put(chunk, mi * 16 + (lane & 15), ni * 16 + 4 * (lane >> 4), acc[2 * C + mi][ni]);
+    use(32 * C, chunk);
+  }(), ...);
+}
+
+template <class S, class F, int... C>
+__device__ __forceinline__ void chunks_of(float* chunk, int lane, const f32x16 (&acc)[WideTile::MI][WideTile::NI], F&& use,
+                                          std::integer_sequence<int, C...>) {
+  using Chunk = ResultChunk<S::kRowsN>;
+  ([&] {
+#pragma unroll
+    for (int ni = 0; ni < WideTile::NI; ++ni)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        Chunk::put(chunk, lane & 31, ni * 32 + 8 * q + 4 * (lane >> 5),
+                   f32x4{acc[C][ni][4 * q], acc[C][ni][4 * q + 1], acc[C][ni][4 * q + 2], acc[C][ni][4 * q + 3]});
+    use(32 * C, chunk);
+  }(), ...);
+}
+
+template <class S, class Acc, class F>
+__device__ __forceinline__ void for_each_chunk(float* chunk, int lane, const Acc& acc, F&& use) {
+  chunks_of<S>(chunk, lane, acc, use, std::make_integer_sequence<int, S::kRowsM / 32>{});
+}
 
 }  // namespace sr
