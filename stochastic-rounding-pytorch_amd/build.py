@@ -3,11 +3,12 @@
 Run ``python build.py`` from anywhere.  The AdamW instantiations are split
 into nine translation units (one per first-moment encoding) that compile in
 parallel; the shared library is linked in place next to the Python package,
-so it travels with the source tree.  Two CPython extensions over torch's
+so it travels with the source tree.  Three CPython extensions over torch's
 tensor type are built alongside it: the host-side group walk
-(csrc/group_walk.cpp -> sr_states/_group_walk<EXT_SUFFIX>) and the native
+(csrc/group_walk.cpp -> sr_states/_group_walk<EXT_SUFFIX>), the native
 entries of the launches (csrc/launch.cpp ->
-sr_states/_launch<EXT_SUFFIX>).
+sr_states/_launch<EXT_SUFFIX>) and those of the matrix operators
+(csrc/matrix.cpp -> sr_states/_matrix<EXT_SUFFIX>).
 """
 
 from __future__ import annotations
@@ -31,6 +32,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 CXX = os.environ.get("CXX", "g++")
 WALK_OUTPUT = ROOT / "sr_states" / f"_group_walk{sysconfig.get_config_var('EXT_SUFFIX')}"
 LAUNCH_OUTPUT = ROOT / "sr_states" / f"_launch{sysconfig.get_config_var('EXT_SUFFIX')}"
+MATRIX_OUTPUT = ROOT / "sr_states" / f"_matrix{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 # -ffp-contract=off: only the explicit fmaf() calls may fuse, matching the
 # eager CPU reference.  Division and sqrt stay IEEE correctly rounded.
@@ -115,6 +117,8 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
     commands.append(walk_command(walk_tmp))
     launch_tmp = LAUNCH_OUTPUT.with_name(LAUNCH_OUTPUT.name + ".tmp")
     commands.append(walk_command(launch_tmp, CSRC / "launch.cpp"))
+    matrix_tmp = MATRIX_OUTPUT.with_name(MATRIX_OUTPUT.name + ".tmp")
+    commands.append(walk_command(matrix_tmp, CSRC / "matrix.cpp"))
     workers = jobs or min(len(commands), max(1, min(16, os.cpu_count() or 1)))
     with ThreadPoolExecutor(workers) as pool:
         for cmd, _ in zip(commands, pool.map(_run, commands)):
@@ -127,6 +131,7 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
     os.replace(tmp, OUTPUT)
     os.replace(walk_tmp, WALK_OUTPUT)
     os.replace(launch_tmp, LAUNCH_OUTPUT)
+    os.replace(matrix_tmp, MATRIX_OUTPUT)
     return OUTPUT
 
 

@@ -311,6 +311,23 @@ def launcher():
     return _launcher
 
 
+_matrix = None
+
+
+def matrix():
+    """The native entries of the matrix operators (sr_states/_matrix), bound to this library."""
+    global _matrix
+    if _matrix is None:
+        from . import _matrix as module
+
+        lib = library()
+        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
+                      for name in ("sr_block_cast", "sr_block_matmul", "sr_block_matmul_workspace", "sr_orthogonalize",
+                                   "sr_orthogonalize_workspace")))
+        _matrix = module
+    return _matrix
+
+
 def low64(value: int) -> int:
     return int(value) & 0xFFFFFFFFFFFFFFFF
 

@@ -15,7 +15,6 @@ The reference package has no counterpart.
 
 from __future__ import annotations
 
-import math
 from typing import NamedTuple
 
 import torch
@@ -30,7 +29,6 @@ from ._optimizer import reject_dtensors
 BLOCK = _lib.BLOCK
 FP8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 _WIDE_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
-_SCALE_TYPES = {torch.float8_e8m0fnu: _lib.SCALE_E8M0, torch.float32: _lib.SCALE_F32}
 
 
 class BlockScaled(NamedTuple):
@@ -54,28 +52,22 @@ class BlockScaled(NamedTuple):
         return self.data.float() * scale.repeat_interleave(BLOCK, 1)[:, :k]
 
 
-def _blocks(n: int) -> int:
-    return -(-n // BLOCK)
+# Checked (dtype, block, axis, rounding) of block_cast, as the native entry takes them: built-in rules
+# can never be replaced, so what was checked once holds for the life of the process.
+_CASTS: dict = {}
 
 
-def _row_stride(x: torch.Tensor, what: str) -> int:
-    """The distance between rows of a 2-D tensor with consecutive columns."""
-    rows, cols = x.shape
-    stride = x.stride(0) if rows > 1 else max(cols, 1)
-    if (cols > 1 and x.stride(1) != 1) or stride < cols:
-        raise ValueError(f"{what} requires consecutive columns and rows that do not overlap")
-    return stride
-
-
-def _new_output(rows: int, k: int, dtype, square: bool, device):
-    """An empty BlockScaled; rows start on 16 bytes, which the product's asynchronous loads need."""
-    data = torch.empty_strided((rows, k), (-(-k // 16) * 16, 1), dtype=dtype, device=device)
-    scale = torch.empty((_blocks(rows) if square else rows, _blocks(k)), dtype=torch.float8_e8m0fnu, device=device)
-    return BlockScaled(data, scale)
-
-
-def _address(x: torch.Tensor) -> int:
-    return x.data_ptr()
+def _cast_plan(dtype, block, axis, rounding):
+    if dtype not in FP8_DTYPES:
+        raise ValueError(f"block casts give torch.float8_e4m3fn or torch.float8_e5m2, not {dtype}")
+    code, rule = native_codes(dtype, rounding)
+    block = tuple(block)
+    if block not in ((1, BLOCK), (BLOCK, BLOCK)):
+        raise ValueError(f"block must be (1, {BLOCK}) or ({BLOCK}, {BLOCK})")
+    axes = axis if isinstance(axis, tuple) else (axis,)
+    if axes not in ((1,), (0,), (1, 0), (0, 1)):
+        raise ValueError("axis must be 1, 0, (1, 0) or (0, 1)")
+    return code, rule, int(block[0] == BLOCK), "".join(str(int(a)) for a in axes)
 
 
 def block_cast(
@@ -105,78 +97,31 @@ def block_cast(
     contiguous only where its last size is one.  Nothing is recorded for
     autograd.
     """
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"expected a tensor, got {type(x).__name__}")
-    reject_dtensors(x)
-    if x.dtype not in _WIDE_DTYPES:
-        raise TypeError(f"expected FP32, BF16 or FP16 input, got {x.dtype}")
-    if dtype not in FP8_DTYPES:
-        raise ValueError(f"block casts give torch.float8_e4m3fn or torch.float8_e5m2, not {dtype}")
-    code, rule = native_codes(dtype, rounding)
-    block = tuple(block)
-    if block not in ((1, BLOCK), (BLOCK, BLOCK)):
-        raise ValueError(f"block must be (1, {BLOCK}) or ({BLOCK}, {BLOCK})")
-    axes = axis if isinstance(axis, tuple) else (axis,)
-    if axes not in ((1,), (0,), (1, 0), (0, 1)):
-        raise ValueError("axis must be 1, 0, (1, 0) or (0, 1)")
-    if x.dim() != 2:
-        raise ValueError(f"block_cast takes a matrix, not {x.dim()} dimensions")
-    device = x.device
-    if device.type != "cuda":
-        raise ValueError("block_cast requires a GPU tensor")
-    validate_device(device)
-    stride = _row_stride(x, "block_cast")
-    rows, cols = x.shape
-    square = block[0] == BLOCK
-    result = {}
-    out = {}
-    for a in axes:
-        q = _new_output(*((rows, cols) if a == 1 else (cols, rows)), dtype, square, device)
-        result[a] = q
-        out[a] = _lib.BlockOutput(_address(q.data), _address(q.scale), q.data.stride(0), max(q.scale.shape[1], 1))
-    if rows and cols:
-        with _lib.on_device(device):
-            _lib.call(
-                "sr_block_cast", _address(x), stride, rows, cols, _lib.DTYPE_CODES[x.dtype], code, rule, int(square),
-                _lib.low32(seed), _lib.low32(offset), out.get(1), out.get(0), _lib.stream_handle(device),
-            )
-    return result[axes[0]] if len(axes) == 1 else tuple(result[a] for a in axes)
+    try:
+        plan = _CASTS[dtype, block, axis, rounding]
+    except KeyError:
+        plan = _CASTS[dtype, block, axis, rounding] = _cast_plan(dtype, block, axis, rounding)
+    except TypeError:  # an unhashable argument
+        plan = _cast_plan(dtype, block, axis, rounding)
+    device = _device_of(x)
+    q = _lib.matrix().block_cast(x, *plan, seed & 0xFFFFFFFF, offset & 0xFFFFFFFF, _stream(device))
+    if not isinstance(q, tuple):
+        _lib.check("sr_block_cast", q)
+    return BlockScaled(q[0], q[1]) if len(q) == 2 else (BlockScaled(q[0], q[1]), BlockScaled(q[2], q[3]))
 
 
-def _operand(q: BlockScaled, name: str) -> _lib.BlockMatrix:
-    """The checked C record of one operand."""
-    data, scale = q
-    for t in (data, scale):
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{name} must be a BlockScaled pair of tensors")
-    reject_dtensors(data, scale)
-    if data.dtype not in FP8_DTYPES:
-        raise TypeError(f"{name}: data must be FP8 (E4M3 or E5M2), got {data.dtype}")
-    if scale.dtype not in _SCALE_TYPES:
-        raise TypeError(f"{name}: scales must be torch.float8_e8m0fnu or torch.float32, got {scale.dtype}")
-    if data.dim() != 2 or scale.dim() != 2:
-        raise ValueError(f"{name}: data and scales must be matrices")
-    if data.device.type != "cuda" or scale.device != data.device:
-        raise ValueError(f"{name}: data and scales must be on the same GPU device")
-    rows, k = data.shape
-    if scale.shape[1] != _blocks(k) or scale.shape[0] not in (rows, _blocks(rows)):
-        raise ValueError(
-            f"{name}: scales of a {rows} x {k} matrix are {rows} x {_blocks(k)} or {_blocks(rows)} x {_blocks(k)}, "
-            f"not {tuple(scale.shape)}"
-        )
-    return _lib.BlockMatrix(
-        _address(data), _address(scale), _row_stride(data, f"{name}: data"), _row_stride(scale, f"{name}: scale"),
-        rows, _lib.DTYPE_CODES[data.dtype], _SCALE_TYPES[scale.dtype], 1 if scale.shape[0] == rows else BLOCK, 0,
-    )
+def _device_of(*tensors):
+    """The first tensor's device, checked where it is a GPU; the native entries refuse everything else."""
+    reject_dtensors(*tensors)
+    device = getattr(tensors[0], "device", None)
+    if device is not None and device.type == "cuda":
+        validate_device(device)
+        return device
+    return None
 
 
-def _span(x: torch.Tensor):
-    """First and one past the last byte a 2-D tensor touches."""
-    start = x.data_ptr()
-    if not x.numel():
-        return start, start
-    last = sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
-    return start, start + (last + 1) * x.element_size()
+def _stream(device) -> int:
+    return 0 if device is None else _lib.stream_handle(device)
 
 
 def block_matmul(
@@ -193,42 +138,18 @@ def block_matmul(
     ``out_dtype`` (BF16 by default, FP32 or FP16) or into ``out``, which has
     consecutive columns and shares no memory with the operands.
     """
-    left, right = _operand(a, "a"), _operand(b, "b")
-    device, k = a[0].device, a[0].shape[1]
-    if b[0].device != device:
-        raise ValueError("a and b must be on the same GPU device")
-    if b[0].shape[1] != k:
-        raise ValueError(f"a and b contract {k} and {b[0].shape[1]} values")
-    if left.scale_type != right.scale_type:
-        raise TypeError("a and b must have scales of one type")
-    validate_device(device)
-    m, n = left.rows, right.rows
-    if out is None:
-        dtype = torch.bfloat16 if out_dtype is None else out_dtype
-        if dtype not in _WIDE_DTYPES:
-            raise TypeError(f"out_dtype must be FP32, BF16 or FP16, not {dtype}")
-        out = torch.empty((m, n), dtype=dtype, device=device)
-        stride = n
+    (a_data, a_scale), (b_data, b_scale) = a, b
+    if out_dtype is None:
+        code = -1  # out's, or BF16
+    elif out_dtype in _WIDE_DTYPES:
+        code = _lib.DTYPE_CODES[out_dtype]
     else:
-        if out.dtype not in _WIDE_DTYPES or (out_dtype is not None and out.dtype != out_dtype):
-            raise TypeError(f"out has dtype {out.dtype}")
-        if out.shape != (m, n) or out.device != device:
-            raise ValueError(f"out must be a {m} x {n} tensor on {device}")
-        stride = _row_stride(out, "out")
-        start, end = _span(out)
-        for t in (*a, *b):
-            first, last = _span(t)
-            if start < last and first < end:
-                raise ValueError("out must not overlap the operands")
-    if m and n:
-        size = _lib.library().sr_block_matmul_workspace(m, n, k)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        with _lib.on_device(device):
-            _lib.call(
-                "sr_block_matmul", left, right, k, _address(out), stride, _lib.DTYPE_CODES[out.dtype],
-                _address(workspace) if size else None, _lib.stream_handle(device),
-            )
-    return out
+        raise TypeError(f"out_dtype must be FP32, BF16 or FP16, not {out_dtype}")
+    device = _device_of(a_data, a_scale, b_data, b_scale, out)
+    result = _lib.matrix().block_matmul(a_data, a_scale, b_data, b_scale, code, out, _stream(device))
+    if not isinstance(result, torch.Tensor):
+        _lib.check("sr_block_matmul", result)
+    return result
 
 
 _LINEAR_NAMES = ("input", "weight", "gradient")
@@ -239,51 +160,39 @@ _LINEAR_FORMATS = (
 )
 
 
-def _matrix(x: torch.Tensor, cols: int) -> torch.Tensor:
-    """x as rows of ``cols`` consecutive values, copied only where its layout needs it."""
-    x = x.reshape(math.prod(x.shape[:-1]), cols)
-    if (cols > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < cols):
-        x = x.contiguous()
-    return x
+# Checked formats of block_linear, as the native entries take them.
+_LINEAR_CODES: dict = {}
+
+
+def _linear_codes(formats):
+    chosen = _LINEAR_FORMATS if formats is None else resolve_formats(_LINEAR_NAMES, formats, backend="hip")
+    for name, fmt in zip(_LINEAR_NAMES, chosen):
+        if fmt.dtype not in FP8_DTYPES:
+            raise ValueError(f"{name} format must be FP8, not {fmt.dtype}")
+    return tuple(code for fmt in chosen for code in native_codes(fmt.dtype, fmt.rounding))
 
 
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, formats, seed):
-        rows = _matrix(x, weight.shape[1])
+    def forward(ctx, x, weight, codes, seed):
         need_x, need_w = ctx.needs_input_grad[:2]
-
-        def cast(t, k, **options):
-            fmt = formats[k]
-            return block_cast(t, dtype=fmt.dtype, rounding=fmt.rounding, seed=state_key(seed, k), **options)
-
-        ctx.cast, ctx.like, ctx.weight_dtype = cast, (x.shape, x.dtype), weight.dtype
+        seeds = tuple(state_key(seed, k) for k in range(3))
         # The weight gradient contracts the tokens, so it needs the input's blocks along them; the input gradient
         # contracts the weight's rows, and its square blocks only turn.
-        qx, qx_t = cast(rows, 0, axis=(1, 0)) if need_w else (cast(rows, 0), None)
-        square = {"block": (BLOCK, BLOCK)}
-        qw, qw_t = cast(_matrix(weight, weight.shape[1]), 1, axis=(1, 0), **square) if need_x else (
-            cast(_matrix(weight, weight.shape[1]), 1, **square), None)
-        ctx.save_for_backward(*(qx_t or (None, None)), *(qw_t or (None, None)))
-        y = block_matmul(qx, qw, out_dtype=x.dtype)
-        return y.view(*x.shape[:-1], weight.shape[0])
+        out = _lib.matrix().linear_forward(x, weight, codes, seeds, need_x, need_w, _stream(x.device))
+        if not isinstance(out, tuple):
+            _lib.check("block_linear", out)
+        ctx.save_for_backward(*out[1:])
+        ctx.options = (*codes[4:], seeds[2], _lib.DTYPE_CODES[x.dtype], _lib.DTYPE_CODES[weight.dtype])
+        return out[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x_data, x_scale, w_data, w_scale = ctx.saved_tensors
-        shape, dtype = ctx.like
-        need_x, need_w = ctx.needs_input_grad[:2]
-        rows = _matrix(dy, dy.shape[-1])
-        axes = (1,) * need_x + (0,) * need_w
-        q = ctx.cast(rows, 2, axis=axes if len(axes) > 1 else axes[0])
-        q = dict(zip(axes, q if len(axes) > 1 else (q,)))
-        dx = dw = None
-        if need_x:
-            dx = block_matmul(q[1], BlockScaled(w_data, w_scale), out_dtype=dtype).view(shape)
-        if need_w:
-            dw = block_matmul(q[0], BlockScaled(x_data, x_scale), out_dtype=ctx.weight_dtype)
-        return dx, dw, None, None
+        out = _lib.matrix().linear_backward(dy, *ctx.saved_tensors, *ctx.options, _stream(dy.device))
+        if not isinstance(out, tuple):
+            _lib.check("block_linear", out)
+        return *out, None, None
 
 
 def block_linear(
@@ -311,16 +220,18 @@ def block_linear(
     be an update key that differs by layer and step (:func:`sr_states.update_key`).
     Only the FP8 copies are kept for the backward pass.
     """
-    chosen = _LINEAR_FORMATS if formats is None else resolve_formats(_LINEAR_NAMES, formats, backend="hip")
-    for name, fmt in zip(_LINEAR_NAMES, chosen):
-        if fmt.dtype not in FP8_DTYPES:
-            raise ValueError(f"{name} format must be FP8, not {fmt.dtype}")
+    try:
+        codes = _LINEAR_CODES[formats]
+    except KeyError:
+        codes = _LINEAR_CODES[formats] = _linear_codes(formats)
+    except TypeError:  # a dict of formats
+        codes = _linear_codes(formats)
     for name, t in (("x", x), ("weight", weight)):
-        reject_dtensors(t)
         if t.dtype not in _WIDE_DTYPES:
             raise TypeError(f"{name} must be FP32, BF16 or FP16, not {t.dtype}")
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x {tuple(x.shape)} and weight {tuple(weight.shape)} do not match")
     if x.device.type != "cuda" or weight.device != x.device:
         raise ValueError("x and weight must be on the same GPU device")
-    return _BlockLinear.apply(x, weight, chosen, _lib.low32(seed))
+    _device_of(x, weight)
+    return _BlockLinear.apply(x, weight, codes, _lib.low32(seed))

@@ -99,39 +99,20 @@ def orthogonalize(
     Matrices that are not contiguous are copied first.  Nothing is recorded
     for autograd.
     """
-    if not isinstance(x, torch.Tensor):
-        raise TypeError(f"expected a tensor, got {type(x).__name__}")
     reject_dtensors(x)
-    if x.dtype not in _DTYPES:
-        raise TypeError(f"expected FP32, BF16 or FP16 input, got {x.dtype}")
     if dtype not in _DTYPES:
         raise TypeError(f"dtype must be FP32, BF16 or FP16, not {dtype}")
     ns = _newton_schulz(steps, tuple(coefficients), float(eps))
-    if x.dim() < 2:
-        raise ValueError(f"orthogonalize takes matrices, not {x.dim()} dimensions")
-    device = x.device
-    if device.type != "cuda":
-        raise ValueError("orthogonalize requires a GPU tensor")
-    validate_device(device)
-    out = torch.empty(x.shape, dtype=dtype, device=device)
-    if not x.numel():
-        return out
-    x = x.detach()
-    if not x.is_contiguous():
-        x = x.contiguous()
-    rows, cols = x.shape[-2:]
-    size = rows * cols
-    batch = x.numel() // size
-    each = min(batch, _batch_size(rows, cols))
-    with _lib.on_device(device):
-        workspace = _workspace(each, rows, cols, device)
-        for first in range(0, batch, each):
-            _lib.call(
-                "sr_orthogonalize", x.data_ptr() + first * size * x.element_size(),
-                out.data_ptr() + first * size * out.element_size(), min(each, batch - first), size, size, rows, cols,
-                _lib.DTYPE_CODES[x.dtype], _lib.DTYPE_CODES[dtype], ns, workspace.data_ptr(),
-                _lib.stream_handle(device),
-            )
+    device = getattr(x, "device", None)
+    stream = 0
+    if device is not None and device.type == "cuda":  # the native entry refuses everything else
+        validate_device(device)
+        stream = _lib.stream_handle(device)
+    out = _lib.matrix().orthogonalize(
+        x, _lib.DTYPE_CODES[dtype], ns.a, ns.b, ns.c, ns.eps, ns.steps, _WORKSPACE_BYTES, stream
+    )
+    if not isinstance(out, torch.Tensor):
+        _lib.check("sr_orthogonalize", out)
     return out
 
 
