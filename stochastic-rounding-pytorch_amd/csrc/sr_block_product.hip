@@ -18,6 +18,8 @@ void fill(BlockProductKernels& k) {
   k.tile[kTile128][1] = reinterpret_cast<const void*>(&block_product_kernel<MODE, FA, FB, Tile128, true>);
   k.tile[kTile64][0] = reinterpret_cast<const void*>(&block_product_kernel<MODE, FA, FB, Tile64, false>);
   k.tile[kTile64][1] = reinterpret_cast<const void*>(&block_product_kernel<MODE, FA, FB, Tile64, true>);
+  k.tile[kTile64x2][1] = reinterpret_cast<const void*>(&block_product_kernel<MODE, FA, FB, Tile64x2, true>);
+  k.tile[kTile64x4][1] = reinterpret_cast<const void*>(&block_product_kernel<MODE, FA, FB, Tile64x4, true>);
 }
 
 template <int FB>

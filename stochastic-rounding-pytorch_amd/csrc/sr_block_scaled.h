@@ -476,11 +476,14 @@ __device__ __forceinline__ void block_mma(f32x4& acc, const Fragment<MODE, FA>& 
 }
 
 template <int MODE, int FA, int FB, class S, bool ASYNC>
-__global__ __launch_bounds__(S::kThreads, 2) void block_product_kernel(BlockProductArgs g) {
-  constexpr int kStages = 2 * S::kStage + ScaleArea<S>::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
+__global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void block_product_kernel(BlockProductArgs g) {
+  static_assert(ASYNC || S::kGroups == 1, "groups take aligned rows");
+  constexpr int kStages = S::kLds + ScaleArea<S>::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
   constexpr int kLds = kStages > kChunks ? kStages : kChunks;
+  static_assert(S::kSums <= kLds, "the groups' sums");
   __shared__ __align__(1024) char lds[kLds];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = all % S::kWaves, group = all / S::kWaves;
   uint32_t tile_m, tile_n;
   band_tile(xcd_run(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tile_m, tile_n);
   const int row0 = tile_m * S::BM, col0 = tile_n * S::BN;
@@ -488,7 +491,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void block_product_kernel(BlockProd
 
   Stager<S> stager;
   stager.init(g.a, g.b, row0, col0, wave, lane);
-  char* area = lds + 2 * S::kStage;
+  char* own = lds + group * 2 * S::kStage;  // this group's stages
+  char* area = lds + S::kLds;
   const int period = ScaleArea<S>::period(g);
 
   f32x4 acc[S::MI][S::NI] = {};
@@ -514,48 +518,48 @@ __global__ __launch_bounds__(S::kThreads, 2) void block_product_kernel(BlockProd
     }
   };
 
-  // Stage kt lies in buffer kt % 2.  At its barrier it has landed for every
-  // wave, and every wave is done with the other buffer and the scales before.
   auto refill = [&](int kt) {
     if ((kt & (period - 1)) == 0) {
       ScaleArea<S>::fill(area, g, row0, col0, kt, stages);
-      stage_barrier();
+      lds_barrier();
     }
   };
   if constexpr (ASYNC) {
     const int whole = static_cast<int>(g.k / kStageBytes);
-    if (whole > 0) stager.load_async(lds, 0, wave);
-    for (int kt = 0; kt < whole; ++kt) {
-      stage_barrier();
-      refill(kt);
-      if (kt + 1 < whole) stager.load_async(lds + (~kt & 1) * S::kStage, (kt + 1) * kStageBytes, wave);
-      multiply(lds + (kt & 1) * S::kStage, kt);
-    }
+    walk_stages<S>(
+        whole, group, [&](int kt, int buffer) { stager.load_async(own + buffer * S::kStage, kt * kStageBytes, wave); }, refill,
+        [&](int kt, int buffer) { multiply(own + buffer * S::kStage, kt); });
     if (whole < stages) {  // the contracted axis ends inside a stage
       stage_barrier();
       refill(whole);
-      char* stage = lds + (whole & 1) * S::kStage;
-      stager.load_through(stage, static_cast<int64_t>(whole) * kStageBytes, g.k, wave, lane);
-      stage_barrier();
-      multiply(stage, whole);
+      if (group == 0) stager.load_through(lds, static_cast<int64_t>(whole) * kStageBytes, g.k, wave, lane);
+      lds_barrier();
+      if (group == 0) multiply(lds, whole);
     }
   } else {
-    i32x4 regs[S::kLoads];
-    if (stages > 0) {
-      stager.load(regs, 0, g.k, wave, lane);
-      stager.store(lds, regs, wave, lane);
-    }
-    for (int kt = 0; kt < stages; ++kt) {
-      stage_barrier();
+    // Two sets of registers, so that a stage's loads have two stages' time.
+    i32x4 even[S::kLoads], odd[S::kLoads];
+    auto load = [&](i32x4 (&regs)[S::kLoads], int kt) {
+      if (kt < stages) stager.load(regs, static_cast<int64_t>(kt) * kStageBytes, g.k, wave, lane);
+    };
+    auto step = [&](int kt, i32x4 (&next)[S::kLoads], i32x4 (&after)[S::kLoads]) {
+      lds_barrier();
       refill(kt);
-      const bool more = kt + 1 < stages;
-      if (more) stager.load(regs, static_cast<int64_t>(kt + 1) * kStageBytes, g.k, wave, lane);
+      load(after, kt + 2);
       multiply(lds + (kt & 1) * S::kStage, kt);
-      if (more) stager.store(lds + (~kt & 1) * S::kStage, regs, wave, lane);
+      if (kt + 1 < stages) stager.store(lds + (~kt & 1) * S::kStage, next, wave, lane);
+    };
+    load(even, 0);
+    load(odd, 1);
+    if (stages > 0) stager.store(lds, even, wave, lane);
+    for (int kt = 0; kt < stages; kt += 2) {
+      step(kt, odd, even);
+      if (kt + 1 < stages) step(kt + 1, even, odd);
     }
   }
   stage_barrier();
-  store_chunks<kLds, S>(g, lds, row0, col0, wave, lane, acc);
+  add_groups<S>(lds, group, acc);
+  if (group == 0) store_chunks<kLds, S>(g, lds, row0, col0, wave, lane, acc);
 }
 
 // Few rows of A (at most 16): one 16-column tile of the result per workgroup,

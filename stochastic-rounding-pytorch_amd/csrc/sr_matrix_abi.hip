@@ -140,9 +140,13 @@ int sr_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t 
     g.tiles_n = (g.n + S::BN - 1) / S::BN;
     return launch(kernel, static_cast<uint64_t>(g.tiles_m) * g.tiles_n, S::kThreads, &g, stream);
   };
-  // The larger tile where it still gives the chip's 256 CUs work.
-  if (tiles(128) >= 256) return launch_tiles(fn.tile[sr::kTile128][async], sr::Tile128{});
-  return launch_tiles(fn.tile[sr::kTile64][async], sr::Tile64{});
+  const sr::BlockTile tile = sr::tile_by_count(tiles);
+  switch (async || tile == sr::kTile128 ? tile : sr::kTile64) {
+    case sr::kTile128: return launch_tiles(fn.tile[sr::kTile128][async], sr::Tile128{});
+    case sr::kTile64x2: return launch_tiles(fn.tile[sr::kTile64x2][1], sr::Tile64x2{});
+    case sr::kTile64x4: return launch_tiles(fn.tile[sr::kTile64x4][1], sr::Tile64x4{});
+    default: return launch_tiles(fn.tile[sr::kTile64][async], sr::Tile64{});
+  }
 }
 
 }  // extern "C"

@@ -394,11 +394,14 @@ __device__ __forceinline__ void with_result(const NsArgs& a, F&& store) {
 //   kNsLast        the same into the results or the parameters; TURNED where
 //                  these are the transpose of the workspace's orientation
 template <int OP, class S, bool TURNED>
-__global__ __launch_bounds__(S::kThreads, 2) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
+__global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
                                                                     uint32_t tiles, uint32_t matrices, MatrixTable t) {
-  constexpr int kLds = ns_lds<OP, TURNED, S>(2 * S::kStage);
+  constexpr int kLds = ns_lds<OP, TURNED, S>(S::kLds);
+  static_assert(S::kSums <= kLds, "the groups' sums");
   __shared__ __align__(1024) char lds[kLds];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = all % S::kWaves, group = all / S::kWaves;
+  char* own = lds + group * 2 * S::kStage;  // this group's stages
   const NsTile tile = ns_tile<OP, S>(a, tiles_m, tiles_n, tiles, matrices);
   const int wave_m = wave / S::WN * S::kRowsM, wave_n = wave % S::WN * S::kRowsN;
   const int stages = tile.stages;
@@ -407,30 +410,31 @@ __global__ __launch_bounds__(S::kThreads, 2) void ns_product_kernel(NsArgs a, ui
 
   f32x4 acc[S::MI][S::NI] = {};
   const uint32_t fragment = fragment_offset(lane);
-  stager.load_async(lds, 0, wave);
-  for (int kt = 0; kt < stages; ++kt) {
-    // Stage kt has landed for every wave, and every wave is done with the other buffer.
-    stage_barrier();
-    if (kt + 1 < stages) stager.load_async(lds + (~kt & 1) * S::kStage, (kt + 1) * kStageBytes, wave);
-    const char* stage = lds + (kt & 1) * S::kStage;
+  walk_stages<S>(
+      stages, group, [&](int kt, int buffer) { stager.load_async(own + buffer * S::kStage, kt * kStageBytes, wave); },
+      [](int) {},
+      [&](int, int buffer) {
+        const char* stage = own + buffer * S::kStage;
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      const char* sa = stage + wave_m * kStageBytes + (fragment ^ (64 * ks));
-      const char* sb = stage + (S::BM + wave_n) * kStageBytes + (fragment ^ (64 * ks));
-      f16x8 fb[S::NI];
+        for (int ks = 0; ks < 2; ++ks) {
+          const char* sa = stage + wave_m * kStageBytes + (fragment ^ (64 * ks));
+          const char* sb = stage + (S::BM + wave_n) * kStageBytes + (fragment ^ (64 * ks));
+          f16x8 fb[S::NI];
 #pragma unroll
-      for (int ni = 0; ni < S::NI; ++ni)
-        fb[ni] = __builtin_bit_cast(f16x8, read_chunk(sb + ni * 16 * kStageBytes));
+          for (int ni = 0; ni < S::NI; ++ni)
+            fb[ni] = __builtin_bit_cast(f16x8, read_chunk(sb + ni * 16 * kStageBytes));
 #pragma unroll
-      for (int mi = 0; mi < S::MI; ++mi) {
-        const f16x8 fa = __builtin_bit_cast(f16x8, read_chunk(sa + mi * 16 * kStageBytes));
+          for (int mi = 0; mi < S::MI; ++mi) {
+            const f16x8 fa = __builtin_bit_cast(f16x8, read_chunk(sa + mi * 16 * kStageBytes));
 #pragma unroll
-        for (int ni = 0; ni < S::NI; ++ni)
-          acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[ni], fa, acc[mi][ni], 0, 0, 0);
-      }
-    }
-  }
+            for (int ni = 0; ni < S::NI; ++ni)
+              acc[mi][ni] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[ni], fa, acc[mi][ni], 0, 0, 0);
+          }
+        }
+      });
   stage_barrier();
+  add_groups<S>(lds, group, acc);
+  if (group > 0) return;
   with_result<OP>(a, [&](auto encoding, auto muon) {
     ns_store<OP, TURNED, decltype(encoding)::value, decltype(muon)::value, kLds, S>(a, t, tile, lds, wave, lane, acc);
   });
@@ -450,6 +454,199 @@ __global__ __launch_bounds__(TileWide::kThreads, 2) void ns_wide_kernel(NsArgs a
   WideTile::run(lds, stager, tile.stages, wave, lane, acc);
   with_result<OP>(a, [&](auto encoding, auto muon) {
     ns_store<OP, TURNED, decltype(encoding)::value, decltype(muon)::value, kLds, TileWide>(a, t, tile, lds, wave, lane, acc);
+  });
+}
+
+// ---------------------------------------------------------------------------
+// Small matrices: all steps of one matrix in one workgroup.
+//
+// With at most 64 rows (padded) and 768 columns, H fits the LDS and X the
+// registers of sixteen waves, so that the steps need no memory and no further
+// launches: 64 x 576 takes 32 us so, and a chain of 16 launches of 3 to 5 us
+each took 70.  Wave w
+// computes tile (w / 4, w % 4) of G and P, and of X the column tiles w, w + 16, ...:
+// lane l holds rows 16 i + 4 (l / 16) .. + 3 of its column 16 t + l % 16.
+//
+// LDS rows are runs of 16-byte chunks, chunk c of row r at place c ^ (r % 8) of
+// its group of eight, as in the stages above.  G and P are symmetric, so a
+// lane's four values of a column are stored as four neighbours of that row.
+// The step needs H with its rows as the contracted axis: the transposing LDS
+// read gives lane i of sixteen the values at column i of four rows, when lane i
+// points at columns 4 (i % 4) .. + 3 of row i / 4.
+// ---------------------------------------------------------------------------
+constexpr int kSmallRows = 64, kSmallCols = 768, kSmallThreads = 1024;
+constexpr int kSmallTiles = kSmallCols / 16 / 16;  // column tiles of a wave, at most
+
+#if defined(__HIP_DEVICE_COMPILE__)
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f16x4 read_turned(const char* p) {
+  return __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+#else
+__device__ inline f16x4 read_turned(const char*) { return {}; }
+#endif
+
+// Byte offset of column `col` (a multiple of 4) of row `row` in rows of `stride` bytes.
+__device__ __forceinline__ int swizzled(int row, int col, int stride) {
+  return row * stride + (((col >> 3) ^ (row & 7)) << 4) + ((col & 4) << 1);
+}
+
+// One value of the result, in the caller's orientation.
+template <int E, bool MUON>
+__device__ __forceinline__ void finish_one(const NsArgs& a, void* out, int row, int col, float y) {
+  if (row >= a.rows || col >= a.cols) return;
+  const int64_t i = static_cast<int64_t>(row) * a.cols + col;
+  const float r = MUON ? fmaf(y, a.neg_lr, decode<E>(load1<E>(out, i)) * a.decay) : y;
+  store1<E>(out, i, encode<E>(r, 0u));
+}
+
+__global__ __launch_bounds__(kSmallThreads, 4) void ns_small_kernel(NsArgs a, int steps, MatrixTable t) {
+  __shared__ __align__(1024) char small_lds[2 * (2 * kSmallRows * kSmallRows + kSmallRows * kSmallCols)];
+  __shared__ float scratch[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int across = lane & 15, quarter = lane >> 4;
+  const int matrix = blockIdx.x, n = a.n;
+  char* gram = small_lds;                           // 64 x 64
+  char* poly = gram + kSmallRows * kSmallRows * 2;  // 64 x 64
+  char* h = poly + kSmallRows * kSmallRows * 2;     // 64 x n
+  const int stride = 2 * n;
+  const float* from = a.x + static_cast<int64_t>(matrix) * a.m * n;
+
+  float sum = threadIdx.x < a.partials ? a.partial[matrix * kNsPartials + threadIdx.x] : 0.0f;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (lane == 0) scratch[wave] = sum;
+  f32x4 x[kSmallTiles][4];
+#pragma unroll
+  for (int c = 0; c < kSmallTiles; ++c) {
+    const int col = 16 * (wave + 16 * c) + across;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[c][i][j] = 16 * (wave + 16 * c) < n ? from[(16 * i + 4 * quarter + j) * n + col] : 0.0f;
+  }
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) sum += scratch[w];
+  const float inverse = 1.0f / (sqrtf(sum) + a.eps);
+
+  // Places in H whose swizzle does not change over the loops: 16 rows further are 16 strides, 16 column tiles further
+  // (the wave's next) 512 bytes, 64 columns further 128 bytes.
+  uint32_t own_h[4];  // of this lane's column of its first tile, row 4 quarter + j
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    own_h[j] = swizzled(4 * quarter + j, (16 * wave + across) & ~3, stride) + 2 * (across & 3);
+  uint32_t turned_h[2];  // what it points at in the transposing reads of rows 0 .. 3 and 4 .. 7
+#pragma unroll
+  for (int u = 0; u < 2; ++u) turned_h[u] = swizzled(8 * quarter + across / 4 + 4 * u, 16 * wave + 4 * (across & 3), stride);
+  uint32_t chunk_h[2], chunk_s[2];  // chunk 4 u + quarter of row `across` of H, and of G or P
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    chunk_h[u] = swizzled(across, 8 * (4 * u + quarter), stride);
+    chunk_s[u] = swizzled(across, 8 * (4 * u + quarter), 2 * kSmallRows);
+  }
+  const uint32_t rows16 = 16 * stride;
+
+  // H = X in FP16; every wave its column tiles.
+  auto store_h = [&] {
+#pragma unroll
+    for (int c = 0; c < kSmallTiles; ++c) {
+      if (16 * (wave + 16 * c) >= n) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          *reinterpret_cast<_Float16*>(h + own_h[j] + i * rows16 + 512 * c) = static_cast<_Float16>(x[c][i][j] * kNsScale);
+    }
+  };
+#pragma unroll
+  for (int c = 0; c < kSmallTiles; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[c][i][j] *= inverse;
+  store_h();
+  __syncthreads();
+
+  const int tile_i = wave >> 2, tile_j = wave & 3;
+  auto fragment = [](const char* p) { return __builtin_bit_cast(f16x8, read_chunk(p)); };
+  // Where a lane's four values of a symmetric tile belong: row of tile j, columns of tile i.
+  const int own = swizzled(16 * tile_j + across, 16 * tile_i + 4 * quarter, 2 * kSmallRows);
+  for (int step = 0; step < steps; ++step) {
+    f32x4 sums[2] = {};
+    const char *rows_i = h + tile_i * rows16, *rows_j = h + tile_j * rows16;
+    for (int k = 0; k < stride; k += 128) {  // 64 columns, which n is a multiple of
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        sums[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fragment(rows_i + chunk_h[u] + k), fragment(rows_j + chunk_h[u] + k),
+                                                         sums[u], 0, 0, 0);
+    }
+    f16x4 g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = static_cast<_Float16>((sums[0][j] + sums[1][j]) * kNsInverse);
+    *reinterpret_cast<f16x4*>(gram + own) = g;
+    __syncthreads();
+    f32x4 square{};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      square = __builtin_amdgcn_mfma_f32_16x16x32_f16(fragment(gram + 32 * kSmallRows * tile_i + chunk_s[k]),
+                                                      fragment(gram + 32 * kSmallRows * tile_j + chunk_s[k]), square, 0, 0, 0);
+    f16x4 p;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float v = fmaf(a.c * kNsInverse, square[j], a.b * static_cast<float>(g[j]));
+      p[j] = static_cast<_Float16>(16 * tile_j + across == 16 * tile_i + 4 * quarter + j ? v + kNsShift * kNsScale : v);
+    }
+    *reinterpret_cast<f16x4*>(poly + own) = p;
+    __syncthreads();
+    f16x8 left[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) left[i][k] = fragment(poly + 32 * kSmallRows * i + chunk_s[k]);
+#pragma unroll
+    for (int c = 0; c < kSmallTiles; ++c) {
+      if (16 * (wave + 16 * c) >= n) break;
+      f16x8 right[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const char* rows = h + 2 * k * rows16 + 512 * c;
+        right[k] = __builtin_shufflevector(read_turned(rows + turned_h[0]), read_turned(rows + turned_h[1]), 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f32x4 v{};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v = __builtin_amdgcn_mfma_f32_16x16x32_f16(left[i][k], right[k], v, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float own_h = static_cast<float>(static_cast<_Float16>(x[c][i][j] * kNsScale)) * kNsInverse;
+          x[c][i][j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, own_h, a.a * x[c][i][j]));
+        }
+      }
+    }
+    // A wave reads and writes only its own columns of H in the step, and all of it in the next G.
+    if (step + 1 < steps) {
+      store_h();
+      __syncthreads();
+    }
+  }
+
+  void* out = reinterpret_cast<void*>(t.p[matrix]);
+  with_result<kNsLast>(a, [&](auto encoding, auto muon) {
+#pragma unroll
+    for (int c = 0; c < kSmallTiles; ++c) {
+      const int col = 16 * (wave + 16 * c) + across;
+      if (16 * (wave + 16 * c) >= n) break;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int row = 16 * i + 4 * quarter + j;
+          finish_one<decltype(encoding)::value, decltype(muon)::value>(a, out, a.tall ? col : row, a.tall ? row : col, x[c][i][j]);
+        }
+    }
   });
 }
 

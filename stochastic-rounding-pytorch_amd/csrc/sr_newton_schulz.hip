@@ -69,34 +69,29 @@ int product(const NsArgs& a, int matrices, const sr::MatrixTable& t, hipStream_t
   return launched("Newton-Schulz product launch");
 }
 
-// Tiles of a launch of S.
-template <int OP, class S>
-int64_t tile_count(const NsArgs& a, int matrices) {
-  const int64_t tm = (a.m + S::BM - 1) / S::BM, tn = (a.n + S::BN - 1) / S::BN;
-  return (OP == sr::kNsGram || OP == sr::kNsPolynomial ? S::BM / S::BN * (tm * (tm + 1) / 2) : tm * tn) * matrices;
-}
-
-// The largest tile that still gives the chip's 256 CUs work.  The symmetric
-// launches stop at 128 x 128: their triangles have few large tiles (8
+// The symmetric launches stop at 128 x 128 tiles, and the others take 256 x
+// 256 ones where these fill the chip: a triangle has few large tiles (8
 // matrices of 2048 x 2048: G 122 us on 256 x 256 tiles and 102 on 128 x 128,
 // the step 200 and 244).
-template <int OP>
+template <int OP, bool TURNED = false>
 int product_by_size(const NsArgs& a, int matrices, const sr::MatrixTable& t, hipStream_t s) {
   constexpr bool kSymmetric = OP == sr::kNsGram || OP == sr::kNsPolynomial;
-  const int tile = !kSymmetric && tile_count<OP, sr::TileWide>(a, matrices) >= 256 ? 256
-                   : tile_count<OP, sr::Tile128>(a, matrices) >= 256              ? 128
-                                                                                   : 64;
-  if constexpr (OP == sr::kNsLast) {
-    if (a.tall)
-      return tile == 256 ? product<OP, sr::TileWide, true>(a, matrices, t, s)
-             : tile == 128 ? product<OP, sr::Tile128, true>(a, matrices, t, s)
-                           : product<OP, sr::Tile64, true>(a, matrices, t, s);
+  if constexpr (OP == sr::kNsLast && !TURNED) {
+    if (a.tall) return product_by_size<OP, true>(a, matrices, t, s);
   }
+  auto tiles = [&](int64_t side) {
+    const int64_t tm = (a.m + side - 1) / side, tn = (a.n + side - 1) / side;
+    return (kSymmetric ? tm * (tm + 1) / 2 : tm * tn) * matrices;
+  };
   if constexpr (!kSymmetric) {
-    if (tile == 256) return product<OP, sr::TileWide>(a, matrices, t, s);
+    if (tiles(256) >= 256) return product<OP, sr::TileWide, TURNED>(a, matrices, t, s);
   }
-  return tile == 128 ? product<OP, sr::Tile128>(a, matrices, t, s)
-                     : product<OP, sr::Tile64>(a, matrices, t, s);
+  switch (sr::tile_by_count(tiles)) {
+    case sr::kTile128: return product<OP, sr::Tile128, TURNED>(a, matrices, t, s);
+    case sr::kTile64x2: return product<OP, sr::Tile64x2, TURNED>(a, matrices, t, s);
+    case sr::kTile64x4: return product<OP, sr::Tile64x4, TURNED>(a, matrices, t, s);
+    default: return product<OP, sr::Tile64, TURNED>(a, matrices, t, s);
+  }
 }
 
 // The whole update of up to SR_MATRIX_BATCH matrices.  `ue` is the momentum's
@@ -134,6 +129,10 @@ int run(NsArgs a, const sr::MatrixTable& t, int matrices, int g_dtype, int ue, c
     load_momentum<sr::ENC_BF16_RN>(a, t, ue, grid, s);
   }
   if (int rc = launched("ns_load_kernel launch")) return rc;
+  if (a.m == sr::kSmallRows && a.n <= sr::kSmallCols) {
+    sr::ns_small_kernel<<<matrices, sr::kSmallThreads, 0, s>>>(a, ns.steps, t);
+    return launched("ns_small_kernel launch");
+  }
   a.ht_next = turned[0];
   sr::ns_scale_kernel<<<dim3(static_cast<uint32_t>(tiles), matrices), sr::kNsThreads, 0, s>>>(a);
   if (int rc = launched("ns_scale_kernel launch")) return rc;

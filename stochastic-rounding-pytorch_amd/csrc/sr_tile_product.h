@@ -44,14 +44,21 @@ typedef int chunk_any __attribute__((ext_vector_type(4), aligned(1)));
 constexpr int kStageBytes = 128;  // of each operand row
 constexpr int kChunk = 16;
 
-// BM x BN results by WM x WN waves.
-template <int BM_, int BN_, int WM_, int WN_>
+// BM x BN results by WM x WN waves; two stages in LDS.  With GROUPS > 1 so many
+// such sets of waves take every GROUPS-th stage each, with stages of their own,
+// and add their sums at the end: for launches with few tiles, whose time is
+// the latency of one tile's walk.
+template <int BM_, int BN_, int WM_, int WN_, int GROUPS_ = 1>
 struct TileShape {
+  static constexpr int kGroups = GROUPS_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
-  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int kWaves = WM * WN;                         // of one group
+  static constexpr int kThreads = 64 * kWaves * kGroups;
   static constexpr int kRowsM = BM / WM, kRowsN = BN / WN;      // of one wave
   static constexpr int MI = kRowsM / 16, NI = kRowsN / 16;      // its 16x16 tiles
   static constexpr int kStage = (BM + BN) * kStageBytes;        // bytes of one LDS stage
+  static constexpr int kLds = 2 * kStage * kGroups;             // all stages
+  static constexpr int kSums = (kGroups - 1) * BM * BN * 4;     // the other groups' sums
   static constexpr int kLoads = (BM + BN) / 8 / kWaves;         // chunks a lane stages
   static_assert(BM % 8 == 0 && ((BM + BN) / 8) % kWaves == 0 && kRowsM % 16 == 0 && kRowsN % 16 == 0, "tile shape");
 };
@@ -67,6 +74,51 @@ struct Operand {
 // workgroup's other waves.
 __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// The same without waiting for loads, for what only LDS accesses must order.
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Walks `stages` stages, a group every kGroups-th: load(stage, buffer) starts a
+// stage's loads into one of the group's two buffers, use(stage, buffer) takes
+// one that has landed for all its waves.  between(stage) runs on every wave
+// before the stages from `stage` on (a multiple of kGroups), when every wave
+// is done with those before.  Past the end a group loads the last stage
+// again and uses nothing.
+template <class S, class Load, class Between, class Use>
+__device__ __forceinline__ void walk_stages(int stages, int group, Load&& load, Between&& between, Use&& use) {
+  if (stages <= 0) return;
+  auto start = [&](int kt, int buffer) { load(kt < stages ? kt : stages - 1, buffer); };
+  start(group, 0);
+  for (int base = 0, buffer = 0; base < stages; base += S::kGroups, buffer ^= 1) {
+    stage_barrier();
+    between(base);
+    if (base + S::kGroups < stages) start(base + S::kGroups + group, buffer ^ 1);
+    if (S::kGroups == 1 || base + group < stages) use(base + group, buffer);
+  }
+}
+
+// Adds the groups' sums into group 0's, in the groups' order, through LDS that
+// every wave is done with; only group 0 may go on to use acc, and after it the LDS.
+template <class S>
+__device__ __forceinline__ void add_groups(char* lds, int group, f32x4 (&acc)[S::MI][S::NI]) {
+  if constexpr (S::kGroups > 1) {
+    constexpr int kTiles = S::MI * S::NI, kThreadsOfGroup = S::kThreads / S::kGroups;
+    const int t = threadIdx.x - group * kThreadsOfGroup;
+    f32x4* sums = reinterpret_cast<f32x4*>(lds);
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) sums[((group - 1) * kTiles + i) * kThreadsOfGroup + t] = acc[i / S::NI][i % S::NI];
+    }
+    lds_barrier();
+    if (group == 0) {
+#pragma unroll
+      for (int g = 0; g < S::kGroups - 1; ++g)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) acc[i / S::NI][i % S::NI] += sums[(g * kTiles + i) * kThreadsOfGroup + t];
+    }
+    lds_barrier();
+  }
 }
 
 // The tiles of a grid are numbered so that each XCD, which gets every eighth
