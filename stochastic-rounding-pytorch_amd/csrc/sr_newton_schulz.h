@@ -463,7 +463,7 @@ __global__ __launch_bounds__(TileWide::kThreads, 2) void ns_wide_kernel(NsArgs a
 // With at most 64 rows (padded) and 768 columns, H fits the LDS and X the
 // registers of sixteen waves, so that the steps need no memory and no further
 // launches: 64 x 576 takes 32 us so, and a chain of 16 launches of 3 to 5 us
-each took 70.  Wave w
+// each took 70.  Wave w
 // computes tile (w / 4, w % 4) of G and P, and of X the column tiles w, w + 16, ...:
 // lane l holds rows 16 i + 4 (l / 16) .. + 3 of its column 16 t + l % 16.
 //
