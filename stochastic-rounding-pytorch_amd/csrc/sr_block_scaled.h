@@ -586,19 +586,30 @@ __global__ __launch_bounds__(64 * kRowWaves) void block_product_rows_kernel(Bloc
     scale_b[j] = g.scale_b + ((r < g.n ? r : g.n - 1) >> g.shift_b) * g.ld_scale_b * size;
   }
   f32x4 acc{};
-  const int stages = static_cast<int>((g.k + kStageBytes - 1) / kStageBytes);
-  for (int kb = wave; kb < stages; kb += kRowWaves) {
+  const int whole = static_cast<int>(g.k / kStageBytes);
+  auto block = [&](int kb, auto load) {
     Scales<MODE, 1, 1> s;
-    s.a[0] = Scales<MODE, 1, 1>::read(scale_a + kb * size, g.scale_f32);
+    s.a[0] = Scales<MODE, 1, 1>::read(scale_a + static_cast<int64_t>(kb) * size, g.scale_f32);
 #pragma unroll
-    for (int j = 0; j < Scales<MODE, 1, 1>::kPerB; ++j) s.b[0][j] = Scales<MODE, 1, 1>::read(scale_b[j] + kb * size, g.scale_f32);
+    for (int j = 0; j < Scales<MODE, 1, 1>::kPerB; ++j)
+      s.b[0][j] = Scales<MODE, 1, 1>::read(scale_b[j] + static_cast<int64_t>(kb) * size, g.scale_f32);
     const int64_t at = static_cast<int64_t>(kb) * kStageBytes + (lane >> 4) * kChunk;
     Fragment<MODE, FA> a;
     Fragment<MODE, FB> b;
-    a.set(load_chunk(pa, at, g.k), load_chunk(pa, at + 64, g.k));
-    b.set(load_chunk(pb, at, g.k), load_chunk(pb, at + 64, g.k));
+    a.set(load(pa, at), load(pa, at + 64));
+    b.set(load(pb, at), load(pb, at + 64));
     block_mma(acc, a, b, s, 0, 0);
+  };
+  // A wave's blocks are few, so that the loads of two run together.
+  auto inside = [](const char* row, int64_t at) { return load_whole_chunk(row, at); };
+  int kb = wave;
+  for (; kb + kRowWaves < whole; kb += 2 * kRowWaves) {
+    block(kb, inside);
+    block(kb + kRowWaves, inside);
   }
+  if (kb < whole) block(kb, inside);
+  if (g.k % kStageBytes && whole % kRowWaves == wave)
+    block(whole, [&](const char* row, int64_t at) { return load_chunk(row, at, g.k); });
   sums[wave][lane] = acc;
   __syncthreads();
   if (wave) return;

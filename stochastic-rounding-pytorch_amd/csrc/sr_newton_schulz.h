@@ -204,34 +204,57 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a) {
   }
 }
 
-// Four consecutive values of row `row` of the result, in the caller's
-// orientation: stored with encoding E, or (MUON) applied to the parameter.
+// Four consecutive values of row `row` of the parameter, in its orientation;
+// zeros outside.  Loads come apart from the stores below: between a store and a
+// load that might read it the compiler keeps their order, and each load would
+// wait for memory by itself.
+template <int E>
+__device__ __forceinline__ f32x4 load_parameter(const NsArgs& a, const void* p, int row, int col) {
+  f32x4 v{};
+  if (row >= a.rows || col >= a.cols) return v;
+  const int64_t i = static_cast<int64_t>(row) * a.cols + col;
+  if (a.cols - col >= 4) {
+    uint32_t w[group_words(E)];
+    float r[4];
+    load_group<E>(p, i, w);
+    decode_group<E>(w, r);
+    v = f32x4{r[0], r[1], r[2], r[3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < a.cols - col) v[j] = decode<E>(load1<E>(p, i + j));
+  }
+  return v;
+}
+
+// Stores four consecutive values of row `row` of the result with encoding E, or
+// (MUON) of the parameter, whose values were `old`, updated by them.
 template <int E, bool MUON>
-__device__ __forceinline__ void finish(const NsArgs& a, const MatrixTable& t, int matrix, int row, int col,
-                                       const f32x4& y) {
+__device__ __forceinline__ void finish(const NsArgs& a, void* out, int row, int col, const f32x4& y, const f32x4& old) {
   if (row >= a.rows || col >= a.cols) return;
   const int live = a.cols - col < 4 ? a.cols - col : 4;
   const int64_t i = static_cast<int64_t>(row) * a.cols + col;
-  void* out = reinterpret_cast<void*>(t.p[matrix]);
+  float r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = MUON ? fmaf(y[j], a.neg_lr, old[j] * a.decay) : y[j];
   if (live == 4) {
     uint32_t w[group_words(E)];
-    float r[4];
-    if constexpr (MUON) {
-      load_group<E>(out, i, w);
-      decode_group<E>(w, r);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = MUON ? fmaf(y[j], a.neg_lr, r[j] * a.decay) : y[j];
     encode_group<E>(r, 0u, w);
     store_group<E>(out, i, w);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (j < live) {
-        const float r = MUON ? fmaf(y[j], a.neg_lr, decode<E>(load1<E>(out, i + j)) * a.decay) : y[j];
-        store1<E>(out, i + j, encode<E>(r, 0u));
-      }
+      if (j < live) store1<E>(out, i + j, encode<E>(r[j], 0u));
   }
+}
+
+// Loads what the kernel will need of its arguments at once: they may lie in
+// host memory, where each load that waits by itself costs a microsecond or two.
+__device__ __forceinline__ void need_arguments(const NsArgs& a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" ::"s"(a.m), "s"(a.n), "s"(a.a), "s"(a.b), "s"(a.c), "s"(a.x), "s"(a.h), "s"(a.ht), "s"(a.ht_next),
+               "s"(a.g), "s"(a.p));
+#endif
 }
 
 enum NsOp { kNsGram, kNsPolynomial, kNsStep, kNsLast };
@@ -292,12 +315,28 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
   float* chunk = reinterpret_cast<float*>(lds + wave * kWaveBytes);
   T* turned = reinterpret_cast<T*>(lds + wave * kWaveBytes + Chunk::kBytes);
   _Float16* out = (OP == kNsGram ? a.g : a.p) + square;  // kSymmetric
+  void* result = reinterpret_cast<void*>(t.p[tile.matrix]);  // kNsLast
 
   auto use = [&](int first, const float* from) {
     // The workspace's sizes are multiples of 64, so a chunk of 32 x 32 or 32 x 64 is inside or outside as a whole.
     const int row0 = wave_row + first;
     if (row0 >= a.m || wave_col >= width) return;
     const int col = wave_col + Chunk::block_col(lane);
+    // What the sums are combined with: G, or X and the parameter, of all of the lane's rows.
+    using Old = std::conditional_t<OP == kNsPolynomial, f16x4, f32x4>;
+    Old old[Chunk::kBlocks][4];
+    f32x4 parameter[Chunk::kBlocks][4];
+#pragma unroll
+    for (int i = 0; i < Chunk::kBlocks; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = row0 + Chunk::block_row(i, lane) + k;
+        if constexpr (OP == kNsPolynomial)
+          old[i][k] = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
+        else if constexpr (OP != kNsGram)
+          old[i][k] = *reinterpret_cast<const f32x4*>(a.x + base + static_cast<int64_t>(row) * a.n + col);
+        if constexpr (MUON && !TURNED) parameter[i][k] = load_parameter<E>(a, result, row, col);
+      }
 #pragma unroll
     for (int i = 0; i < Chunk::kBlocks; ++i) {
       const int r0 = Chunk::block_row(i, lane);
@@ -311,30 +350,28 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
           for (int j = 0; j < 4; ++j) block[k][j] = static_cast<_Float16>(v[j] * kNsInverse);
           *reinterpret_cast<f16x4*>(out + static_cast<int64_t>(row) * a.m + col) = block[k];
         } else if constexpr (OP == kNsPolynomial) {
-          const f16x4 g = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float p = fmaf(a.c * kNsInverse, v[j], a.b * static_cast<float>(g[j]));
+            const float p = fmaf(a.c * kNsInverse, v[j], a.b * static_cast<float>(old[i][k][j]));
             block[k][j] = static_cast<_Float16>(row == col + j ? p + kNsShift * kNsScale : p);
           }
           *reinterpret_cast<f16x4*>(out + static_cast<int64_t>(row) * a.m + col) = block[k];
         } else {
-          const int64_t at = base + static_cast<int64_t>(row) * a.n + col;
-          const f32x4 x = *reinterpret_cast<const f32x4*>(a.x + at);
           f32x4 y;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float h = static_cast<float>(static_cast<_Float16>(x[j] * kNsScale)) * kNsInverse;
-            y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x[j]));
+            const float x = old[i][k][j], h = static_cast<float>(static_cast<_Float16>(x * kNsScale)) * kNsInverse;
+            y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x));
           }
           if constexpr (OP == kNsStep) {
+            const int64_t at = base + static_cast<int64_t>(row) * a.n + col;
 #pragma unroll
             for (int j = 0; j < 4; ++j) block[k][j] = static_cast<_Float16>(y[j] * kNsScale);
             *reinterpret_cast<f32x4*>(a.x + at) = y;
             *reinterpret_cast<f16x4*>(a.h + at) = block[k];
           } else {
             block[k] = y;
-            if constexpr (!TURNED) finish<E, MUON>(a, t, tile.matrix, row, col, y);
+            if constexpr (!TURNED) finish<E, MUON>(a, result, row, col, y, parameter[i][k]);
           }
         }
       }
@@ -347,16 +384,25 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
         }
       }
     }
-    if constexpr (kTurns) {
-      if (!kSymmetric || tile.mirrored)
-        Chunk::template store_turned<T, T4>(turned, lane, [&](int c, int r, const T4& v) {
-          if constexpr (OP == kNsLast) {
-            finish<E, MUON>(a, t, tile.matrix, wave_col + c, row0 + r, v);
-          } else {
-            _Float16* to = kSymmetric ? out : a.ht_next + base;
-            *reinterpret_cast<f16x4*>(to + static_cast<int64_t>(wave_col + c) * a.m + row0 + r) = v;
-          }
-        });
+    if constexpr (OP == kNsLast && TURNED) {
+      f32x4 before[Chunk::kTurnedBlocks];
+      if constexpr (MUON) {
+#pragma unroll
+        for (int i = 0; i < Chunk::kTurnedBlocks; ++i)
+          before[i] = load_parameter<E>(a, result, wave_col + Chunk::turned_col(i, lane), row0 + Chunk::turned_row(lane));
+      }
+#pragma unroll
+      for (int i = 0; i < Chunk::kTurnedBlocks; ++i)
+        finish<E, MUON>(a, result, wave_col + Chunk::turned_col(i, lane), row0 + Chunk::turned_row(lane),
+                        Chunk::template get_turned<T, T4>(turned, i, lane), before[i]);
+    } else if constexpr (kTurns) {
+      if (!kSymmetric || tile.mirrored) {
+        _Float16* to = kSymmetric ? out : a.ht_next + base;
+#pragma unroll
+        for (int i = 0; i < Chunk::kTurnedBlocks; ++i)
+          *reinterpret_cast<f16x4*>(to + static_cast<int64_t>(wave_col + Chunk::turned_col(i, lane)) * a.m + row0 +
+                                    Chunk::turned_row(lane)) = Chunk::template get_turned<T, T4>(turned, i, lane);
+      }
     }
   };
   for_each_chunk<S>(chunk, lane, acc, use);
@@ -402,6 +448,7 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void ns_pr
   const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = all % S::kWaves, group = all / S::kWaves;
   char* own = lds + group * 2 * S::kStage;  // this group's stages
+  need_arguments(a);
   const NsTile tile = ns_tile<OP, S>(a, tiles_m, tiles_n, tiles, matrices);
   const int wave_m = wave / S::WN * S::kRowsM, wave_n = wave % S::WN * S::kRowsN;
   const int stages = tile.stages;
@@ -447,6 +494,7 @@ __global__ __launch_bounds__(TileWide::kThreads, 2) void ns_wide_kernel(NsArgs a
   constexpr int kLds = ns_lds<OP, TURNED, TileWide>(2 * TileWide::kStage);
   __shared__ __align__(1024) char lds[kLds];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  need_arguments(a);
   const NsTile tile = ns_tile<OP, TileWide>(a, tiles_m, tiles_n, tiles, matrices);
   Stager<TileWide> stager;
   stager.init(tile.a, tile.b, tile.row0, tile.col0, wave, lane);

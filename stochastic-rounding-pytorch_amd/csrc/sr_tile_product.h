@@ -153,17 +153,37 @@ __device__ __forceinline__ void triangle_tile(uint32_t id, uint32_t wide, uint32
   col = id - wide * (r * (r + 1) / 2);
 }
 
-// The 16 bytes at `at` of a row that ends at `end`; zeros from there on.
+// The 16 bytes at `at` of a row, all inside it.
+__device__ __forceinline__ i32x4 load_whole_chunk(const char* row, int64_t at) {
+  const chunk_any v = *(const __attribute__((address_space(1))) chunk_any*)(row + at);
+  return i32x4{v[0], v[1], v[2], v[3]};
+}
+
+// The 16 bytes at `at` of a row of `end` bytes (at least 1, the same for the
+// wave); zeros from its end on.  Without a branch per lane, at whose end each
+// load would wait for memory by itself: a chunk that passes the end is
+// read where it still fits and shifted, and rows shorter than a chunk are read
+// byte by byte at clamped places.
 __device__ __forceinline__ i32x4 load_chunk(const char* row, int64_t at, int64_t end) {
-  if (at + kChunk <= end) {
-    const chunk_any v = *(const __attribute__((address_space(1))) chunk_any*)(row + at);
-    return i32x4{v[0], v[1], v[2], v[3]};
+  if (end >= kChunk) {
+    const int64_t from = at < end - kChunk ? at : end - kChunk;
+    const i32x4 v = load_whole_chunk(row, from);
+    const int skip = at - from < kChunk ? static_cast<int>(at - from) : kChunk;  // bytes before the chunk
+    const uint64_t lo = static_cast<uint32_t>(v[0]) | static_cast<uint64_t>(static_cast<uint32_t>(v[1])) << 32;
+    const uint64_t hi = static_cast<uint32_t>(v[2]) | static_cast<uint64_t>(static_cast<uint32_t>(v[3])) << 32;
+    const int bits = 8 * (skip & 7);
+    // lo and hi shifted by less than a word, then by a word.
+    const uint64_t low = (lo >> bits) | ((hi << 1) << (63 - bits)), high = hi >> bits;
+    const uint64_t a = skip >= 16 ? 0 : (skip >= 8 ? high : low), b = skip >= 8 ? 0 : high;
+    return i32x4{static_cast<int>(a), static_cast<int>(a >> 32), static_cast<int>(b), static_cast<int>(b >> 32)};
   }
   uint32_t words[4] = {0, 0, 0, 0};
 #pragma unroll
-  for (int j = 0; j < kChunk; ++j)
-    if (at + j < end)
-      words[j >> 2] |= static_cast<uint32_t>(*(const __attribute__((address_space(1))) uint8_t*)(row + at + j)) << (8 * (j & 3));
+  for (int j = 0; j < kChunk; ++j) {
+    const int64_t from = at + j < end ? at + j : end - 1;
+    const uint32_t byte = *(const __attribute__((address_space(1))) uint8_t*)(row + from);
+    words[j >> 2] |= (at + j < end ? byte : 0u) << (8 * (j & 3));
+  }
   return i32x4{(int)words[0], (int)words[1], (int)words[2], (int)words[3]};
 }
 
@@ -224,10 +244,13 @@ struct Stager {
   // stage that ends inside its 128 bytes: bytes from `end` on become zero.
   __device__ void load(i32x4 (&regs)[S::kLoads], int64_t k, int64_t end, int wave, int lane) const {
     const int64_t chunk = ((lane & 7) ^ (lane >> 3)) * kChunk;
+    // Whole stages load without a branch per chunk: at its end a branch waits for its own load.
+    if (k + kStageBytes <= end) {
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) {
-      const char* row = (i < kLoadsA ? a : b) + (offset[i] - chunk);
-      regs[i] = load_chunk(row, k + chunk, end);
+      for (int i = 0; i < S::kLoads; ++i) regs[i] = load_whole_chunk((i < kLoadsA ? a : b) + offset[i], k);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) regs[i] = load_chunk((i < kLoadsA ? a : b) + (offset[i] - chunk), k + chunk, end);
     }
   }
 
@@ -382,14 +405,13 @@ struct ResultChunk {
   static __device__ __forceinline__ void put_turned(T* turned, int col, int row, const T4& v) {
     *reinterpret_cast<T4*>(turned + col * kTurnedStride + row) = v;
   }
-  // Calls store(column, row, four values from that row on) for all of it.
-  template <class T, class T4, class F>
-  static __device__ __forceinline__ void store_turned(const T* turned, int lane, F&& store) {
-#pragma unroll
-    for (int i = 0; i < CN * kTurnedLanes / 64; ++i) {
-      const int col = i * (64 / kTurnedLanes) + lane / kTurnedLanes, row = 4 * (lane % kTurnedLanes);
-      store(col, row, *reinterpret_cast<const T4*>(turned + col * kTurnedStride + row));
-    }
+  // Turned block `i` of this lane: four values of column turned_col(i) from row turned_row() on.
+  static constexpr int kTurnedBlocks = CN * kTurnedLanes / 64;
+  static __device__ __forceinline__ int turned_col(int i, int lane) { return i * (64 / kTurnedLanes) + lane / kTurnedLanes; }
+  static __device__ __forceinline__ int turned_row(int lane) { return 4 * (lane % kTurnedLanes); }
+  template <class T, class T4>
+  static __device__ __forceinline__ T4 get_turned(const T* turned, int i, int lane) {
+    return *reinterpret_cast<const T4*>(turned + turned_col(i, lane) * kTurnedStride + turned_row(lane));
   }
 };
 
