@@ -6,13 +6,14 @@ namespace sr {
 namespace {
 
 template <int XE, int QE>
-void fill(const void* (&k)[2]) {
-  k[0] = reinterpret_cast<const void*>(&block_cast_kernel<XE, QE, false>);
-  k[1] = reinterpret_cast<const void*>(&block_cast_kernel<XE, QE, true>);
+void fill(const void* (&k)[kCastKinds]) {
+  k[kCastRowBlocks] = reinterpret_cast<const void*>(&block_cast_kernel<XE, QE, false>);
+  k[kCastSquare] = reinterpret_cast<const void*>(&block_cast_kernel<XE, QE, true>);
+  k[kCastSplit] = reinterpret_cast<const void*>(&block_cast_split_kernel<XE, QE>);
 }
 
 template <int XE>
-void fill_formats(const void* (&k)[4][2]) {
+void fill_formats(const void* (&k)[4][kCastKinds]) {
   fill<XE, ENC_E4M3_RN>(k[0]);
   fill<XE, ENC_E4M3_SR>(k[1]);
   fill<XE, ENC_E5M2_RN>(k[2]);

@@ -27,28 +27,55 @@ struct BlockCastArgs {
   int64_t ldx, rows, cols;
   sr_block_output by_rows, by_cols;
   uint32_t counter_base;  // seed + offset (mod 2^32)
-  uint32_t tiles_n;
+  uint32_t tiles_n;       // blocks of 128 columns
+  uint32_t row_groups;    // block_cast_split_kernel: workgroups of the row orientation
+};
+
+// The format of encoding QE.
+template <int QE>
+struct CastFormat {
+  static constexpr bool kE4M3 = QE == ENC_E4M3_RN || QE == ENC_E4M3_SR;
+  using F = std::conditional_t<kE4M3, E4M3, E5M2>;
+  static constexpr int kTop = kE4M3 ? 8 : 15;  // the largest value is 1.75 2^kTop
 };
 
 // The exponent e of a block's scale 2^e from the bits of its largest finite
-// magnitude: with amax = f 2^E, 1 <= f < 2, and the format's maximum
-// 1.75 2^top, e = E - top, one more where f > 1.75; 0 where amax is 0.
-// Subnormal amax are far below 2^(top - 127), where e stays at -127.
-template <int TOP>
+// magnitude: with amax = f 2^E, 1 <= f < 2, e = E - top, one more where
+// f > 1.75; 0 where amax is 0.  Subnormal amax are far below 2^(top - 127),
+// where e stays at -127.
+template <int QE>
 __device__ __forceinline__ int block_exponent(uint32_t amax) {
-  const int e = static_cast<int>(amax >> 23) - 127 - TOP + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  const int e = static_cast<int>(amax >> 23) - 127 - CastFormat<QE>::kTop + ((amax & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   return amax == 0 ? 0 : (e > -127 ? e : -127);
 }
 
 // 2^-e, e in [-127, 120]: always a normal number.
 __device__ __forceinline__ float inverse_scale(int e) { return bits_f32(static_cast<uint32_t>(127 - e) << 23); }
 
+__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t umin(uint32_t a, uint32_t b) { return a < b ? a : b; }
+
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+__device__ __forceinline__ uint32_t magnitude(float x) { return f32_bits(x) & 0x7FFFFFFFu; }
+
 __device__ __forceinline__ uint32_t finite_magnitude(float x) {
-  const uint32_t a = f32_bits(x) & 0x7FFFFFFFu;
-  return a < 0x7F800000u ? a : 0u;
+  const uint32_t a = magnitude(x);
+  return a < kInfBits ? a : 0u;
 }
 
-__device__ __forceinline__ uint32_t umax(uint32_t a, uint32_t b) { return a > b ? a : b; }
+// The largest finite magnitude of eight values; `finite`: all of them are.
+__device__ __forceinline__ uint32_t largest(const float (&x)[8], bool finite) {
+  uint32_t m = 0;
+  if (finite) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) m = umax(umax(m, magnitude(x[j])), magnitude(x[j + 1]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = umax(m, finite_magnitude(x[j]));
+  }
+  return m;
+}
 
 // Byte j of each of four words, for j = 0..3: a 4 x 4 byte transpose.
 __device__ __forceinline__ void transpose_bytes(uint32_t (&w)[4]) {
@@ -68,64 +95,157 @@ __device__ __forceinline__ uint32_t max_of_16(uint32_t m) {
   return umax(m, __builtin_amdgcn_update_dpp(0u, m, 0x121, 0xF, 0xF, true));
 }
 
-template <int XE, int QE, bool SQUARE>
-__global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs a) {
-  constexpr int TOP = (QE == ENC_E4M3_RN || QE == ENC_E4M3_SR) ? 8 : 15;
-  constexpr int XB = enc_bytes(XE);
-  __shared__ uint32_t turned[kCastTile * 32];
-  __shared__ __align__(16) uint32_t partial[SQUARE ? 1 : 16][kCastTile];
-  __shared__ __align__(16) int exponents[kCastTile];
-  __shared__ uint32_t whole[4];
-  const int t = threadIdx.x, group = t >> 4, lane = t & 15;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x / a.tiles_n) * kCastTile;
-  const int64_t col0 = static_cast<int64_t>(blockIdx.x % a.tiles_n) * kCastTile;
-  const int64_t c = col0 + 8 * lane;
-  const int live = c >= a.cols ? 0 : (a.cols - c < 8 ? static_cast<int>(a.cols - c) : 8);
-
-  // Rows of this thread: band k, row 64 k + 4 group + i.
-  float x[2][4][8];
+// Eight values from `p`, of which the first `live` are there; zeros for the rest.
+template <int XE>
+__device__ __forceinline__ void load_eight(const char* p, int live, float (&x)[8]) {
+  if (live == 8) {
+    uint32_t w[2 * group_words(XE)];
+    load_words<16, true>(p, w);
+    if constexpr (enc_bytes(XE) == 4) load_words<16, true>(p + 16, w + 4);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
+    for (int h = 0; h < 2; ++h) {
+      uint32_t words[group_words(XE)];
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < group_words(XE); ++j) words[j] = w[h * group_words(XE) + j];
+      decode_group<XE>(words, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[4 * h + j] = v[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = j < live ? decode<XE>(load1<XE>(p, j)) : 0.0f;
+  }
+}
+
+// The hashes of eight consecutive counters.
+template <int QE>
+__device__ __forceinline__ void hash_eight(uint32_t counter, uint32_t (&hash)[2][4]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) hash[j >> 2][j & 3] = enc_stochastic(QE) ? h32(counter + static_cast<uint32_t>(j)) : 0u;
+}
+
+// Four values, scaled into the format's range, as FP8.  Where they are finite
+// and (stochastic) zeros or at least the format's smallest normal number, the
+// rule is an addition: the random bits as far below the format's last bit as
+// FP32 has bits, and a truncation, after which the convert is exact.  The
+// general rule takes the rest (4% of the waves' groups of normally
+// distributed values for stochastic E4M3, none for the others); 8192 x 2048
+// in both orientations took 34 us with it alone.
+template <int QE>
+__device__ __forceinline__ uint32_t encode_scaled(const float (&y)[4], const uint32_t (&hash)[4], bool finite) {
+  using F = typename CastFormat<QE>::F;
+  uint32_t bits[4], word[1];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bits[j] = f32_bits(y[j]);
+  bool plain = finite;
+  if constexpr (enc_stochastic(QE)) {
+    uint32_t smallest = 0xFFFFFFFFu;  // of 2 |y| - 1, for zeros the largest of all
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) smallest = umin(umin(smallest, 2 * bits[j] - 1), 2 * bits[j + 1] - 1);
+    plain = plain && smallest >= (static_cast<uint32_t>(127 + F::kEmin) << 24) - 1;
+  }
+  if (plain) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (enc_stochastic(QE)) {
+      constexpr int kShift = 9 + F::kM;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bits[j] = (bits[j] + (~hash[j] >> kShift)) & ~(0xFFFFFFFFu >> kShift);
+    }
+    if constexpr (CastFormat<QE>::kE4M3) {
+      const int low = __builtin_amdgcn_cvt_pk_fp8_f32(bits_f32(bits[0]), bits_f32(bits[1]), 0, false);
+      word[0] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(bits_f32(bits[2]), bits_f32(bits[3]), low, true));
+    } else {
+      const int low = __builtin_amdgcn_cvt_pk_bf8_f32(bits_f32(bits[0]), bits_f32(bits[1]), 0, false);
+      word[0] = static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_bf8_f32(bits_f32(bits[2]), bits_f32(bits[3]), low, true));
+    }
+#endif
+  } else {
+    encode_group_with<QE>(bits, hash, word);
+  }
+  return word[0];
+}
+
+// One row's eight values under their block's scale.
+template <int QE>
+__device__ __forceinline__ void encode_row(const float (&x)[8], int e, const uint32_t (&hash)[2][4], bool finite,
+                                           uint32_t (&words)[2]) {
+  const float inv = inverse_scale(e);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float y[4] = {x[4 * h] * inv, x[4 * h + 1] * inv, x[4 * h + 2] * inv, x[4 * h + 3] * inv};
+    words[h] = encode_scaled<QE>(y, hash[h], finite);
+  }
+}
+
+// Stores the first `live` of eight bytes.
+__device__ __forceinline__ void store_eight(char* q, const uint32_t (&words)[2], int live) {
+  if (live == 8) {
+    *(SR_GLOBAL group8*)(q) = group8{words[0], words[1]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < live) *gptr_mut<uint8_t>(q + j) = static_cast<uint8_t>(words[j >> 2] >> (8 * (j & 3)));
+  }
+}
+
+__device__ __forceinline__ void store_exponent(const sr_block_output& to, int64_t row, int64_t col, int e) {
+  *gptr_mut<uint8_t>(static_cast<char*>(to.scale) + row * to.ld_scale + col) = static_cast<uint8_t>(e + 127);
+}
+
+template <class T>
+__device__ __forceinline__ int live_of(T at, T end, int width) {
+  return at >= end ? 0 : (end - at < width ? static_cast<int>(end - at) : width);
+}
+
+// The tile of 128 rows and 8 LANES columns from (row0, col0), by a workgroup
+// of 256 threads: groups of LANES threads share rows, four neighbouring ones in
+// each of BANDS bands.
+template <int XE, int QE, bool SQUARE, int LANES>
+__device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, int64_t col0, bool want_rows, bool want_cols) {
+  constexpr int kGroups = kCastThreads / LANES, kBands = kCastTile / (4 * kGroups), kCols = 8 * LANES;
+  constexpr int kTurn = 32 / LANES;
+  __shared__ uint32_t turned[kCols * 32];
+  __shared__ __align__(16) uint32_t partial[SQUARE ? 1 : kGroups][kCols];
+  __shared__ __align__(16) int exponents[kCols];
+  __shared__ uint32_t whole[4];
+  const int t = threadIdx.x, group = t / LANES, lane = t % LANES;
+  const int64_t c = col0 + 8 * lane;
+  const int live = live_of(c, a.cols, 8);
+
+  // Rows of this thread: band k, row 4 (kGroups k + group) + i.
+  float x[kBands][4][8];
+#pragma unroll
+  for (int k = 0; k < kBands; ++k)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t r = row0 + 64 * k + 4 * group + i;
-      const char* p = a.x + (r * a.ldx + c) * XB;
-      if (r < a.rows && live == 8) {
-        uint32_t w[2 * group_words(XE)];
-        if constexpr (XB == 4) {
-          load_words<16, true>(p, w);
-          load_words<16, true>(p + 16, w + 4);
-        } else {
-          load_words<16, true>(p, w);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t words[group_words(XE)];
-          float v[4];
-#pragma unroll
-          for (int j = 0; j < group_words(XE); ++j) words[j] = w[h * group_words(XE) + j];
-          decode_group<XE>(words, v);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[k][i][4 * h + j] = v[j];
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[k][i][j] = r < a.rows && j < live ? decode<XE>(load1<XE>(p, j)) : 0.0f;
-      }
+      const int64_t r = row0 + 4 * (kGroups * k + group) + i;
+      load_eight<XE>(a.x + (r * a.ldx + c) * enc_bytes(XE), r < a.rows ? live : 0, x[k][i]);
     }
-  }
 
-  const bool want_rows = a.by_rows.data != nullptr, want_cols = a.by_cols.data != nullptr;
+  uint32_t m[8] = {}, any = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+#pragma unroll
+    for (int k = 0; k < kBands; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) m[j] = umax(umax(m[j], magnitude(x[k][i][j])), magnitude(x[k][i + 1][j]));
+    any = umax(any, m[j]);
+  }
+  const bool finite = any < kInfBits;
   int tile_exp = 0;  // SQUARE
   int col_exp[8];    // of this thread's columns
   if (SQUARE || want_cols) {
-    uint32_t m[8] = {};
+    if (!finite) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
+      for (int j = 0; j < 8; ++j) {
+        m[j] = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < kBands; ++k)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) m[j] = umax(m[j], finite_magnitude(x[k][i][j]));
+          for (int i = 0; i < 4; ++i) m[j] = umax(m[j], finite_magnitude(x[k][i][j]));
+      }
+    }
     if constexpr (SQUARE) {
       uint32_t tile = 0;
 #pragma unroll
@@ -135,22 +255,20 @@ __global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs 
       tile = umax(tile, __shfl_xor(tile, 32));
       if ((t & 63) == 0) whole[t >> 6] = tile;
       __syncthreads();
-      tile_exp = block_exponent<TOP>(umax(umax(whole[0], whole[1]), umax(whole[2], whole[3])));
+      tile_exp = block_exponent<QE>(umax(umax(whole[0], whole[1]), umax(whole[2], whole[3])));
 #pragma unroll
       for (int j = 0; j < 8; ++j) col_exp[j] = tile_exp;
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) partial[group][8 * lane + j] = m[j];
       __syncthreads();
-      if (t < kCastTile) {
+      if (t < kCols) {
         uint32_t col = 0;
 #pragma unroll
-        for (int h = 0; h < 16; ++h) col = umax(col, partial[h][t]);
-        const int e = block_exponent<TOP>(col);
+        for (int h = 0; h < kGroups; ++h) col = umax(col, partial[h][t]);
+        const int e = block_exponent<QE>(col);
         exponents[t] = e;
-        if (col0 + t < a.cols)
-          *gptr_mut<uint8_t>(static_cast<char*>(a.by_cols.scale) + (col0 + t) * a.by_cols.ld_scale + row0 / kCastTile) =
-              static_cast<uint8_t>(e + 127);
+        if (col0 + t < a.cols) store_exponent(a.by_cols, col0 + t, row0 / kCastTile, e);
       }
       __syncthreads();
 #pragma unroll
@@ -159,46 +277,21 @@ __global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs 
   }
 
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (row0 + 64 * k >= a.rows && !want_cols) break;
+  for (int k = 0; k < kBands; ++k) {
+    if (row0 + 4 * kGroups * k >= a.rows && !want_cols) break;
     uint32_t by_col[2][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int64_t r = row0 + 64 * k + 4 * group + i;
-      const uint32_t counter = a.counter_base + static_cast<uint32_t>(r) * static_cast<uint32_t>(a.cols) + static_cast<uint32_t>(c);
-      uint32_t hash[2][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) hash[j >> 2][j & 3] = enc_stochastic(QE) ? h32(counter + static_cast<uint32_t>(j)) : 0u;
-      uint32_t bits[4], word[1], words[2];
+      const int64_t r = row0 + 4 * (kGroups * k + group) + i;
+      uint32_t hash[2][4], words[2];
+      hash_eight<QE>(a.counter_base + static_cast<uint32_t>(r) * static_cast<uint32_t>(a.cols) + static_cast<uint32_t>(c), hash);
       if (want_rows) {
         int e = tile_exp;
-        if constexpr (!SQUARE) {
-          uint32_t m = 0;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) m = umax(m, finite_magnitude(x[k][i][j]));
-          e = block_exponent<TOP>(max_of_16(m));
-        }
-        const float inv = inverse_scale(e);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) bits[j] = f32_bits(x[k][i][4 * h + j] * inv);
-          encode_group_with<QE>(bits, hash[h], word);
-          words[h] = word[0];
-        }
+        if constexpr (!SQUARE) e = block_exponent<QE>(max_of_16(largest(x[k][i], finite)));
+        encode_row<QE>(x[k][i], e, hash, finite, words);
         if (r < a.rows) {
-          char* q = static_cast<char*>(a.by_rows.data) + r * a.by_rows.ld + c;
-          if (live == 8) {
-            *(SR_GLOBAL group8*)(q) = group8{words[0], words[1]};
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (j < live) *gptr_mut<uint8_t>(q + j) = static_cast<uint8_t>(words[j >> 2] >> (8 * (j & 3)));
-          }
-          if constexpr (!SQUARE)
-            if (lane == 0)
-              *gptr_mut<uint8_t>(static_cast<char*>(a.by_rows.scale) + r * a.by_rows.ld_scale + col0 / kCastTile) =
-                  static_cast<uint8_t>(e + 127);
+          store_eight(static_cast<char*>(a.by_rows.data) + r * a.by_rows.ld + c, words, live);
+          if (!SQUARE && lane == 0) store_exponent(a.by_rows, r, col0 / kCastTile, e);
         }
       }
       if (want_cols) {
@@ -208,42 +301,41 @@ __global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs 
         } else {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            float y[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) bits[j] = f32_bits(x[k][i][4 * h + j] * inverse_scale(col_exp[4 * h + j]));
-            encode_group_with<QE>(bits, hash[h], word);
-            by_col[h][i] = word[0];
+            for (int j = 0; j < 4; ++j) y[j] = x[k][i][4 * h + j] * inverse_scale(col_exp[4 * h + j]);
+            by_col[h][i] = encode_scaled<QE>(y, hash[h], finite);
           }
         }
       }
     }
     if (want_cols) {
-      // Column 8 lane + j, rows 64 k + 4 group .. + 3, at word (row / 4) ^ (2 lane) of its column's 32: the lanes
-      // of a wave then meet in a bank two at a time, and those that read a column below do not.
+      // Column 8 lane + j, rows 4 (kGroups k + group) .. + 3, at word (row / 4) ^ (kTurn lane) of its column's 32: the
+      // lanes of a wave then meet in a bank two at a time, and those that read a column below do not.
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         transpose_bytes(by_col[h]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) turned[(8 * lane + 4 * h + j) * 32 + ((16 * k + group) ^ (2 * lane))] = by_col[h][j];
+        for (int j = 0; j < 4; ++j)
+          turned[(8 * lane + 4 * h + j) * 32 + ((kGroups * k + group) ^ (kTurn * lane))] = by_col[h][j];
       }
     }
   }
 
   if (SQUARE && t == 0) {
-    const uint8_t byte = static_cast<uint8_t>(tile_exp + 127);
-    const int64_t rb = row0 / kCastTile, cb = col0 / kCastTile;
-    if (want_rows) *gptr_mut<uint8_t>(static_cast<char*>(a.by_rows.scale) + rb * a.by_rows.ld_scale + cb) = byte;
-    if (want_cols) *gptr_mut<uint8_t>(static_cast<char*>(a.by_cols.scale) + cb * a.by_cols.ld_scale + rb) = byte;
+    if (want_rows) store_exponent(a.by_rows, row0 / kCastTile, col0 / kCastTile, tile_exp);
+    if (want_cols) store_exponent(a.by_cols, col0 / kCastTile, row0 / kCastTile, tile_exp);
   }
   if (!want_cols) return;
   __syncthreads();
   const int word_at = t & 31, half = t >> 5;
   const int64_t r = row0 + 4 * word_at;
-  const int live_r = r >= a.rows ? 0 : (a.rows - r < 4 ? static_cast<int>(a.rows - r) : 4);
+  const int live_r = live_of(r, a.rows, 4);
 #pragma unroll
-  for (int k = 0; k < kCastTile / 8; ++k) {
+  for (int k = 0; k < kCols / 8; ++k) {
     const int col = 8 * k + half;
     if (col0 + col >= a.cols) break;
-    const uint32_t word = turned[col * 32 + (word_at ^ (2 * (col >> 3)))];
+    const uint32_t word = turned[col * 32 + (word_at ^ (kTurn * (col >> 3)))];
     char* q = static_cast<char*>(a.by_cols.data) + (col0 + col) * a.by_cols.ld + r;
     if (live_r == 4) {
       *(SR_GLOBAL group4*)(q) = word;
@@ -253,6 +345,45 @@ __global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs 
         if (j < live_r) *gptr_mut<uint8_t>(q + j) = static_cast<uint8_t>(word >> (8 * j));
     }
   }
+}
+
+template <int XE, int QE, bool SQUARE>
+__global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs a) {
+  cast_tile<XE, QE, SQUARE, 16>(a, static_cast<int64_t>(blockIdx.x / a.tiles_n) * kCastTile,
+                                static_cast<int64_t>(blockIdx.x % a.tiles_n) * kCastTile, a.by_rows.data != nullptr,
+                                a.by_cols.data != nullptr);
+}
+
+// Few tiles: each orientation by workgroups of its own, which read x twice but
+// are many.  Of the row orientation a workgroup takes 16 rows of 128
+// columns, of the other one 128 rows of 64 columns.
+constexpr int kSplitRows = kCastThreads / 16, kSplitLanes = 8;
+constexpr uint64_t kSplitBelow = 256;  // tiles
+
+template <int XE, int QE>
+__global__ __launch_bounds__(kCastThreads) void block_cast_split_kernel(BlockCastArgs a) {
+  if (blockIdx.x >= a.row_groups) {
+    const uint32_t id = blockIdx.x - a.row_groups, tiles = 2 * a.tiles_n;
+    cast_tile<XE, QE, false, kSplitLanes>(a, static_cast<int64_t>(id / tiles) * kCastTile,
+                                          static_cast<int64_t>(id % tiles) * 8 * kSplitLanes, false, true);
+    return;
+  }
+  const int lane = threadIdx.x & 15;
+  const int64_t r = static_cast<int64_t>(blockIdx.x / a.tiles_n) * kSplitRows + (threadIdx.x >> 4);
+  const int64_t block = blockIdx.x % a.tiles_n, c = block * kCastTile + 8 * lane;
+  if (r >= a.rows) return;  // sixteen lanes together
+  const int live = live_of(c, a.cols, 8);
+  float x[8];
+  load_eight<XE>(a.x + (r * a.ldx + c) * enc_bytes(XE), live, x);
+  uint32_t any = largest(x, true);
+  const bool finite = any < kInfBits;
+  if (!finite) any = largest(x, false);
+  const int e = block_exponent<QE>(max_of_16(any));
+  uint32_t hash[2][4], words[2];
+  hash_eight<QE>(a.counter_base + static_cast<uint32_t>(r) * static_cast<uint32_t>(a.cols) + static_cast<uint32_t>(c), hash);
+  encode_row<QE>(x, e, hash, finite, words);
+  store_eight(static_cast<char*>(a.by_rows.data) + r * a.by_rows.ld + c, words, live);
+  if (lane == 0) store_exponent(a.by_rows, r, block, e);
 }
 
 // ---------------------------------------------------------------------------

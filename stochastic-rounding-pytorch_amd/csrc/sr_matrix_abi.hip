@@ -92,8 +92,14 @@ int sr_block_cast(const void* x, int64_t ldx, int64_t rows, int64_t cols, int x_
   a.cols = cols;
   a.counter_base = seed + offset;
   a.tiles_n = static_cast<uint32_t>(blocks(cols));
-  const void* fn = casts()[x_dtype == SR_F32 ? 0 : (x_dtype == SR_BF16 ? 1 : 2)][2 * (dtype == SR_E5M2) + (rule == SR_STOCHASTIC)][square != 0];
-  return launch(fn, static_cast<uint64_t>(blocks(rows)) * a.tiles_n, sr::kCastThreads, &a, stream);
+  const auto& kinds = casts()[x_dtype == SR_F32 ? 0 : (x_dtype == SR_BF16 ? 1 : 2)][2 * (dtype == SR_E5M2) + (rule == SR_STOCHASTIC)];
+  const uint64_t tiles = static_cast<uint64_t>(blocks(rows)) * a.tiles_n;
+  if (!square && tiles < sr::kSplitBelow) {
+    const int64_t rows_groups = (rows + sr::kSplitRows - 1) / sr::kSplitRows * a.tiles_n;
+    a.row_groups = a.by_rows.data ? static_cast<uint32_t>(rows_groups) : 0;
+    return launch(kinds[sr::kCastSplit], a.row_groups + (a.by_cols.data ? 2 * tiles : 0), sr::kCastThreads, &a, stream);
+  }
+  return launch(kinds[square ? sr::kCastSquare : sr::kCastRowBlocks], tiles, sr::kCastThreads, &a, stream);
 }
 
 int64_t sr_block_matmul_workspace(int64_t, int64_t, int64_t) { return 0; }
