@@ -71,7 +71,7 @@ int sr_matrix_abi_version(void);
  * rows x ceil(cols / 128).  `by_cols` receives blocks along the rows, both
  * transposed: data cols x rows, scale cols x ceil(rows / 128).  Blocks are
  * 1 x 128 along those axes, or 128 x 128 with `square` (one scale row per 128
- * rows of data).  One pass over x fills both. */
+ * rows of data).  One call fills both. */
 int sr_block_cast(const void* x, int64_t ldx, int64_t rows, int64_t cols, int x_dtype, int dtype, int rule,
                   int square, uint32_t seed, uint32_t offset, const sr_block_output* by_rows,
                   const sr_block_output* by_cols, void* stream);
@@ -80,13 +80,9 @@ int sr_block_cast(const void* x, int64_t ldx, int64_t rows, int64_t cols, int x_
  * contracted values:
  *   out[i,j] = sum over blocks of scale_a scale_b sum in the block of a b
  * summed in FP32 and rounded once.  Both matrices have the same scale type.
- * m = a->rows and n = b->rows.  `workspace` holds sr_block_matmul_workspace
- * bytes (NULL when that is 0). */
+ * m = a->rows and n = b->rows. */
 int sr_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t k, void* out, int64_t ldo,
-                    int out_dtype, void* workspace, void* stream);
-
-/* Bytes of workspace sr_block_matmul needs for these sizes. */
-int64_t sr_block_matmul_workspace(int64_t m, int64_t n, int64_t k);
+                    int out_dtype, void* stream);
 
 /* ---- orthogonalised updates -------------------------------------------- */
 

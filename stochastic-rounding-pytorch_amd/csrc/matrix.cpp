@@ -6,7 +6,7 @@
 // makes the tensor checks, allocates the results and calls the C ABI's entry
 // points through the addresses the Python side binds once.
 //
-// bind(block_cast, block_matmul, block_matmul_workspace, orthogonalize, orthogonalize_workspace)
+// bind(block_cast, block_matmul, orthogonalize, orthogonalize_workspace)
 //   Keep the addresses of these sr_ entry points, taken from the loaded library.
 //
 // block_cast(x, code, rule, square, axes, seed, offset, stream) -> tuple or int
@@ -50,12 +50,10 @@ namespace {
 
 using CastFn = decltype(&sr_block_cast);
 using MatmulFn = decltype(&sr_block_matmul);
-using MatmulWorkspaceFn = decltype(&sr_block_matmul_workspace);
 using OrthogonalizeFn = decltype(&sr_orthogonalize);
 using WorkspaceFn = decltype(&sr_orthogonalize_workspace);
 CastFn g_cast = nullptr;
 MatmulFn g_matmul = nullptr;
-MatmulWorkspaceFn g_matmul_workspace = nullptr;
 OrthogonalizeFn g_orthogonalize = nullptr;
 WorkspaceFn g_workspace = nullptr;
 PyObject* g_out_of_memory = nullptr;  // torch.OutOfMemoryError
@@ -218,11 +216,7 @@ at::Tensor matmul(const Scaled& a, const Scaled& b, int out_code, at::Tensor out
     if (out_code < 0) out_code = SR_BF16;
     out = at::empty({m, n}, options.dtype(scalar_type(out_code)));
   }
-  if (m && n) {
-    at::Tensor workspace;
-    if (const int64_t size = g_matmul_workspace(m, n, k)) workspace = at::empty({size}, options.dtype(c10::ScalarType::Byte));
-    checked(g_matmul(&left, &right, k, memory(out), stride, out_code, workspace.defined() ? memory(workspace) : nullptr, stream));
-  }
+  if (m && n) checked(g_matmul(&left, &right, k, memory(out), stride, out_code, stream));
   return out;
 }
 
@@ -236,7 +230,7 @@ at::Tensor as_rows(const at::Tensor& x) {
   return flat;
 }
 
-bool bound() { return g_cast && g_matmul && g_matmul_workspace && g_orthogonalize && g_workspace; }
+bool bound() { return g_cast && g_matmul && g_orthogonalize && g_workspace; }
 
 // Runs `body` as the entries promise; nullptr with an exception set, the
 // status, or what `result` makes of the outcome.
@@ -299,11 +293,10 @@ PyObject* wrap_all(std::initializer_list<const at::Tensor*> tensors) {
 }
 
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long cast, matmul, matmul_workspace, orthogonalize, workspace;
-  if (!PyArg_ParseTuple(args, "KKKKK", &cast, &matmul, &matmul_workspace, &orthogonalize, &workspace)) return nullptr;
+  unsigned long long cast, matmul, orthogonalize, workspace;
+  if (!PyArg_ParseTuple(args, "KKKK", &cast, &matmul, &orthogonalize, &workspace)) return nullptr;
   g_cast = reinterpret_cast<CastFn>(address(cast));
   g_matmul = reinterpret_cast<MatmulFn>(address(matmul));
-  g_matmul_workspace = reinterpret_cast<MatmulWorkspaceFn>(address(matmul_workspace));
   g_orthogonalize = reinterpret_cast<OrthogonalizeFn>(address(orthogonalize));
   g_workspace = reinterpret_cast<WorkspaceFn>(address(workspace));
   if (!bound()) {

@@ -7,9 +7,9 @@ namespace {
 
 template <int XE, int QE>
 void fill(const void* (&k)[kCastKinds]) {
-  k[kCastRowBlocks] = reinterpret_cast<const void*>(&block_cast_kernel<XE, QE, false>);
-  k[kCastSquare] = reinterpret_cast<const void*>(&block_cast_kernel<XE, QE, true>);
-  k[kCastSplit] = reinterpret_cast<const void*>(&block_cast_split_kernel<XE, QE>);
+  k[kCastParts] = reinterpret_cast<const void*>(&block_cast_parts_kernel<XE, QE>);
+  k[kCastWhole] = reinterpret_cast<const void*>(&block_cast_tile_kernel<XE, QE, false>);
+  k[kCastSquare] = reinterpret_cast<const void*>(&block_cast_tile_kernel<XE, QE, true>);
 }
 
 template <int XE>

@@ -12,15 +12,27 @@ namespace sr {
 // ---------------------------------------------------------------------------
 // Cast to FP8 with a power of two for each block of 128.
 //
-// A workgroup takes a 128 x 128 tile of x into registers, so that one read
-// serves both orientations.  Sixteen lanes share a row, eight values each (one
-// 16-byte load of BF16): a row's maximum is four rotations inside them.  A
-// thread holds four neighbouring rows of each 64-row band; the columns' maxima
-// cross LDS once, and the encoded bytes of the transposed orientation are
-// turned 4 x 4 in registers and cross it once.  Rows leave as 128 bytes of
-// sixteen lanes, columns as 128 bytes of 32.
+// Sixteen lanes share a row, eight values each (one 16-byte load of BF16): its
+// maximum is four rotations inside them.  Blocks along the columns need
+// 128 rows: a thread holds four neighbouring ones, the columns' maxima cross LDS
+// once, and the encoded bytes are turned 4 x 4 in registers and cross it
+// once.  Rows leave as 128 bytes of sixteen lanes, columns as 128 bytes of 32.
+//
+// Three kernels:
+//   square   square blocks: both orientations hold the same bytes
+//   whole    both orientations of a tile from one read of it, with one hash for
+//            each value
+//   parts    workgroups of one orientation each, smaller than a tile: for one
+//            orientation alone, and for both of so few tiles that the chip's CUs
+//            would idle (measured, nearest: 128 tiles 5.4 us against 6.2, 256
+//            tiles 7.5 against 6.9; stochastic 256 tiles 12.1 against 9.6)
+//
+// 8192 x 2048 BF16, 67 MB with both results (13 us at a copy's rate): whole 17 us
+// nearest, 24 stochastic, square 14.4; rows alone 11, 15.  The stochastic
+// ones are bound by arithmetic, half of it the hash (31 operations for a value
+// of both orientations, of which the hash is 17).
 // ---------------------------------------------------------------------------
-constexpr int kCastTile = 128, kCastThreads = 256;
+constexpr int kCastTile = 128;
 
 struct BlockCastArgs {
   const char* x;
@@ -28,7 +40,7 @@ struct BlockCastArgs {
   sr_block_output by_rows, by_cols;
   uint32_t counter_base;  // seed + offset (mod 2^32)
   uint32_t tiles_n;       // blocks of 128 columns
-  uint32_t row_groups;    // block_cast_split_kernel: workgroups of the row orientation
+  uint32_t first;         // the launch's first workgroup
 };
 
 // The format of encoding QE.
@@ -130,8 +142,7 @@ __device__ __forceinline__ void hash_eight(uint32_t counter, uint32_t (&hash)[2]
 // rule is an addition: the random bits as far below the format's last bit as
 // FP32 has bits, and a truncation, after which the convert is exact.  The
 // general rule takes the rest (4% of the waves' groups of normally
-// distributed values for stochastic E4M3, none for the others); 8192 x 2048
-// in both orientations took 34 us with it alone.
+// distributed values for stochastic E4M3, next to none for the others).
 template <int QE>
 __device__ __forceinline__ uint32_t encode_scaled(const float (&y)[4], const uint32_t (&hash)[4], bool finite) {
   using F = typename CastFormat<QE>::F;
@@ -199,51 +210,41 @@ __device__ __forceinline__ int live_of(T at, T end, int width) {
 }
 
 // The tile of 128 rows and 8 LANES columns from (row0, col0), by a workgroup
-// of 256 threads: groups of LANES threads share rows, four neighbouring ones in
-// each of BANDS bands.
+// of 32 LANES threads, of which LANES share four neighbouring rows.
 template <int XE, int QE, bool SQUARE, int LANES>
 __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, int64_t col0, bool want_rows, bool want_cols) {
-  constexpr int kGroups = kCastThreads / LANES, kBands = kCastTile / (4 * kGroups), kCols = 8 * LANES;
+  constexpr int kGroups = 32, kThreads = kGroups * LANES, kCols = 8 * LANES;
   constexpr int kTurn = 32 / LANES;
   __shared__ uint32_t turned[kCols * 32];
   __shared__ __align__(16) uint32_t partial[SQUARE ? 1 : kGroups][kCols];
   __shared__ __align__(16) int exponents[kCols];
-  __shared__ uint32_t whole[4];
+  __shared__ uint32_t whole[kThreads / 64];
   const int t = threadIdx.x, group = t / LANES, lane = t % LANES;
-  const int64_t c = col0 + 8 * lane;
+  const int64_t r0 = row0 + 4 * group, c = col0 + 8 * lane;
   const int live = live_of(c, a.cols, 8);
 
-  // Rows of this thread: band k, row 4 (kGroups k + group) + i.
-  float x[kBands][4][8];
+  float x[4][8];
 #pragma unroll
-  for (int k = 0; k < kBands; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t r = row0 + 4 * (kGroups * k + group) + i;
-      load_eight<XE>(a.x + (r * a.ldx + c) * enc_bytes(XE), r < a.rows ? live : 0, x[k][i]);
-    }
+  for (int i = 0; i < 4; ++i)
+    load_eight<XE>(a.x + ((r0 + i) * a.ldx + c) * enc_bytes(XE), r0 + i < a.rows ? live : 0, x[i]);
 
   uint32_t m[8] = {}, any = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
 #pragma unroll
-    for (int k = 0; k < kBands; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; i += 2) m[j] = umax(umax(m[j], magnitude(x[k][i][j])), magnitude(x[k][i + 1][j]));
+    for (int i = 0; i < 4; i += 2) m[j] = umax(umax(m[j], magnitude(x[i][j])), magnitude(x[i + 1][j]));
     any = umax(any, m[j]);
   }
   const bool finite = any < kInfBits;
   int tile_exp = 0;  // SQUARE
-  int col_exp[8];    // of this thread's columns
-  if (SQUARE || want_cols) {
+  int col_exp[8];    // otherwise, of this thread's columns
+  {
     if (!finite) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         m[j] = 0;
 #pragma unroll
-        for (int k = 0; k < kBands; ++k)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) m[j] = umax(m[j], finite_magnitude(x[k][i][j]));
+        for (int i = 0; i < 4; ++i) m[j] = umax(m[j], finite_magnitude(x[i][j]));
       }
     }
     if constexpr (SQUARE) {
@@ -255,9 +256,9 @@ __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, 
       tile = umax(tile, __shfl_xor(tile, 32));
       if ((t & 63) == 0) whole[t >> 6] = tile;
       __syncthreads();
-      tile_exp = block_exponent<QE>(umax(umax(whole[0], whole[1]), umax(whole[2], whole[3])));
 #pragma unroll
-      for (int j = 0; j < 8; ++j) col_exp[j] = tile_exp;
+      for (int w = 0; w < kThreads / 64; ++w) tile = umax(tile, whole[w]);
+      tile_exp = block_exponent<QE>(tile);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) partial[group][8 * lane + j] = m[j];
@@ -276,64 +277,58 @@ __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, 
     }
   }
 
+  uint32_t by_col[2][4];
 #pragma unroll
-  for (int k = 0; k < kBands; ++k) {
-    if (row0 + 4 * kGroups * k >= a.rows && !want_cols) break;
-    uint32_t by_col[2][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t r = row0 + 4 * (kGroups * k + group) + i;
-      uint32_t hash[2][4], words[2];
-      hash_eight<QE>(a.counter_base + static_cast<uint32_t>(r) * static_cast<uint32_t>(a.cols) + static_cast<uint32_t>(c), hash);
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = r0 + i;
+    uint32_t hash[2][4], words[2];
+    hash_eight<QE>(a.counter_base + static_cast<uint32_t>(r) * static_cast<uint32_t>(a.cols) + static_cast<uint32_t>(c), hash);
+    if constexpr (SQUARE) {
+      encode_row<QE>(x[i], tile_exp, hash, finite, words);
+      if (want_rows && r < a.rows) store_eight(static_cast<char*>(a.by_rows.data) + r * a.by_rows.ld + c, words, live);
+    } else {
       if (want_rows) {
-        int e = tile_exp;
-        if constexpr (!SQUARE) e = block_exponent<QE>(max_of_16(largest(x[k][i], finite)));
-        encode_row<QE>(x[k][i], e, hash, finite, words);
+        const int e = block_exponent<QE>(max_of_16(largest(x[i], finite)));
+        encode_row<QE>(x[i], e, hash, finite, words);
         if (r < a.rows) {
           store_eight(static_cast<char*>(a.by_rows.data) + r * a.by_rows.ld + c, words, live);
-          if (!SQUARE && lane == 0) store_exponent(a.by_rows, r, col0 / kCastTile, e);
+          if (lane == 0) store_exponent(a.by_rows, r, col0 / kCastTile, e);
         }
       }
-      if (want_cols) {
-        if (SQUARE && want_rows) {  // the same bytes
-          by_col[0][i] = words[0];
-          by_col[1][i] = words[1];
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] = x[k][i][4 * h + j] * inverse_scale(col_exp[4 * h + j]);
-            by_col[h][i] = encode_scaled<QE>(y, hash[h], finite);
-          }
-        }
-      }
-    }
-    if (want_cols) {
-      // Column 8 lane + j, rows 4 (kGroups k + group) .. + 3, at word (row / 4) ^ (kTurn lane) of its column's 32: the
-      // lanes of a wave then meet in a bank two at a time, and those that read a column below do not.
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        transpose_bytes(by_col[h]);
+        float y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          turned[(8 * lane + 4 * h + j) * 32 + ((kGroups * k + group) ^ (kTurn * lane))] = by_col[h][j];
+        for (int j = 0; j < 4; ++j) y[j] = x[i][4 * h + j] * inverse_scale(col_exp[4 * h + j]);
+        words[h] = encode_scaled<QE>(y, hash[h], finite);
       }
     }
+    by_col[0][i] = words[0];
+    by_col[1][i] = words[1];
+  }
+  if constexpr (SQUARE) {
+    if (t == 0) {
+      if (want_rows) store_exponent(a.by_rows, row0 / kCastTile, col0 / kCastTile, tile_exp);
+      if (want_cols) store_exponent(a.by_cols, col0 / kCastTile, row0 / kCastTile, tile_exp);
+    }
+    if (!want_cols) return;
   }
 
-  if (SQUARE && t == 0) {
-    if (want_rows) store_exponent(a.by_rows, row0 / kCastTile, col0 / kCastTile, tile_exp);
-    if (want_cols) store_exponent(a.by_cols, col0 / kCastTile, row0 / kCastTile, tile_exp);
+  // Column 8 lane + j, rows r0 .. r0 + 3, at word group ^ (kTurn lane) of its column's 32: the lanes of a wave then
+  // meet in a bank two at a time, and those that read a column below do not.
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    transpose_bytes(by_col[h]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) turned[(8 * lane + 4 * h + j) * 32 + (group ^ (kTurn * lane))] = by_col[h][j];
   }
-  if (!want_cols) return;
   __syncthreads();
-  const int word_at = t & 31, half = t >> 5;
+  const int word_at = t & 31, part = t >> 5;
   const int64_t r = row0 + 4 * word_at;
   const int live_r = live_of(r, a.rows, 4);
 #pragma unroll
-  for (int k = 0; k < kCols / 8; ++k) {
-    const int col = 8 * k + half;
+  for (int k = 0; k < kCols * 32 / kThreads; ++k) {
+    const int col = kThreads / 32 * k + part;
     if (col0 + col >= a.cols) break;
     const uint32_t word = turned[col * 32 + (word_at ^ (kTurn * (col >> 3)))];
     char* q = static_cast<char*>(a.by_cols.data) + (col0 + col) * a.by_cols.ld + r;
@@ -347,30 +342,36 @@ __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, 
   }
 }
 
+constexpr int kTileThreads = 512, kPartThreads = 256;
+constexpr uint64_t kWholeTiles = 256;  // see above
+
 template <int XE, int QE, bool SQUARE>
-__global__ __launch_bounds__(kCastThreads) void block_cast_kernel(BlockCastArgs a) {
-  cast_tile<XE, QE, SQUARE, 16>(a, static_cast<int64_t>(blockIdx.x / a.tiles_n) * kCastTile,
-                                static_cast<int64_t>(blockIdx.x % a.tiles_n) * kCastTile, a.by_rows.data != nullptr,
-                                a.by_cols.data != nullptr);
+__global__ __launch_bounds__(kTileThreads, SQUARE ? 6 : 4) void block_cast_tile_kernel(BlockCastArgs a) {
+  const uint32_t tile = a.first + blockIdx.x;
+  cast_tile<XE, QE, SQUARE, 16>(a, static_cast<int64_t>(tile / a.tiles_n) * kCastTile,
+                              static_cast<int64_t>(tile % a.tiles_n) * kCastTile, a.by_rows.data != nullptr,
+                              a.by_cols.data != nullptr);
 }
 
-// Few tiles: each orientation by workgroups of its own, which read x twice but
-// are many.  Of the row orientation a workgroup takes 16 rows of 128
-// columns, of the other one 128 rows of 64 columns.
-constexpr int kSplitRows = kCastThreads / 16, kSplitLanes = 8;
-constexpr uint64_t kSplitBelow = 256;  // tiles
+// The workgroups of a band of 128 rows: where the row orientation is asked
+// for, eight times tiles_n of 16 rows x 128 columns, along the rows first; then
+// two times tiles_n of 64 columns.
+constexpr int kPartRows = kPartThreads / 16, kPartLanes = 8;
+constexpr int kRowParts = kCastTile / kPartRows, kColParts = kCastTile / (8 * kPartLanes);
 
 template <int XE, int QE>
-__global__ __launch_bounds__(kCastThreads) void block_cast_split_kernel(BlockCastArgs a) {
-  if (blockIdx.x >= a.row_groups) {
-    const uint32_t id = blockIdx.x - a.row_groups, tiles = 2 * a.tiles_n;
-    cast_tile<XE, QE, false, kSplitLanes>(a, static_cast<int64_t>(id / tiles) * kCastTile,
-                                          static_cast<int64_t>(id % tiles) * 8 * kSplitLanes, false, true);
+__global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void block_cast_parts_kernel(BlockCastArgs a) {
+  const uint32_t row_parts = a.by_rows.data ? kRowParts : 0, parts = row_parts + (a.by_cols.data ? kColParts : 0);
+  const uint32_t id = a.first + blockIdx.x, band = id / (parts * a.tiles_n), within = id - band * parts * a.tiles_n;
+  const int64_t row0 = static_cast<int64_t>(band) * kCastTile;
+  if (within >= row_parts * a.tiles_n) {
+    cast_tile<XE, QE, false, kPartLanes>(a, row0, static_cast<int64_t>(within - row_parts * a.tiles_n) * 8 * kPartLanes, false, true);
     return;
   }
+  const uint32_t part = within / a.tiles_n;
+  const int64_t block = within - part * a.tiles_n;
   const int lane = threadIdx.x & 15;
-  const int64_t r = static_cast<int64_t>(blockIdx.x / a.tiles_n) * kSplitRows + (threadIdx.x >> 4);
-  const int64_t block = blockIdx.x % a.tiles_n, c = block * kCastTile + 8 * lane;
+  const int64_t r = row0 + kPartRows * part + (threadIdx.x >> 4), c = block * kCastTile + 8 * lane;
   if (r >= a.rows) return;  // sixteen lanes together
   const int live = live_of(c, a.cols, 8);
   float x[8];

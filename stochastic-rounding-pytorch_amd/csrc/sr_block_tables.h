@@ -29,8 +29,7 @@ struct BlockProductKernels {
 };
 // [A is E5M2][B is E5M2][ProductMode]
 using BlockProductTable = BlockProductKernels[2][2][3];
-// Casts with blocks of one row by whole tiles, with square blocks, and with blocks of one row by orientation.
-enum BlockCastKind { kCastRowBlocks, kCastSquare, kCastSplit, kCastKinds };
+enum BlockCastKind { kCastParts, kCastWhole, kCastSquare, kCastKinds };
 // [FP32, BF16, FP16 input][E4M3 nearest, stochastic, E5M2 nearest, stochastic][kind]
 using BlockCastTable = const void* [3][4][kCastKinds];
 

@@ -1,6 +1,8 @@
 // sr_matrix_abi.hip -- extern "C" entry points of the block-scaled operators (sr_matrix_hip.h).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "../../include/sr_matrix_hip.h"
 #include "sr_block_scaled.h"
 #include "sr_block_tables.h"
@@ -92,20 +94,22 @@ int sr_block_cast(const void* x, int64_t ldx, int64_t rows, int64_t cols, int x_
   a.cols = cols;
   a.counter_base = seed + offset;
   a.tiles_n = static_cast<uint32_t>(blocks(cols));
-  const auto& kinds = casts()[x_dtype == SR_F32 ? 0 : (x_dtype == SR_BF16 ? 1 : 2)][2 * (dtype == SR_E5M2) + (rule == SR_STOCHASTIC)];
   const uint64_t tiles = static_cast<uint64_t>(blocks(rows)) * a.tiles_n;
-  if (!square && tiles < sr::kSplitBelow) {
-    const int64_t rows_groups = (rows + sr::kSplitRows - 1) / sr::kSplitRows * a.tiles_n;
-    a.row_groups = a.by_rows.data ? static_cast<uint32_t>(rows_groups) : 0;
-    return launch(kinds[sr::kCastSplit], a.row_groups + (a.by_cols.data ? 2 * tiles : 0), sr::kCastThreads, &a, stream);
+  const bool rows_too = a.by_rows.data, cols_too = a.by_cols.data;
+  const sr::BlockCastKind kind = square ? sr::kCastSquare : (rows_too && cols_too && tiles >= sr::kWholeTiles ? sr::kCastWhole : sr::kCastParts);
+  const void* fn = casts()[x_dtype == SR_F32 ? 0 : (x_dtype == SR_BF16 ? 1 : 2)][2 * (dtype == SR_E5M2) + (rule == SR_STOCHASTIC)][kind];
+  const uint64_t groups = tiles * (kind == sr::kCastParts ? sr::kRowParts * rows_too + sr::kColParts * cols_too : 1);
+  if (groups > 0xFFFFFFFFu) return fail(SR_ERR_ARGUMENT, "%lld x %lld matrix", (long long)rows, (long long)cols);
+  constexpr uint64_t kLaunch = 0x7FFFFF / 2;  // a launch has fewer than 2^32 threads
+  for (uint64_t first = 0; first < groups; first += kLaunch) {
+    a.first = static_cast<uint32_t>(first);
+    if (int rc = launch(fn, std::min(kLaunch, groups - first), kind == sr::kCastParts ? sr::kPartThreads : sr::kTileThreads, &a, stream)) return rc;
   }
-  return launch(kinds[square ? sr::kCastSquare : sr::kCastRowBlocks], tiles, sr::kCastThreads, &a, stream);
+  return SR_OK;
 }
 
-int64_t sr_block_matmul_workspace(int64_t, int64_t, int64_t) { return 0; }
-
 int sr_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t k, void* out, int64_t ldo,
-                    int out_dtype, void* workspace, void* stream) {
+                    int out_dtype, void* stream) {
   if (k < 0 || k > kMaxLd) return fail(SR_ERR_ARGUMENT, "%lld contracted values", (long long)k);
   if (int rc = check_matrix(a, "a", k)) return rc;
   if (int rc = check_matrix(b, "b", k)) return rc;

@@ -186,9 +186,8 @@ MATRIX_SIGNATURES = {
     ),
     "sr_block_matmul": (
         _int,
-        [ctypes.POINTER(BlockMatrix), ctypes.POINTER(BlockMatrix), _i64, _vp, _i64, _int, _vp, _vp],
+        [ctypes.POINTER(BlockMatrix), ctypes.POINTER(BlockMatrix), _i64, _vp, _i64, _int, _vp],
     ),
-    "sr_block_matmul_workspace": (_i64, [_i64, _i64, _i64]),
     "sr_orthogonalize_workspace": (_i64, [_i64, _i64, _i64]),
     "sr_orthogonalize": (
         _int,
@@ -322,8 +321,7 @@ def matrix():
 
         lib = library()
         module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                      for name in ("sr_block_cast", "sr_block_matmul", "sr_block_matmul_workspace", "sr_orthogonalize",
-                                   "sr_orthogonalize_workspace")))
+                      for name in ("sr_block_cast", "sr_block_matmul", "sr_orthogonalize", "sr_orthogonalize_workspace")))
         _matrix = module
     return _matrix
 

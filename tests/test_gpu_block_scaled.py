@@ -82,6 +82,18 @@ def test_cast_of_special_values(cuda, dtype, square):
             _assert_cast(got, x, dtype, rule, square, axis, 1)
 
 
+@pytest.mark.parametrize("x_dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype, rule", [(E4M3, "nearest"), (E4M3, "stochastic"), (E5M2, "nearest"), (E5M2, "stochastic")])
+def test_cast_of_many_blocks_in_both_orientations(cuda, x_dtype, dtype, rule):
+    x = torch.empty(2050, 2101, device=cuda, dtype=x_dtype).copy_(_spread((2050, 2101), cuda, 6))
+    x[5, 7], x[600, 1300], x[600, 1301], x[2049, 2100] = float("nan"), float("inf"), -float("inf"), float("nan")
+    x[128:256, 256:384] = 0
+    x[300:400, 100] *= 2.0**-12
+    by_rows, by_cols = sr_states.block_cast(x, dtype=dtype, axis=(1, 0), rounding=rule, seed=4)
+    _assert_cast(by_rows, x, dtype, rule, False, 1, 4)
+    _assert_cast(by_cols, x, dtype, rule, False, 0, 4)
+
+
 def test_cast_is_the_plain_cast_of_the_scaled_values(cuda):
     x = _spread((64, 256), cuda, 8)
     got = sr_states.block_cast(x, seed=21)

@@ -59,7 +59,7 @@ def test_invalid_arguments_fail_before_any_device_work():
     good = _matrix()
 
     def matmul(a=good, b=good, k=128, out=1 << 20, ldo=4, dtype=_lib.SR_BF16):
-        return lib.sr_block_matmul(a, b, k, out, ldo, dtype, None, None)
+        return lib.sr_block_matmul(a, b, k, out, ldo, dtype, None)
 
     for call, message in [
         (lambda: matmul(a=_matrix(dtype=_lib.SR_BF16)), b"E4M3 or E5M2"),
