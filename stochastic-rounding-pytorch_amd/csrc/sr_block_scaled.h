@@ -491,20 +491,20 @@ __device__ __forceinline__ float e8m0_value(uint32_t byte) {
   return bits_f32(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7FC00000u : byte << 23));
 }
 
-// The scales of a workgroup's rows, 32 bytes of each at a time (32 exponent
-// bytes or 8 FP32 factors), in LDS beside the stages.  Read from memory stage
-// by stage they would cost more than they weigh: the scales of one stage lie in a
-// cache line of their own for every row, and an access to 64 lines takes
-// 64 cycles (measured at 8192 x 8192 x 2048 on 128 x 128 tiles: 202 us with a
-// load per fragment and stage, 144 so).
-// Rows are 36 bytes apart: 32 rows' same bytes then lie in different banks.
-template <class S>
+// The scales of a workgroup's rows, 32 bytes of each at a time, in LDS beside
+// the stages: 32 exponent bytes where the instructions take them, else 8 FP32
+// factors.  Read from memory stage by stage they would cost more than they
+// weigh: the scales of one stage lie in a cache line of their own for every
+// row, and an access to 64 lines takes 64 cycles (measured at
+// 8192 x 8192 x 2048 on 128 x 128 tiles: 202 us with a load per fragment and
+// stage, 144 so).  Rows are 36 bytes apart: 32 rows' same bytes then lie in
+// different banks.
+template <int MODE, class S>
 struct ScaleArea {
   static constexpr int kRow = 36, kFill = 32, kBytes = (S::BM + S::BN) * kRow;
+  static constexpr int kPeriod = MODE == kExponents ? kFill : kFill / 4;
 
-  static __device__ __forceinline__ int period(const BlockProductArgs& g) { return g.scale_f32 ? kFill / 4 : kFill; }
-
-  // Blocks [first, first + period) of every row; rows past the end repeat the last one.
+  // Blocks [first, first + kPeriod) of every row; rows past the end repeat the last one.
   static __device__ void fill(char* area, const BlockProductArgs& g, int row0, int col0, int first, int total) {
     const int size = g.scale_f32 ? 4 : 1;
     for (int r = threadIdx.x; r < S::BM + S::BN; r += S::kThreads) {
@@ -513,8 +513,14 @@ struct ScaleArea {
       const char* from = (of_a ? g.scale_a : g.scale_b) +
                          (((at < rows ? at : rows - 1) >> (of_a ? g.shift_a : g.shift_b)) * (of_a ? g.ld_scale_a : g.ld_scale_b) + first) * size;
       const int64_t end = static_cast<int64_t>(total - first) * size;
-      const i32x4 lo = load_chunk(from, 0, end), hi = load_chunk(from, 16, end);
       int* to = reinterpret_cast<int*>(area + r * kRow);
+      const i32x4 lo = load_chunk(from, 0, end);
+      if (MODE == kWide && !g.scale_f32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) to[j] = static_cast<int>(f32_bits(e8m0_value(lo[j >> 2] >> (8 * (j & 3)) & 255)));
+        continue;
+      }
+      const i32x4 hi = load_chunk(from, 16, end);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         to[j] = lo[j];
@@ -534,24 +540,27 @@ struct Scales {
   using Value = std::conditional_t<kExp, int, float>;
   Value a[MI], b[NI][kPerB];
 
+  // From memory, in the matrices' own type.
   static __device__ __forceinline__ Value read(const char* p, bool f32) {
     if constexpr (kExp) return *reinterpret_cast<const uint8_t*>(p);
     else if constexpr (MODE == kFactors) return *reinterpret_cast<const float*>(p);
     else return f32 ? *reinterpret_cast<const float*>(p) : e8m0_value(*reinterpret_cast<const uint8_t*>(p));
   }
 
-  // `wave_m`, `wave_n`: this wave's first rows of A and B in the area; `slot`: the block's place in a row.
+  // From the area.  `wave_m`, `wave_n`: this wave's first rows of A and B in it; `slot`: the block's place in a row.
   template <class S>
-  __device__ __forceinline__ void load(const char* area, int wave_m, int wave_n, int slot, bool f32, int lane) {
-    const char* at = area + (f32 ? 4 * slot : slot);
-    const char* pa = at + (wave_m + (lane & 15)) * ScaleArea<S>::kRow;
-    const char* pb = at + (S::BM + wave_n + (kExp ? lane & 15 : 4 * (lane >> 4))) * ScaleArea<S>::kRow;
+  __device__ __forceinline__ void load(const char* area, int wave_m, int wave_n, int slot, int lane) {
+    using T = std::conditional_t<kExp, uint8_t, float>;
+    constexpr int kRow = ScaleArea<MODE, S>::kRow;
+    const char* at = area + slot * sizeof(T);
+    const char* pa = at + (wave_m + (lane & 15)) * kRow;
+    const char* pb = at + (S::BM + wave_n + (kExp ? lane & 15 : 4 * (lane >> 4))) * kRow;
 #pragma unroll
-    for (int i = 0; i < MI; ++i) a[i] = read(pa + i * 16 * ScaleArea<S>::kRow, f32);
+    for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const T*>(pa + i * 16 * kRow);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int j = 0; j < kPerB; ++j) b[i][j] = read(pb + (i * 16 + j) * ScaleArea<S>::kRow, f32);
+      for (int j = 0; j < kPerB; ++j) b[i][j] = *reinterpret_cast<const T*>(pb + (i * 16 + j) * kRow);
   }
 };
 
@@ -610,7 +619,8 @@ __device__ __forceinline__ void block_mma(f32x4& acc, const Fragment<MODE, FA>& 
 template <int MODE, int FA, int FB, class S, bool ASYNC>
 __global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void block_product_kernel(BlockProductArgs g) {
   static_assert(ASYNC || S::kGroups == 1, "groups take aligned rows");
-  constexpr int kStages = S::kLds + ScaleArea<S>::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
+  using Area = ScaleArea<MODE, S>;
+  constexpr int kStages = S::kLds + Area::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
   constexpr int kLds = kStages > kChunks ? kStages : kChunks;
   static_assert(S::kSums <= kLds, "the groups' sums");
   __shared__ __align__(1024) char lds[kLds];
@@ -625,14 +635,13 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void block
   stager.init(g.a, g.b, row0, col0, wave, lane);
   char* own = lds + group * 2 * S::kStage;  // this group's stages
   char* area = lds + S::kLds;
-  const int period = ScaleArea<S>::period(g);
 
   f32x4 acc[S::MI][S::NI] = {};
   const uint32_t fragment = fragment_offset(lane);
   const int stages = static_cast<int>((g.k + kStageBytes - 1) / kStageBytes);
   auto multiply = [&](const char* stage, int kt) {
     Scales<MODE, S::MI, S::NI> scales;
-    scales.template load<S>(area, wave_m, wave_n, kt & (period - 1), g.scale_f32, lane);
+    scales.template load<S>(area, wave_m, wave_n, kt & (Area::kPeriod - 1), lane);
     const char* sa = stage + wave_m * kStageBytes + fragment;
     const char* sb = stage + (S::BM + wave_n) * kStageBytes + fragment;
     const char* sa2 = stage + wave_m * kStageBytes + (fragment ^ 64);
@@ -651,8 +660,8 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void block
   };
 
   auto refill = [&](int kt) {
-    if ((kt & (period - 1)) == 0) {
-      ScaleArea<S>::fill(area, g, row0, col0, kt, stages);
+    if ((kt & (Area::kPeriod - 1)) == 0) {
+      Area::fill(area, g, row0, col0, kt, stages);
       lds_barrier();
     }
   };
@@ -669,24 +678,30 @@ __global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void block
       if (group == 0) multiply(lds, whole);
     }
   } else {
-    // Two sets of registers, so that a stage's loads have two stages' time.
-    i32x4 even[S::kLoads], odd[S::kLoads];
+    // Two sets of registers, so that a stage's loads have two stages' time, where they are small enough (of the 128
+    // tile, with FP16 instructions, two did not fit: 4096 x 4096 x 1000 took 129 us so).
+    constexpr bool kTwo = S::kLoads <= 4;
+    i32x4 even[S::kLoads], odd[kTwo ? S::kLoads : 1];
     auto load = [&](i32x4 (&regs)[S::kLoads], int kt) {
       if (kt < stages) stager.load(regs, static_cast<int64_t>(kt) * kStageBytes, g.k, wave, lane);
     };
     auto step = [&](int kt, i32x4 (&next)[S::kLoads], i32x4 (&after)[S::kLoads]) {
       lds_barrier();
       refill(kt);
-      load(after, kt + 2);
+      load(after, kTwo ? kt + 2 : kt + 1);
       multiply(lds + (kt & 1) * S::kStage, kt);
       if (kt + 1 < stages) stager.store(lds + (~kt & 1) * S::kStage, next, wave, lane);
     };
     load(even, 0);
-    load(odd, 1);
+    if constexpr (kTwo) load(odd, 1);
     if (stages > 0) stager.store(lds, even, wave, lane);
-    for (int kt = 0; kt < stages; kt += 2) {
-      step(kt, odd, even);
-      if (kt + 1 < stages) step(kt + 1, even, odd);
+    if constexpr (kTwo) {
+      for (int kt = 0; kt < stages; kt += 2) {
+        step(kt, odd, even);
+        if (kt + 1 < stages) step(kt + 1, even, odd);
+      }
+    } else {
+      for (int kt = 0; kt < stages; ++kt) step(kt, even, even);
     }
   }
   stage_barrier();
