@@ -38,7 +38,7 @@ constexpr float kNsScale = 8192.0f, kNsInverse = 1.0f / 8192.0f;  // 2^13
 constexpr float kNsProduct = kNsInverse * kNsInverse;             // of a product of two scaled operands
 constexpr float kNsShift = 1.5f;
 constexpr int kNsPad = 64;        // rows and columns of the workspace are padded to it
-constexpr int kNsPartials = 512;  // partial sums of squares per matrix
+constexpr int kNsPartials = 1024; // partial sums of squares per matrix
 constexpr int kNsThreads = 256;
 
 // The matrices of one launch.
@@ -54,6 +54,7 @@ struct NsArgs {
   int m, n;        // padded: m <= n, X is m x n, transposed where rows > cols
   int tall;
   int partials;    // partial sums per matrix in use
+  int keep;        // the first kernel writes V
   float a, b, c, eps;
   float* x;
   _Float16* h;
@@ -76,9 +77,35 @@ __device__ __forceinline__ float group_sum(float v, float* scratch) {
   return scratch[0] + scratch[1] + scratch[2] + scratch[3];
 }
 
-// Reads the gradients (GE) and, with UE >= 0, updates the momenta; leaves V in
-// FP32, in the workspace's orientation, and partial sums of its squares.
-// 64 x 64 tiles, of which a workgroup takes every gridDim.x-th.
+// Four consecutive values of a row with encoding E, the first `live` of them
+// there; zeros for the rest.
+template <int E>
+__device__ __forceinline__ f32x4 load_four(const void* from, int64_t i, int live) {
+  f32x4 v{};
+  if (live == 4) {
+    uint32_t w[group_words(E)];
+    float r[4];
+    load_group<E>(from, i, w);
+    decode_group<E>(w, r);
+    v = f32x4{r[0], r[1], r[2], r[3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      if (j < live) v[j] = decode<E>(load1<E>(from, i + j));
+  }
+  return v;
+}
+
+// How many of the columns col .. col + 3 of row `row` the caller's matrices have.
+__device__ __forceinline__ int live_four(const NsArgs& a, int row, int col) {
+  return row >= a.rows || col >= a.cols ? 0 : (a.cols - col < 4 ? a.cols - col : 4);
+}
+
+// Partial sums of the squares of V, which is the gradient (GE) or, with
+// UE >= 0, what the momentum update makes of it; V itself in FP32, in the
+// workspace's orientation, where a.keep asks for it.  64 x 64 tiles, of which a
+// workgroup takes every gridDim.x-th; a tile's loads come before its stores,
+// which might change what a later load reads for all that the compiler knows.
 template <int GE, int UE>
 __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTable t) {
   __shared__ float turned[kNsPad][kNsPad + 1];
@@ -92,65 +119,49 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTab
   float sum = 0.0f;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int r0 = tile / tiles_c * kNsPad, c = tile % tiles_c * kNsPad + tc;
-    const int live = c >= a.cols ? 0 : (a.cols - c < 4 ? a.cols - c : 4);
+    f32x4 v[4], old[4];
 #pragma unroll
     for (int pass = 0; pass < 4; ++pass) {
       const int r = r0 + 16 * pass + tr;
       const int64_t i = static_cast<int64_t>(r) * a.cols + c;
-      float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if (r < a.rows && live) {
-        float gv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const bool full = live == 4;
-        if (full) {
-          uint32_t w[group_words(GE)];
-          load_group<GE>(g, i, w);
-          decode_group<GE>(w, gv);
-        } else {
+      v[pass] = load_four<GE>(g, i, live_four(a, r, c));
+      if constexpr (UE >= 0) old[pass] = load_four<UE>(u, i, live_four(a, r, c));
+    }
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < live) gv[j] = decode<GE>(load1<GE>(g, i + j));
+    for (int pass = 0; pass < 4; ++pass) {
+      const int r = r0 + 16 * pass + tr;
+      if constexpr (UE >= 0) {
+        const int64_t i = static_cast<int64_t>(r) * a.cols + c;
+        const uint32_t counter = t.counter[matrix] + static_cast<uint32_t>(i);
+        const int live = live_four(a, r, c);
+        float uv[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float gv = v[pass][j];
+          uv[j] = old[pass][j] * a.momentum + gv;
+          v[pass][j] = j < live ? (a.nesterov ? uv[j] * a.momentum + gv : uv[j]) : 0.0f;
         }
-        if constexpr (UE < 0) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[j] = gv[j];
-        } else {
-          float uv[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-          const uint32_t counter = t.counter[matrix] + static_cast<uint32_t>(i);
+        if (live == 4) {
           uint32_t w[group_words(UE)];
-          if (full) {
-            load_group<UE>(u, i, w);
-            decode_group<UE>(w, uv);
-          } else {
+          encode_group<UE>(uv, counter, w);
+          store_group<UE>(u, i, w);
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j < live) uv[j] = decode<UE>(load1<UE>(u, i + j));
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uv[j] = uv[j] * a.momentum + gv[j];
-            v[j] = a.nesterov ? uv[j] * a.momentum + gv[j] : uv[j];
-          }
-          if (full) {
-            encode_group<UE>(uv, counter, w);
-            store_group<UE>(u, i, w);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (j < live) store1<UE>(u, i + j, encode<UE>(uv[j], counter + static_cast<uint32_t>(j)));
-              else v[j] = 0.0f;
-          }
+          for (int j = 0; j < 3; ++j)
+            if (j < live) store1<UE>(u, i + j, encode<UE>(uv[j], counter + static_cast<uint32_t>(j)));
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fmaf(v[j], v[j], sum);
+      for (int j = 0; j < 4; ++j) sum = fmaf(v[pass][j], v[pass][j], sum);
+      if (!a.keep) continue;
       if (a.tall) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) turned[tc + j][16 * pass + tr] = v[j];
+        for (int j = 0; j < 4; ++j) turned[tc + j][16 * pass + tr] = v[pass][j];
       } else {
-        *reinterpret_cast<f32x4*>(x + static_cast<int64_t>(r) * a.n + c) = f32x4{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<f32x4*>(x + static_cast<int64_t>(r) * a.n + c) = v[pass];
       }
     }
-    if (a.tall) {
+    if (a.keep && a.tall) {
       __syncthreads();
 #pragma unroll
       for (int pass = 0; pass < 4; ++pass) {
@@ -165,74 +176,78 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTab
   if (threadIdx.x == 0) a.partial[matrix * kNsPartials + blockIdx.x] = sum;
 }
 
-// X = V / (|V|_F + eps) and its FP16 copies H and H^T, one 64 x 64 tile per workgroup.
-__global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a) {
-  __shared__ _Float16 turned[kNsPad][kNsPad + 8];
+// X = V / (|V|_F + eps) and its FP16 copies H and H^T, one 64 x 64 tile per
+// workgroup.  V comes from the caller's matrices (GE), which is less to read
+// and spares writing it in FP32 first (8192 x 2048 BF16: 14 us for the sum and 36
+// for the rest, 40 and 31 the other way), or with
+// GE < 0 from X.
+template <int GE>
+__global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTable t) {
+  __shared__ float turned[kNsPad][kNsPad + 1];
   __shared__ float scratch[4];
   const int matrix = blockIdx.y;
-  const float* partial = a.partial + matrix * kNsPartials;
-  float sum = 0.0f;
-  for (int i = threadIdx.x; i < a.partials; i += kNsThreads) sum += partial[i];
-  const float norm = sqrtf(group_sum(sum, scratch)) + a.eps;
   const int64_t base = static_cast<int64_t>(matrix) * a.m * a.n;
   float* x = a.x + base;
   _Float16* h = a.h + base;
   _Float16* ht = a.ht_next + base;
-  const int tiles_n = a.n / kNsPad;
-  const int r0 = blockIdx.x / tiles_n * kNsPad, c0 = blockIdx.x % tiles_n * kNsPad;
+  const bool flip = GE >= 0 && a.tall;  // V's tiles lie as H^T's
+  const int tiles_c = (flip ? a.m : a.n) / kNsPad;
+  const int r0 = blockIdx.x / tiles_c * kNsPad, c0 = blockIdx.x % tiles_c * kNsPad;
   const int tr = threadIdx.x >> 4, tc = 4 * (threadIdx.x & 15);
+  f32x4 v[4];
 #pragma unroll
   for (int pass = 0; pass < 4; ++pass) {
-    const int64_t i = static_cast<int64_t>(r0 + 16 * pass + tr) * a.n + c0 + tc;
-    f32x4 v = *reinterpret_cast<const f32x4*>(x + i);
+    const int r = r0 + 16 * pass + tr, c = c0 + tc;
+    if constexpr (GE >= 0)
+      v[pass] = load_four<GE>(reinterpret_cast<const void*>(t.g[matrix]), static_cast<int64_t>(r) * a.cols + c, live_four(a, r, c));
+    else
+      v[pass] = *reinterpret_cast<const f32x4*>(x + static_cast<int64_t>(r) * a.n + c);
+  }
+  const float* partial = a.partial + matrix * kNsPartials;
+  float sum = 0.0f;
+  for (int i = threadIdx.x; i < a.partials; i += kNsThreads) sum += partial[i];
+  const float norm = sqrtf(group_sum(sum, scratch)) + a.eps;
+  auto store_x = [&](int row, int col, const f32x4& y, const f16x4& w) {
+    const int64_t i = static_cast<int64_t>(row) * a.n + col;
+    *reinterpret_cast<f32x4*>(x + i) = y;
+    *reinterpret_cast<f16x4*>(h + i) = w;
+  };
+  auto store_turned = [&](int row, int col, const f16x4& w) {
+    *reinterpret_cast<f16x4*>(ht + static_cast<int64_t>(row) * a.m + col) = w;
+  };
+  auto halves = [](const f32x4& y) {
     f16x4 w;
 #pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = static_cast<_Float16>(y[j] * kNsScale);
+    return w;
+  };
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int row = 16 * pass + tr;
+#pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[j] = v[j] / norm;
-      w[j] = static_cast<_Float16>(v[j] * kNsScale);
-      turned[tc + j][16 * pass + tr] = w[j];
+      v[pass][j] = v[pass][j] / norm;
+      turned[tc + j][row] = v[pass][j];
     }
-    *reinterpret_cast<f32x4*>(x + i) = v;
-    *reinterpret_cast<f16x4*>(h + i) = w;
+    if (flip) store_turned(r0 + row, c0 + tc, halves(v[pass]));
+    else store_x(r0 + row, c0 + tc, v[pass], halves(v[pass]));
   }
   __syncthreads();
 #pragma unroll
   for (int pass = 0; pass < 4; ++pass) {
     const int row = 16 * pass + tr;
-    *reinterpret_cast<f16x4*>(ht + static_cast<int64_t>(c0 + row) * a.m + r0 + tc) =
-        *reinterpret_cast<const f16x4*>(&turned[row][tc]);
+    const f32x4 y{turned[row][tc], turned[row][tc + 1], turned[row][tc + 2], turned[row][tc + 3]};
+    if (flip) store_x(c0 + row, r0 + tc, y, halves(y));
+    else store_turned(c0 + row, r0 + tc, halves(y));
   }
-}
-
-// Four consecutive values of row `row` of the parameter, in its orientation;
-// zeros outside.  Loads come apart from the stores below: between a store and a
-// load that might read it the compiler keeps their order, and each load would
-// wait for memory by itself.
-template <int E>
-__device__ __forceinline__ f32x4 load_parameter(const NsArgs& a, const void* p, int row, int col) {
-  f32x4 v{};
-  if (row >= a.rows || col >= a.cols) return v;
-  const int64_t i = static_cast<int64_t>(row) * a.cols + col;
-  if (a.cols - col >= 4) {
-    uint32_t w[group_words(E)];
-    float r[4];
-    load_group<E>(p, i, w);
-    decode_group<E>(w, r);
-    v = f32x4{r[0], r[1], r[2], r[3]};
-  } else {
-#pragma unroll
-    for (int j = 0; j < 3; ++j)
-      if (j < a.cols - col) v[j] = decode<E>(load1<E>(p, i + j));
-  }
-  return v;
 }
 
 // Stores four consecutive values of row `row` of the result with encoding E, or
 // (MUON) of the parameter, whose values were `old`, updated by them.
 template <int E, bool MUON>
 __device__ __forceinline__ void finish(const NsArgs& a, void* out, int row, int col, const f32x4& y, const f32x4& old) {
-  if (row >= a.rows || col >= a.cols) return;
-  const int live = a.cols - col < 4 ? a.cols - col : 4;
+  const int live = live_four(a, row, col);
+  if (!live) return;
   const int64_t i = static_cast<int64_t>(row) * a.cols + col;
   float r[4];
 #pragma unroll
@@ -335,7 +350,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
           old[i][k] = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
         else if constexpr (OP != kNsGram)
           old[i][k] = *reinterpret_cast<const f32x4*>(a.x + base + static_cast<int64_t>(row) * a.n + col);
-        if constexpr (MUON && !TURNED) parameter[i][k] = load_parameter<E>(a, result, row, col);
+        if constexpr (MUON && !TURNED) parameter[i][k] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
       }
 #pragma unroll
     for (int i = 0; i < Chunk::kBlocks; ++i) {
@@ -389,7 +404,10 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
       if constexpr (MUON) {
 #pragma unroll
         for (int i = 0; i < Chunk::kTurnedBlocks; ++i)
-          before[i] = load_parameter<E>(a, result, wave_col + Chunk::turned_col(i, lane), row0 + Chunk::turned_row(lane));
+          {
+          const int row = wave_col + Chunk::turned_col(i, lane), col = row0 + Chunk::turned_row(lane);
+          before[i] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
+        }
       }
 #pragma unroll
       for (int i = 0; i < Chunk::kTurnedBlocks; ++i)

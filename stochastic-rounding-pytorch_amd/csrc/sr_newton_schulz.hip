@@ -118,7 +118,9 @@ int run(NsArgs a, const sr::MatrixTable& t, int matrices, int g_dtype, int ue, c
 
   const int64_t tiles = static_cast<int64_t>(a.m / sr::kNsPad) * (a.n / sr::kNsPad);
   a.partials = static_cast<int>(tiles < sr::kNsPartials ? tiles : sr::kNsPartials);
-  const dim3 grid(a.partials, matrices);
+  const dim3 grid(a.partials, matrices), all(static_cast<uint32_t>(tiles), matrices);
+  const bool small = a.m == sr::kSmallRows && a.n <= sr::kSmallCols;
+  a.keep = ue >= 0 || small;
   if (ue < 0) {
     if (g_dtype == SR_F32) sr::ns_load_kernel<sr::ENC_F32, -1><<<grid, sr::kNsThreads, 0, s>>>(a, t);
     else if (g_dtype == SR_BF16) sr::ns_load_kernel<sr::ENC_BF16_RN, -1><<<grid, sr::kNsThreads, 0, s>>>(a, t);
@@ -129,12 +131,15 @@ int run(NsArgs a, const sr::MatrixTable& t, int matrices, int g_dtype, int ue, c
     load_momentum<sr::ENC_BF16_RN>(a, t, ue, grid, s);
   }
   if (int rc = launched("ns_load_kernel launch")) return rc;
-  if (a.m == sr::kSmallRows && a.n <= sr::kSmallCols) {
+  if (small) {
     sr::ns_small_kernel<<<matrices, sr::kSmallThreads, 0, s>>>(a, ns.steps, t);
     return launched("ns_small_kernel launch");
   }
   a.ht_next = turned[0];
-  sr::ns_scale_kernel<<<dim3(static_cast<uint32_t>(tiles), matrices), sr::kNsThreads, 0, s>>>(a);
+  if (ue >= 0) sr::ns_scale_kernel<-1><<<all, sr::kNsThreads, 0, s>>>(a, t);
+  else if (g_dtype == SR_F32) sr::ns_scale_kernel<sr::ENC_F32><<<all, sr::kNsThreads, 0, s>>>(a, t);
+  else if (g_dtype == SR_BF16) sr::ns_scale_kernel<sr::ENC_BF16_RN><<<all, sr::kNsThreads, 0, s>>>(a, t);
+  else sr::ns_scale_kernel<sr::ENC_F16_RN><<<all, sr::kNsThreads, 0, s>>>(a, t);
   if (int rc = launched("ns_scale_kernel launch")) return rc;
   for (int step = 0; step < ns.steps; ++step) {
     a.ht = turned[step & 1];
