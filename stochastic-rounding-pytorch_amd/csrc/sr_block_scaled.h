@@ -461,7 +461,8 @@ __device__ __forceinline__ void store_chunks(const BlockProductArgs& g, char* ld
   const int wave_row = row0 + wave / S::WN * S::kRowsM, wave_col = col0 + wave % S::WN * S::kRowsN;
   float* chunk = reinterpret_cast<float*>(lds + wave * Chunk::kBytes);
   with_output(g, row0, col0, S::BM, S::BN, [&](auto out, auto edge) {
-    for_each_chunk<S>(chunk, lane, acc, [&](int first, const float* from) {
+    for_each_chunk<S>(chunk, lane, acc, [&](auto number, const float* from) {
+      constexpr int first = 32 * decltype(number)::value;
 #pragma unroll
       for (int i = 0; i < Chunk::kBlocks; ++i)
 #pragma unroll

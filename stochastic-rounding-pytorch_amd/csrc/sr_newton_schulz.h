@@ -332,26 +332,61 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
   _Float16* out = (OP == kNsGram ? a.g : a.p) + square;  // kSymmetric
   void* result = reinterpret_cast<void*>(t.p[tile.matrix]);  // kNsLast
 
-  auto use = [&](int first, const float* from) {
-    // The workspace's sizes are multiples of 64, so a chunk of 32 x 32 or 32 x 64 is inside or outside as a whole.
-    const int row0 = wave_row + first;
-    if (row0 >= a.m || wave_col >= width) return;
-    const int col = wave_col + Chunk::block_col(lane);
-    // What the sums are combined with: G, or X and the parameter, of all of the lane's rows.
-    using Old = std::conditional_t<OP == kNsPolynomial, f16x4, f32x4>;
-    Old old[Chunk::kBlocks][4];
-    f32x4 parameter[Chunk::kBlocks][4];
+  // What the sums of a chunk are combined with: G, or X and the parameter, of all of the lane's rows.  A chunk's loads
+  // go out before the stores of the one before it: memory operations are waited for in their order, so that loads
+  // behind stores wait for these too (8192 x 2048: STORETIMES).
+  using Old = std::conditional_t<OP == kNsPolynomial, f16x4, f32x4>;
+  Old old[2][Chunk::kBlocks][4];
+  // (The registers of wide tiles do not hold two chunks of X and the parameter.)
+  constexpr bool kAhead = !(MUON && std::is_same_v<S, TileWide>);
+  f32x4 parameter[2][Chunk::kBlocks][4], across[2][Chunk::kTurnedBlocks];
+  constexpr int kChunks = S::kRowsM / 32;
+  // The workspace's sizes are multiples of 64, so a chunk of 32 x 32 or 32 x 64 is inside or outside as a whole.
+  auto inside = [&](int number) { return wave_row + 32 * number < a.m && wave_col < width; };
+  auto load = [&](int number) {
+    const bool in = inside(number);
+    const int row0 = in ? wave_row + 32 * number : 0, col = (in ? wave_col : 0) + Chunk::block_col(lane);
 #pragma unroll
     for (int i = 0; i < Chunk::kBlocks; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int row = row0 + Chunk::block_row(i, lane) + k;
         if constexpr (OP == kNsPolynomial)
-          old[i][k] = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
+          old[number & 1][i][k] = *reinterpret_cast<const f16x4*>(a.g + square + static_cast<int64_t>(row) * a.m + col);
         else if constexpr (OP != kNsGram)
-          old[i][k] = *reinterpret_cast<const f32x4*>(a.x + base + static_cast<int64_t>(row) * a.n + col);
-        if constexpr (MUON && !TURNED) parameter[i][k] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
+          old[number & 1][i][k] = *reinterpret_cast<const f32x4*>(a.x + base + static_cast<int64_t>(row) * a.n + col);
       }
+  };
+  auto load_parameter = [&](int number) {
+    const bool in = inside(number);
+    const int row0 = in ? wave_row + 32 * number : 0, col0 = in ? wave_col : 0;
+    if constexpr (MUON && TURNED) {
+#pragma unroll
+      for (int i = 0; i < Chunk::kTurnedBlocks; ++i) {
+        const int row = col0 + Chunk::turned_col(i, lane), col = row0 + Chunk::turned_row(lane);
+        across[number & 1][i] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
+      }
+    } else if constexpr (MUON) {
+      const int col = col0 + Chunk::block_col(lane);
+#pragma unroll
+      for (int i = 0; i < Chunk::kBlocks; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = row0 + Chunk::block_row(i, lane) + k;
+          parameter[number & 1][i][k] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
+        }
+    }
+  };
+
+  auto use = [&](auto number, const float* from) {
+    constexpr int kNumber = decltype(number)::value;
+    constexpr int kLoad = kAhead ? kNumber + 1 : kNumber;
+    if constexpr (kLoad < kChunks) {
+      load(kLoad);
+      load_parameter(kLoad);
+    }
+    if (!inside(kNumber)) return;
+    const int row0 = wave_row + 32 * kNumber, col = wave_col + Chunk::block_col(lane);
 #pragma unroll
     for (int i = 0; i < Chunk::kBlocks; ++i) {
       const int r0 = Chunk::block_row(i, lane);
@@ -367,7 +402,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
         } else if constexpr (OP == kNsPolynomial) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float p = fmaf(a.c * kNsInverse, v[j], a.b * static_cast<float>(old[i][k][j]));
+            const float p = fmaf(a.c * kNsInverse, v[j], a.b * static_cast<float>(old[kNumber & 1][i][k][j]));
             block[k][j] = static_cast<_Float16>(row == col + j ? p + kNsShift * kNsScale : p);
           }
           *reinterpret_cast<f16x4*>(out + static_cast<int64_t>(row) * a.m + col) = block[k];
@@ -375,7 +410,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
           f32x4 y;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float x = old[i][k][j], h = static_cast<float>(static_cast<_Float16>(x * kNsScale)) * kNsInverse;
+            const float x = old[kNumber & 1][i][k][j], h = static_cast<float>(static_cast<_Float16>(x * kNsScale)) * kNsInverse;
             y[j] = fmaf(v[j], kNsProduct, fmaf(-kNsShift, h, a.a * x));
           }
           if constexpr (OP == kNsStep) {
@@ -386,7 +421,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
             *reinterpret_cast<f16x4*>(a.h + at) = block[k];
           } else {
             block[k] = y;
-            if constexpr (!TURNED) finish<E, MUON>(a, result, row, col, y, parameter[i][k]);
+            if constexpr (!TURNED) finish<E, MUON>(a, result, row, col, y, parameter[kNumber & 1][i][k]);
           }
         }
       }
@@ -400,19 +435,10 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
       }
     }
     if constexpr (OP == kNsLast && TURNED) {
-      f32x4 before[Chunk::kTurnedBlocks];
-      if constexpr (MUON) {
-#pragma unroll
-        for (int i = 0; i < Chunk::kTurnedBlocks; ++i)
-          {
-          const int row = wave_col + Chunk::turned_col(i, lane), col = row0 + Chunk::turned_row(lane);
-          before[i] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
-        }
-      }
 #pragma unroll
       for (int i = 0; i < Chunk::kTurnedBlocks; ++i)
         finish<E, MUON>(a, result, wave_col + Chunk::turned_col(i, lane), row0 + Chunk::turned_row(lane),
-                        Chunk::template get_turned<T, T4>(turned, i, lane), before[i]);
+                        Chunk::template get_turned<T, T4>(turned, i, lane), across[kNumber & 1][i]);
     } else if constexpr (kTurns) {
       if (!kSymmetric || tile.mirrored) {
         _Float16* to = kSymmetric ? out : a.ht_next + base;
@@ -423,6 +449,10 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
       }
     }
   };
+  if constexpr (kAhead) {
+    load(0);
+    load_parameter(0);
+  }
   for_each_chunk<S>(chunk, lane, acc, use);
 }
 

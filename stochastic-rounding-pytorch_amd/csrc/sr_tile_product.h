@@ -416,8 +416,8 @@ struct ResultChunk {
 };
 
 // The 32-row chunks of a wave of S's results: for each, fills it from the
-// accumulators and calls use(first row, chunk) with the rows counted from the
-// wave's first.  16 x 16 tiles acc[MI][NI] of f32x4, or 32 x 32 ones of f32x16.
+// accumulators and calls use(its number, chunk), the number as a constant.
+// 16 x 16 tiles acc[MI][NI] of f32x4, or 32 x 32 ones of f32x16.
 // (Folds, not loops: accumulators live in registers only where every index is
 // known, and the unroller gives up on bodies this long.)
 template <class S, class F, int... C>
@@ -430,7 +430,7 @@ __device__ __forceinline__ void chunks_of(float* chunk, int lane, const f32x4 (&
 #pragma unroll
       for (int ni = 0; ni < S::NI; ++ni)
         Chunk::put(chunk, mi * 16 + (lane & 15), ni * 16 + 4 * (lane >> 4), acc[2 * C + mi][ni]);
-    use(32 * C, chunk);
+    use(std::integral_constant<int, C>{}, chunk);
   }(), ...);
 }
 
@@ -445,7 +445,7 @@ __device__ __forceinline__ void chunks_of(float* chunk, int lane, const f32x16 (
       for (int q = 0; q < 4; ++q)
         Chunk::put(chunk, lane & 31, ni * 32 + 8 * q + 4 * (lane >> 5),
                    f32x4{acc[C][ni][4 * q], acc[C][ni][4 * q + 1], acc[C][ni][4 * q + 2], acc[C][ni][4 * q + 3]});
-    use(32 * C, chunk);
+    use(std::integral_constant<int, C>{}, chunk);
   }(), ...);
 }
 
