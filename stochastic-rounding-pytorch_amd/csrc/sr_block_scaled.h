@@ -618,7 +618,7 @@ __device__ __forceinline__ void block_mma(f32x4& acc, const Fragment<MODE, FA>& 
 }
 
 template <int MODE, int FA, int FB, class S, bool ASYNC>
-__global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void block_product_kernel(BlockProductArgs g) {
+__global__ __launch_bounds__(S::kThreads, S::kMinWaves) void block_product_kernel(BlockProductArgs g) {
   static_assert(ASYNC || S::kGroups == 1, "groups take aligned rows");
   using Area = ScaleArea<MODE, S>;
   constexpr int kStages = S::kLds + Area::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;

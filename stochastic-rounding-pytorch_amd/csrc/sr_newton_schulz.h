@@ -77,28 +77,56 @@ __device__ __forceinline__ float group_sum(float v, float* scratch) {
   return scratch[0] + scratch[1] + scratch[2] + scratch[3];
 }
 
-// Four consecutive values of a row with encoding E, the first `live` of them
-// there; zeros for the rest.
+// How many of the columns col .. col + 3 of row `row` the caller's matrices have.
+__device__ __forceinline__ int live_four(const NsArgs& a, int row, int col) {
+  return row >= a.rows || col >= a.cols ? 0 : (a.cols - col < 4 ? a.cols - col : 4);
+}
+
+// The values of columns col .. col + 3 of row `row` of a matrix of the
+// caller's with encoding E; zeros outside.  Without a branch per lane, at whose
+// end each load would wait for memory by itself: what passes the edges is
+// read where it still fits and shifted (1023 x 767: 14 us with branches, 11 so).
 template <int E>
-__device__ __forceinline__ f32x4 load_four(const void* from, int64_t i, int live) {
+__device__ __forceinline__ f32x4 load_four(const NsArgs& a, const void* from, int row, int col) {
+  const int live = live_four(a, row, col);
   f32x4 v{};
-  if (live == 4) {
-    uint32_t w[group_words(E)];
-    float r[4];
-    load_group<E>(from, i, w);
-    decode_group<E>(w, r);
-    v = f32x4{r[0], r[1], r[2], r[3]};
-  } else {
+  if (a.cols < 4) {
 #pragma unroll
     for (int j = 0; j < 3; ++j)
-      if (j < live) v[j] = decode<E>(load1<E>(from, i + j));
+      if (j < live) v[j] = decode<E>(load1<E>(from, static_cast<int64_t>(row) * a.cols + col + j));
+    return v;
+  }
+  const int at_row = row < a.rows ? row : a.rows - 1, at_col = col < a.cols - 4 ? col : a.cols - 4, shift = col - at_col;
+  uint32_t w[group_words(E)];
+  float r[4];
+  load_group<E>(from, static_cast<int64_t>(at_row) * a.cols + at_col, w);
+  decode_group<E>(w, r);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float x = 0.0f;
+#pragma unroll
+    for (int s = 3; s >= 0; --s)
+      if (j + s < 4) x = shift == s ? r[j + s] : x;
+    v[j] = j < live ? x : 0.0f;
   }
   return v;
 }
 
-// How many of the columns col .. col + 3 of row `row` the caller's matrices have.
-__device__ __forceinline__ int live_four(const NsArgs& a, int row, int col) {
-  return row >= a.rows || col >= a.cols ? 0 : (a.cols - col < 4 ? a.cols - col : 4);
+// Loads what the kernel will need of its arguments at once: they may lie in
+// host memory, where each load that waits by itself costs a microsecond or two.
+__device__ __forceinline__ void need_arguments(const NsArgs& a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" ::"s"(a.m), "s"(a.n), "s"(a.a), "s"(a.b), "s"(a.c), "s"(a.x), "s"(a.h), "s"(a.ht), "s"(a.ht_next),
+               "s"(a.g), "s"(a.p));
+#endif
+}
+
+__device__ __forceinline__ void need_arguments(const NsArgs& a, const MatrixTable& t, int matrix) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" ::"s"(a.m), "s"(a.n), "s"(a.rows), "s"(a.cols), "s"(a.tall), "s"(a.keep), "s"(a.partials), "s"(a.eps),
+               "s"(a.x), "s"(a.h), "s"(a.ht_next), "s"(a.partial), "s"(a.momentum), "s"(a.nesterov), "s"(t.g[matrix]),
+               "s"(t.u[matrix]), "s"(t.counter[matrix]));
+#endif
 }
 
 // Partial sums of the squares of V, which is the gradient (GE) or, with
@@ -111,6 +139,7 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTab
   __shared__ float turned[kNsPad][kNsPad + 1];
   __shared__ float scratch[4];
   const int matrix = blockIdx.y;
+  need_arguments(a, t, matrix);
   const void* g = reinterpret_cast<const void*>(t.g[matrix]);
   void* u = reinterpret_cast<void*>(t.u[matrix]);
   float* x = a.x + static_cast<int64_t>(matrix) * a.m * a.n;
@@ -123,9 +152,8 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTab
 #pragma unroll
     for (int pass = 0; pass < 4; ++pass) {
       const int r = r0 + 16 * pass + tr;
-      const int64_t i = static_cast<int64_t>(r) * a.cols + c;
-      v[pass] = load_four<GE>(g, i, live_four(a, r, c));
-      if constexpr (UE >= 0) old[pass] = load_four<UE>(u, i, live_four(a, r, c));
+      v[pass] = load_four<GE>(a, g, r, c);
+      if constexpr (UE >= 0) old[pass] = load_four<UE>(a, u, r, c);
     }
 #pragma unroll
     for (int pass = 0; pass < 4; ++pass) {
@@ -186,6 +214,7 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTa
   __shared__ float turned[kNsPad][kNsPad + 1];
   __shared__ float scratch[4];
   const int matrix = blockIdx.y;
+  need_arguments(a, t, matrix);
   const int64_t base = static_cast<int64_t>(matrix) * a.m * a.n;
   float* x = a.x + base;
   _Float16* h = a.h + base;
@@ -199,14 +228,14 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTa
   for (int pass = 0; pass < 4; ++pass) {
     const int r = r0 + 16 * pass + tr, c = c0 + tc;
     if constexpr (GE >= 0)
-      v[pass] = load_four<GE>(reinterpret_cast<const void*>(t.g[matrix]), static_cast<int64_t>(r) * a.cols + c, live_four(a, r, c));
+      v[pass] = load_four<GE>(a, reinterpret_cast<const void*>(t.g[matrix]), r, c);
     else
       v[pass] = *reinterpret_cast<const f32x4*>(x + static_cast<int64_t>(r) * a.n + c);
   }
   const float* partial = a.partial + matrix * kNsPartials;
   float sum = 0.0f;
   for (int i = threadIdx.x; i < a.partials; i += kNsThreads) sum += partial[i];
-  const float norm = sqrtf(group_sum(sum, scratch)) + a.eps;
+  const float inverse = 1.0f / (sqrtf(group_sum(sum, scratch)) + a.eps);
   auto store_x = [&](int row, int col, const f32x4& y, const f16x4& w) {
     const int64_t i = static_cast<int64_t>(row) * a.n + col;
     *reinterpret_cast<f32x4*>(x + i) = y;
@@ -226,7 +255,7 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTa
     const int row = 16 * pass + tr;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[pass][j] = v[pass][j] / norm;
+      v[pass][j] *= inverse;
       turned[tc + j][row] = v[pass][j];
     }
     if (flip) store_turned(r0 + row, c0 + tc, halves(v[pass]));
@@ -261,15 +290,6 @@ __device__ __forceinline__ void finish(const NsArgs& a, void* out, int row, int 
     for (int j = 0; j < 4; ++j)
       if (j < live) store1<E>(out, i + j, encode<E>(r[j], 0u));
   }
-}
-
-// Loads what the kernel will need of its arguments at once: they may lie in
-// host memory, where each load that waits by itself costs a microsecond or two.
-__device__ __forceinline__ void need_arguments(const NsArgs& a) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("" ::"s"(a.m), "s"(a.n), "s"(a.a), "s"(a.b), "s"(a.c), "s"(a.x), "s"(a.h), "s"(a.ht), "s"(a.ht_next),
-               "s"(a.g), "s"(a.p));
-#endif
 }
 
 enum NsOp { kNsGram, kNsPolynomial, kNsStep, kNsLast };
@@ -334,7 +354,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
 
   // What the sums of a chunk are combined with: G, or X and the parameter, of all of the lane's rows.  A chunk's loads
   // go out before the stores of the one before it: memory operations are waited for in their order, so that loads
-  // behind stores wait for these too (8192 x 2048: STORETIMES).
+  // behind stores wait for these too.
   using Old = std::conditional_t<OP == kNsPolynomial, f16x4, f32x4>;
   Old old[2][Chunk::kBlocks][4];
   // (The registers of wide tiles do not hold two chunks of X and the parameter.)
@@ -364,7 +384,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
 #pragma unroll
       for (int i = 0; i < Chunk::kTurnedBlocks; ++i) {
         const int row = col0 + Chunk::turned_col(i, lane), col = row0 + Chunk::turned_row(lane);
-        across[number & 1][i] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
+        across[number & 1][i] = load_four<E>(a, result, row, col);
       }
     } else if constexpr (MUON) {
       const int col = col0 + Chunk::block_col(lane);
@@ -373,7 +393,7 @@ __device__ __forceinline__ void ns_store(const NsArgs& a, const MatrixTable& t, 
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int row = row0 + Chunk::block_row(i, lane) + k;
-          parameter[number & 1][i][k] = load_four<E>(result, static_cast<int64_t>(row) * a.cols + col, live_four(a, row, col));
+          parameter[number & 1][i][k] = load_four<E>(a, result, row, col);
         }
     }
   };
@@ -488,7 +508,7 @@ __device__ __forceinline__ void with_result(const NsArgs& a, F&& store) {
 //   kNsLast        the same into the results or the parameters; TURNED where
 //                  these are the transpose of the workspace's orientation
 template <int OP, class S, bool TURNED>
-__global__ __launch_bounds__(S::kThreads, S::kThreads <= 512 ? 2 : 4) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
+__global__ __launch_bounds__(S::kThreads, S::kMinWaves) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
                                                                     uint32_t tiles, uint32_t matrices, MatrixTable t) {
   constexpr int kLds = ns_lds<OP, TURNED, S>(S::kLds);
   static_assert(S::kSums <= kLds, "the groups' sums");

@@ -54,6 +54,7 @@ struct TileShape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int kWaves = WM * WN;                         // of one group
   static constexpr int kThreads = 64 * kWaves * kGroups;
+  static constexpr int kMinWaves = kThreads <= 512 ? 2 : (kWaves * kGroups + 3) / 4;  // of a SIMD, for its registers
   static constexpr int kRowsM = BM / WM, kRowsN = BN / WN;      // of one wave
   static constexpr int MI = kRowsM / 16, NI = kRowsN / 16;      // its 16x16 tiles
   static constexpr int kStage = (BM + BN) * kStageBytes;        // bytes of one LDS stage

@@ -43,6 +43,14 @@ def test_orthogonalize_equals_the_definition(cuda, shape, x_dtype):
     assert oracle.relative(got, oracle.orthogonalize(x)) < LIMIT
 
 
+@pytest.mark.parametrize("shape", [(2003, 2101), (2101, 2003), (8, 1101, 2050), (8, 2050, 1101), (24, 640, 700)])
+def test_orthogonalize_of_many_tiles(cuda, shape):
+    x = _matrix(shape, cuda, 2, torch.bfloat16)
+    got = sr_states.orthogonalize(x, dtype=torch.float32)
+    for g, one in zip(got.view(-1, *shape[-2:])[::5], x.view(-1, *shape[-2:])[::5]):
+        assert oracle.relative(g, oracle.orthogonalize(one)) < LIMIT
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
 def test_orthogonalize_result_types(cuda, dtype):
     for shape in ((96, 130), (130, 96), (50, 20)):
@@ -173,6 +181,18 @@ def test_step_types_shapes_and_options(cuda, p_dtype, g_dtype, shape, nesterov, 
     u, want, size = _expected(p, g, m, **HYPER, nesterov=nesterov, update_scale=update_scale)
     stored = sr_states.cast(u, dtype=torch.bfloat16, seed=sr_states.state_key(5, 0))
     sr_states.hip_muon_step_(p, g, m, **HYPER, nesterov=nesterov, update_scale=update_scale, seed=5)
+    assert torch.equal(m, stored)
+    _assert_parameter(p, want, size)
+
+
+@pytest.mark.parametrize("p_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1023, 767), (767, 1023), (4099, 4170), (4170, 4099)])
+def test_step_of_large_tensors(cuda, p_dtype, shape):
+    p, g = _matrix(shape, cuda, 1, p_dtype, 0.05), _matrix(shape, cuda, 2, p_dtype, 0.1)
+    m = _matrix(shape, cuda, 3, torch.bfloat16, 0.3)
+    u, want, size = _expected(p, g, m, **HYPER, nesterov=True, update_scale="spectral")
+    stored = sr_states.cast(u, dtype=torch.bfloat16, seed=sr_states.state_key(5, 0))
+    sr_states.hip_muon_step_(p, g, m, **HYPER, nesterov=True, update_scale="spectral", seed=5)
     assert torch.equal(m, stored)
     _assert_parameter(p, want, size)
 
