@@ -388,7 +388,18 @@ __global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void bloc
 }
 
 // ---------------------------------------------------------------------------
-// Product of two block-scaled matrices.
+// Product of two block-scaled matrices: out = sum over blocks of
+// scale_a scale_b (sum over the block of a b).
+//
+// Both operands have the contracted axis last, so that a stage, 128 bytes of
+// every row of a tile, is one scaled block of each row and one 16x16x128
+// instruction per 16 x 16 results.  Tiles of 128 x 128 results and of 64 x 64
+// (see tile_by_count); rows of at most 16 take the kernel at the end.
+//
+// Large products are bound by the card's power: 8192 x 8192 x 2048 takes 146 us
+// (1880 TFLOP/s) in a kernel by itself and 175 us call after call, alike with
+// 256 x 256 tiles.  Small ones are bound by latency: 4.3 us of arguments, first
+// stage and result, then 0.5 to 1 us a stage (501 x 2304 x 768: 6.7 us).
 // ---------------------------------------------------------------------------
 struct BlockProductArgs {
   Operand a, b;
@@ -713,7 +724,8 @@ __global__ __launch_bounds__(S::kThreads, S::kMinWaves) void block_product_kerne
 // Few rows of A (at most 16): one 16-column tile of the result per workgroup,
 // whose waves take the blocks of the contracted axis in turn and add their
 // sums through LDS in wave order.  The operands go from memory to registers:
-// each byte of B is used once.
+// each byte of B is used once.  1 x 8192 x 2048 takes 5.5 us (3.1 TB/s of B), of
+// which a launch and its arguments are about 3.
 constexpr int kRowWaves = 8;
 
 template <int MODE, int FA, int FB>

@@ -38,8 +38,9 @@ constexpr float kNsScale = 8192.0f, kNsInverse = 1.0f / 8192.0f;  // 2^13
 constexpr float kNsProduct = kNsInverse * kNsInverse;             // of a product of two scaled operands
 constexpr float kNsShift = 1.5f;
 constexpr int kNsPad = 64;        // rows and columns of the workspace are padded to it
-constexpr int kNsPartials = 1024; // partial sums of squares per matrix
+constexpr int kNsPartials = 512;  // partial sums of squares per matrix
 constexpr int kNsThreads = 256;
+constexpr int kNsLoadThreads = 512;
 
 // The matrices of one launch.
 struct MatrixTable {
@@ -68,13 +69,17 @@ struct NsArgs {
   int muon, out_dtype;  // last step: update p in out_dtype, or store the result
 };
 
-// Sum over the workgroup's 256 threads, in a fixed order; valid in thread 0.
+// Sum over the workgroup's THREADS threads, in a fixed order; the same in all of them.
+template <int THREADS>
 __device__ __forceinline__ float group_sum(float v, float* scratch) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
   __syncthreads();
-  return scratch[0] + scratch[1] + scratch[2] + scratch[3];
+  v = scratch[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) v += scratch[w];
+  return v;
 }
 
 // How many of the columns col .. col + 3 of row `row` the caller's matrices have.
@@ -85,7 +90,7 @@ __device__ __forceinline__ int live_four(const NsArgs& a, int row, int col) {
 // The values of columns col .. col + 3 of row `row` of a matrix of the
 // caller's with encoding E; zeros outside.  Without a branch per lane, at whose
 // end each load would wait for memory by itself: what passes the edges is
-// read where it still fits and shifted (1023 x 767: 14 us with branches, 11 so).
+// read where it still fits and shifted (1023 x 767 took 3 us longer with branches).
 template <int E>
 __device__ __forceinline__ f32x4 load_four(const NsArgs& a, const void* from, int row, int col) {
   const int live = live_four(a, row, col);
@@ -135,9 +140,10 @@ __device__ __forceinline__ void need_arguments(const NsArgs& a, const MatrixTabl
 // workgroup takes every gridDim.x-th; a tile's loads come before its stores,
 // which might change what a later load reads for all that the compiler knows.
 template <int GE, int UE>
-__global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTable t) {
+__global__ __launch_bounds__(kNsLoadThreads) void ns_load_kernel(NsArgs a, MatrixTable t) {
   __shared__ float turned[kNsPad][kNsPad + 1];
-  __shared__ float scratch[4];
+  __shared__ float scratch[kNsLoadThreads / 64];
+  constexpr int kRows = kNsLoadThreads / 16, kPasses = kNsPad / kRows;
   const int matrix = blockIdx.y;
   need_arguments(a, t, matrix);
   const void* g = reinterpret_cast<const void*>(t.g[matrix]);
@@ -148,16 +154,16 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTab
   float sum = 0.0f;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int r0 = tile / tiles_c * kNsPad, c = tile % tiles_c * kNsPad + tc;
-    f32x4 v[4], old[4];
+    f32x4 v[kPasses], old[kPasses];
 #pragma unroll
-    for (int pass = 0; pass < 4; ++pass) {
-      const int r = r0 + 16 * pass + tr;
+    for (int pass = 0; pass < kPasses; ++pass) {
+      const int r = r0 + kRows * pass + tr;
       v[pass] = load_four<GE>(a, g, r, c);
       if constexpr (UE >= 0) old[pass] = load_four<UE>(a, u, r, c);
     }
 #pragma unroll
-    for (int pass = 0; pass < 4; ++pass) {
-      const int r = r0 + 16 * pass + tr;
+    for (int pass = 0; pass < kPasses; ++pass) {
+      const int r = r0 + kRows * pass + tr;
       if constexpr (UE >= 0) {
         const int64_t i = static_cast<int64_t>(r) * a.cols + c;
         const uint32_t counter = t.counter[matrix] + static_cast<uint32_t>(i);
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTab
       if (!a.keep) continue;
       if (a.tall) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) turned[tc + j][16 * pass + tr] = v[pass][j];
+        for (int j = 0; j < 4; ++j) turned[tc + j][kRows * pass + tr] = v[pass][j];
       } else {
         *reinterpret_cast<f32x4*>(x + static_cast<int64_t>(r) * a.n + c) = v[pass];
       }
@@ -192,23 +198,23 @@ __global__ __launch_bounds__(kNsThreads) void ns_load_kernel(NsArgs a, MatrixTab
     if (a.keep && a.tall) {
       __syncthreads();
 #pragma unroll
-      for (int pass = 0; pass < 4; ++pass) {
-        const int row = 16 * pass + tr;
+      for (int pass = 0; pass < kPasses; ++pass) {
+        const int row = kRows * pass + tr;
         *reinterpret_cast<f32x4*>(x + static_cast<int64_t>(c - tc + row) * a.n + r0 + tc) =
             f32x4{turned[row][tc], turned[row][tc + 1], turned[row][tc + 2], turned[row][tc + 3]};
       }
       __syncthreads();
     }
   }
-  sum = group_sum(sum, scratch);
+  sum = group_sum<kNsLoadThreads>(sum, scratch);
   if (threadIdx.x == 0) a.partial[matrix * kNsPartials + blockIdx.x] = sum;
 }
 
 // X = V / (|V|_F + eps) and its FP16 copies H and H^T, one 64 x 64 tile per
 // workgroup.  V comes from the caller's matrices (GE), which is less to read
-// and spares writing it in FP32 first (8192 x 2048 BF16: 14 us for the sum and 36
-// for the rest, 40 and 31 the other way), or with
-// GE < 0 from X.
+// and spares writing it in FP32 first, or with GE < 0 from X.  Bound by memory:
+// 8192 x 2048 BF16 takes 16 us for the sum and 36 for the rest (161 MB, 4.5
+// TB/s); 40 and 31 where the first wrote V for the second.
 template <int GE>
 __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTable t) {
   __shared__ float turned[kNsPad][kNsPad + 1];
@@ -235,7 +241,7 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTa
   const float* partial = a.partial + matrix * kNsPartials;
   float sum = 0.0f;
   for (int i = threadIdx.x; i < a.partials; i += kNsThreads) sum += partial[i];
-  const float inverse = 1.0f / (sqrtf(group_sum(sum, scratch)) + a.eps);
+  const float inverse = 1.0f / (sqrtf(group_sum<kNsThreads>(sum, scratch)) + a.eps);
   auto store_x = [&](int row, int col, const f32x4& y, const f16x4& w) {
     const int64_t i = static_cast<int64_t>(row) * a.n + col;
     *reinterpret_cast<f32x4*>(x + i) = y;
@@ -507,6 +513,9 @@ __device__ __forceinline__ void with_result(const NsArgs& a, F&& store) {
 //   kNsStep        X <- a X - s H + (P + s I) H, and the new H and H^T
 //   kNsLast        the same into the results or the parameters; TURNED where
 //                  these are the transpose of the workspace's orientation
+// Few tiles are bound by the latency of a tile's walk (768 x 2304: G 12.5 us, P
+// 6.9, step 11.9), many by what a CU reads from its L2 (G of 8 x 2048 x 2048
+// 109 us, 710 TFLOP/s of the computed half and diagonal).
 template <int OP, class S, bool TURNED>
 __global__ __launch_bounds__(S::kThreads, S::kMinWaves) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
                                                                     uint32_t tiles, uint32_t matrices, MatrixTable t) {
@@ -555,7 +564,9 @@ __global__ __launch_bounds__(S::kThreads, S::kMinWaves) void ns_product_kernel(N
   });
 }
 
-// The same launches on wide tiles.
+// The same launches on wide tiles.  The step of 8192 x 2048 takes 91 us: 51 for
+// the product (1355 TFLOP/s) and the rest for 192 MB of X, H and H^T at 4.6
+// TB/s.
 template <int OP, bool TURNED>
 __global__ __launch_bounds__(TileWide::kThreads, 2) void ns_wide_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
                                                                         uint32_t tiles, uint32_t matrices, MatrixTable t) {

@@ -41,7 +41,7 @@ template <int GE>
 void load_momentum(const NsArgs& a, const sr::MatrixTable& t, int ue, dim3 grid, hipStream_t s) {
   switch (ue) {
 #define SR_CASE(E) \
-  case sr::E: sr::ns_load_kernel<GE, sr::E><<<grid, sr::kNsThreads, 0, s>>>(a, t); break;
+  case sr::E: sr::ns_load_kernel<GE, sr::E><<<grid, sr::kNsLoadThreads, 0, s>>>(a, t); break;
     SR_CASE(ENC_F32)
     SR_CASE(ENC_BF16_RN)
     SR_CASE(ENC_BF16_SR)
@@ -128,9 +128,9 @@ int run(NsArgs a, const sr::MatrixTable& t, int matrices, int g_dtype, int ue, c
   const bool small = a.m == sr::kSmallRows && a.n <= sr::kSmallCols;
   a.keep = ue >= 0 || small;
   if (ue < 0) {
-    if (g_dtype == SR_F32) sr::ns_load_kernel<sr::ENC_F32, -1><<<grid, sr::kNsThreads, 0, s>>>(a, t);
-    else if (g_dtype == SR_BF16) sr::ns_load_kernel<sr::ENC_BF16_RN, -1><<<grid, sr::kNsThreads, 0, s>>>(a, t);
-    else sr::ns_load_kernel<sr::ENC_F16_RN, -1><<<grid, sr::kNsThreads, 0, s>>>(a, t);
+    if (g_dtype == SR_F32) sr::ns_load_kernel<sr::ENC_F32, -1><<<grid, sr::kNsLoadThreads, 0, s>>>(a, t);
+    else if (g_dtype == SR_BF16) sr::ns_load_kernel<sr::ENC_BF16_RN, -1><<<grid, sr::kNsLoadThreads, 0, s>>>(a, t);
+    else sr::ns_load_kernel<sr::ENC_F16_RN, -1><<<grid, sr::kNsLoadThreads, 0, s>>>(a, t);
   } else if (g_dtype == SR_F32) {
     load_momentum<sr::ENC_F32>(a, t, ue, grid, s);
   } else {
