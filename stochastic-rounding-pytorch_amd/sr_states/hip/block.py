@@ -174,8 +174,10 @@ def _linear_codes(formats):
 
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, codes, seed):
-        need_x, need_w = ctx.needs_input_grad[:2]
+    def forward(ctx, x, weight, codes, seed, recorded):
+        # needs_input_grad says which tensors require gradients in every grad mode, and the mode is always off in here:
+        # `recorded` is the caller's.
+        need_x, need_w = (recorded and need for need in ctx.needs_input_grad[:2])
         seeds = tuple(state_key(seed, k) for k in range(3))
         # The weight gradient contracts the tokens, so it needs the input's blocks along them; the input gradient
         # contracts the weight's rows, and its square blocks only turn.
@@ -192,7 +194,7 @@ class _BlockLinear(torch.autograd.Function):
         out = _lib.matrix().linear_backward(dy, *ctx.saved_tensors, *ctx.options, _stream(dy.device))
         if not isinstance(out, tuple):
             _lib.check("block_linear", out)
-        return *out, None, None
+        return *out, None, None, None
 
 
 def block_linear(
@@ -218,7 +220,8 @@ def block_linear(
     nearest for the first two and stochastic for the gradient.  Tensor k of
     that order uses the random stream ``state_key(seed, k)``, so ``seed`` should
     be an update key that differs by layer and step (:func:`sr_states.update_key`).
-    Only the FP8 copies are kept for the backward pass.
+    Only the FP8 copies are kept for the backward pass; without grad mode
+    those that it alone would need are not made.
     """
     try:
         codes = _LINEAR_CODES[formats]
@@ -234,4 +237,4 @@ def block_linear(
     if x.device.type != "cuda" or weight.device != x.device:
         raise ValueError("x and weight must be on the same GPU device")
     _device_of(x, weight)
-    return _BlockLinear.apply(x, weight, codes, _lib.low32(seed))
+    return _BlockLinear.apply(x, weight, codes, _lib.low32(seed), torch.is_grad_enabled())
