@@ -498,6 +498,36 @@ __device__ __forceinline__ void store_chunks(const BlockProductArgs& g, char* ld
 // takes the FP16 instructions (4e-8) at half the rate.
 enum ProductMode { kExponents, kFactors, kWide, kProductModes };
 
+// A block's sum times two FP32 scales.  It lies between 2^-32 and 2^39 or is 0,
+// but the scales' product, or that of the sum and one scale, can leave FP32's range
+// on the way to a result inside it (2^100 by 2^30 with a small sum gave infinity,
+// with a sum of 0 NaN).  Scales between 2^-62 and 2^62, and zeros, are `near`:
+// their product is safe, and one multiplication and the fused one into the result do.  With others each
+// scale is taken as two factors of about half its exponent.  With T the
+// result's exponent and S the sum's, both partial products below are then
+// near 2^((T + S) / 2) and 2^((T - S) / 2): inside the range wherever 2^T is.
+__device__ __forceinline__ bool near_scale(uint32_t bits) {
+  const uint32_t a = bits & 0x7FFFFFFFu;
+  return a == 0 || a - (65u << 23) < (124u << 23);
+}
+
+// The power of two with half the exponent of `s`, rounded down; subnormal numbers, infinities and NaN count as 2^-127
+// and 2^128.
+__device__ __forceinline__ uint32_t half_power_bits(float s) { return (((f32_bits(s) >> 23 & 255u) + 127u) >> 1) << 23; }
+
+// acc + part * sa * sb; FAR: any scales, otherwise near ones.
+template <bool FAR>
+__device__ __forceinline__ float add_scaled(float acc, float part, float sa, float sb) {
+  if constexpr (FAR) {
+    const uint32_t a = half_power_bits(sa), b = half_power_bits(sb);
+    // s 2^-h is exact: 2^-h as the power of two with the opposite exponent.
+    const float rest_a = sa * bits_f32((254u << 23) - a), rest_b = sb * bits_f32((254u << 23) - b);
+    return fmaf(part * rest_a * rest_b, bits_f32(a) * bits_f32(b), acc);
+  } else {
+    return fmaf(part, sa * sb, acc);
+  }
+}
+
 // The FP32 value of an E8M0 byte.
 __device__ __forceinline__ float e8m0_value(uint32_t byte) {
   return bits_f32(byte == 0 ? 0x00400000u : (byte == 255 ? 0x7FC00000u : byte << 23));
@@ -516,9 +546,11 @@ struct ScaleArea {
   static constexpr int kRow = 36, kFill = 32, kBytes = (S::BM + S::BN) * kRow;
   static constexpr int kPeriod = MODE == kExponents ? kFill : kFill / 4;
 
-  // Blocks [first, first + kPeriod) of every row; rows past the end repeat the last one.
-  static __device__ void fill(char* area, const BlockProductArgs& g, int row0, int col0, int first, int total) {
+  // Blocks [first, first + kPeriod) of every row; rows past the end repeat the last one.  Sets *far where a factor is
+  // not a near one.
+  static __device__ void fill(char* area, int* far, const BlockProductArgs& g, int row0, int col0, int first, int total) {
     const int size = g.scale_f32 ? 4 : 1;
+    bool near = true;
     for (int r = threadIdx.x; r < S::BM + S::BN; r += S::kThreads) {
       const bool of_a = r < S::BM;
       const int at = of_a ? row0 + r : col0 + r - S::BM, rows = of_a ? g.m : g.n;
@@ -529,16 +561,22 @@ struct ScaleArea {
       const i32x4 lo = load_chunk(from, 0, end);
       if (MODE == kWide && !g.scale_f32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) to[j] = static_cast<int>(f32_bits(e8m0_value(lo[j >> 2] >> (8 * (j & 3)) & 255)));
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t bits = f32_bits(e8m0_value(lo[j >> 2] >> (8 * (j & 3)) & 255));
+          near = near && near_scale(bits);
+          to[j] = static_cast<int>(bits);
+        }
         continue;
       }
       const i32x4 hi = load_chunk(from, 16, end);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
+        if (MODE != kExponents) near = near && near_scale(lo[j]) && near_scale(hi[j]);
         to[j] = lo[j];
         to[4 + j] = hi[j];
       }
     }
+    if (MODE != kExponents && !near) *far = 1;
   }
 };
 
@@ -608,7 +646,7 @@ struct Fragment<kWide, FMT> {
 
 // One block of 128 of a 16 x 16 tile of results: B's rows first (see
 // sr_tile_product.h).
-template <int MODE, int FA, int FB, int MI, int NI>
+template <bool FAR, int MODE, int FA, int FB, int MI, int NI>
 __device__ __forceinline__ void block_mma(f32x4& acc, const Fragment<MODE, FA>& a, const Fragment<MODE, FB>& b,
                                           const Scales<MODE, MI, NI>& s, int mi, int ni) {
   if constexpr (MODE == kExponents) {
@@ -624,20 +662,73 @@ __device__ __forceinline__ void block_mma(f32x4& acc, const Fragment<MODE, FA>& 
       for (int i = 0; i < 4; ++i) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(b.v[i], a.v[i], part, 0, 0, 0);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = fmaf(part[j], s.a[mi] * s.b[ni][j], acc[j]);
+    for (int j = 0; j < 4; ++j) acc[j] = add_scaled<FAR>(acc[j], part[j], s.a[mi], s.b[ni][j]);
   }
 }
 
+// A tile's sums once more where some of its scales are not near ones: a stage at a time by the first group of waves,
+// with few values in registers, so that the ordinary walk keeps its own.  Every wave is done with the LDS, before and
+// after.
+template <int MODE, int FA, int FB, class S>
+__device__ __forceinline__ void sum_far_scales(const BlockProductArgs& g, char* lds, char* area, int* far, int row0, int col0,
+                                               int wave, int group, int stages, f32x4 (&acc)[S::MI][S::NI]) {
+  using Area = ScaleArea<MODE, S>;
+  const int wave_m = wave / S::WN * S::kRowsM, wave_n = wave % S::WN * S::kRowsN;
+  int lane = threadIdx.x & 63;
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(lane));  // nothing computed from it is kept over the ordinary walk
+#endif
+  Stager<S> stager;
+  stager.init(g.a, g.b, row0, col0, wave, lane);
+  const uint32_t fragment = fragment_offset(lane);
+#pragma unroll
+  for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+    for (int ni = 0; ni < S::NI; ++ni) acc[mi][ni] = f32x4{};
+  for (int kt = 0; kt < stages; ++kt) {
+    if (kt % Area::kPeriod == 0) Area::fill(area, far, g, row0, col0, kt, stages);
+    if (group == 0) stager.load_through(lds, static_cast<int64_t>(kt) * kStageBytes, g.k, wave, lane);
+    lds_barrier();
+    if (group == 0) {
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < S::NI; ++ni) {
+          const int row = wave_m + 16 * mi, col = wave_n + 16 * ni;
+          const char* sa = lds + row * kStageBytes;
+          const char* sb = lds + (S::BM + col) * kStageBytes;
+          Scales<MODE, 1, 1> scales;
+          scales.template load<S>(area, row, col, kt % Area::kPeriod, lane);
+          Fragment<MODE, FA> a;
+          Fragment<MODE, FB> b;
+          a.set(read_chunk(sa + fragment), read_chunk(sa + (fragment ^ 64)));
+          b.set(read_chunk(sb + fragment), read_chunk(sb + (fragment ^ 64)));
+          block_mma<true>(acc[mi][ni], a, b, scales, 0, 0);
+          asm volatile("" ::: "memory");  // the next tile's reads stay behind this one's
+        }
+    }
+    lds_barrier();
+  }
+}
+
+// Waves of a SIMD: as many workgroups of a small tile as its stages leave room for in a CU (three with unaligned rows'
+// registers), two of the large one.
+template <class S>
+constexpr int kProductWaves = S::BM > 64 ? S::kMinWaves : (S::kGroups > 1 ? 4 : 3);
+
 template <int MODE, int FA, int FB, class S, bool ASYNC>
-__global__ __launch_bounds__(S::kThreads, S::kMinWaves) void block_product_kernel(BlockProductArgs g) {
+__global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void block_product_kernel(BlockProductArgs g) {
   static_assert(ASYNC || S::kGroups == 1, "groups take aligned rows");
   using Area = ScaleArea<MODE, S>;
   constexpr int kStages = S::kLds + Area::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
   constexpr int kLds = kStages > kChunks ? kStages : kChunks;
   static_assert(S::kSums <= kLds, "the groups' sums");
-  __shared__ __align__(1024) char lds[kLds];
+  // One array: beside a second one the compiler lets the stages' asynchronous loads land before any read of LDS.
+  __shared__ __align__(1024) char lds[kLds + 16];
+  int* far = reinterpret_cast<int*>(lds + kLds);  // a scale so far is not a near one
   const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = all % S::kWaves, group = all / S::kWaves;
+  if (MODE != kExponents && threadIdx.x == 0) *far = 0;  // a barrier comes before the first fill
   uint32_t tile_m, tile_n;
   band_tile(xcd_run(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tile_m, tile_n);
   const int row0 = tile_m * S::BM, col0 = tile_n * S::BN;
@@ -667,13 +758,13 @@ __global__ __launch_bounds__(S::kThreads, S::kMinWaves) void block_product_kerne
       Fragment<MODE, FA> a;
       a.set(read_chunk(sa + mi * 16 * kStageBytes), read_chunk(sa2 + mi * 16 * kStageBytes));
 #pragma unroll
-      for (int ni = 0; ni < S::NI; ++ni) block_mma(acc[mi][ni], a, b[ni], scales, mi, ni);
+      for (int ni = 0; ni < S::NI; ++ni) block_mma<false>(acc[mi][ni], a, b[ni], scales, mi, ni);
     }
   };
 
   auto refill = [&](int kt) {
     if ((kt & (Area::kPeriod - 1)) == 0) {
-      Area::fill(area, g, row0, col0, kt, stages);
+      Area::fill(area, far, g, row0, col0, kt, stages);
       lds_barrier();
     }
   };
@@ -717,6 +808,10 @@ __global__ __launch_bounds__(S::kThreads, S::kMinWaves) void block_product_kerne
     }
   }
   stage_barrier();
+  if constexpr (MODE != kExponents) {
+    if (__builtin_amdgcn_readfirstlane(*far))
+      sum_far_scales<MODE, FA, FB, S>(g, lds, area, far, row0, col0, wave, group, stages, acc);
+  }
   add_groups<S>(lds, group, acc);
   if (group == 0) store_chunks<kLds, S>(g, lds, row0, col0, wave, lane, acc);
 }
@@ -758,7 +853,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void block_product_rows_kernel(Bloc
     Fragment<MODE, FB> b;
     a.set(load(pa, at), load(pa, at + 64));
     b.set(load(pb, at), load(pb, at + 64));
-    block_mma(acc, a, b, s, 0, 0);
+    block_mma<true>(acc, a, b, s, 0, 0);
   };
   // A wave's blocks are few, so that the loads of two run together.
   auto inside = [](const char* row, int64_t at) { return load_whole_chunk(row, at); };
