@@ -20,6 +20,10 @@
 // subtracted in FP32: on the large singular values P lies between -3 and 0,
 // and half the magnitude halves the rounding of its diagonal.
 //
+// The norm.  Squares of FP32 values need twice its exponents (a norm above 1.8e19
+// would overflow, values below 1e-23 would vanish), so they are summed in
+// FP64, and X is V 2^-h times a factor near one, 2^h being the norm's power of two.
+//
 // Workspace.  Rows and columns are padded to multiples of 64 with zeros, which
 // every step keeps, so the products have no edges along their contracted
 // axis.  Per padded element: X in FP32, H, and two buffers of H^T, which one
@@ -38,9 +42,9 @@ constexpr float kNsScale = 8192.0f, kNsInverse = 1.0f / 8192.0f;  // 2^13
 constexpr float kNsProduct = kNsInverse * kNsInverse;             // of a product of two scaled operands
 constexpr float kNsShift = 1.5f;
 constexpr int kNsPad = 64;        // rows and columns of the workspace are padded to it
-constexpr int kNsPartials = 512;  // partial sums of squares per matrix
+constexpr int kNsPartials = 256;  // partial sums of squares per matrix
 constexpr int kNsThreads = 256;
-constexpr int kNsLoadThreads = 512;
+constexpr int kNsLoadThreads = 1024;
 
 // The matrices of one launch.
 struct MatrixTable {
@@ -63,7 +67,7 @@ struct NsArgs {
   _Float16* ht_next;
   _Float16* g;
   _Float16* p;
-  float* partial;
+  double* partial;
   float momentum, decay, neg_lr;  // Muon
   int nesterov;
   int muon, out_dtype;  // last step: update p in out_dtype, or store the result
@@ -71,7 +75,7 @@ struct NsArgs {
 
 // Sum over the workgroup's THREADS threads, in a fixed order; the same in all of them.
 template <int THREADS>
-__device__ __forceinline__ float group_sum(float v, float* scratch) {
+__device__ __forceinline__ double group_sum(double v, double* scratch) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
   if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = v;
@@ -80,6 +84,28 @@ __device__ __forceinline__ float group_sum(float v, float* scratch) {
 #pragma unroll
   for (int w = 1; w < THREADS / 64; ++w) v += scratch[w];
   return v;
+}
+
+// What divides V, from the sum of its squares: V / (|V|_F + eps) = (V 2^-shift) * factor.
+struct NsDivisor {
+  int shift;
+  float factor;
+  __device__ __forceinline__ float operator()(float v) const { return ldexpf(v, -shift) * factor; }
+};
+
+// The sum is a normal number of FP64, 0, infinite or NaN.  A divisor of 0 has only zeros to divide, which stay.
+__device__ __forceinline__ NsDivisor ns_divisor(double sum, float eps) {
+  uint64_t bits;
+  __builtin_memcpy(&bits, &sum, 8);
+  const int exponent = static_cast<int>(bits >> 52) & 0x7FF;
+  int h = 0;
+  if (exponent != 0 && exponent != 0x7FF) {  // sum = [1, 4) 2^2h
+    h = (exponent - 1023) >> 1;
+    bits -= static_cast<uint64_t>(static_cast<int64_t>(2 * h)) << 52;
+    __builtin_memcpy(&sum, &bits, 8);
+  }
+  const float divisor = sqrtf(static_cast<float>(sum)) + ldexpf(eps, -h);
+  return {h, divisor == 0.0f ? 0.0f : 1.0f / divisor};
 }
 
 // How many of the columns col .. col + 3 of row `row` the caller's matrices have.
@@ -142,7 +168,7 @@ __device__ __forceinline__ void need_arguments(const NsArgs& a, const MatrixTabl
 template <int GE, int UE>
 __global__ __launch_bounds__(kNsLoadThreads) void ns_load_kernel(NsArgs a, MatrixTable t) {
   __shared__ float turned[kNsPad][kNsPad + 1];
-  __shared__ float scratch[kNsLoadThreads / 64];
+  __shared__ double scratch[kNsLoadThreads / 64];
   constexpr int kRows = kNsLoadThreads / 16, kPasses = kNsPad / kRows;
   const int matrix = blockIdx.y;
   need_arguments(a, t, matrix);
@@ -151,7 +177,7 @@ __global__ __launch_bounds__(kNsLoadThreads) void ns_load_kernel(NsArgs a, Matri
   float* x = a.x + static_cast<int64_t>(matrix) * a.m * a.n;
   const int tiles_c = (a.tall ? a.m : a.n) / kNsPad, tiles = (a.m / kNsPad) * (a.n / kNsPad);
   const int tr = threadIdx.x >> 4, tc = 4 * (threadIdx.x & 15);
-  float sum = 0.0f;
+  double sum = 0.0;
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int r0 = tile / tiles_c * kNsPad, c = tile % tiles_c * kNsPad + tc;
     f32x4 v[kPasses], old[kPasses];
@@ -186,7 +212,7 @@ __global__ __launch_bounds__(kNsLoadThreads) void ns_load_kernel(NsArgs a, Matri
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum = fmaf(v[pass][j], v[pass][j], sum);
+      for (int j = 0; j < 4; ++j) sum = fma(static_cast<double>(v[pass][j]), static_cast<double>(v[pass][j]), sum);
       if (!a.keep) continue;
       if (a.tall) {
 #pragma unroll
@@ -218,7 +244,7 @@ __global__ __launch_bounds__(kNsLoadThreads) void ns_load_kernel(NsArgs a, Matri
 template <int GE>
 __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTable t) {
   __shared__ float turned[kNsPad][kNsPad + 1];
-  __shared__ float scratch[4];
+  __shared__ double scratch[4];
   const int matrix = blockIdx.y;
   need_arguments(a, t, matrix);
   const int64_t base = static_cast<int64_t>(matrix) * a.m * a.n;
@@ -238,10 +264,9 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTa
     else
       v[pass] = *reinterpret_cast<const f32x4*>(x + static_cast<int64_t>(r) * a.n + c);
   }
-  const float* partial = a.partial + matrix * kNsPartials;
-  float sum = 0.0f;
-  for (int i = threadIdx.x; i < a.partials; i += kNsThreads) sum += partial[i];
-  const float inverse = 1.0f / (sqrtf(group_sum<kNsThreads>(sum, scratch)) + a.eps);
+  static_assert(kNsPartials <= kNsThreads, "a partial sum for each thread");
+  const double sum = static_cast<int>(threadIdx.x) < a.partials ? a.partial[matrix * kNsPartials + threadIdx.x] : 0.0;
+  const NsDivisor scaled = ns_divisor(group_sum<kNsThreads>(sum, scratch), a.eps);
   auto store_x = [&](int row, int col, const f32x4& y, const f16x4& w) {
     const int64_t i = static_cast<int64_t>(row) * a.n + col;
     *reinterpret_cast<f32x4*>(x + i) = y;
@@ -261,7 +286,7 @@ __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTa
     const int row = 16 * pass + tr;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      v[pass][j] *= inverse;
+      v[pass][j] = scaled(v[pass][j]);
       turned[tc + j][row] = v[pass][j];
     }
     if (flip) store_turned(r0 + row, c0 + tc, halves(v[pass]));
@@ -629,7 +654,7 @@ __device__ __forceinline__ void finish_one(const NsArgs& a, void* out, int row, 
 
 __global__ __launch_bounds__(kSmallThreads, 4) void ns_small_kernel(NsArgs a, int steps, MatrixTable t) {
   __shared__ __align__(1024) char small_lds[2 * (2 * kSmallRows * kSmallRows + kSmallRows * kSmallCols)];
-  __shared__ float scratch[16];
+  __shared__ double scratch[16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int across = lane & 15, quarter = lane >> 4;
   const int matrix = blockIdx.x, n = a.n;
@@ -639,7 +664,7 @@ __global__ __launch_bounds__(kSmallThreads, 4) void ns_small_kernel(NsArgs a, in
   const int stride = 2 * n;
   const float* from = a.x + static_cast<int64_t>(matrix) * a.m * n;
 
-  float sum = threadIdx.x < a.partials ? a.partial[matrix * kNsPartials + threadIdx.x] : 0.0f;
+  double sum = static_cast<int>(threadIdx.x) < a.partials ? a.partial[matrix * kNsPartials + threadIdx.x] : 0.0;
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   if (lane == 0) scratch[wave] = sum;
@@ -653,10 +678,10 @@ __global__ __launch_bounds__(kSmallThreads, 4) void ns_small_kernel(NsArgs a, in
       for (int j = 0; j < 4; ++j) x[c][i][j] = 16 * (wave + 16 * c) < n ? from[(16 * i + 4 * quarter + j) * n + col] : 0.0f;
   }
   __syncthreads();
-  sum = 0.0f;
+  sum = 0.0;
 #pragma unroll
   for (int w = 0; w < 16; ++w) sum += scratch[w];
-  const float inverse = 1.0f / (sqrtf(sum) + a.eps);
+  const NsDivisor scaled = ns_divisor(sum, a.eps);
 
   // Places in H whose swizzle does not change over the loops: 16 rows further are 16 strides, 16 column tiles further
   // (the wave's next) 512 bytes, 64 columns further 128 bytes.
@@ -692,7 +717,7 @@ __global__ __launch_bounds__(kSmallThreads, 4) void ns_small_kernel(NsArgs a, in
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[c][i][j] *= inverse;
+      for (int j = 0; j < 4; ++j) x[c][i][j] = scaled(x[c][i][j]);
   store_h();
   __syncthreads();
 

@@ -19,7 +19,7 @@ struct Layout {
   int64_t x, h, square, partial;
   Layout(int64_t batch, int64_t m, int64_t n)
       : x(aligned(batch * m * n * 4)), h(aligned(batch * m * n * 2)), square(aligned(batch * m * m * 2)),
-        partial(aligned(batch * sr::kNsPartials * 4)) {}
+        partial(aligned(batch * sr::kNsPartials * 8)) {}
   int64_t total() const { return x + 3 * h + 2 * square + partial; }
 };
 
@@ -120,7 +120,7 @@ int run(NsArgs a, const sr::MatrixTable& t, int matrices, int g_dtype, int ue, c
   w += 3 * layout.h;
   a.g = reinterpret_cast<_Float16*>(w);
   a.p = reinterpret_cast<_Float16*>(w + layout.square);
-  a.partial = reinterpret_cast<float*>(w + 2 * layout.square);
+  a.partial = reinterpret_cast<double*>(w + 2 * layout.square);
 
   const int64_t tiles = static_cast<int64_t>(a.m / sr::kNsPad) * (a.n / sr::kNsPad);
   a.partials = static_cast<int>(tiles < sr::kNsPartials ? tiles : sr::kNsPartials);

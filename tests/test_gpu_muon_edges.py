@@ -1,0 +1,55 @@
+"""Edges of the orthogonalised updates: norms at the ends of FP32's range, steps that are refused.
+
+Tolerances are those of test_gpu_muon.py.
+"""
+
+from __future__ import annotations
+
+import _matrix_oracle as oracle
+import pytest
+import sr_states
+import torch
+
+pytestmark = pytest.mark.gpu
+LIMIT = 4e-3
+
+
+def _matrix(shape, device, seed, dtype=torch.float32, std=1.0):
+    gen = torch.Generator(device=device).manual_seed(seed)
+    return (torch.randn(shape, device=device, generator=gen) * std).to(dtype)
+
+
+# Sums of squares from 1e-66 to beyond 1e77, in one workgroup, in tiles, tall and in a batch.
+@pytest.mark.parametrize("shape", [(50, 70), (200, 300), (300, 200), (2, 150, 90)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("std", [6e37, 1e25, 1e19, 1e-19, 1e-25, 1e-35])
+def test_orthogonalize_over_the_range_of_norms(cuda, shape, dtype, std):
+    x = _matrix(shape, cuda, 1, torch.float64, std).to(dtype)
+    assert x.isfinite().all()
+    eps = 1e-7 if std > 1 else 0.0
+    got = sr_states.orthogonalize(x, eps=eps)
+    want = oracle.orthogonalize(x, eps=eps)
+    assert float(want.abs().max()) > 0.01
+    assert oracle.relative(got, want) < LIMIT
+
+
+def test_a_norm_of_zero_or_beyond_every_number(cuda):
+    for shape in ((50, 70), (200, 300)):
+        zero = torch.zeros(shape, device=cuda)
+        assert torch.equal(sr_states.orthogonalize(zero, eps=0.0), torch.zeros(shape, device=cuda, dtype=torch.bfloat16))
+        infinite = _matrix(shape, cuda, 1)
+        infinite[3, 4] = float("inf")
+        assert sr_states.orthogonalize(infinite).isnan().any()
+
+
+@pytest.mark.parametrize("shape", [(50, 70), (200, 300), (300, 200)])
+@pytest.mark.parametrize("std", [1e30, 1e-30])
+def test_step_over_the_range_of_norms(cuda, shape, std):
+    p, g, m = _matrix(shape, cuda, 1), _matrix(shape, cuda, 2, std=std), _matrix(shape, cuda, 3, std=std)
+    u = m * 0.9 + g
+    update = oracle.orthogonalize(u * 0.9 + g, eps=0.0) * max(1.0, shape[0] / shape[1]) ** 0.5
+    want = p.double() - 0.5 * update
+    fmt = sr_states.StateFormat(torch.float32, "nearest")
+    sr_states.hip_muon_step_(p, g, m, lr=0.5, momentum_factor=0.9, eps=0.0, seed=1, formats=(fmt,))
+    assert torch.equal(m, u)
+    assert float((p.double() - want).norm()) <= LIMIT * float((0.5 * update).norm()) + 2.0**-22 * float(want.norm())
