@@ -102,7 +102,9 @@ typedef struct sr_newton_schulz {
 /* Matrices one launch takes; longer batches run in turn. */
 #define SR_MATRIX_BATCH 64
 
-/* Bytes of workspace for `batch` matrices of this shape. */
+/* Bytes of workspace for `batch` matrices of this shape; 0 for none, and for a
+ * shape that the entries below refuse (a side above 2^20, or more than 2^31
+ * elements). */
 int64_t sr_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols);
 
 /* out[i] = the orthogonalised x[i] (each contiguous rows x cols; x FP32, BF16

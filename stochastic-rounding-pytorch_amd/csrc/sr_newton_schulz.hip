@@ -23,9 +23,11 @@ struct Layout {
   int64_t total() const { return x + 3 * h + 2 * square + partial; }
 };
 
+bool fits(int64_t rows, int64_t cols) { return rows <= kMaxSide && cols <= kMaxSide && rows * cols <= kMaxElements; }
+
 int check_shape(int64_t batch, int64_t rows, int64_t cols, const sr_newton_schulz* ns) {
   if (batch < 0 || rows < 0 || cols < 0) return fail(SR_ERR_ARGUMENT, "negative size");
-  if (rows > kMaxSide || cols > kMaxSide || rows * cols > kMaxElements)
+  if (!fits(rows, cols))
     return fail(SR_ERR_ARGUMENT, "%lld x %lld matrices are too large", (long long)rows, (long long)cols);
   if (!ns) return fail(SR_ERR_ARGUMENT, "null argument");
   if (ns->steps < 1) return fail(SR_ERR_ARGUMENT, "%d steps", ns->steps);
@@ -176,7 +178,7 @@ int momentum_enc(int dtype, int rule) {
 extern "C" {
 
 int64_t sr_orthogonalize_workspace(int64_t batch, int64_t rows, int64_t cols) {
-  if (batch <= 0 || rows <= 0 || cols <= 0 || rows > kMaxSide || cols > kMaxSide) return 0;
+  if (batch <= 0 || rows <= 0 || cols <= 0 || !fits(rows, cols)) return 0;
   const int64_t m = padded(rows < cols ? rows : cols), n = padded(rows < cols ? cols : rows);
   return Layout(batch < SR_MATRIX_BATCH ? batch : SR_MATRIX_BATCH, m, n).total();
 }

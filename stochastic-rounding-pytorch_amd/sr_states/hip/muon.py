@@ -68,14 +68,18 @@ def _newton_schulz(steps: int, coefficients: tuple, eps: float) -> _lib.NewtonSc
     return _lib.NewtonSchulz(a, b, c, eps, steps)
 
 
-def _workspace(batch: int, rows: int, cols: int, device) -> torch.Tensor:
-    return torch.empty(_lib.library().sr_orthogonalize_workspace(batch, rows, cols), dtype=torch.uint8, device=device)
-
-
-def _batch_size(rows: int, cols: int) -> int:
-    """Matrices per launch: as many as the library takes, within the workspace's limit."""
+def _batch_size(count: int, rows: int, cols: int) -> int:
+    """Matrices of ``count`` per launch: as many as the library takes, within the workspace's limit."""
     one = _lib.library().sr_orthogonalize_workspace(1, rows, cols)
-    return max(1, min(_lib.MATRIX_BATCH, _WORKSPACE_BYTES // max(one, 1)))
+    return max(1, min(count, _lib.MATRIX_BATCH, _WORKSPACE_BYTES // max(one, 1)))
+
+
+def _workspace_bytes(count: int, rows: int, cols: int) -> int:
+    """Bytes of workspace of the launches that update ``count`` matrices; raises for matrices the library refuses."""
+    size = _lib.library().sr_orthogonalize_workspace(_batch_size(count, rows, cols), rows, cols)
+    if not size:
+        raise ValueError(f"{rows} x {cols} matrices are too large")
+    return size
 
 
 def orthogonalize(
@@ -138,7 +142,7 @@ def _validate_hyper(lr, momentum, weight_decay, update_scale):
         raise ValueError(f"update_scale must be one of {UPDATE_SCALES}")
 
 
-def _launch(tensors, shape, keys, codes, hyper, ns, device):
+def _launch(tensors, shape, keys, codes, hyper, ns, workspace):
     """Queue the update of same-shaped (parameter, gradient, momentum) rows; keys are (key, offset)."""
     lr, momentum, nesterov, weight_decay, update_scale = hyper
     parameter, gradient, _ = tensors[0]
@@ -147,9 +151,9 @@ def _launch(tensors, shape, keys, codes, hyper, ns, device):
     hparams = _lib.MuonHparams(
         momentum, 1 - lr * weight_decay, -lr * _update_scale(update_scale, rows, cols), int(nesterov)
     )
-    each = min(len(tensors), _batch_size(rows, cols))
+    device = workspace.device
+    each = _batch_size(len(tensors), rows, cols)
     with _lib.on_device(device):
-        workspace = _workspace(each, rows, cols, device)
         for first in range(0, len(tensors), each):
             part = range(first, min(first + each, len(tensors)))
             table = (_lib.MuonRow * len(part))(
@@ -216,8 +220,9 @@ def hip_muon_step_(
         validate_device(device)
         validate_no_overlap(_spans(tensors))
         if parameter.numel():
+            workspace = torch.empty(_workspace_bytes(1, *shape), dtype=torch.uint8, device=device)
             _launch([tensors], shape, [(_lib.low32(seed), _lib.low32(offset))], codes[0],
-                    (lr, momentum_factor, nesterov, weight_decay, update_scale), ns, device)
+                    (lr, momentum_factor, nesterov, weight_decay, update_scale), ns, workspace)
     finally:
         _lib.set_grad_enabled(grad)
 
@@ -295,14 +300,6 @@ class MuonHip(StateOptimizer):
     def _hyper(self, group):
         return group["lr"], group["momentum"], group["nesterov"], group["weight_decay"], group["update_scale"]
 
-    def _step_parameter(self, parameter, state, group, formats, step, seed, offset):
-        lr, momentum, nesterov, weight_decay, update_scale = self._hyper(group)
-        hip_muon_step_(
-            parameter, parameter.grad, state["momentum_buffer"], lr=lr, momentum_factor=momentum, nesterov=nesterov,
-            weight_decay=weight_decay, update_scale=update_scale, ns_steps=group["ns_steps"],
-            ns_coefficients=group["ns_coefficients"], eps=group["eps"], seed=seed, offset=offset, formats=formats,
-        )
-
     def _step_group(self, group, formats, items, rng_step):
         if _lib.capturing():
             raise RuntimeError(
@@ -312,7 +309,8 @@ class MuonHip(StateOptimizer):
         _validate_hyper(*(group[name] for name in ("lr", "momentum", "weight_decay", "update_scale")))
         ns = _newton_schulz(group["ns_steps"], tuple(group["ns_coefficients"]), float(group["eps"]))
         codes = native_codes(formats[0].dtype, formats[0].rounding)
-        # The whole group is checked before its first launch.
+        # The whole group is checked, and its workspaces are there, before its first launch: a step that is refused or
+        # runs out of memory has changed nothing.
         buckets, spans = {}, {}
         for parameter, state, index, _, offset in items:
             tensors = (parameter, parameter.grad, state["momentum_buffer"])
@@ -328,8 +326,13 @@ class MuonHip(StateOptimizer):
             keys.append((update_key(group["sr_seed"], rng_step, index), offset))
         for device_spans in spans.values():
             validate_no_overlap(device_spans)
+        # The launches of a device follow each other on its stream, so one workspace serves them all.
+        sizes = {}
+        for (device, shape, _, _), (rows, _) in buckets.items():
+            sizes[device] = max(sizes.get(device, 0), _workspace_bytes(len(rows), *shape))
+        workspaces = {d: torch.empty(size, dtype=torch.uint8, device=d) for d, size in sizes.items()}
         for (device, shape, _, _), (rows, keys) in buckets.items():
-            _launch(rows, shape, keys, codes, self._hyper(group), ns, device)
+            _launch(rows, shape, keys, codes, self._hyper(group), ns, workspaces[device])
 
 
 class MuonHipRN(MuonHip):

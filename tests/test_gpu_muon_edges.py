@@ -36,7 +36,7 @@ def test_orthogonalize_over_the_range_of_norms(cuda, shape, dtype, std):
 def test_a_norm_of_zero_or_beyond_every_number(cuda):
     for shape in ((50, 70), (200, 300)):
         zero = torch.zeros(shape, device=cuda)
-        assert torch.equal(sr_states.orthogonalize(zero, eps=0.0), torch.zeros(shape, device=cuda, dtype=torch.bfloat16))
+        assert torch.equal(sr_states.orthogonalize(zero, eps=0.0), zero.bfloat16())
         infinite = _matrix(shape, cuda, 1)
         infinite[3, 4] = float("inf")
         assert sr_states.orthogonalize(infinite).isnan().any()
@@ -53,3 +53,44 @@ def test_step_over_the_range_of_norms(cuda, shape, std):
     sr_states.hip_muon_step_(p, g, m, lr=0.5, momentum_factor=0.9, eps=0.0, seed=1, formats=(fmt,))
     assert torch.equal(m, u)
     assert float((p.double() - want).norm()) <= LIMIT * float((0.5 * update).norm()) + 2.0**-22 * float(want.norm())
+
+
+def _optimizer(shapes, device):
+    """An optimizer after a first step over the matrices that are not too large, with gradients for a second one."""
+    params = [torch.nn.Parameter(_matrix(shape, device, k)) for k, shape in enumerate(shapes)]
+    opt = sr_states.MuonHip(params, seed=3)
+    for step in range(2):
+        for k, p in enumerate(params):
+            p.grad = _matrix(p.shape, device, 10 * step + k) if step or p.shape[0] <= 1 << 20 else None
+        if not step:
+            opt.step()
+    return params, opt
+
+
+def _unchanged(params, opt, step):
+    before = [(p.detach().clone(), opt.state[p]["momentum_buffer"].clone()) for p in params[:2]]
+    with pytest.raises((RuntimeError, ValueError)) as error:
+        step()
+    for p, (value, momentum) in zip(params, before):
+        assert torch.equal(p, value) and torch.equal(opt.state[p]["momentum_buffer"], momentum)
+    return str(error.value)
+
+
+def test_a_step_with_a_matrix_that_is_too_large_changes_nothing(cuda):
+    params, opt = _optimizer([(64, 96), (130, 70), ((1 << 20) + 1, 2)], cuda)
+    assert "too large" in _unchanged(params, opt, opt.step)
+    with pytest.raises((RuntimeError, ValueError), match="too large"):
+        sr_states.orthogonalize(params[2].detach())
+
+
+def test_a_step_without_memory_for_a_workspace_changes_nothing(cuda, monkeypatch):
+    params, opt = _optimizer([(64, 96), (130, 70), (900, 900)], cuda)
+    empty = torch.empty
+
+    def small_only(*args, **options):
+        if options.get("dtype") == torch.uint8 and args[0] > 900 * 900 * 4:
+            raise torch.OutOfMemoryError("no memory for a workspace")
+        return empty(*args, **options)
+
+    monkeypatch.setattr(torch, "empty", small_only)
+    assert "no memory" in _unchanged(params, opt, opt.step)
