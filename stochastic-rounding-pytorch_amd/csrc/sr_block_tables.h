@@ -8,7 +8,6 @@
 namespace sr {
 
 using Tile128 = TileShape<128, 128, 2, 2>;
-using Tile96 = TileShape<96, 96, 1, 3, 3>;
 using Tile64 = TileShape<64, 64, 2, 2>;
 using Tile64x2 = TileShape<64, 64, 2, 2, 2>;
 using Tile64x4 = TileShape<64, 64, 2, 2, 4>;

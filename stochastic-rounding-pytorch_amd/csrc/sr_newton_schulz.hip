@@ -74,10 +74,7 @@ int product(const NsArgs& a, int matrices, const sr::MatrixTable& t, hipStream_t
 // The symmetric launches stop at 128 x 128 tiles, and the others take 256 x
 // 256 ones where these fill the chip: a triangle has few large tiles (8
 // matrices of 2048 x 2048: G 122 us on 256 x 256 tiles and 102 on 128 x 128,
-// the step 200 and 244).  A triangle of more than 512 small tiles gives some
-// CUs three and most two; where 96 x 96 ones are at most one a CU, they are
-// better balanced (2048 rows: 253 of them in place of 528; G of 2048 x 8192
-// 77 us and 64).
+// the step 200 and 244).
 template <int OP, bool TURNED = false>
 int product_by_size(const NsArgs& a, int matrices, const sr::MatrixTable& t, hipStream_t s) {
   constexpr bool kSymmetric = OP == sr::kNsGram || OP == sr::kNsPolynomial;
@@ -90,9 +87,6 @@ int product_by_size(const NsArgs& a, int matrices, const sr::MatrixTable& t, hip
   };
   if constexpr (!kSymmetric) {
     if (tiles(256) >= 256) return product<OP, sr::TileWide, TURNED>(a, matrices, t, s);
-  }
-  if constexpr (kSymmetric) {
-    if (tiles(64) > 512 && tiles(96) <= 256) return product<OP, sr::Tile96, TURNED>(a, matrices, t, s);
   }
   switch (sr::tile_by_count(tiles)) {
     case sr::kTile128: return product<OP, sr::Tile128, TURNED>(a, matrices, t, s);

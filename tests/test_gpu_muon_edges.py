@@ -94,3 +94,15 @@ def test_a_step_without_memory_for_a_workspace_changes_nothing(cuda, monkeypatch
 
     monkeypatch.setattr(torch, "empty", small_only)
     assert "no memory" in _unchanged(params, opt, opt.step)
+
+
+# Both sides of the lines between tile shapes: 256 and 512 tiles of 64 x 64 on a triangle, and 256 of 128 x 128.
+@pytest.mark.parametrize("shape", [
+    (1410, 1500), (1472, 1480), (1984, 2050), (2040, 2100), (2112, 2150), (2170, 2180), (2816, 2900), (2890, 2900),
+    (12, 570, 600), (3, 1150, 1200), (7, 760, 790), (2, 1400, 1450), (25, 380, 400),
+])
+def test_orthogonalize_on_both_sides_of_the_tile_shapes(cuda, shape):
+    x = _matrix(shape, cuda, 1, torch.bfloat16)
+    got = sr_states.orthogonalize(x)
+    for g, one in zip(got.view(-1, *shape[-2:])[::6], x.view(-1, *shape[-2:])[::6]):
+        assert oracle.relative(g, oracle.orthogonalize(one)) < LIMIT
