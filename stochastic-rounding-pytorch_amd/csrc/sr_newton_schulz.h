@@ -341,7 +341,8 @@ __device__ __forceinline__ NsTile ns_tile(const NsArgs& a, uint32_t tiles_m, uin
   r.matrix = id / tiles;
   uint32_t tile_m, tile_n;
   if constexpr (kSymmetric) {
-    triangle_tile(id % tiles, S::BM / S::BN, tile_m, tile_n);
+    static_assert(S::BM == S::BN, "a triangle of square tiles");
+    triangle_tile(id % tiles, tile_m, tile_n);
   } else {
     band_tile(id % tiles, tiles_m, tiles_n, tile_m, tile_n);
   }

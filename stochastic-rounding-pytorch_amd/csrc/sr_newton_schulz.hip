@@ -61,7 +61,7 @@ template <int OP, class S, bool TURNED = false>
 int product(const NsArgs& a, int matrices, const sr::MatrixTable& t, hipStream_t s) {
   constexpr bool kSymmetric = OP == sr::kNsGram || OP == sr::kNsPolynomial;
   const uint32_t tm = (a.m + S::BM - 1) / S::BM, tn = ((kSymmetric ? a.m : a.n) + S::BN - 1) / S::BN;
-  const uint32_t tiles = kSymmetric ? S::BM / S::BN * (tm * (tm + 1) / 2) : tm * tn;
+  const uint32_t tiles = kSymmetric ? tm * (tm + 1) / 2 : tm * tn;
   if (static_cast<uint64_t>(tiles) * matrices > 0x3FFFFFu) return fail(SR_ERR_ARGUMENT, "%u tiles exceed a launch", tiles);
   if constexpr (std::is_same_v<S, sr::TileWide>) {
     sr::ns_wide_kernel<OP, TURNED><<<tiles * matrices, S::kThreads, 0, s>>>(a, tm, tn, tiles, matrices, t);

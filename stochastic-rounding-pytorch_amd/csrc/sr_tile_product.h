@@ -142,16 +142,13 @@ __device__ __forceinline__ void band_tile(uint32_t id, uint32_t tm, uint32_t tn,
   col = within / height;
 }
 
-// The lower triangle's tile of index id, counted row by row, of tiles that are
-// `wide` (1 or 2) times as high as wide: row r has wide * (r + 1) tiles, up to
-// those on its diagonal block.
-__device__ __forceinline__ void triangle_tile(uint32_t id, uint32_t wide, uint32_t& row, uint32_t& col) {
-  const uint32_t half = id / wide;
-  uint32_t r = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(half) + 1.0f) - 1.0f) * 0.5f);
-  while (r * (r + 1) / 2 > half) --r;
-  while ((r + 1) * (r + 2) / 2 <= half) ++r;
+// The lower triangle's tile of index id, counted row by row: row r has r + 1 tiles.
+__device__ __forceinline__ void triangle_tile(uint32_t id, uint32_t& row, uint32_t& col) {
+  uint32_t r = static_cast<uint32_t>((sqrtf(8.0f * static_cast<float>(id) + 1.0f) - 1.0f) * 0.5f);
+  while (r * (r + 1) / 2 > id) --r;
+  while ((r + 1) * (r + 2) / 2 <= id) ++r;
   row = r;
-  col = id - wide * (r * (r + 1) / 2);
+  col = id - r * (r + 1) / 2;
 }
 
 // The 16 bytes at `at` of a row, all inside it.
