@@ -107,13 +107,23 @@ __device__ __forceinline__ uint32_t max_of_16(uint32_t m) {
   return umax(m, __builtin_amdgcn_update_dpp(0u, m, 0x121, 0xF, 0xF, true));
 }
 
+// Eight values of two bytes, and eight bytes, in one access each that promises one element's alignment (rows start
+// anywhere; sr_group_access.h's types of these sizes promise more, their groups being of larger elements).
+typedef uint32_t eight_halves __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t eight_bytes __attribute__((ext_vector_type(2), aligned(1)));
+
 // Eight values from `p`, of which the first `live` are there; zeros for the rest.
 template <int XE>
 __device__ __forceinline__ void load_eight(const char* p, int live, float (&x)[8]) {
   if (live == 8) {
     uint32_t w[2 * group_words(XE)];
-    load_words<16, true>(p, w);
-    if constexpr (enc_bytes(XE) == 4) load_words<16, true>(p + 16, w + 4);
+    if constexpr (enc_bytes(XE) == 4) {
+      load_words<16, true>(p, w);
+      load_words<16, true>(p + 16, w + 4);
+    } else {
+      const eight_halves values = *(const SR_GLOBAL eight_halves*)(p);
+      __builtin_memcpy(w, &values, 16);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       uint32_t words[group_words(XE)];
@@ -192,7 +202,7 @@ __device__ __forceinline__ void encode_row(const float (&x)[8], int e, const uin
 // Stores the first `live` of eight bytes.
 __device__ __forceinline__ void store_eight(char* q, const uint32_t (&words)[2], int live) {
   if (live == 8) {
-    *(SR_GLOBAL group8*)(q) = group8{words[0], words[1]};
+    *(SR_GLOBAL eight_bytes*)(q) = eight_bytes{words[0], words[1]};
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
