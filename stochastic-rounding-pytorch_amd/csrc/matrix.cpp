@@ -36,6 +36,7 @@
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/GradMode.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
@@ -212,6 +213,10 @@ at::Tensor matmul(const Scaled& a, const Scaled& b, int out_code, at::Tensor out
       const auto [first, last] = span(*t);
       if (start < last && first < end) value_error("out must not overlap the operands");
     }
+    // As torch's own out= functions: the write is not differentiable, and whoever saved the tensor must notice it.
+    if (out.requires_grad() && c10::GradMode::is_enabled())
+      throw Refusal(PyExc_RuntimeError, "out requires grad, and block_matmul records no gradients: call it under torch.no_grad()");
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
   } else {
     if (out_code < 0) out_code = SR_BF16;
     out = at::empty({m, n}, options.dtype(scalar_type(out_code)));

@@ -136,7 +136,8 @@ def block_matmul(
     Either may be E4M3 or E5M2 with blocks of one row or of 128; both have E8M0
     scales or both FP32 ones.  Products are summed in FP32 and rounded once, to
     ``out_dtype`` (BF16 by default, FP32 or FP16) or into ``out``, which has
-    consecutive columns and shares no memory with the operands.
+    consecutive columns, shares no memory with the operands and, in grad mode,
+    requires no gradient.  Nothing is recorded for autograd.
     """
     (a_data, a_scale), (b_data, b_scale) = a, b
     if out_dtype is None:

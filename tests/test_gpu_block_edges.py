@@ -95,3 +95,36 @@ def test_scales_far_apart_and_far_from_one(cuda, m, n, dtype, scale, log_a, log_
         if out == torch.float16:
             limit = limit + 2.0**-25
         assert float(((got.double() - want).abs() - limit).max()) <= 0
+
+
+def _operands(device):
+    return (sr_states.block_cast(_values((rows, 128), device, rows)) for rows in (8, 16))
+
+
+def test_a_result_that_requires_a_gradient_is_refused(cuda):
+    a, b = _operands(cuda)
+    leaf = torch.zeros(8, 16, device=cuda, requires_grad=True)
+    for out in (leaf, leaf * 1.0):
+        with pytest.raises(RuntimeError, match="requires grad"):
+            sr_states.block_matmul(a, b, out=out)
+        assert not out.any()
+    with torch.no_grad():  # as torch's own out= functions
+        assert sr_states.block_matmul(a, b, out=leaf) is leaf
+    assert torch.equal(leaf, sr_states.block_matmul(a, b, out_dtype=torch.float32))
+
+
+def test_a_result_written_over_a_saved_tensor_is_noticed(cuda):
+    a, b = _operands(cuda)
+    x = torch.ones(8, 16, device=cuda, requires_grad=True)
+    saved = torch.full((8, 16), 2.0, device=cuda)
+    product = x * saved
+    version = saved._version
+    sr_states.block_matmul(a, b, out=saved)
+    assert saved._version > version
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
+    with torch.inference_mode():
+        inside = torch.empty(8, 16, device=cuda)
+        sr_states.block_matmul(a, b, out=inside)
+    # Nothing tracks an inference tensor.
+    assert sr_states.block_matmul(a, b, out=inside) is inside
