@@ -128,3 +128,123 @@ def test_a_result_written_over_a_saved_tensor_is_noticed(cuda):
         sr_states.block_matmul(a, b, out=inside)
     # Nothing tracks an inference tensor.
     assert sr_states.block_matmul(a, b, out=inside) is inside
+
+
+@pytest.mark.parametrize("dtypes", [(torch.float16, torch.float16), (torch.float16, torch.float32),
+                                    (torch.float32, torch.float16)])
+@pytest.mark.parametrize("shape", [(300,), (70, 300), (2, 3, 300)])
+def test_linear_of_fp16_and_of_one_row(cuda, dtypes, shape):
+    seed, n = 5, 140
+    x = _values(shape, cuda, 1, dtypes[0]).requires_grad_()
+    w = (_values((n, 300), cuda, 2) * 0.05).to(dtypes[1]).requires_grad_()
+    y = sr_states.block_linear(x, w, seed=seed)
+    dy = (_values(tuple(y.shape), cuda, 3) * 0.1).to(y.dtype)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert (y.dtype, dx.dtype, dw.dtype) == (dtypes[0], *dtypes) and dx.shape == x.shape and dw.shape == w.shape
+    keys = [sr_states.state_key(seed, k) for k in range(3)]
+    rows, grads = x.detach().reshape(-1, 300), dy.reshape(-1, n)
+    wanted = (
+        oracle.product(oracle.block_cast(rows, E4M3, "nearest", False, 1, keys[0]),
+                       oracle.block_cast(w.detach(), E4M3, "nearest", True, 1, keys[1])),
+        oracle.product(oracle.block_cast(grads, E4M3, "stochastic", False, 1, keys[2]),
+                       oracle.block_cast(w.detach(), E4M3, "nearest", True, 0, keys[1])),
+        oracle.product(oracle.block_cast(grads, E4M3, "stochastic", False, 0, keys[2]),
+                       oracle.block_cast(rows, E4M3, "nearest", False, 0, keys[0])),
+    )
+    for got, (want, magnitude), k in zip((y, dx, dw), wanted, (300, n, rows.shape[0])):
+        got = got.detach().reshape(want.shape)
+        inner = k * 2.0**-24 + (0 if got.dtype == torch.float32 else 2.0**-13)
+        limit = HALF_ULP[got.dtype] * want.abs() + inner * magnitude * (1 + HALF_ULP[got.dtype])
+        if got.dtype == torch.float16:
+            limit = limit + 2.0**-25
+        assert float(((got.double() - want).abs() - limit).max()) <= 0
+
+
+def test_linear_gradients_of_an_expanded_and_of_a_strided_gradient(cuda):
+    x, w = _values((60, 200), cuda, 1), _values((50, 200), cuda, 2)
+
+    def gradients(dy):
+        leaves = x.clone().requires_grad_(), w.clone().requires_grad_()
+        return torch.autograd.grad(sr_states.block_linear(*leaves, seed=3), leaves, dy)
+
+    for dy in (torch.ones((), device=cuda).expand(60, 50), _values((50,), cuda, 3).expand(60, 50),
+               _values((50, 60), cuda, 4).t(), _values((60, 57), cuda, 5)[:, 3:53]):
+        for got, want in zip(gradients(dy), gradients(dy.contiguous())):
+            assert torch.equal(got, want)
+    # Only one of the two is wanted.
+    leaf = x.clone().requires_grad_()
+    dy = _values((60, 50), cuda, 6)
+    sr_states.block_linear(leaf, w, seed=3).backward(dy)
+    assert torch.equal(leaf.grad, gradients(dy)[0])
+    leaf = w.clone().requires_grad_()
+    sr_states.block_linear(x, leaf, seed=3).backward(dy)
+    assert torch.equal(leaf.grad, gradients(dy)[1])
+
+
+def test_linear_under_autocast_checkpointing_and_compilation(cuda):
+    from torch.utils.checkpoint import checkpoint
+
+    x, w = _values((60, 200), cuda, 1, torch.bfloat16), _values((50, 200), cuda, 2)
+    dy = _values((60, 50), cuda, 3, torch.bfloat16)
+
+    def gradients(call):
+        leaves = x.clone().requires_grad_(), w.clone().requires_grad_()
+        y = call(*leaves)
+        y.backward(dy)
+        return y.detach(), *(leaf.grad for leaf in leaves)
+
+    def layer(x, w):
+        return sr_states.block_linear(x, w, seed=3)
+
+    def cast(x, w):
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            return layer(x, w)
+
+    want = gradients(layer)
+    for call in (cast, lambda x, w: checkpoint(layer, x, w, use_reentrant=False),
+                 lambda x, w: checkpoint(layer, x, w, use_reentrant=True), torch.compile(layer, backend="eager")):
+        for a, b in zip(gradients(call), want):
+            assert torch.equal(a, b)
+
+
+def test_linear_on_a_side_stream(cuda):
+    x, w = _values((300, 512), cuda, 1, torch.bfloat16).requires_grad_(), _values((256, 512), cuda, 2).requires_grad_()
+    dy = _values((300, 256), cuda, 3, torch.bfloat16)
+    want = torch.autograd.grad(sr_states.block_linear(x, w, seed=1), (x, w), dy)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        late = dy.clone()
+        for _ in range(20):
+            late = late * 1.0
+        got = torch.autograd.grad(sr_states.block_linear(x, w, seed=1), (x, w), late)
+    stream.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [E4M3, E5M2])
+def test_products_of_subnormal_values(cuda, dtype):
+    """Zeros and the three smallest magnitudes of the format, through each kind of instruction."""
+    lowest = 2.0 ** (oracle.FORMATS[dtype][1] - oracle.FORMATS[dtype][0])
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    for m in (5, 40, 2100):
+        a, b = ((torch.randint(-3, 4, (rows, 256), device=cuda, generator=gen) * lowest).to(dtype)
+                for rows in (m, 2000))
+        for scales in (torch.float8_e8m0fnu, torch.float32):
+            operands = [BlockScaled(t, torch.ones(t.shape[0], 2, device=cuda).to(scales)) for t in (a, b)]
+            want, magnitude = oracle.product(*operands)
+            assert float(want.abs().max()) > 0
+            for out in (torch.float32, torch.bfloat16):
+                got = sr_states.block_matmul(*operands, out_dtype=out)
+                inner = 256 * 2.0**-24 + (0 if out == torch.float32 else 2.0**-13)
+                limit = HALF_ULP[out] * want.abs() + inner * magnitude * (1 + HALF_ULP[out])
+                assert float(((got.double() - want).abs() - limit).max()) <= 0
+
+
+@pytest.mark.parametrize("rule", ["nearest", "stochastic"])
+def test_cast_of_many_columns_alone(cuda, rule):
+    x = _values((4100, 2050), cuda, 1, torch.bfloat16)
+    got = sr_states.block_cast(x, dtype=E5M2, axis=0, rounding=rule, seed=9)
+    value, scale = oracle.block_cast(x, E5M2, rule, False, 0, 9)
+    assert torch.equal(got.data.double(), value) and torch.equal(got.scale.double(), scale)

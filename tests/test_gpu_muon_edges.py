@@ -106,3 +106,36 @@ def test_orthogonalize_on_both_sides_of_the_tile_shapes(cuda, shape):
     got = sr_states.orthogonalize(x)
     for g, one in zip(got.view(-1, *shape[-2:])[::6], x.view(-1, *shape[-2:])[::6]):
         assert oracle.relative(g, oracle.orthogonalize(one)) < LIMIT
+
+
+def test_batches_beyond_a_launch(cuda):
+    """More matrices than a launch takes, too large for one workgroup each."""
+    x = _matrix((70, 90, 130), cuda, 1)
+    got = sr_states.orthogonalize(x)
+    for k in (0, 63, 64, 69):
+        assert oracle.relative(got[k], oracle.orthogonalize(x[k])) < LIMIT
+    params = [torch.nn.Parameter(t.clone()) for t in x]
+    grads = _matrix((70, 90, 130), cuda, 2)
+    for p, g in zip(params, grads):
+        p.grad = g.clone()
+    sr_states.MuonHip(params, lr=0.5, momentum=0.9, seed=1).step()
+    for k in (0, 63, 64, 69):
+        update = 0.5 * oracle.orthogonalize(grads[k] * 0.9 + grads[k])
+        off = float((params[k].detach().double() - (x[k].double() - update)).norm())
+        assert off <= LIMIT * float(update.norm()) + 2.0**-22 * float(x[k].norm())
+
+
+def test_step_on_a_side_stream(cuda):
+    params = [_matrix((200, 300), cuda, k) for k in range(3)]
+    momentum = params[2].bfloat16()
+    copies = params[0].clone(), momentum.clone()
+    sr_states.hip_muon_step_(copies[0], params[1], copies[1], lr=0.1, momentum_factor=0.9, seed=1)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        late = params[1].clone()
+        for _ in range(20):
+            late = late * 1.0
+        sr_states.hip_muon_step_(params[0], late, momentum, lr=0.1, momentum_factor=0.9, seed=1)
+    stream.synchronize()
+    assert torch.equal(params[0], copies[0]) and torch.equal(momentum, copies[1])
