@@ -284,7 +284,10 @@ class MuonHip(StateOptimizer):
 
     def add_param_group(self, param_group):
         params = param_group["params"]
-        params = [params] if isinstance(params, torch.Tensor) else list(params)
+        if isinstance(params, torch.Tensor):
+            params = [params]
+        elif not isinstance(params, set):  # which torch refuses, below
+            params = list(params)
         for parameter in params:
             # Named parameters come as (name, parameter).
             matrix = parameter[1] if isinstance(parameter, tuple) else parameter
