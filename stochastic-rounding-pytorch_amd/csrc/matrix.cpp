@@ -108,8 +108,10 @@ const at::Tensor& tensor(PyObject* object) {
   return THPVariable_Unpack(object);
 }
 
-// Device memory of a tensor that has elements.
+// Device memory of a tensor that has elements.  A lazily negated view (torch's negative bit) holds other values than its
+// memory: inputs are resolved before they come here.
 void* memory(const at::Tensor& x) {
+  if (x.is_neg()) value_error("lazily negated views cannot be used: call resolve_neg()");
   void* p = const_cast<void*>(x.const_data_ptr());
   if (!p && x.numel()) value_error("tensors without device memory cannot be used");
   return p;
@@ -142,8 +144,9 @@ void checked(int status) {
 }
 
 // The casts of x: by_rows (axis 1) and by_cols (axis 0), where asked for.  The caller has x's device current.
-void cast_into(const at::Tensor& x, int code, int rule, bool square, uint32_t seed, uint32_t offset, Scaled* by_rows,
+void cast_into(const at::Tensor& given, int code, int rule, bool square, uint32_t seed, uint32_t offset, Scaled* by_rows,
                Scaled* by_cols, void* stream) {
+  const at::Tensor x = given.resolve_neg();
   const int x_code = dtype_code(x.scalar_type());
   if (!wide(x_code)) type_error("expected FP32, BF16 or FP16 input, got " + name_of(x.scalar_type()));
   if (x.dim() != 2) value_error("block_cast takes a matrix, not " + std::to_string(x.dim()) + " dimensions");
@@ -435,7 +438,7 @@ PyObject* orthogonalize(PyObject*, PyObject* args) {
         const auto options = at::TensorOptions().device(x.device());
         out = at::empty(x.sizes(), options.dtype(scalar_type(out_code)));
         if (!x.numel()) return;
-        const at::Tensor from = x.detach().contiguous();
+        const at::Tensor from = x.detach().resolve_neg().contiguous();
         const int64_t rows = x.size(-2), cols = x.size(-1), size = rows * cols, batch = x.numel() / size;
         const int64_t one = std::max<int64_t>(g_workspace(1, rows, cols), 1);
         const int64_t each = std::min<int64_t>({batch, SR_MATRIX_BATCH, std::max<int64_t>(static_cast<int64_t>(limit) / one, 1)});

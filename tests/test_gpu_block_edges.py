@@ -248,3 +248,28 @@ def test_cast_of_many_columns_alone(cuda, rule):
     got = sr_states.block_cast(x, dtype=E5M2, axis=0, rounding=rule, seed=9)
     value, scale = oracle.block_cast(x, E5M2, rule, False, 0, 9)
     assert torch.equal(got.data.double(), value) and torch.equal(got.scale.double(), scale)
+
+
+def test_lazily_negated_views(cuda):
+    """Imaginary parts of conjugates, among others, are views whose memory holds the opposite values."""
+    x, w, dy = _values((40, 60), cuda, 1), _values((30, 60), cuda, 2), _values((40, 30), cuda, 3)
+
+    def view(t):
+        negated = torch._neg_view(-t)
+        assert negated.is_neg() and torch.equal(negated, t)
+        return negated
+
+    def gradients(x, dy):
+        leaf = w.clone().requires_grad_()
+        y = sr_states.block_linear(x, leaf, seed=1)
+        return y, *torch.autograd.grad(y, leaf, dy)
+
+    for got, want in zip(gradients(view(x), view(dy)), gradients(x, dy)):
+        assert torch.equal(got, want)
+    assert torch.equal(sr_states.orthogonalize(view(x)), sr_states.orthogonalize(x))
+    for axis in (0, 1):
+        got, want = (sr_states.block_cast(t, axis=axis, seed=1) for t in (view(x), x))
+        assert torch.equal(got.dequantize(), want.dequantize())
+    q = sr_states.block_cast(x)
+    with pytest.raises(ValueError, match="negated"):
+        sr_states.block_matmul(q, q, out=view(_values((40, 40), cuda, 4)))
