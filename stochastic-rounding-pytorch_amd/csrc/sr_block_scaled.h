@@ -24,11 +24,13 @@ namespace sr {
 //            each value
 //   parts    workgroups of one orientation each, smaller than a tile: for one
 //            orientation alone, and for both of so few tiles that the chip's CUs
-//            would idle (measured, nearest: 128 tiles 5.4 us against 6.2, 256
-//            tiles 7.5 against 6.9; stochastic 256 tiles 12.1 against 9.6)
+//            would idle (parts against whole, nearest: 128 tiles 5.6 us and 6.4, 192
+//            level at 6.8, 256 7.6 and 7.0; stochastic: 128 tiles 7.4 and 8.9, 192
+//            10.2 and 9.4, 256 11.5 and 9.6)
 //
-// 8192 x 2048 BF16, 67 MB with both results (13 us at a copy's rate): whole 17 us
-// nearest, 24 stochastic, square 14.4; rows alone 11, 15.  The stochastic
+// 8192 x 2048 BF16 to E4M3, calls one after the other; 67 MB with both results (13
+// us at a copy's rate), 50 with one (10): whole 17 us nearest, 23.5 stochastic,
+// square 14 and 18, rows alone 11 and 15, columns alone 12 and 16.  The stochastic
 // ones are bound by arithmetic, half of it the hash (31 operations for a value
 // of both orientations, of which the hash is 17).
 // ---------------------------------------------------------------------------
@@ -406,10 +408,13 @@ __global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void bloc
 // instruction per 16 x 16 results.  Tiles of 128 x 128 results and of 64 x 64
 // (see tile_by_count); rows of at most 16 take the kernel at the end.
 //
-// Large products are bound by the card's power: 8192 x 8192 x 2048 takes 146 us
-// (1880 TFLOP/s) in a kernel by itself and 175 us call after call, alike with
-// 256 x 256 tiles.  Small ones are bound by latency: 4.3 us of arguments, first
-// stage and result, then 0.5 to 1 us a stage (501 x 2304 x 768: 6.7 us).
+// 8192 x 8192 x 2048 takes 144 us (1900 TFLOP/s) when the card is rested: the matrix
+// cores work 43% of the cycles and the LDS 33%, and every stage of a workgroup
+// waits once for its loads.  Call after call it takes 145 to 175 as the clock
+// falls under the load (1.7 GHz after 20 calls, 2.4 at rest; zeros as data: 122), and
+// 256 x 256 tiles are level.  Small ones are bound by latency: 4.3 us of
+// arguments, first stage and result, then 0.5 to 1 us a stage (501 x 2304 x 768: 6.7
+// us).
 // ---------------------------------------------------------------------------
 struct BlockProductArgs {
   Operand a, b;

@@ -239,7 +239,7 @@ __global__ __launch_bounds__(kNsLoadThreads) void ns_load_kernel(NsArgs a, Matri
 // X = V / (|V|_F + eps) and its FP16 copies H and H^T, one 64 x 64 tile per
 // workgroup.  V comes from the caller's matrices (GE), which is less to read
 // and spares writing it in FP32 first, or with GE < 0 from X.  Bound by memory:
-// 8192 x 2048 BF16 takes 16 us for the sum and 36 for the rest (161 MB, 4.5
+// 8192 x 2048 BF16 takes 18 us for the sum and 36 for the rest (168 MB, 4.7
 // TB/s); 40 and 31 where the first wrote V for the second.
 template <int GE>
 __global__ __launch_bounds__(kNsThreads) void ns_scale_kernel(NsArgs a, MatrixTable t) {
@@ -539,9 +539,10 @@ __device__ __forceinline__ void with_result(const NsArgs& a, F&& store) {
 //   kNsStep        X <- a X - s H + (P + s I) H, and the new H and H^T
 //   kNsLast        the same into the results or the parameters; TURNED where
 //                  these are the transpose of the workspace's orientation
-// Few tiles are bound by the latency of a tile's walk (768 x 2304: G 12.5 us, P
-// 6.9, step 11.9), many by what a CU reads from its L2 (G of 8 x 2048 x 2048
-// 109 us, 710 TFLOP/s of the computed half and diagonal).
+// Few tiles are bound by the latency of a tile's walk (768 x 2304: G 12.6 us, P
+// 7.2, step 11.6), many by what a CU reads from its L2 (G of 8 x 2048 x 2048
+// 108 us, 676 TFLOP/s of the computed half and diagonal; G of 2048 x 8192, 528
+// tiles of 64 x 64 on 256 CUs, 77 us with the matrix cores busy 20% of the cycles).
 template <int OP, class S, bool TURNED>
 __global__ __launch_bounds__(S::kThreads, S::kMinWaves) void ns_product_kernel(NsArgs a, uint32_t tiles_m, uint32_t tiles_n,
                                                                     uint32_t tiles, uint32_t matrices, MatrixTable t) {
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(S::kThreads, S::kMinWaves) void ns_product_kernel(N
   });
 }
 
-// The same launches on wide tiles.  The step of 8192 x 2048 takes 91 us: 51 for
+// The same launches on wide tiles.  The step of 8192 x 2048 takes 92 us: 51 for
 // the product (1355 TFLOP/s) and the rest for 192 MB of X, H and H^T at 4.6
 // TB/s.
 template <int OP, bool TURNED>
