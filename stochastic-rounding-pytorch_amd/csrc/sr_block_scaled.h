@@ -514,23 +514,41 @@ __device__ __forceinline__ void store_chunks(const BlockProductArgs& g, char* ld
 enum ProductMode { kExponents, kFactors, kWide, kProductModes };
 
 // A block's sum times two FP32 scales.  It lies between 2^-32 and 2^39 or is 0,
-// but the scales' product, or that of the sum and one scale, can leave FP32's range
-// on the way to a result inside it (2^100 by 2^30 with a small sum gave infinity,
-// with a sum of 0 NaN).  Scales between 2^-62 and 2^62, and zeros, are `near`:
-// their product is safe, and one multiplication and the fused one into the result do.  With others each
-// scale is taken as two factors of about half its exponent.  With T the
-// result's exponent and S the sum's, both partial products below are then
-// near 2^((T + S) / 2) and 2^((T - S) / 2): inside the range wherever 2^T is.
-__device__ __forceinline__ bool near_scale(uint32_t bits) {
-  const uint32_t a = bits & 0x7FFFFFFFu;
-  return a == 0 || a - (65u << 23) < (124u << 23);
-}
+// but the scales' product, or that of the sum and one scale, can leave FP32's
+// range on the way to a result inside it (2^100 by 2^30 with a small sum gave
+// infinity, with a sum of 0 NaN).  Scales between 2^-62 and 2^62, and zeros, are
+// `near`: their product is safe, and one multiplication and the fused one into
+// the result do.  A tile that has others looks at its scales' largest and
+// smallest products, and where these are no normal numbers it sums again with
+// each scale as two factors of about half its exponent.  With T the result's
+// exponent and S the sum's, both partial products below are then near
+// 2^((T + S) / 2) and 2^((T - S) / 2): inside the range wherever 2^T is.  (A tile
+// that sums again takes four times as long; one that only looks, 1 to 2 us more.)
+struct ScaleRange {
+  uint32_t high = 0, low = 0xFFFFFFFFu;  // magnitudes; the lowest is of those that are not 0, less one
+  __device__ __forceinline__ void add(uint32_t bits) {
+    const uint32_t m = bits & 0x7FFFFFFFu;
+    high = umax(high, m);
+    low = umin(low, m - 1);
+  }
+  __device__ __forceinline__ void add(const ScaleRange& other) {
+    high = umax(high, other.high);
+    low = umin(low, other.low);
+  }
+  __device__ __forceinline__ bool near() const { return high <= (189u << 23) && low >= (65u << 23) - 1; }
+  __device__ __forceinline__ bool zeros() const { return low == 0xFFFFFFFFu; }
+  // Whether every product with a factor of `other`'s is 0 or a normal number.
+  __device__ __forceinline__ bool normal_with(const ScaleRange& other) const {
+    if (zeros() || other.zeros()) return umax(high, other.high) < kInfBits;
+    return bits_f32(high) * bits_f32(other.high) <= 0x1p127f && bits_f32(low + 1) * bits_f32(other.low + 1) >= 0x1p-126f;
+  }
+};
 
 // The power of two with half the exponent of `s`, rounded down; subnormal numbers, infinities and NaN count as 2^-127
 // and 2^128.
 __device__ __forceinline__ uint32_t half_power_bits(float s) { return (((f32_bits(s) >> 23 & 255u) + 127u) >> 1) << 23; }
 
-// acc + part * sa * sb; FAR: any scales, otherwise near ones.
+// acc + part * sa * sb; FAR: any scales, otherwise such as have a normal product.
 template <bool FAR>
 __device__ __forceinline__ float add_scaled(float acc, float part, float sa, float sb) {
   if constexpr (FAR) {
@@ -561,37 +579,69 @@ struct ScaleArea {
   static constexpr int kRow = 36, kFill = 32, kBytes = (S::BM + S::BN) * kRow;
   static constexpr int kPeriod = MODE == kExponents ? kFill : kFill / 4;
 
-  // Blocks [first, first + kPeriod) of every row; rows past the end repeat the last one.  Sets *far where a factor is
-  // not a near one.
-  static __device__ void fill(char* area, int* far, const BlockProductArgs& g, int row0, int col0, int first, int total) {
+  // Row r of the area for blocks [first, first + kPeriod), of which `total` - first are there (values past them mean
+  // nothing): rows of A, then of B; rows past the operand's end repeat its last one.
+  static __device__ __forceinline__ void row(const BlockProductArgs& g, int row0, int col0, int r, int first, int total,
+                                             int (&words)[8]) {
     const int size = g.scale_f32 ? 4 : 1;
-    bool near = true;
+    const bool of_a = r < S::BM;
+    const int at = of_a ? row0 + r : col0 + r - S::BM, rows = of_a ? g.m : g.n;
+    const char* from = (of_a ? g.scale_a : g.scale_b) +
+                       (((at < rows ? at : rows - 1) >> (of_a ? g.shift_a : g.shift_b)) * (of_a ? g.ld_scale_a : g.ld_scale_b) + first) * size;
+    const int64_t end = static_cast<int64_t>(total - first) * size;
+    const i32x4 lo = load_chunk(from, 0, end);
+    if (MODE == kWide && !g.scale_f32) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) words[j] = static_cast<int>(f32_bits(e8m0_value(lo[j >> 2] >> (8 * (j & 3)) & 255)));
+      return;
+    }
+    const i32x4 hi = load_chunk(from, 16, end);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      words[j] = lo[j];
+      words[4 + j] = hi[j];
+    }
+  }
+
+  // These blocks of every row.  Sets *far where a factor is not a near one.
+  static __device__ void fill(char* area, int* far, const BlockProductArgs& g, int row0, int col0, int first, int total) {
+    ScaleRange range;
     for (int r = threadIdx.x; r < S::BM + S::BN; r += S::kThreads) {
-      const bool of_a = r < S::BM;
-      const int at = of_a ? row0 + r : col0 + r - S::BM, rows = of_a ? g.m : g.n;
-      const char* from = (of_a ? g.scale_a : g.scale_b) +
-                         (((at < rows ? at : rows - 1) >> (of_a ? g.shift_a : g.shift_b)) * (of_a ? g.ld_scale_a : g.ld_scale_b) + first) * size;
-      const int64_t end = static_cast<int64_t>(total - first) * size;
+      int words[8];
+      row(g, row0, col0, r, first, total, words);
       int* to = reinterpret_cast<int*>(area + r * kRow);
-      const i32x4 lo = load_chunk(from, 0, end);
-      if (MODE == kWide && !g.scale_f32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const uint32_t bits = f32_bits(e8m0_value(lo[j >> 2] >> (8 * (j & 3)) & 255));
-          near = near && near_scale(bits);
-          to[j] = static_cast<int>(bits);
-        }
-        continue;
-      }
-      const i32x4 hi = load_chunk(from, 16, end);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (MODE != kExponents) near = near && near_scale(lo[j]) && near_scale(hi[j]);
-        to[j] = lo[j];
-        to[4 + j] = hi[j];
+      for (int j = 0; j < 8; ++j) {
+        if (MODE != kExponents) range.add(j < total - first ? words[j] : 0);
+        to[j] = words[j];
       }
     }
-    if (MODE != kExponents && !near) *far = 1;
+    if (MODE != kExponents && !range.near()) *far = 1;
+  }
+
+  // Whether every product of a factor of A and one of B that a tile's rows hold is 0 or a normal number, for tiles with
+  // factors that are not near ones: what the ordinary walk summed is right then.  `scratch`: LDS, an entry a wave.
+  // Every wave is done with the LDS, before and after.
+  static __device__ bool products_are_normal(ScaleRange* scratch, const BlockProductArgs& g, int row0, int col0, int total) {
+    static_assert(S::BM + S::BN <= S::kThreads && S::BM % 64 == 0 && S::BN % 64 == 0, "a row for a thread, waves of one operand");
+    ScaleRange range;
+    if (static_cast<int>(threadIdx.x) < S::BM + S::BN) {
+      for (int first = 0; first < total; first += kPeriod) {
+        int words[8];
+        row(g, row0, col0, threadIdx.x, first, total, words);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) range.add(j < total - first ? words[j] : 0);
+      }
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) range.add(ScaleRange{__shfl_xor(range.high, d), __shfl_xor(range.low, d)});
+    if ((threadIdx.x & 63) == 0) scratch[threadIdx.x >> 6] = range;
+    lds_barrier();
+    ScaleRange sides[2];
+#pragma unroll
+    for (int w = 0; w < (S::BM + S::BN) / 64; ++w) sides[w * 64 < S::BM ? 0 : 1].add(scratch[w]);
+    lds_barrier();
+    return sides[0].normal_with(sides[1]);
   }
 };
 
@@ -681,7 +731,7 @@ __device__ __forceinline__ void block_mma(f32x4& acc, const Fragment<MODE, FA>& 
   }
 }
 
-// A tile's sums once more where some of its scales are not near ones: a stage at a time by the first group of waves,
+// A tile's sums once more where products of its scales leave FP32's normal range: a stage at a time by the first group of waves,
 // with few values in registers, so that the ordinary walk keeps its own.  Every wave is done with the LDS, before and
 // after.
 template <int MODE, int FA, int FB, class S>
@@ -824,7 +874,8 @@ __global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void block_product_k
   }
   stage_barrier();
   if constexpr (MODE != kExponents) {
-    if (__builtin_amdgcn_readfirstlane(*far))
+    if (__builtin_expect(__builtin_amdgcn_readfirstlane(*far), 0) &&
+        !Area::products_are_normal(reinterpret_cast<ScaleRange*>(lds), g, row0, col0, stages))
       sum_far_scales<MODE, FA, FB, S>(g, lds, area, far, row0, col0, wave, group, stages, acc);
   }
   add_groups<S>(lds, group, acc);

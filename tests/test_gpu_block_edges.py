@@ -273,3 +273,33 @@ def test_lazily_negated_views(cuda):
     q = sr_states.block_cast(x)
     with pytest.raises(ValueError, match="negated"):
         sr_states.block_matmul(q, q, out=view(_values((40, 40), cuda, 4)))
+
+
+@pytest.mark.parametrize("k", [128, 768, 1024, 1100])
+@pytest.mark.parametrize("m, n", [(40, 70), (300, 2000), (2100, 2000)])
+def test_scales_of_one_value_in_either_type_give_one_result(cuda, m, n, k):
+    """Powers of two as E8M0 and as FP32, for whole and partial runs of blocks."""
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    operands = []
+    for rows in (m, n):
+        codes = torch.randint(100, 150, (rows, -(-k // 128)), device=cuda, generator=gen, dtype=torch.uint8)
+        operands.append((_values((rows, k), cuda, rows).to(E4M3), codes.view(torch.float8_e8m0fnu)))
+    got, want = (sr_states.block_matmul(*(BlockScaled(data, scale.to(dtype)) for data, scale in operands),
+                                        out_dtype=torch.float32) for dtype in (torch.float8_e8m0fnu, torch.float32))
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m, n, k", [(40, 70, 300), (300, 2000, 1024), (2100, 2000, 208)])
+def test_one_small_scale_leaves_the_other_rows_alone(cuda, m, n, k, out):
+    """A row scaled by 2^-80, as of a gradient of next to nothing, has products that are normal numbers."""
+    gen = torch.Generator(device=cuda).manual_seed(4)
+    data = [_values((rows, k), cuda, rows).to(E4M3) for rows in (m, n)]
+    scales = [torch.rand(rows, -(-k // 128), device=cuda, generator=gen) + 0.1 for rows in (m, n)]
+    b = BlockScaled(data[1], scales[1])
+    plain = sr_states.block_matmul(BlockScaled(data[0], scales[0]), b, out_dtype=out)
+    scales[0][7] *= 2.0**-80
+    small = sr_states.block_matmul(BlockScaled(data[0], scales[0]), b, out_dtype=out)
+    others = torch.arange(m, device=cuda) != 7
+    assert torch.equal(small[others], plain[others])
+    assert torch.equal(small[7].float() * 2.0**80, plain[7].float())
