@@ -84,6 +84,65 @@ int sr_block_cast(const void* x, int64_t ldx, int64_t rows, int64_t cols, int x_
 int sr_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t k, void* out, int64_t ldo,
                     int out_dtype, void* stream);
 
+/* ---- rows sorted into groups ------------------------------------------- */
+
+/* Groups that one call takes. */
+#define SR_MATRIX_GROUPS 4096
+
+/* How many rows each of `count` groups has, in order from row 0 on: device
+ * memory, int64 where `wide`, else int32, read when the stream comes to it.
+ * Sizes below zero count as zero, and groups end where the matrix does. */
+typedef struct sr_groups {
+  const void* sizes;
+  int count;
+  int wide;
+} sr_groups;
+
+/* Columns of a matrix whose contracted axis is `rows` rows in `groups` groups
+ * that each start on a multiple of 128 columns: room for any sizes. */
+int64_t sr_grouped_columns(int64_t rows, int64_t groups);
+
+/* sr_block_cast with 1 x 128 blocks, whose blocks along the rows are those of
+ * each group by itself: in `by_cols` (wanted; data cols x
+ * sr_grouped_columns(rows, count)) a group's columns start on the next
+ * multiple of 128 behind the group before, and zeros with a scale of 1 fill
+ * what belongs to no row.  `by_rows` is that of sr_block_cast, with the rows
+ * behind the last group. */
+int sr_grouped_block_cast(const void* x, int64_t ldx, int64_t rows, int64_t cols, int x_dtype, int dtype, int rule,
+                          uint32_t seed, uint32_t offset, const sr_groups* groups, const sr_block_output* by_rows,
+                          const sr_block_output* by_cols, void* stream);
+
+/* One orientation of the casts of several matrices, `stride` bytes and
+ * `stride_scale` scales apart. */
+typedef struct sr_block_stack {
+  sr_block_output out;
+  int64_t stride;
+  int64_t stride_scale;
+} sr_block_stack;
+
+/* sr_block_cast of `count` matrices (at most SR_MATRIX_GROUPS), each by
+ * itself, `x_stride` elements apart.  Value (i, r, c) uses counter
+ * (i * rows + r) * cols + c + seed + offset. */
+int sr_stacked_block_cast(const void* x, int64_t x_stride, int64_t ldx, int64_t count, int64_t rows, int64_t cols, int x_dtype,
+                          int dtype, int rule, int square, uint32_t seed, uint32_t offset, const sr_block_stack* by_rows,
+                          const sr_block_stack* by_cols, void* stream);
+
+/* out[t] = a[t] b[i]^T for the rows t of every group i, where b is
+ * groups->count matrices, `b_stride` bytes and `b_stride_scale` scales apart;
+ * otherwise as sr_block_matmul.  Rows behind the last group become zeros with
+ * `zero_behind`, and keep what they hold without it. */
+int sr_grouped_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t b_stride, int64_t b_stride_scale,
+                            int64_t k, const sr_groups* groups, void* out, int64_t ldo, int out_dtype, int zero_behind,
+                            void* stream);
+
+/* out[i] = a[:, columns of group i] b[:, columns of group i]^T for every group,
+ * zeros for one without rows; results are `out_stride` elements apart.  Both
+ * matrices have `columns` columns laid out as sr_grouped_block_cast's `by_cols`
+ * (a multiple of 128; rows start on 16 bytes).  The values behind a group's
+ * rows in its last block of 128 take part: a cast leaves zeros there. */
+int sr_grouped_block_contract(const sr_block_matrix* a, const sr_block_matrix* b, int64_t columns, const sr_groups* groups,
+                              void* out, int64_t ldo, int64_t out_stride, int out_dtype, void* stream);
+
 /* ---- orthogonalised updates -------------------------------------------- */
 
 /* Newton-Schulz orthogonalisation of a matrix X (rows x cols): X / (|X|_F +

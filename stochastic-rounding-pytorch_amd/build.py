@@ -60,7 +60,10 @@ def units() -> list[tuple[Path, list[str], Path]]:
     jobs.append((CSRC / "sr_matrix_abi.hip", [], BUILD / "sr_matrix_abi.o"))
     jobs.append((CSRC / "sr_block_cast.hip", [], BUILD / "sr_block_cast.o"))
     jobs.append((CSRC / "sr_newton_schulz.hip", [], BUILD / "sr_newton_schulz.o"))
+    jobs.append((CSRC / "sr_grouped_abi.hip", [], BUILD / "sr_grouped_abi.o"))
+    jobs.append((CSRC / "sr_grouped_cast.hip", [], BUILD / "sr_grouped_cast.o"))
     for e5m2 in range(2):
+        jobs.append((CSRC / "sr_grouped_product.hip", [f"-DSR_A_E5M2={e5m2}"], BUILD / f"sr_grouped_product_a{e5m2}.o"))
         jobs.append((CSRC / "sr_block_product.hip", [f"-DSR_A_E5M2={e5m2}"], BUILD / f"sr_block_product_a{e5m2}.o"))
     for enc in range(9):
         jobs.append((CSRC / "sr_adamw.hip", [f"-DSR_M_ENC={enc}"], BUILD / f"sr_adamw_m{enc}.o"))

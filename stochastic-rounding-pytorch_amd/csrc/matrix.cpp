@@ -6,7 +6,8 @@
 // makes the tensor checks, allocates the results and calls the C ABI's entry
 // points through the addresses the Python side binds once.
 //
-// bind(block_cast, block_matmul, orthogonalize, orthogonalize_workspace)
+// bind(block_cast, block_matmul, orthogonalize, orthogonalize_workspace, grouped_columns, grouped_block_cast,
+//      stacked_block_cast, grouped_block_matmul, grouped_block_contract)
 //   Keep the addresses of these sr_ entry points, taken from the loaded library.
 //
 // block_cast(x, code, rule, square, axes, seed, offset, stream) -> tuple or int
@@ -26,6 +27,14 @@
 //
 // orthogonalize(x, out_code, a, b, c, eps, steps, batch limit bytes, stream) -> tensor or int
 //
+// grouped_cast(x, sizes, code, rule, square, axes, seed, offset, stream) -> tuple or int
+//   As block_cast, of a matrix whose rows are in groups of `sizes`, or (None) of a stack of matrices.
+// grouped_matmul(a_data, a_scale, b_data, b_scale, sizes, out_code, out, stream) -> tensor or int
+//   Each group's rows of a by its matrix of b, or its columns of a by its columns of b where b is a matrix.
+// grouped_linear_forward(x, weight, sizes, formats, seed, need_x, need_weight, stream)
+// grouped_linear_backward(dy, sizes, x_t data, x_t scale, w_t data, w_t scale, formats, seed, dx_code, dw_code, stream)
+//   As linear_forward and linear_backward.
+//
 // Errors of the tensors raise TypeError or ValueError before anything is
 // launched.  Every entry runs with the first tensor's device current and the
 // GIL released around the launch; `stream` is the raw handle of a stream on
@@ -44,6 +53,7 @@
 #include <exception>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "../../include/sr_matrix_hip.h"
 
@@ -57,6 +67,11 @@ CastFn g_cast = nullptr;
 MatmulFn g_matmul = nullptr;
 OrthogonalizeFn g_orthogonalize = nullptr;
 WorkspaceFn g_workspace = nullptr;
+decltype(&sr_grouped_columns) g_columns = nullptr;
+decltype(&sr_grouped_block_cast) g_grouped_cast = nullptr;
+decltype(&sr_stacked_block_cast) g_stacked_cast = nullptr;
+decltype(&sr_grouped_block_matmul) g_grouped_matmul = nullptr;
+decltype(&sr_grouped_block_contract) g_grouped_contract = nullptr;
 PyObject* g_out_of_memory = nullptr;  // torch.OutOfMemoryError
 
 // A refusal, raised as `type`.
@@ -119,9 +134,10 @@ void* memory(const at::Tensor& x) {
 
 int64_t blocks(int64_t n) { return (n + SR_BLOCK - 1) / SR_BLOCK; }
 
-// The distance between rows of a matrix with consecutive columns.
+// The distance between rows of a matrix with consecutive columns; an empty one has any strides.
 int64_t row_stride(const at::Tensor& x, const std::string& what) {
   const int64_t rows = x.size(0), cols = x.size(1);
+  if (!x.numel()) return std::max<int64_t>(cols, 1);
   const int64_t stride = rows > 1 ? x.stride(0) : std::max<int64_t>(cols, 1);
   if ((cols > 1 && x.stride(1) != 1) || stride < cols)
     value_error(what + " requires consecutive columns and rows that do not overlap");
@@ -166,6 +182,10 @@ void cast_into(const at::Tensor& given, int code, int rule, bool square, uint32_
                    by_cols ? &out[1] : nullptr, stream));
 }
 
+// The distance between matrices of a stack, and a matrix of it.
+int64_t stack_stride(const at::Tensor& x) { return x.size(0) > 1 ? x.stride(0) : 0; }
+at::Tensor matrix_of(const at::Tensor& x) { return x.dim() == 3 ? x.select(0, 0) : x; }
+
 sr_block_matrix operand(const at::Tensor& data, const at::Tensor& scale, const std::string& name) {
   const int code = dtype_code(data.scalar_type());
   if (code != SR_E4M3 && code != SR_E5M2) type_error(name + ": data must be FP8 (E4M3 or E5M2), got " + name_of(data.scalar_type()));
@@ -194,6 +214,44 @@ std::pair<uintptr_t, uintptr_t> span(const at::Tensor& x) {
   return {start, start + static_cast<uintptr_t>((last + 1) * x.element_size())};
 }
 
+std::string shape_of(at::IntArrayRef shape) {
+  std::string text;
+  for (int64_t n : shape) text += (text.empty() ? "" : " x ") + std::to_string(n);
+  return text;
+}
+
+// Makes `out` a new tensor of this shape and dtype where it is not defined, and else checks that it can take the result
+// of these operands; sets out_code.  Returns the distance between its rows.
+int64_t result_of(at::Tensor& out, at::IntArrayRef shape, int& out_code, const Scaled& a, const Scaled& b, const char* name) {
+  if (!out.defined()) {
+    if (out_code < 0) out_code = SR_BF16;
+    out = at::empty(shape, at::TensorOptions().device(a.data.device()).dtype(scalar_type(out_code)));
+    return shape.back();
+  }
+  if (!wide(dtype_code(out.scalar_type())) || (out_code >= 0 && dtype_code(out.scalar_type()) != out_code))
+    type_error("out has dtype " + name_of(out.scalar_type()));
+  out_code = dtype_code(out.scalar_type());
+  if (out.sizes() != shape || out.device() != a.data.device())
+    value_error("out must be a " + shape_of(shape) + " tensor on " + a.data.device().str());
+  int64_t stride = std::max<int64_t>(shape.back(), 1);
+  if (out.numel()) {
+    stride = row_stride(matrix_of(out), "out");
+    if (out.dim() == 3 && out.size(0) > 1 && out.stride(0) < (out.size(1) - 1) * stride + out.size(2))
+      value_error("out requires matrices that do not overlap");
+  }
+  const auto [start, end] = span(out);
+  for (const at::Tensor* t : {&a.data, &a.scale, &b.data, &b.scale}) {
+    const auto [first, last] = span(*t);
+    if (start < last && first < end) value_error("out must not overlap the operands");
+  }
+  // As torch's own out= functions: the write is not differentiable, and whoever saved the tensor must notice it.
+  if (out.requires_grad() && c10::GradMode::is_enabled())
+    throw Refusal(PyExc_RuntimeError,
+                  std::string("out requires grad, and ") + name + " records no gradients: call it under torch.no_grad()");
+  if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+  return stride;
+}
+
 // The caller has the operands' device current.
 at::Tensor matmul(const Scaled& a, const Scaled& b, int out_code, at::Tensor out, void* stream) {
   const sr_block_matrix left = operand(a.data, a.scale, "a"), right = operand(b.data, b.scale, "b");
@@ -202,28 +260,7 @@ at::Tensor matmul(const Scaled& a, const Scaled& b, int out_code, at::Tensor out
   if (b.data.size(1) != k)
     value_error("a and b contract " + std::to_string(k) + " and " + std::to_string(b.data.size(1)) + " values");
   if (left.scale_type != right.scale_type) type_error("a and b must have scales of one type");
-  const auto options = at::TensorOptions().device(a.data.device());
-  int64_t stride = n;
-  if (out.defined()) {
-    if (!wide(dtype_code(out.scalar_type())) || (out_code >= 0 && dtype_code(out.scalar_type()) != out_code))
-      type_error("out has dtype " + name_of(out.scalar_type()));
-    out_code = dtype_code(out.scalar_type());
-    if (out.dim() != 2 || out.size(0) != m || out.size(1) != n || out.device() != a.data.device())
-      value_error("out must be a " + std::to_string(m) + " x " + std::to_string(n) + " tensor on " + a.data.device().str());
-    stride = row_stride(out, "out");
-    const auto [start, end] = span(out);
-    for (const at::Tensor* t : {&a.data, &a.scale, &b.data, &b.scale}) {
-      const auto [first, last] = span(*t);
-      if (start < last && first < end) value_error("out must not overlap the operands");
-    }
-    // As torch's own out= functions: the write is not differentiable, and whoever saved the tensor must notice it.
-    if (out.requires_grad() && c10::GradMode::is_enabled())
-      throw Refusal(PyExc_RuntimeError, "out requires grad, and block_matmul records no gradients: call it under torch.no_grad()");
-    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
-  } else {
-    if (out_code < 0) out_code = SR_BF16;
-    out = at::empty({m, n}, options.dtype(scalar_type(out_code)));
-  }
+  const int64_t stride = result_of(out, {m, n}, out_code, a, b, "block_matmul");
   if (m && n) checked(g_matmul(&left, &right, k, memory(out), stride, out_code, stream));
   return out;
 }
@@ -238,7 +275,126 @@ at::Tensor as_rows(const at::Tensor& x) {
   return flat;
 }
 
-bool bound() { return g_cast && g_matmul && g_orthogonalize && g_workspace; }
+// ---- rows sorted into groups ----
+
+// The groups that a tensor of sizes describes, on `device`.
+sr_groups groups_of(const at::Tensor& sizes, const at::Device& device) {
+  const bool wide = sizes.scalar_type() == c10::ScalarType::Long;
+  if (!wide && sizes.scalar_type() != c10::ScalarType::Int) type_error("sizes must be torch.int32 or torch.int64, got " + name_of(sizes.scalar_type()));
+  if (sizes.dim() != 1 || !sizes.is_contiguous()) value_error("sizes must be one row of consecutive numbers");
+  if (sizes.device() != device) value_error("sizes must be on the same GPU device");
+  if (sizes.size(0) > SR_MATRIX_GROUPS)
+    value_error(std::to_string(sizes.size(0)) + " groups: at most " + std::to_string(SR_MATRIX_GROUPS));
+  return {memory(sizes), static_cast<int>(sizes.size(0)), wide};
+}
+
+// The casts of the rows of x, blocks along the rows ending with each group.
+void cast_groups_into(const at::Tensor& given, const at::Tensor& sizes, int code, int rule, uint32_t seed, uint32_t offset,
+                      Scaled* by_rows, Scaled* by_cols, void* stream) {
+  const at::Tensor x = given.resolve_neg();
+  const int x_code = dtype_code(x.scalar_type());
+  if (!wide(x_code)) type_error("expected FP32, BF16 or FP16 input, got " + name_of(x.scalar_type()));
+  if (x.dim() != 2) value_error("groups are rows of a matrix, not of " + std::to_string(x.dim()) + " dimensions");
+  if (!x.is_cuda()) value_error("grouped_block_cast requires a GPU tensor");
+  const sr_groups groups = groups_of(sizes, x.device());
+  const int64_t stride = row_stride(x, "grouped_block_cast"), rows = x.size(0), cols = x.size(1);
+  const int64_t columns = g_columns(rows, groups.count);
+  if (by_cols) *by_cols = new_scaled(cols, columns, code, false, x.device());
+  if (!by_cols || !columns) {  // nothing depends on the groups
+    if (by_rows) cast_into(x, code, rule, false, seed, offset, by_rows, nullptr, stream);
+    return;
+  }
+  sr_block_output out[2] = {};
+  if (by_rows) {
+    *by_rows = new_scaled(rows, cols, code, false, x.device());
+    out[0] = {memory(by_rows->data), memory(by_rows->scale), by_rows->data.stride(0), std::max<int64_t>(blocks(cols), 1)};
+  }
+  out[1] = {memory(by_cols->data), memory(by_cols->scale), by_cols->data.stride(0), blocks(columns)};
+  if (cols)
+    checked(g_grouped_cast(memory(x), stride, rows, cols, x_code, code, rule, seed, offset, &groups, by_rows ? &out[0] : nullptr,
+                           &out[1], stream));
+}
+
+// A stack of matrices, rows on 16 bytes.
+Scaled new_stack(int64_t count, int64_t rows, int64_t k, int code, bool square, const at::Device& device) {
+  const auto options = at::TensorOptions().device(device);
+  const int64_t ld = (k + 15) / 16 * 16;
+  return {at::empty_strided({count, rows, k}, {rows * ld, ld, 1}, options.dtype(scalar_type(code))),
+          at::empty({count, square ? blocks(rows) : rows, blocks(k)}, options.dtype(c10::ScalarType::Float8_e8m0fnu))};
+}
+
+// The casts of every matrix of x.
+void cast_stack_into(const at::Tensor& given, int code, int rule, bool square, uint32_t seed, uint32_t offset, Scaled* by_rows,
+                     Scaled* by_cols, void* stream) {
+  const at::Tensor x = given.resolve_neg();
+  const int x_code = dtype_code(x.scalar_type());
+  if (!wide(x_code)) type_error("expected FP32, BF16 or FP16 input, got " + name_of(x.scalar_type()));
+  if (x.dim() != 3) value_error("a stack of matrices has three dimensions, not " + std::to_string(x.dim()));
+  if (!x.is_cuda()) value_error("grouped_block_cast requires a GPU tensor");
+  const int64_t count = x.size(0), rows = x.size(1), cols = x.size(2);
+  if (count > SR_MATRIX_GROUPS) value_error(std::to_string(count) + " matrices: at most " + std::to_string(SR_MATRIX_GROUPS));
+  sr_block_stack out[2] = {};
+  auto make = [&](Scaled* to, sr_block_stack& stack, int64_t r, int64_t c) {
+    if (!to) return;
+    *to = new_stack(count, r, c, code, square, x.device());
+    stack = {{memory(to->data), memory(to->scale), to->data.stride(1), std::max<int64_t>(blocks(c), 1)},
+             to->data.stride(0),
+             to->scale.size(1) * to->scale.size(2)};
+  };
+  make(by_rows, out[0], rows, cols);
+  make(by_cols, out[1], cols, rows);
+  if (x.numel())
+    checked(g_stacked_cast(memory(x), stack_stride(x), row_stride(matrix_of(x), "grouped_block_cast"), count, rows, cols, x_code,
+                           code, rule, square, seed, offset, by_rows ? &out[0] : nullptr, by_cols ? &out[1] : nullptr, stream));
+}
+
+// The caller has the operands' device current.
+at::Tensor grouped_product(const Scaled& a, const Scaled& b, const at::Tensor& sizes, int out_code, at::Tensor out, void* stream) {
+  const bool stacked = b.data.dim() == 3;
+  const sr_block_matrix left = operand(a.data, a.scale, "a");
+  if (stacked && (b.scale.dim() != 3 || b.scale.size(0) != b.data.size(0)))
+    value_error("b: a stack of matrices has a stack of as many scales");
+  const sr_groups groups = groups_of(sizes, a.data.device());
+  const int64_t k = a.data.size(1);
+  if (b.data.device() != a.data.device()) value_error("a and b must be on the same GPU device");
+  if (b.data.dim() < 2 || b.data.size(-1) != k)
+    value_error("a and b contract " + std::to_string(k) + " and " + std::to_string(b.data.dim() ? b.data.size(-1) : 0) + " values");
+  if (stacked && b.data.size(0) != groups.count)
+    value_error("b has " + std::to_string(b.data.size(0)) + " matrices for " + std::to_string(groups.count) + " groups");
+  const int64_t m = left.rows, n = b.data.size(-2), count = groups.count;
+  const bool given = out.defined();
+  if (stacked) {
+    const int64_t stride = result_of(out, {m, n}, out_code, a, b, "grouped_block_matmul");
+    if (!m || !n) return out;
+    if (!count) return given ? out : out.zero_();
+    const sr_block_matrix right = operand(matrix_of(b.data), matrix_of(b.scale), "b");
+    if (left.scale_type != right.scale_type) type_error("a and b must have scales of one type");
+    checked(g_grouped_matmul(&left, &right, stack_stride(b.data), stack_stride(b.scale), k, &groups, memory(out), stride, out_code,
+                             !given, stream));
+    return out;
+  }
+  const sr_block_matrix right = operand(b.data, b.scale, "b");
+  if (left.scale_type != right.scale_type) type_error("a and b must have scales of one type");
+  if (k % SR_BLOCK) value_error("the columns of padded groups are a multiple of " + std::to_string(SR_BLOCK) + ", not " + std::to_string(k));
+  for (const sr_block_matrix* x : {&left, &right})
+    if (k && (reinterpret_cast<uintptr_t>(x->data) % 16 || x->ld % 16)) value_error("rows of padded groups must start on 16 bytes");
+  const int64_t stride = result_of(out, {count, m, n}, out_code, a, b, "grouped_block_matmul");
+  if (out.numel())
+    checked(g_grouped_contract(&left, &right, k, &groups, memory(out), stride, out.size(0) > 1 ? out.stride(0) : m * stride, out_code,
+                               stream));
+  return out;
+}
+
+// A stack with consecutive columns and rows that do not overlap, copied only where its layout needs it.
+at::Tensor as_stack(const at::Tensor& x) {
+  const bool copy = (x.size(2) > 1 && x.stride(2) != 1) || (x.size(1) > 1 && x.stride(1) < x.size(2));
+  return copy ? x.contiguous() : x;
+}
+
+bool bound() {
+  return g_cast && g_matmul && g_orthogonalize && g_workspace && g_columns && g_grouped_cast && g_stacked_cast &&
+         g_grouped_matmul && g_grouped_contract;
+}
 
 // Runs `body` as the entries promise; nullptr with an exception set, the
 // status, or what `result` makes of the outcome.
@@ -300,13 +456,28 @@ PyObject* wrap_all(std::initializer_list<const at::Tensor*> tensors) {
   return tuple;
 }
 
+// The casts of the axes `wanted`, flat.
+PyObject* wrap_casts(const std::string& wanted, const Scaled& by_rows, const Scaled& by_cols) {
+  const Scaled &first = wanted[0] == '1' ? by_rows : by_cols, &second = wanted[0] == '1' ? by_cols : by_rows;
+  if (wanted.size() == 1) return wrap_all({&first.data, &first.scale});
+  return wrap_all({&first.data, &first.scale, &second.data, &second.scale});
+}
+
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long cast, matmul, orthogonalize, workspace;
-  if (!PyArg_ParseTuple(args, "KKKK", &cast, &matmul, &orthogonalize, &workspace)) return nullptr;
-  g_cast = reinterpret_cast<CastFn>(address(cast));
-  g_matmul = reinterpret_cast<MatmulFn>(address(matmul));
-  g_orthogonalize = reinterpret_cast<OrthogonalizeFn>(address(orthogonalize));
-  g_workspace = reinterpret_cast<WorkspaceFn>(address(workspace));
+  unsigned long long at[9];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKK", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6], &at[7], &at[8])) return nullptr;
+  auto keep = [](auto& function, unsigned long long value) {
+    function = reinterpret_cast<std::remove_reference_t<decltype(function)>>(address(value));
+  };
+  keep(g_cast, at[0]);
+  keep(g_matmul, at[1]);
+  keep(g_orthogonalize, at[2]);
+  keep(g_workspace, at[3]);
+  keep(g_columns, at[4]);
+  keep(g_grouped_cast, at[5]);
+  keep(g_stacked_cast, at[6]);
+  keep(g_grouped_matmul, at[7]);
+  keep(g_grouped_contract, at[8]);
   if (!bound()) {
     PyErr_SetString(PyExc_ValueError, "null entry point address");
     return nullptr;
@@ -334,11 +505,7 @@ PyObject* block_cast(PyObject*, PyObject* args) {
                   wanted.find('1') != std::string::npos ? &by_rows : nullptr,
                   wanted.find('0') != std::string::npos ? &by_cols : nullptr, address(stream));
       },
-      [&]() -> PyObject* {
-        const Scaled &first = wanted[0] == '1' ? by_rows : by_cols, &second = wanted[0] == '1' ? by_cols : by_rows;
-        if (wanted.size() == 1) return wrap_all({&first.data, &first.scale});
-        return wrap_all({&first.data, &first.scale, &second.data, &second.scale});
-      });
+      [&] { return wrap_casts(wanted, by_rows, by_cols); });
 }
 
 PyObject* block_matmul(PyObject*, PyObject* args) {
@@ -420,6 +587,103 @@ PyObject* linear_backward(PyObject*, PyObject* args) {
       [&] { return wrap_all({&dx, &dw}); });
 }
 
+PyObject* grouped_cast(PyObject*, PyObject* args) {
+  PyObject *object, *sizes_object;
+  int code, rule, square;
+  const char* axes;
+  unsigned long long seed, offset, stream;
+  if (!PyArg_ParseTuple(args, "OOiiisKKK", &object, &sizes_object, &code, &rule, &square, &axes, &seed, &offset, &stream))
+    return nullptr;
+  const at::Tensor& x = tensor(object);
+  at::Tensor sizes;
+  if (sizes_object != Py_None) sizes = tensor(sizes_object);
+  const std::string wanted(axes);
+  Scaled by_rows, by_cols;
+  return run(
+      x.device(),
+      [&] {
+        Scaled* rows = wanted.find('1') != std::string::npos ? &by_rows : nullptr;
+        Scaled* cols = wanted.find('0') != std::string::npos ? &by_cols : nullptr;
+        const uint32_t s = static_cast<uint32_t>(seed), o = static_cast<uint32_t>(offset);
+        if (!sizes.defined()) {
+          cast_stack_into(x, code, rule, square, s, o, rows, cols, address(stream));
+        } else {
+          if (square) value_error("groups of rows take blocks of one row");
+          cast_groups_into(x, sizes, code, rule, s, o, rows, cols, address(stream));
+        }
+      },
+      [&] { return wrap_casts(wanted, by_rows, by_cols); });
+}
+
+PyObject* grouped_matmul(PyObject*, PyObject* args) {
+  PyObject *a_data, *a_scale, *b_data, *b_scale, *sizes_object, *out_object;
+  int out_code;
+  unsigned long long stream;
+  if (!PyArg_ParseTuple(args, "OOOOOiOK", &a_data, &a_scale, &b_data, &b_scale, &sizes_object, &out_code, &out_object, &stream))
+    return nullptr;
+  for (PyObject* object : {a_data, a_scale, b_data, b_scale})
+    if (!THPVariable_Check(object)) type_error("operands must be BlockScaled pairs of tensors");
+  const Scaled a{tensor(a_data), tensor(a_scale)}, b{tensor(b_data), tensor(b_scale)};
+  const at::Tensor& sizes = tensor(sizes_object);
+  at::Tensor out;
+  if (out_object != Py_None) out = tensor(out_object);
+  const bool given = out.defined();
+  at::Tensor result;
+  return run(
+      a.data.device(), [&] { result = grouped_product(a, b, sizes, out_code, out, address(stream)); },
+      [&]() -> PyObject* {
+        if (!given) return wrap(result);
+        Py_INCREF(out_object);
+        return out_object;
+      });
+}
+
+PyObject* grouped_linear_forward(PyObject*, PyObject* args) {
+  PyObject *x_object, *w_object, *sizes_object;
+  int format[6], need_x, need_w;
+  unsigned long long seed[3], stream;
+  if (!PyArg_ParseTuple(args, "OOO(iiiiii)(KKK)ppK", &x_object, &w_object, &sizes_object, &format[0], &format[1], &format[2],
+                        &format[3], &format[4], &format[5], &seed[0], &seed[1], &seed[2], &need_x, &need_w, &stream))
+    return nullptr;
+  const at::Tensor &x = tensor(x_object), &w = tensor(w_object), &sizes = tensor(sizes_object);
+  Scaled qx, qx_t, qw, qw_t;
+  at::Tensor y;
+  return run(
+      x.device(),
+      [&] {
+        const at::Tensor rows = as_rows(x.detach()), weight = as_stack(w.detach());
+        cast_groups_into(rows, sizes, format[0], format[1], static_cast<uint32_t>(seed[0]), 0, &qx, need_w ? &qx_t : nullptr, address(stream));
+        cast_stack_into(weight, format[2], format[3], true, static_cast<uint32_t>(seed[1]), 0, &qw, need_x ? &qw_t : nullptr, address(stream));
+        y = grouped_product(qx, qw, sizes, dtype_code(x.scalar_type()), at::Tensor(), address(stream));
+      },
+      [&] { return wrap_all({&y, &qx_t.data, &qx_t.scale, &qw_t.data, &qw_t.scale}); });
+}
+
+PyObject* grouped_linear_backward(PyObject*, PyObject* args) {
+  PyObject *dy_object, *sizes_object, *x_data, *x_scale, *w_data, *w_scale;
+  int code, rule, dx_code, dw_code;
+  unsigned long long seed, stream;
+  if (!PyArg_ParseTuple(args, "OOOOOOiiKiiK", &dy_object, &sizes_object, &x_data, &x_scale, &w_data, &w_scale, &code, &rule, &seed,
+                        &dx_code, &dw_code, &stream))
+    return nullptr;
+  const at::Tensor &dy = tensor(dy_object), &sizes = tensor(sizes_object);
+  const bool need_w = x_data != Py_None, need_x = w_data != Py_None;
+  Scaled x, w, by_rows, by_cols;
+  if (need_w) x = {tensor(x_data), tensor(x_scale)};
+  if (need_x) w = {tensor(w_data), tensor(w_scale)};
+  at::Tensor dx, dw;
+  return run(
+      dy.device(),
+      [&] {
+        const at::Tensor rows = as_rows(dy.detach());
+        cast_groups_into(rows, sizes, code, rule, static_cast<uint32_t>(seed), 0, need_x ? &by_rows : nullptr,
+                         need_w ? &by_cols : nullptr, address(stream));
+        if (need_x) dx = grouped_product(by_rows, w, sizes, dx_code, at::Tensor(), address(stream));
+        if (need_w) dw = grouped_product(by_cols, x, sizes, dw_code, at::Tensor(), address(stream));
+      },
+      [&] { return wrap_all({&dx, &dw}); });
+}
+
 PyObject* orthogonalize(PyObject*, PyObject* args) {
   PyObject* object;
   int out_code;
@@ -473,6 +737,10 @@ PyMethodDef methods[] = {
     {"block_matmul", guarded<block_matmul>, METH_VARARGS, "Multiply two block-scaled matrices."},
     {"linear_forward", guarded<linear_forward>, METH_VARARGS, "Forward pass of the block-scaled linear layer."},
     {"linear_backward", guarded<linear_backward>, METH_VARARGS, "Gradients of the block-scaled linear layer."},
+    {"grouped_cast", guarded<grouped_cast>, METH_VARARGS, "Cast rows in groups, or a stack of matrices, to FP8 with block scales."},
+    {"grouped_matmul", guarded<grouped_matmul>, METH_VARARGS, "Multiply each group's rows by its matrix, or contract its columns."},
+    {"grouped_linear_forward", guarded<grouped_linear_forward>, METH_VARARGS, "Forward pass of the grouped linear layer."},
+    {"grouped_linear_backward", guarded<grouped_linear_backward>, METH_VARARGS, "Gradients of the grouped linear layer."},
     {"orthogonalize", guarded<orthogonalize>, METH_VARARGS, "Orthogonalise matrices."},
     {nullptr, nullptr, 0, nullptr},
 };

@@ -222,9 +222,11 @@ __device__ __forceinline__ int live_of(T at, T end, int width) {
 }
 
 // The tile of 128 rows and 8 LANES columns from (row0, col0), by a workgroup
-// of 32 LANES threads, of which LANES share four neighbouring rows.
+// of 32 LANES threads, of which LANES share four neighbouring rows.  The columns
+// are stored up to row `stored`, zeros behind the matrix's last row.
 template <int XE, int QE, bool SQUARE, int LANES>
-__device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, int64_t col0, bool want_rows, bool want_cols) {
+__device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, int64_t col0, bool want_rows, bool want_cols,
+                                          int64_t stored) {
   constexpr int kGroups = 32, kThreads = kGroups * LANES, kCols = 8 * LANES;
   constexpr int kTurn = 32 / LANES;
   __shared__ uint32_t turned[kCols * 32];
@@ -337,7 +339,7 @@ __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, 
   __syncthreads();
   const int word_at = t & 31, part = t >> 5;
   const int64_t r = row0 + 4 * word_at;
-  const int live_r = live_of(r, a.rows, 4);
+  const int live_r = live_of(r, stored, 4);
 #pragma unroll
   for (int k = 0; k < kCols * 32 / kThreads; ++k) {
     const int col = kThreads / 32 * k + part;
@@ -357,12 +359,17 @@ __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, 
 constexpr int kTileThreads = 512, kPartThreads = 256;
 constexpr uint64_t kWholeTiles = 256;  // see above
 
+// Tile `tile` of a matrix.
 template <int XE, int QE, bool SQUARE>
-__global__ __launch_bounds__(kTileThreads, SQUARE ? 6 : 4) void block_cast_tile_kernel(BlockCastArgs a) {
-  const uint32_t tile = a.first + blockIdx.x;
+__device__ __forceinline__ void cast_whole(const BlockCastArgs& a, uint32_t tile) {
   cast_tile<XE, QE, SQUARE, 16>(a, static_cast<int64_t>(tile / a.tiles_n) * kCastTile,
                               static_cast<int64_t>(tile % a.tiles_n) * kCastTile, a.by_rows.data != nullptr,
-                              a.by_cols.data != nullptr);
+                              a.by_cols.data != nullptr, a.rows);
+}
+
+template <int XE, int QE, bool SQUARE>
+__global__ __launch_bounds__(kTileThreads, SQUARE ? 6 : 4) void block_cast_tile_kernel(BlockCastArgs a) {
+  cast_whole<XE, QE, SQUARE>(a, a.first + blockIdx.x);
 }
 
 // The workgroups of a band of 128 rows: where the row orientation is asked
@@ -371,19 +378,11 @@ __global__ __launch_bounds__(kTileThreads, SQUARE ? 6 : 4) void block_cast_tile_
 constexpr int kPartRows = kPartThreads / 16, kPartLanes = 8;
 constexpr int kRowParts = kCastTile / kPartRows, kColParts = kCastTile / (8 * kPartLanes);
 
+// 16 rows from row0 on of the block of 128 columns of index `block`.
 template <int XE, int QE>
-__global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void block_cast_parts_kernel(BlockCastArgs a) {
-  const uint32_t row_parts = a.by_rows.data ? kRowParts : 0, parts = row_parts + (a.by_cols.data ? kColParts : 0);
-  const uint32_t id = a.first + blockIdx.x, band = id / (parts * a.tiles_n), within = id - band * parts * a.tiles_n;
-  const int64_t row0 = static_cast<int64_t>(band) * kCastTile;
-  if (within >= row_parts * a.tiles_n) {
-    cast_tile<XE, QE, false, kPartLanes>(a, row0, static_cast<int64_t>(within - row_parts * a.tiles_n) * 8 * kPartLanes, false, true);
-    return;
-  }
-  const uint32_t part = within / a.tiles_n;
-  const int64_t block = within - part * a.tiles_n;
+__device__ __forceinline__ void cast_row_part(const BlockCastArgs& a, int64_t row0, int64_t block) {
   const int lane = threadIdx.x & 15;
-  const int64_t r = row0 + kPartRows * part + (threadIdx.x >> 4), c = block * kCastTile + 8 * lane;
+  const int64_t r = row0 + (threadIdx.x >> 4), c = block * kCastTile + 8 * lane;
   if (r >= a.rows) return;  // sixteen lanes together
   const int live = live_of(c, a.cols, 8);
   float x[8];
@@ -397,6 +396,26 @@ __global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void bloc
   encode_row<QE>(x, e, hash, finite, words);
   store_eight(static_cast<char*>(a.by_rows.data) + r * a.by_rows.ld + c, words, live);
   if (lane == 0) store_exponent(a.by_rows, r, block, e);
+}
+
+// Workgroup `id` of a matrix.
+template <int XE, int QE>
+__device__ __forceinline__ void cast_parts(const BlockCastArgs& a, uint32_t id) {
+  const uint32_t row_parts = a.by_rows.data ? kRowParts : 0, parts = row_parts + (a.by_cols.data ? kColParts : 0);
+  const uint32_t band = id / (parts * a.tiles_n), within = id - band * parts * a.tiles_n;
+  const int64_t row0 = static_cast<int64_t>(band) * kCastTile;
+  if (within >= row_parts * a.tiles_n) {
+    cast_tile<XE, QE, false, kPartLanes>(a, row0, static_cast<int64_t>(within - row_parts * a.tiles_n) * 8 * kPartLanes, false,
+                                         true, a.rows);
+    return;
+  }
+  const uint32_t part = within / a.tiles_n;
+  cast_row_part<XE, QE>(a, row0 + kPartRows * part, within - part * a.tiles_n);
+}
+
+template <int XE, int QE>
+__global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void block_cast_parts_kernel(BlockCastArgs a) {
+  cast_parts<XE, QE>(a, a.first + blockIdx.x);
 }
 
 // ---------------------------------------------------------------------------
@@ -781,22 +800,25 @@ __device__ __forceinline__ void sum_far_scales(const BlockProductArgs& g, char* 
 template <class S>
 constexpr int kProductWaves = S::BM > 64 ? S::kMinWaves : (S::kGroups > 1 ? 4 : 3);
 
-template <int MODE, int FA, int FB, class S, bool ASYNC>
-__global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void block_product_kernel(BlockProductArgs g) {
-  static_assert(ASYNC || S::kGroups == 1, "groups take aligned rows");
-  using Area = ScaleArea<MODE, S>;
-  constexpr int kStages = S::kLds + Area::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
+// LDS of a tile, beside 16 bytes behind it.
+template <int MODE, class S>
+constexpr int product_lds() {
+  constexpr int kStages = S::kLds + ScaleArea<MODE, S>::kBytes, kChunks = S::kWaves * ResultChunk<S::kRowsN>::kBytes;
   constexpr int kLds = kStages > kChunks ? kStages : kChunks;
   static_assert(S::kSums <= kLds, "the groups' sums");
-  // One array: beside a second one the compiler lets the stages' asynchronous loads land before any read of LDS.
-  __shared__ __align__(1024) char lds[kLds + 16];
+  return kLds;
+}
+
+// The results from (row0, col0) on.
+template <int MODE, int FA, int FB, class S, bool ASYNC>
+__device__ __forceinline__ void product_tile(const BlockProductArgs& g, char* lds, int row0, int col0) {
+  static_assert(ASYNC || S::kGroups == 1, "groups take aligned rows");
+  using Area = ScaleArea<MODE, S>;
+  constexpr int kLds = product_lds<MODE, S>();
   int* far = reinterpret_cast<int*>(lds + kLds);  // a scale so far is not a near one
   const int lane = threadIdx.x & 63, all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = all % S::kWaves, group = all / S::kWaves;
   if (MODE != kExponents && threadIdx.x == 0) *far = 0;  // a barrier comes before the first fill
-  uint32_t tile_m, tile_n;
-  band_tile(xcd_run(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tile_m, tile_n);
-  const int row0 = tile_m * S::BM, col0 = tile_n * S::BN;
   const int wave_m = wave / S::WN * S::kRowsM, wave_n = wave % S::WN * S::kRowsN;
 
   Stager<S> stager;
@@ -882,6 +904,15 @@ __global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void block_product_k
   if (group == 0) store_chunks<kLds, S>(g, lds, row0, col0, wave, lane, acc);
 }
 
+template <int MODE, int FA, int FB, class S, bool ASYNC>
+__global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void block_product_kernel(BlockProductArgs g) {
+  // One array: beside a second one the compiler lets the stages' asynchronous loads land before any read of LDS.
+  __shared__ __align__(1024) char lds[product_lds<MODE, S>() + 16];
+  uint32_t tile_m, tile_n;
+  band_tile(xcd_run(blockIdx.x, g.tiles_m * g.tiles_n), g.tiles_m, g.tiles_n, tile_m, tile_n);
+  product_tile<MODE, FA, FB, S, ASYNC>(g, lds, tile_m * S::BM, tile_n * S::BN);
+}
+
 // Few rows of A (at most 16): one 16-column tile of the result per workgroup,
 // whose waves take the blocks of the contracted axis in turn and add their
 // sums through LDS in wave order.  The operands go from memory to registers:
@@ -890,10 +921,8 @@ __global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void block_product_k
 constexpr int kRowWaves = 8;
 
 template <int MODE, int FA, int FB>
-__global__ __launch_bounds__(64 * kRowWaves) void block_product_rows_kernel(BlockProductArgs g) {
-  __shared__ f32x4 sums[kRowWaves][64];
+__device__ __forceinline__ void product_rows(const BlockProductArgs& g, f32x4 (&sums)[kRowWaves][64], int col0) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col0 = static_cast<int>(xcd_run(blockIdx.x, g.tiles_n)) * 16;
   const int row_a = (lane & 15) < g.m ? lane & 15 : g.m - 1;
   const int row_b = col0 + (lane & 15) < g.n ? col0 + (lane & 15) : g.n - 1;
   const char* pa = g.a.base + row_a * g.a.ld;
@@ -939,6 +968,12 @@ __global__ __launch_bounds__(64 * kRowWaves) void block_product_rows_kernel(Bloc
   with_output(g, 0, col0, 16, 16, [&](auto out, auto edge) {
     store_results<decltype(out)::value, decltype(edge)::value>(g, lane & 15, col0 + 4 * (lane >> 4), acc);
   });
+}
+
+template <int MODE, int FA, int FB>
+__global__ __launch_bounds__(64 * kRowWaves) void block_product_rows_kernel(BlockProductArgs g) {
+  __shared__ f32x4 sums[kRowWaves][64];
+  product_rows<MODE, FA, FB>(g, sums, static_cast<int>(xcd_run(blockIdx.x, g.tiles_n)) * 16);
 }
 
 }  // namespace sr

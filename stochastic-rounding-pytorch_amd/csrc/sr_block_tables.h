@@ -38,8 +38,20 @@ enum BlockCastKind { kCastParts, kCastWhole, kCastSquare, kCastKinds };
 // [FP32, BF16, FP16 input][E4M3 nearest, stochastic, E5M2 nearest, stochastic][kind]
 using BlockCastTable = const void* [3][4][kCastKinds];
 
+struct GroupedProductKernels {
+  const void* rows;                  // tiles of 16 rows
+  const void* tile[kBlockTiles][2];  // as above
+  const void* contract[kBlockTiles];
+};
+using GroupedProductTable = GroupedProductKernels[2][2][3];
+enum GroupedCastKind { kGroupedParts, kGroupedWhole, kStackedParts, kStackedWhole, kStackedSquare, kGroupedCastKinds };
+using GroupedCastTable = const void* [3][4][kGroupedCastKinds];
+
 void register_block_product_e4m3(BlockProductTable& t);
 void register_block_product_e5m2(BlockProductTable& t);
 void register_block_cast(BlockCastTable& t);
+void register_grouped_product_e4m3(GroupedProductTable& t);
+void register_grouped_product_e5m2(GroupedProductTable& t);
+void register_grouped_cast(GroupedCastTable& t);
 
 }  // namespace sr

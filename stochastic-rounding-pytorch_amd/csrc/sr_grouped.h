@@ -1,0 +1,350 @@
+// sr_grouped.h -- block casts and products whose rows are sorted into groups, each with a matrix of its own.
+//
+// The groups' sizes are device memory, and no launch waits for them: a grid has
+// room for any sizes, every wave sums them up by itself (64 groups a step), and
+// workgroups beyond the tiles that there are end at once.  Sizes below zero
+// count as zero and rows beyond the matrix as none, so that no sizes lead out of it.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "sr_block_scaled.h"
+
+namespace sr {
+
+struct Groups {
+  const void* sizes;  // `count` numbers, int64 where `wide`, else int32
+  int count;
+  int wide;
+};
+
+__device__ __forceinline__ uint32_t group_size(const Groups& g, int i, uint32_t limit) {
+  if (i >= g.count) return 0;
+  if (g.wide) {
+    const int64_t n = gptr<int64_t>(g.sizes)[i];
+    return n < 0 ? 0u : (n < static_cast<int64_t>(limit) ? static_cast<uint32_t>(n) : limit);
+  }
+  const int32_t n = gptr<int32_t>(g.sizes)[i];
+  return n < 0 ? 0u : umin(static_cast<uint32_t>(n), limit);
+}
+
+// min(the sum of x over this lane and those before it, limit); every x and the limit are below 2^31.
+__device__ __forceinline__ uint32_t scan_capped(uint32_t x, uint32_t limit) {
+#define SR_SCAN_STEP(control, rows) \
+  x = umin(x + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), control, rows, 0xF, false)), limit)
+  SR_SCAN_STEP(0x111, 0xF);  // 1, 2, 4 and 8 lanes back inside 16
+  SR_SCAN_STEP(0x112, 0xF);
+  SR_SCAN_STEP(0x114, 0xF);
+  SR_SCAN_STEP(0x118, 0xF);
+  SR_SCAN_STEP(0x142, 0xA);  // lane 15 to the next 16, lane 31 to the upper half
+  SR_SCAN_STEP(0x143, 0xC);
+#undef SR_SCAN_STEP
+  return x;
+}
+
+__device__ __forceinline__ uint32_t lane_value(uint32_t x, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), lane));
+}
+
+// 64 groups, one a lane: their first row, rows, first tile and tiles of TILE rows, capped at `limit` rows in all.
+// PADDED: a group's rows are rounded up to whole tiles before they are counted.
+template <int TILE, bool PADDED>
+struct GroupChunk {
+  uint32_t start, rows, first, tiles;
+  uint32_t rows_end, tiles_end;  // of the chunk, uniform
+
+  __device__ __forceinline__ void load(const Groups& g, int chunk, uint32_t rows_before, uint32_t tiles_before, uint32_t limit) {
+    const int lane = threadIdx.x & 63;
+    uint32_t n = group_size(g, chunk + lane, limit);
+    if (PADDED) n = umin((n + TILE - 1) / TILE * TILE, limit);
+    const uint32_t end = umin(scan_capped(n, limit) + rows_before, limit);
+    start = static_cast<uint32_t>(__shfl_up(static_cast<int>(end), 1));
+    if (lane == 0) start = rows_before;
+    rows = end - start;
+    tiles = (rows + TILE - 1) / TILE;
+    first = scan_capped(tiles, 0x7FFFFFFFu) + tiles_before;
+    rows_end = lane_value(end, 63);
+    tiles_end = lane_value(first, 63);
+    first -= tiles;
+  }
+};
+
+// A tile's group (the groups' count: rows behind the last one), uniform.
+struct GroupTile {
+  int group;
+  uint32_t start, rows;   // the group's
+  uint32_t first, tiles;  // its first tile among all and its tiles
+};
+
+// All groups' tiles of TILE rows.
+template <int TILE>
+struct GroupTable {
+  GroupChunk<TILE, false> chunk;  // the first 64 groups
+  uint32_t rows, tiles;           // of all groups
+
+  __device__ __forceinline__ void load(const Groups& g, uint32_t limit) {
+    chunk.load(g, 0, 0, 0, limit);
+    rows = chunk.rows_end;
+    tiles = chunk.tiles_end;
+    for (int at = 64; at < g.count; at += 64) {
+      GroupChunk<TILE, false> next;
+      next.load(g, at, rows, tiles, limit);
+      rows = next.rows_end;
+      tiles = next.tiles_end;
+    }
+  }
+
+  // The group of tile `tile`, counted over all groups and then over the rows behind them.
+  __device__ __forceinline__ GroupTile find(const Groups& g, uint32_t tile, uint32_t limit) const {
+    if (tile >= tiles) return {g.count, rows, limit - rows, tiles, (limit - rows + TILE - 1) / TILE};
+    GroupChunk<TILE, false> c = chunk;
+    int at = 0;
+    while (c.tiles_end <= tile) {
+      at += 64;
+      c.load(g, at, c.rows_end, c.tiles_end, limit);
+    }
+    // The only lane with first <= tile < first + tiles.
+    const int lane = __builtin_ctzll(__ballot(tile - c.first < c.tiles));
+    return {at + lane, lane_value(c.start, lane), lane_value(c.rows, lane), lane_value(c.first, lane), lane_value(c.tiles, lane)};
+  }
+};
+
+// Rows [start, start + rows) of group `group` where every group's rows are padded to whole blocks.
+__device__ __forceinline__ void padded_group(const Groups& g, int group, uint32_t limit, uint32_t& start, uint32_t& rows) {
+  GroupChunk<SR_BLOCK, true> c;
+  uint32_t before = 0;
+  int at = 0;
+  for (;; at += 64) {
+    c.load(g, at, before, 0, limit);
+    if (group < at + 64) break;
+    before = c.rows_end;
+  }
+  start = lane_value(c.start, group - at);
+  rows = lane_value(c.rows, group - at);
+}
+
+// ---------------------------------------------------------------------------
+// Products.
+//
+//   rows      out[t] = a[t] b[g]^T for the rows t of group g, b a stack of matrices
+//   contract  out[g] = a[:, g] b[:, g]^T over the columns of group g, which start
+//             on multiples of 128 and end in zeros
+//
+// Both find their group and go on as a plain product does, on the part of the
+// operands that the group has: what a plain product measured holds for them
+// (sr_block_scaled.h).
+// ---------------------------------------------------------------------------
+struct GroupedProductArgs {
+  BlockProductArgs p;  // m: all rows of a (rows), or of one result (contract)
+  Groups groups;
+  int64_t stride, stride_scale;  // rows: between matrices of b and of its scales, in bytes
+  int64_t stride_out;            // contract: between results, in elements
+  int zero_behind;               // rows: rows behind the last group become zeros
+};
+
+__device__ __forceinline__ int64_t output_bytes(const BlockProductArgs& p, int64_t elements) {
+  return elements * (p.out_dtype == SR_F32 ? 4 : 2);
+}
+
+// The product of the group that tile `q` of TILE rows belongs to.
+template <int TILE>
+__device__ __forceinline__ BlockProductArgs rows_product(const GroupedProductArgs& g, const GroupTile& at) {
+  BlockProductArgs p = g.p;
+  const int64_t size = p.scale_f32 ? 4 : 1;
+  p.a.base += at.start * p.a.ld;
+  p.a.rows = p.m = static_cast<int>(at.rows);
+  p.scale_a += at.start * p.ld_scale_a * size;
+  p.out += output_bytes(p, at.start * p.ldo);
+  p.tiles_m = at.tiles;
+  if (at.group == g.groups.count) {
+    p.k = 0;  // nothing is read
+  } else {
+    p.b.base += at.group * g.stride;
+    p.scale_b += at.group * g.stride_scale;
+  }
+  return p;
+}
+
+template <int MODE, int FA, int FB, class S, bool ASYNC>
+__global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void grouped_product_kernel(GroupedProductArgs g) {
+  __shared__ __align__(1024) char lds[product_lds<MODE, S>() + 16];
+  GroupTable<S::BM> table;
+  const uint32_t limit = static_cast<uint32_t>(g.p.m);
+  table.load(g.groups, limit);
+  const uint32_t behind = g.zero_behind ? (limit - table.rows + S::BM - 1) / S::BM : 0;
+  const uint32_t total = (table.tiles + behind) * g.p.tiles_n;
+  if (blockIdx.x >= total) return;
+  const uint32_t id = xcd_run(blockIdx.x, total);
+  const GroupTile at = table.find(g.groups, id / g.p.tiles_n, limit);
+  const BlockProductArgs p = rows_product<S::BM>(g, at);
+  uint32_t tile_m, tile_n;
+  band_tile(id - at.first * p.tiles_n, p.tiles_m, p.tiles_n, tile_m, tile_n);
+  product_tile<MODE, FA, FB, S, ASYNC>(p, lds, tile_m * S::BM, tile_n * S::BN);
+}
+
+// Groups of few rows: tiles of 16 rows by 16 columns.
+template <int MODE, int FA, int FB>
+__global__ __launch_bounds__(64 * kRowWaves) void grouped_product_rows_kernel(GroupedProductArgs g) {
+  __shared__ f32x4 sums[kRowWaves][64];
+  GroupTable<16> table;
+  const uint32_t limit = static_cast<uint32_t>(g.p.m);
+  table.load(g.groups, limit);
+  const uint32_t behind = g.zero_behind ? (limit - table.rows + 15) / 16 : 0;
+  const uint32_t total = (table.tiles + behind) * g.p.tiles_n;
+  if (blockIdx.x >= total) return;
+  const uint32_t id = xcd_run(blockIdx.x, total);
+  GroupTile at = table.find(g.groups, id / g.p.tiles_n, limit);
+  const uint32_t within = id - at.first * g.p.tiles_n, tile_n = within / at.tiles, tile_m = within - tile_n * at.tiles;
+  at.start += tile_m * 16;
+  at.rows = umin(at.rows - tile_m * 16, 16);
+  product_rows<MODE, FA, FB>(rows_product<16>(g, at), sums, static_cast<int>(tile_n) * 16);
+}
+
+template <int MODE, int FA, int FB, class S, bool ASYNC>
+__global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void grouped_contract_kernel(GroupedProductArgs g) {
+  __shared__ __align__(1024) char lds[product_lds<MODE, S>() + 16];
+  BlockProductArgs p = g.p;
+  const uint32_t each = p.tiles_m * p.tiles_n, id = xcd_run(blockIdx.x, each * static_cast<uint32_t>(g.groups.count));
+  const uint32_t group = id / each;
+  uint32_t start, columns;
+  padded_group(g.groups, static_cast<int>(group), static_cast<uint32_t>(p.k), start, columns);
+  const int64_t size = p.scale_f32 ? 4 : 1;
+  p.a.base += start;
+  p.b.base += start;
+  p.scale_a += start / SR_BLOCK * size;
+  p.scale_b += start / SR_BLOCK * size;
+  p.k = columns;
+  p.out += output_bytes(p, group * g.stride_out);
+  uint32_t tile_m, tile_n;
+  band_tile(id - group * each, p.tiles_m, p.tiles_n, tile_m, tile_n);
+  product_tile<MODE, FA, FB, S, ASYNC>(p, lds, tile_m * S::BM, tile_n * S::BN);
+}
+
+// ---------------------------------------------------------------------------
+// Casts.
+//
+// A group's blocks along the rows start at its first row, and its transposed
+// columns at a multiple of 128, zeros up to the next: a contraction over them
+// then has whole blocks of its own group only.  Tiles of 128 rows of a group do
+// both orientations; rows behind the last group are cast along the columns
+// alone.
+//
+// A stack of matrices is cast matrix by matrix in one launch.
+// ---------------------------------------------------------------------------
+struct GroupedCastArgs {
+  BlockCastArgs c;
+  Groups groups;
+  uint32_t column_blocks;  // of the transposed result
+};
+
+// The part of a cast that a group's rows are; `block`: its first block of transposed columns.
+__device__ __forceinline__ BlockCastArgs cast_of_group(const BlockCastArgs& c, const GroupTile& at, int element_bytes) {
+  BlockCastArgs p = c;
+  p.x += static_cast<int64_t>(at.start) * c.ldx * element_bytes;
+  p.rows = at.rows;
+  p.counter_base += at.start * static_cast<uint32_t>(c.cols);
+  if (p.by_rows.data) {
+    p.by_rows.data = static_cast<char*>(p.by_rows.data) + at.start * c.by_rows.ld;
+    p.by_rows.scale = static_cast<char*>(p.by_rows.scale) + at.start * c.by_rows.ld_scale;
+  }
+  p.by_cols.data = static_cast<char*>(p.by_cols.data) + static_cast<int64_t>(at.first) * SR_BLOCK;
+  p.by_cols.scale = static_cast<char*>(p.by_cols.scale) + at.first;
+  return p;
+}
+
+// Zeros in block `block` of the transposed columns, for `cols` columns from col0 on.
+__device__ __forceinline__ void zero_columns(const BlockCastArgs& c, uint32_t block, int64_t col0, int cols, int threads) {
+  for (int i = threadIdx.x; i < cols * 16; i += threads) {
+    const int64_t col = col0 + (i >> 4);
+    if (col >= c.cols) break;
+    char* q = static_cast<char*>(c.by_cols.data) + col * c.by_cols.ld + static_cast<int64_t>(block) * SR_BLOCK + (i & 15) * 8;
+    *(SR_GLOBAL eight_bytes*)(q) = eight_bytes{0, 0};
+    if ((i & 15) == 0) store_exponent(c.by_cols, col, block, 0);
+  }
+}
+
+template <int XE, int QE>
+__global__ __launch_bounds__(kTileThreads, 4) void grouped_cast_tile_kernel(GroupedCastArgs g) {
+  GroupTable<kCastTile> table;
+  const uint32_t limit = static_cast<uint32_t>(g.c.rows);
+  table.load(g.groups, limit);
+  const uint32_t id = g.c.first + blockIdx.x, tile = id / g.c.tiles_n;
+  const int64_t col0 = static_cast<int64_t>(id - tile * g.c.tiles_n) * kCastTile;
+  if (tile >= table.tiles && tile < g.column_blocks) zero_columns(g.c, tile, col0, kCastTile, kTileThreads);
+  const GroupTile at = table.find(g.groups, tile, limit);
+  const uint32_t within = tile - at.first;
+  if (within >= at.tiles) return;  // behind the rows behind the last group
+  if (at.group == g.groups.count) {
+    // Rows behind the last group have no place in the transposed result.
+    for (int part = 0; part < kCastTile; part += kTileThreads / 16)
+      cast_row_part<XE, QE>(g.c, static_cast<int64_t>(at.start) + within * kCastTile + part, col0 / kCastTile);
+    return;
+  }
+  const BlockCastArgs p = cast_of_group(g.c, at, enc_bytes(XE));
+  cast_tile<XE, QE, false, 16>(p, static_cast<int64_t>(within) * kCastTile, col0, true, true,
+                               static_cast<int64_t>(within + 1) * kCastTile);
+}
+
+// Workgroups of one orientation each: first kColParts times tiles_n of every
+// block of transposed columns, then, where the rows are asked for, those of all
+// rows as they lie.
+template <int XE, int QE>
+__global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void grouped_cast_parts_kernel(GroupedCastArgs g) {
+  constexpr int kCols = 8 * kPartLanes;
+  const uint32_t id = g.c.first + blockIdx.x, each = kColParts * g.c.tiles_n, tile = id / each;
+  if (tile >= g.column_blocks) {
+    const uint32_t row_id = id - each * g.column_blocks, part = row_id / g.c.tiles_n;
+    cast_row_part<XE, QE>(g.c, static_cast<int64_t>(part) * kPartRows, row_id - part * g.c.tiles_n);
+    return;
+  }
+  GroupTable<kCastTile> table;
+  const uint32_t limit = static_cast<uint32_t>(g.c.rows);
+  table.load(g.groups, limit);
+  const int64_t col0 = static_cast<int64_t>(id - tile * each) * kCols;
+  if (tile >= table.tiles) {
+    zero_columns(g.c, tile, col0, kCols, kPartThreads);
+    return;
+  }
+  const GroupTile at = table.find(g.groups, tile, limit);
+  const uint32_t within = tile - at.first;
+  const BlockCastArgs p = cast_of_group(g.c, at, enc_bytes(XE));
+  cast_tile<XE, QE, false, kPartLanes>(p, static_cast<int64_t>(within) * kCastTile, col0, false, true,
+                                       static_cast<int64_t>(within + 1) * kCastTile);
+}
+
+// A stack of matrices of `c`'s shape.
+struct StackedCastArgs {
+  BlockCastArgs c;
+  int64_t stride_x;                                          // between matrices, in bytes
+  int64_t rows_data, rows_scale, cols_data, cols_scale;      // of the results
+  uint32_t each;                                             // workgroups of a matrix
+};
+
+__device__ __forceinline__ BlockCastArgs matrix_of_stack(const StackedCastArgs& s, uint32_t matrix) {
+  BlockCastArgs p = s.c;
+  p.x += matrix * s.stride_x;
+  p.counter_base += matrix * static_cast<uint32_t>(s.c.rows) * static_cast<uint32_t>(s.c.cols);
+  if (p.by_rows.data) {
+    p.by_rows.data = static_cast<char*>(p.by_rows.data) + matrix * s.rows_data;
+    p.by_rows.scale = static_cast<char*>(p.by_rows.scale) + matrix * s.rows_scale;
+  }
+  if (p.by_cols.data) {
+    p.by_cols.data = static_cast<char*>(p.by_cols.data) + matrix * s.cols_data;
+    p.by_cols.scale = static_cast<char*>(p.by_cols.scale) + matrix * s.cols_scale;
+  }
+  return p;
+}
+
+template <int XE, int QE, bool SQUARE>
+__global__ __launch_bounds__(kTileThreads, SQUARE ? 6 : 4) void stacked_cast_tile_kernel(StackedCastArgs s) {
+  const uint32_t id = s.c.first + blockIdx.x, matrix = id / s.each;
+  cast_whole<XE, QE, SQUARE>(matrix_of_stack(s, matrix), id - matrix * s.each);
+}
+
+template <int XE, int QE>
+__global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void stacked_cast_parts_kernel(StackedCastArgs s) {
+  const uint32_t id = s.c.first + blockIdx.x, matrix = id / s.each;
+  cast_parts<XE, QE>(matrix_of_stack(s, matrix), id - matrix * s.each);
+}
+
+}  // namespace sr

@@ -25,6 +25,9 @@ from .hip import (
     block_cast,
     block_linear,
     block_matmul,
+    grouped_block_cast,
+    grouped_block_linear,
+    grouped_block_matmul,
     hip_adamw_step_,
     hip_muon_step_,
     hip_sgdm_step_,
@@ -55,6 +58,9 @@ __all__ = [
     "block_linear",
     "block_matmul",
     "cast",
+    "grouped_block_cast",
+    "grouped_block_linear",
+    "grouped_block_matmul",
     "hip_adamw_step_",
     "hip_muon_step_",
     "hip_sgdm_step_",

@@ -78,6 +78,7 @@ MATRIX_ABI_VERSION = 1
 BLOCK = 128  # values that share a scale along the contracted axis
 SCALE_E8M0, SCALE_F32 = range(2)
 MATRIX_BATCH = 64  # matrices one launch takes
+MATRIX_GROUPS = 4096  # groups one call takes
 
 
 class BlockMatrix(ctypes.Structure):
@@ -101,6 +102,14 @@ class BlockOutput(ctypes.Structure):
         ("ld", ctypes.c_int64),
         ("ld_scale", ctypes.c_int64),
     ]
+
+
+class Groups(ctypes.Structure):
+    _fields_ = [("sizes", ctypes.c_void_p), ("count", ctypes.c_int), ("wide", ctypes.c_int)]
+
+
+class BlockStack(ctypes.Structure):
+    _fields_ = [("out", BlockOutput), ("stride", ctypes.c_int64), ("stride_scale", ctypes.c_int64)]
 
 
 class NewtonSchulz(ctypes.Structure):
@@ -187,6 +196,27 @@ MATRIX_SIGNATURES = {
     "sr_block_matmul": (
         _int,
         [ctypes.POINTER(BlockMatrix), ctypes.POINTER(BlockMatrix), _i64, _vp, _i64, _int, _vp],
+    ),
+    "sr_grouped_columns": (_i64, [_i64, _i64]),
+    "sr_grouped_block_cast": (
+        _int,
+        [_vp, _i64, _i64, _i64, _int, _int, _int, _u32, _u32, ctypes.POINTER(Groups), ctypes.POINTER(BlockOutput),
+         ctypes.POINTER(BlockOutput), _vp],
+    ),
+    "sr_stacked_block_cast": (
+        _int,
+        [_vp, _i64, _i64, _i64, _i64, _i64, _int, _int, _int, _int, _u32, _u32, ctypes.POINTER(BlockStack),
+         ctypes.POINTER(BlockStack), _vp],
+    ),
+    "sr_grouped_block_matmul": (
+        _int,
+        [ctypes.POINTER(BlockMatrix), ctypes.POINTER(BlockMatrix), _i64, _i64, _i64, ctypes.POINTER(Groups), _vp, _i64,
+         _int, _int, _vp],
+    ),
+    "sr_grouped_block_contract": (
+        _int,
+        [ctypes.POINTER(BlockMatrix), ctypes.POINTER(BlockMatrix), _i64, ctypes.POINTER(Groups), _vp, _i64, _i64, _int,
+         _vp],
     ),
     "sr_orthogonalize_workspace": (_i64, [_i64, _i64, _i64]),
     "sr_orthogonalize": (
@@ -321,7 +351,9 @@ def matrix():
 
         lib = library()
         module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
-                      for name in ("sr_block_cast", "sr_block_matmul", "sr_orthogonalize", "sr_orthogonalize_workspace")))
+                      for name in ("sr_block_cast", "sr_block_matmul", "sr_orthogonalize", "sr_orthogonalize_workspace",
+                                   "sr_grouped_columns", "sr_grouped_block_cast", "sr_stacked_block_cast",
+                                   "sr_grouped_block_matmul", "sr_grouped_block_contract")))
         _matrix = module
     return _matrix
 

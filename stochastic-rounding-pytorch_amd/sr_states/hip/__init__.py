@@ -4,6 +4,7 @@ from ._common import is_hip_available
 from .adamw import AdamWHip, AdamWHipRN, hip_adamw_step_
 from .block import BlockScaled, block_cast, block_linear, block_matmul
 from .cast import cast, rn_cast_bf16, sr_cast_bf16
+from .grouped import grouped_block_cast, grouped_block_linear, grouped_block_matmul
 from .muon import MuonHip, MuonHipRN, hip_muon_step_, orthogonalize
 from .sgd import SGDMHip, SGDMHipRN, hip_sgdm_step_
 
@@ -19,6 +20,9 @@ __all__ = [
     "block_linear",
     "block_matmul",
     "cast",
+    "grouped_block_cast",
+    "grouped_block_linear",
+    "grouped_block_matmul",
     "hip_adamw_step_",
     "hip_muon_step_",
     "hip_sgdm_step_",

@@ -37,7 +37,8 @@ class BlockScaled(NamedTuple):
     ``data``: (rows, k) FP8 with consecutive columns.  ``scale``: E8M0 or FP32,
     (rows, ceil(k / 128)) for blocks of one row, or (ceil(rows / 128),
     ceil(k / 128)) for blocks of 128 rows.  Value (r, c) is
-    ``data[r, c] * scale[r or r // 128, c // 128]``.
+    ``data[r, c] * scale[r or r // 128, c // 128]``.  A stack of matrices has
+    one more dimension in front of both.
     """
 
     data: torch.Tensor
@@ -45,11 +46,11 @@ class BlockScaled(NamedTuple):
 
     def dequantize(self) -> torch.Tensor:
         """The FP32 values the matrix stands for."""
-        rows, k = self.data.shape
+        rows, k = self.data.shape[-2:]
         scale = self.scale.float()
-        if scale.shape[0] != rows:
-            scale = scale.repeat_interleave(BLOCK, 0)[:rows]
-        return self.data.float() * scale.repeat_interleave(BLOCK, 1)[:, :k]
+        if scale.shape[-2] != rows:
+            scale = scale.repeat_interleave(BLOCK, -2)[..., :rows, :]
+        return self.data.float() * scale.repeat_interleave(BLOCK, -1)[..., :k]
 
 
 # Checked (dtype, block, axis, rounding) of block_cast, as the native entry takes them: built-in rules
@@ -173,6 +174,16 @@ def _linear_codes(formats):
     return tuple(code for fmt in chosen for code in native_codes(fmt.dtype, fmt.rounding))
 
 
+def _formats_of(formats):
+    try:
+        return _LINEAR_CODES[formats]
+    except KeyError:
+        codes = _LINEAR_CODES[formats] = _linear_codes(formats)
+        return codes
+    except TypeError:  # a dict of formats
+        return _linear_codes(formats)
+
+
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, codes, seed, recorded):
@@ -224,12 +235,7 @@ def block_linear(
     Only the FP8 copies are kept for the backward pass; without grad mode
     those that it alone would need are not made.
     """
-    try:
-        codes = _LINEAR_CODES[formats]
-    except KeyError:
-        codes = _LINEAR_CODES[formats] = _linear_codes(formats)
-    except TypeError:  # a dict of formats
-        codes = _linear_codes(formats)
+    codes = _formats_of(formats)
     for name, t in (("x", x), ("weight", weight)):
         if t.dtype not in _WIDE_DTYPES:
             raise TypeError(f"{name} must be FP32, BF16 or FP16, not {t.dtype}")
