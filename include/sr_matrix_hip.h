@@ -143,6 +143,52 @@ int sr_grouped_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, 
 int sr_grouped_block_contract(const sr_block_matrix* a, const sr_block_matrix* b, int64_t columns, const sr_groups* groups,
                               void* out, int64_t ldo, int64_t out_stride, int out_dtype, void* stream);
 
+/* ---- low-rank adapters ------------------------------------------------- */
+
+/* Adapters that one call takes. */
+#define SR_MATRIX_ADAPTERS 65536
+
+/* `count` low-rank updates of one linear layer: a (count x rank x k) and b
+ * (count x n x rank), contiguous, of one dtype (FP32, BF16 or FP16; rank 1 to
+ * 128). `index` holds each row's adapter (int64 where `wide`, else int32); a
+ * row whose number is outside [0, count) has none.  An adapter's update is
+ * scaled by its number in `scaling`, or by `scale` where that is NULL. */
+typedef struct sr_adapters {
+  const void* a;
+  const void* b;
+  const void* index;
+  const float* scaling;
+  float scale;
+  int count;
+  int rank;
+  int dtype;
+  int wide;
+} sr_adapters;
+
+/* FP32 values that sr_adapter_add leaves in `low` for so many rows; 0 for
+ * shapes that it refuses. */
+int64_t sr_adapter_low(int64_t rows, int64_t k, int64_t rank, int dtype);
+
+/* out[t] = base[t] + s_i (x[t] a_i^T) b_i^T for i = index[t], and base[t] for
+ * rows without an adapter.  x (rows x k), base and out (rows x n; out may be
+ * base itself) have the adapters' dtype.  `low` receives s_i x[t] a_i^T, in
+ * parts, for sr_adapter_backward. */
+int sr_adapter_add(const sr_adapters* g, const void* x, int64_t ldx, int64_t k, const void* base, int64_t ldbase, int64_t n,
+                   int64_t rows, void* out, int64_t ldo, float* low, void* stream);
+
+/* Bytes of workspace for the gradients; 0 for shapes that they refuse. */
+int64_t sr_adapter_workspace(int64_t rows, int64_t k, int64_t n, int64_t count, int64_t rank, int dtype);
+
+/* The gradients of sr_adapter_add for dy (rows x n), each where it is not NULL,
+ * all of the adapters' dtype:
+ *   dx[t] = s_i (dy[t] b_i) a_i                (rows x k; zeros without an adapter)
+ *   da_i  = sum over i's rows of (s_i dy[t] b_i)^T x[t]     (count x rank x k)
+ *   db_i  = sum over i's rows of dy[t]^T (s_i x[t] a_i^T)   (count x n x rank)
+ * Adapters without rows get zeros.  `low` is what sr_adapter_add left. */
+int sr_adapter_backward(const sr_adapters* g, const void* x, int64_t ldx, int64_t k, const void* dy, int64_t lddy, int64_t n,
+                        int64_t rows, const float* low, void* dx, int64_t lddx, void* da, void* db, void* workspace,
+                        void* stream);
+
 /* ---- orthogonalised updates -------------------------------------------- */
 
 /* Newton-Schulz orthogonalisation of a matrix X (rows x cols): X / (|X|_F +

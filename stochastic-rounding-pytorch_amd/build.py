@@ -62,6 +62,9 @@ def units() -> list[tuple[Path, list[str], Path]]:
     jobs.append((CSRC / "sr_newton_schulz.hip", [], BUILD / "sr_newton_schulz.o"))
     jobs.append((CSRC / "sr_grouped_abi.hip", [], BUILD / "sr_grouped_abi.o"))
     jobs.append((CSRC / "sr_grouped_cast.hip", [], BUILD / "sr_grouped_cast.o"))
+    jobs.append((CSRC / "sr_adapter_abi.hip", [], BUILD / "sr_adapter_abi.o"))
+    for dtype in range(3):
+        jobs.append((CSRC / "sr_adapter.hip", [f"-DSR_TYPE={dtype}"], BUILD / f"sr_adapter_t{dtype}.o"))
     for e5m2 in range(2):
         jobs.append((CSRC / "sr_grouped_product.hip", [f"-DSR_A_E5M2={e5m2}"], BUILD / f"sr_grouped_product_a{e5m2}.o"))
         jobs.append((CSRC / "sr_block_product.hip", [f"-DSR_A_E5M2={e5m2}"], BUILD / f"sr_block_product_a{e5m2}.o"))

@@ -7,7 +7,8 @@
 // points through the addresses the Python side binds once.
 //
 // bind(block_cast, block_matmul, orthogonalize, orthogonalize_workspace, grouped_columns, grouped_block_cast,
-//      stacked_block_cast, grouped_block_matmul, grouped_block_contract)
+//      stacked_block_cast, grouped_block_matmul, grouped_block_contract, adapter_low, adapter_workspace, adapter_add,
+//      adapter_backward)
 //   Keep the addresses of these sr_ entry points, taken from the loaded library.
 //
 // block_cast(x, code, rule, square, axes, seed, offset, stream) -> tuple or int
@@ -34,6 +35,10 @@
 // grouped_linear_forward(x, weight, sizes, formats, seed, need_x, need_weight, stream)
 // grouped_linear_backward(dy, sizes, x_t data, x_t scale, w_t data, w_t scale, formats, seed, dx_code, dw_code, stream)
 //   As linear_forward and linear_backward.
+//
+// adapter_add(base, x, a, b, index, scaling, scale, out, stream) -> (tensor, low) or int
+//   base plus each row's low-rank update, into `out` where it is not None, and what the gradients need of it.
+// adapter_backward(dy, x, a, b, index, scaling, scale, low, need_x, need_a, need_b, stream) -> (dx, da, db) or int
 //
 // Errors of the tensors raise TypeError or ValueError before anything is
 // launched.  Every entry runs with the first tensor's device current and the
@@ -72,6 +77,10 @@ decltype(&sr_grouped_block_cast) g_grouped_cast = nullptr;
 decltype(&sr_stacked_block_cast) g_stacked_cast = nullptr;
 decltype(&sr_grouped_block_matmul) g_grouped_matmul = nullptr;
 decltype(&sr_grouped_block_contract) g_grouped_contract = nullptr;
+decltype(&sr_adapter_low) g_adapter_low = nullptr;
+decltype(&sr_adapter_workspace) g_adapter_workspace = nullptr;
+decltype(&sr_adapter_add) g_adapter_add = nullptr;
+decltype(&sr_adapter_backward) g_adapter_backward = nullptr;
 PyObject* g_out_of_memory = nullptr;  // torch.OutOfMemoryError
 
 // A refusal, raised as `type`.
@@ -391,9 +400,93 @@ at::Tensor as_stack(const at::Tensor& x) {
   return copy ? x.contiguous() : x;
 }
 
+// ---- low-rank adapters ----
+
+// The adapters of rows (..., k), checked; `a`, `b` and `index` are made contiguous.
+struct AdapterSet {
+  at::Tensor a, b, index, scaling;
+  sr_adapters g{};
+  int64_t rows = 0, k = 0, n = 0;
+
+  AdapterSet(const at::Tensor& x, const at::Tensor& given_a, const at::Tensor& given_b, const at::Tensor& given_index,
+             const at::Tensor& given_scaling, double scale) {
+    const int code = dtype_code(x.scalar_type());
+    if (!wide(code)) type_error("expected FP32, BF16 or FP16 input, got " + name_of(x.scalar_type()));
+    if (!x.is_cuda()) value_error("adapter_add requires GPU tensors");
+    for (const auto& [t, name] : {std::pair<const at::Tensor&, const char*>{given_a, "a"}, {given_b, "b"}}) {
+      if (t.scalar_type() != x.scalar_type()) type_error(std::string(name) + " must have x's dtype, got " + name_of(t.scalar_type()));
+      if (t.device() != x.device()) value_error(std::string(name) + " must be on x's device");
+      if (t.dim() != 3) value_error(std::string(name) + " is a stack of matrices, not " + std::to_string(t.dim()) + " dimensions");
+    }
+    if (x.dim() < 1) value_error("x has rows of values");
+    k = x.size(-1);
+    n = given_b.size(1);
+    rows = 1;
+    for (int64_t d = 0; d + 1 < x.dim(); ++d) rows *= x.size(d);
+    const int64_t count = given_a.size(0), rank = given_a.size(1);
+    if (given_b.size(0) != count || given_b.size(2) != rank || given_a.size(2) != k)
+      value_error("x of " + std::to_string(k) + " values, a " + shape_of(given_a.sizes()) + " and b " + shape_of(given_b.sizes()) +
+                  " do not match");
+    if (rank < 1 || rank > 128) value_error("adapters have rank 1 to 128, not " + std::to_string(rank));
+    if (count > SR_MATRIX_ADAPTERS) value_error(std::to_string(count) + " adapters: at most " + std::to_string(SR_MATRIX_ADAPTERS));
+    if (given_index.scalar_type() != c10::ScalarType::Int && given_index.scalar_type() != c10::ScalarType::Long)
+      type_error("index must be torch.int32 or torch.int64, got " + name_of(given_index.scalar_type()));
+    if (given_index.device() != x.device()) value_error("index must be on x's device");
+    if (given_index.dim() != x.dim() - 1 || given_index.sizes() != x.sizes().slice(0, x.dim() - 1))
+      value_error("index must hold an adapter for each row of x");
+    if (given_scaling.defined()) {
+      if (given_scaling.scalar_type() != c10::ScalarType::Float) type_error("scaling must be torch.float32, got " + name_of(given_scaling.scalar_type()));
+      if (given_scaling.device() != x.device() || given_scaling.dim() != 1 || given_scaling.size(0) != count)
+        value_error("scaling must hold a number for each adapter on x's device");
+      scaling = given_scaling.detach().resolve_neg().contiguous();
+    }
+    a = given_a.detach().resolve_neg().contiguous();
+    b = given_b.detach().resolve_neg().contiguous();
+    index = given_index.contiguous();
+    g = {memory(a), memory(b), memory(index), scaling.defined() && count ? static_cast<const float*>(memory(scaling)) : nullptr,
+         static_cast<float>(scale), static_cast<int>(count), static_cast<int>(rank), code, index.scalar_type() == c10::ScalarType::Long};
+  }
+};
+
+// base plus the updates; `low` is what the gradients need.
+at::Tensor add_adapters(const at::Tensor& base, const at::Tensor& x, const AdapterSet& set, at::Tensor out, at::Tensor& low, void* stream) {
+  if (base.scalar_type() != x.scalar_type()) type_error("base must have x's dtype, got " + name_of(base.scalar_type()));
+  if (base.device() != x.device()) value_error("base must be on x's device");
+  auto shape = x.sizes().vec();
+  shape.back() = set.n;
+  if (base.sizes() != at::IntArrayRef(shape)) value_error("base must be " + shape_of(shape) + ", not " + shape_of(base.sizes()));
+  const at::Tensor rows = as_rows(x.detach().resolve_neg()), from = as_rows(base.detach().resolve_neg());
+  const bool given = out.defined();
+  at::Tensor to;  // out as rows
+  if (given) {
+    if (out.scalar_type() != x.scalar_type()) type_error("out has dtype " + name_of(out.scalar_type()));
+    if (out.sizes() != base.sizes() || out.device() != x.device()) value_error("out must be a " + shape_of(shape) + " tensor on " + x.device().str());
+    if (out.is_neg()) value_error("lazily negated views cannot be used: call resolve_neg()");
+    if (out.requires_grad() && c10::GradMode::is_enabled())
+      throw Refusal(PyExc_RuntimeError, "out requires grad, and a given out records no gradients: call adapter_add under torch.no_grad()");
+    to = out.dim() == 2 ? out : out.view({set.rows, set.n});
+    row_stride(to, "out");
+    const auto [start, end] = span(out);
+    const bool same = from.const_data_ptr() == to.const_data_ptr() && from.sizes() == to.sizes() && from.strides() == to.strides();
+    for (const at::Tensor* t : {&rows, &set.a, &set.b, &set.index, &set.scaling, &from}) {
+      if (!t->defined() || (t == &from && same)) continue;
+      const auto [first, last] = span(*t);
+      if (start < last && first < end) value_error("out must not overlap the operands, but for base itself");
+    }
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+  } else {
+    out = at::empty(shape, x.options());
+    to = out.view({set.rows, set.n});
+  }
+  low = at::empty({g_adapter_low(set.rows, set.k, set.g.rank, set.g.dtype)}, x.options().dtype(c10::ScalarType::Float));
+  checked(g_adapter_add(&set.g, memory(rows), row_stride(rows, "x"), set.k, memory(from), row_stride(from, "base"), set.n, set.rows,
+                        memory(to), row_stride(to, "out"), static_cast<float*>(memory(low)), stream));
+  return out;
+}
+
 bool bound() {
   return g_cast && g_matmul && g_orthogonalize && g_workspace && g_columns && g_grouped_cast && g_stacked_cast &&
-         g_grouped_matmul && g_grouped_contract;
+         g_grouped_matmul && g_grouped_contract && g_adapter_low && g_adapter_workspace && g_adapter_add && g_adapter_backward;
 }
 
 // Runs `body` as the entries promise; nullptr with an exception set, the
@@ -464,8 +557,10 @@ PyObject* wrap_casts(const std::string& wanted, const Scaled& by_rows, const Sca
 }
 
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long at[9];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKK", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6], &at[7], &at[8])) return nullptr;
+  unsigned long long at[13];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKK", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6], &at[7], &at[8], &at[9],
+                        &at[10], &at[11], &at[12]))
+    return nullptr;
   auto keep = [](auto& function, unsigned long long value) {
     function = reinterpret_cast<std::remove_reference_t<decltype(function)>>(address(value));
   };
@@ -478,6 +573,10 @@ PyObject* bind(PyObject*, PyObject* args) {
   keep(g_stacked_cast, at[6]);
   keep(g_grouped_matmul, at[7]);
   keep(g_grouped_contract, at[8]);
+  keep(g_adapter_low, at[9]);
+  keep(g_adapter_workspace, at[10]);
+  keep(g_adapter_add, at[11]);
+  keep(g_adapter_backward, at[12]);
   if (!bound()) {
     PyErr_SetString(PyExc_ValueError, "null entry point address");
     return nullptr;
@@ -684,6 +783,57 @@ PyObject* grouped_linear_backward(PyObject*, PyObject* args) {
       [&] { return wrap_all({&dx, &dw}); });
 }
 
+PyObject* adapter_add(PyObject*, PyObject* args) {
+  PyObject *base_object, *x_object, *a_object, *b_object, *index_object, *scaling_object, *out_object;
+  double scale;
+  unsigned long long stream;
+  if (!PyArg_ParseTuple(args, "OOOOOOdOK", &base_object, &x_object, &a_object, &b_object, &index_object, &scaling_object, &scale,
+                        &out_object, &stream))
+    return nullptr;
+  const at::Tensor &base = tensor(base_object), &x = tensor(x_object), &a = tensor(a_object), &b = tensor(b_object),
+                   &index = tensor(index_object);
+  at::Tensor scaling, out, low, result;
+  if (scaling_object != Py_None) scaling = tensor(scaling_object);
+  if (out_object != Py_None) out = tensor(out_object);
+  const bool given = out.defined();
+  return run(
+      x.device(), [&] { result = add_adapters(base, x, AdapterSet(x, a, b, index, scaling, scale), out, low, address(stream)); },
+      [&]() -> PyObject* {
+        if (!given) return wrap_all({&result, &low});
+        return Py_BuildValue("(ON)", out_object, wrap(low));
+      });
+}
+
+PyObject* adapter_backward(PyObject*, PyObject* args) {
+  PyObject *dy_object, *x_object, *a_object, *b_object, *index_object, *scaling_object, *low_object;
+  double scale;
+  int need_x, need_a, need_b;
+  unsigned long long stream;
+  if (!PyArg_ParseTuple(args, "OOOOOOdOpppK", &dy_object, &x_object, &a_object, &b_object, &index_object, &scaling_object, &scale,
+                        &low_object, &need_x, &need_a, &need_b, &stream))
+    return nullptr;
+  const at::Tensor &dy = tensor(dy_object), &x = tensor(x_object), &a = tensor(a_object), &b = tensor(b_object),
+                   &index = tensor(index_object), &low = tensor(low_object);
+  at::Tensor scaling, dx, da, db;
+  if (scaling_object != Py_None) scaling = tensor(scaling_object);
+  return run(
+      x.device(),
+      [&] {
+        const AdapterSet set(x, a, b, index, scaling, scale);
+        const at::Tensor rows = as_rows(x.detach().resolve_neg()), from = as_rows(dy.detach().resolve_neg());
+        if (need_x) dx = at::empty(x.sizes(), x.options());
+        if (need_a) da = at::empty(a.sizes(), a.options());
+        if (need_b) db = at::empty(b.sizes(), b.options());
+        const at::Tensor workspace = at::empty({g_adapter_workspace(set.rows, set.k, set.n, set.g.count, set.g.rank, set.g.dtype)},
+                                               x.options().dtype(c10::ScalarType::Byte));
+        auto place = [](const at::Tensor& t) { return t.defined() ? memory(t) : nullptr; };
+        checked(g_adapter_backward(&set.g, memory(rows), row_stride(rows, "x"), set.k, memory(from), row_stride(from, "dy"), set.n,
+                                   set.rows, static_cast<const float*>(memory(low)), place(dx), set.k, place(da), place(db),
+                                   memory(workspace), address(stream)));
+      },
+      [&] { return wrap_all({&dx, &da, &db}); });
+}
+
 PyObject* orthogonalize(PyObject*, PyObject* args) {
   PyObject* object;
   int out_code;
@@ -741,6 +891,8 @@ PyMethodDef methods[] = {
     {"grouped_matmul", guarded<grouped_matmul>, METH_VARARGS, "Multiply each group's rows by its matrix, or contract its columns."},
     {"grouped_linear_forward", guarded<grouped_linear_forward>, METH_VARARGS, "Forward pass of the grouped linear layer."},
     {"grouped_linear_backward", guarded<grouped_linear_backward>, METH_VARARGS, "Gradients of the grouped linear layer."},
+    {"adapter_add", guarded<adapter_add>, METH_VARARGS, "Add each row's low-rank update."},
+    {"adapter_backward", guarded<adapter_backward>, METH_VARARGS, "Gradients of the low-rank updates."},
     {"orthogonalize", guarded<orthogonalize>, METH_VARARGS, "Orthogonalise matrices."},
     {nullptr, nullptr, 0, nullptr},
 };

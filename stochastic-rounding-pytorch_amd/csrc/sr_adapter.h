@@ -1,0 +1,780 @@
+// sr_adapter.h -- low-rank updates of rows that each have an adapter of their own:
+//
+//   y[t] = base[t] + s_i (x[t] a_i^T) b_i^T,  i = index[t]
+//
+// with a_i (rank x k) and b_i (n x rank), and their gradients.  Rows lie in any
+// order: a tile of 16 rows goes once through each adapter that it meets, and
+// keeps of every pass only the rows that are the adapter's.  Nothing of one
+// adapter reaches a row of another, infinities and NaN included.
+//
+//   shrink    low[t] = s_i x[t] a_i^T in FP32
+//   expand    y[t] = base[t] + low[t] b_i^T
+//   contract  sums over an adapter's rows t of low[t][r] x[t][c]: the gradients
+//             of a (low of dy and b, with x) and of b (low of x and a, with dy)
+//
+// The input's gradient is shrink by b^T and expand by a^T.
+//
+// Numbers.  Products of x and the adapters run on their type's matrix
+// instructions; what follows takes `low` as FP32.  With BF16 operands a value
+// of it enters as two BF16 parts, truncated and rest, which keep 15 bits: far
+// below the result's rounding.  FP16 has no exponents for that, so FP16 operands
+// widen to FP32 there.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "../../include/sr_matrix_hip.h"
+#include "sr_group_access.h"
+#include "sr_math.h"
+#include "sr_tile_product.h"
+
+namespace sr {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// Sixteen and eight bytes at the alignment of one element.
+typedef uint32_t halves8 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t halves4 __attribute__((ext_vector_type(2), aligned(2)));
+typedef float floats4 __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kAdapterWaves = 4, kAdapterThreads = 64 * kAdapterWaves;
+constexpr int kRankChunk = 16;  // ranks of one matrix instruction's result
+
+struct Adapters {
+  const char* a;         // count x rank x k, or for gradients its transpose or b's
+  const void* index;     // the rows' adapters, int64 where `wide`, else int32; none where outside [0, count)
+  const float* scaling;  // one for each adapter, or null:
+  float scale;           // for all
+  int count, rank, chunks;  // chunks: of 16 ranks
+  int wide;
+  int64_t rows;
+};
+
+__device__ __forceinline__ int adapter_of(const Adapters& g, int64_t row) {
+  if (row >= g.rows) return -1;
+  if (g.wide) {
+    const int64_t i = gptr<int64_t>(g.index)[row];
+    return i >= 0 && i < g.count ? static_cast<int>(i) : -1;
+  }
+  const int i = gptr<int32_t>(g.index)[row];
+  return i >= 0 && i < g.count ? i : -1;
+}
+
+__device__ __forceinline__ float adapter_scale(const Adapters& g, int adapter) {
+  return g.scaling ? gptr<float>(g.scaling)[adapter < 0 ? 0 : adapter] : g.scale;
+}
+
+// Eight consecutive values of the contracted axis, as a matrix instruction takes them.
+template <int XE>
+struct Eight {
+  uint32_t w[enc_bytes(XE) * 2];
+};
+
+template <int XE>
+__device__ __forceinline__ Eight<XE> load_eight_whole(const char* row, int64_t c) {
+  Eight<XE> e;
+  if constexpr (enc_bytes(XE) == 2) {
+    const halves8 v = *(const SR_GLOBAL halves8*)(row + 2 * c);
+    __builtin_memcpy(e.w, &v, 16);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const floats4 v = *(const SR_GLOBAL floats4*)(row + 4 * c + 16 * h);
+      __builtin_memcpy(e.w + 4 * h, &v, 16);
+    }
+  }
+  return e;
+}
+
+// The same with zeros from place `end` on.
+template <int XE>
+__device__ __forceinline__ Eight<XE> load_eight_to(const char* row, int64_t c, int64_t end) {
+  if (c + 8 <= end) return load_eight_whole<XE>(row, c);
+  Eight<XE> e{};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (c + j < end) {
+      if constexpr (enc_bytes(XE) == 2) e.w[j >> 1] |= static_cast<uint32_t>(gptr<uint16_t>(row)[c + j]) << (16 * (j & 1));
+      else e.w[j] = gptr<uint32_t>(row)[c + j];
+    }
+  }
+  return e;
+}
+
+// acc[4 q + e][i] += sum over the eight places of first and second: see sr_tile_product.h.
+template <int XE>
+__device__ __forceinline__ void mma_eight(f32x4& acc, const Eight<XE>& first, const Eight<XE>& second) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  if constexpr (XE == ENC_BF16_RN) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, first), __builtin_bit_cast(bf16x8, second), acc, 0, 0, 0);
+  } else if constexpr (XE == ENC_F16_RN) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, first), __builtin_bit_cast(f16x8, second), acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f32(first.w[j]), bits_f32(second.w[j]), acc, 0, 0, 0);
+  }
+#endif
+}
+
+// Two FP32 values as BF16, rounded to nearest, and the upper halves of two words.
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{lo, hi}, bf16x2));
+}
+__device__ __forceinline__ uint32_t upper_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
+__device__ __forceinline__ uint32_t lower_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x05040100u); }
+
+// What truncation to BF16 leaves of x; nothing of infinities and NaN.
+__device__ __forceinline__ float bf16_rest(float x) {
+  const uint32_t b = f32_bits(x);
+  return (b & 0x7F800000u) == 0x7F800000u ? 0.0f : x - bits_f32(b & 0xFFFF0000u);
+}
+
+// Four values in T at `p`, of which `live` are there.
+template <int XE>
+__device__ __forceinline__ f32x4 load_four(const char* p, int live) {
+  f32x4 x{};
+  if constexpr (enc_bytes(XE) == 4) {
+    if (live >= 4) {
+      const floats4 v = *(const SR_GLOBAL floats4*)(p);
+      return f32x4{v[0], v[1], v[2], v[3]};
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < live) x[j] = gptr<float>(p)[j];
+  } else {
+    uint32_t w[2] = {0, 0};
+    if (live >= 4) {
+      const halves4 v = *(const SR_GLOBAL halves4*)(p);
+      w[0] = v[0];
+      w[1] = v[1];
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < live) w[j >> 1] |= static_cast<uint32_t>(gptr<uint16_t>(p)[j]) << (16 * (j & 1));
+    }
+    if constexpr (XE == ENC_BF16_RN) {
+      x = f32x4{bits_f32(w[0] << 16), bits_f32(w[0] & 0xFFFF0000u), bits_f32(w[1] << 16), bits_f32(w[1] & 0xFFFF0000u)};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)))));
+    }
+  }
+  return x;
+}
+
+template <int XE>
+__device__ __forceinline__ void store_four(char* p, const f32x4& x, int live) {
+  if constexpr (enc_bytes(XE) == 4) {
+    if (live >= 4) {
+      *(SR_GLOBAL floats4*)(p) = floats4{x[0], x[1], x[2], x[3]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < live) gptr_mut<float>(p)[j] = x[j];
+    }
+  } else {
+    uint32_t w[2];
+    if constexpr (XE == ENC_BF16_RN) {
+      w[0] = pack_bf16(x[0], x[1]);
+      w[1] = pack_bf16(x[2], x[3]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[h] = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x[2 * h]))) |
+               static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x[2 * h + 1]))) << 16;
+    }
+    if (live >= 4) {
+      *(SR_GLOBAL halves4*)(p) = halves4{w[0], w[1]};
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < live) gptr_mut<uint16_t>(p)[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+__device__ __forceinline__ int live_four(int64_t at, int64_t end) { return at >= end ? 0 : (end - at < 4 ? static_cast<int>(end - at) : 4); }
+
+// Calls use(adapter, number) for every adapter that 16 rows meet, in the order of their first rows; `mine` is this
+// lane's.  Uniform.
+template <class F>
+__device__ __forceinline__ void for_each_adapter(int mine, F&& use) {
+  uint32_t todo = static_cast<uint32_t>(__ballot(mine >= 0)) & 0xFFFFu;
+  for (int number = 0; todo; ++number) {
+    const int adapter = __builtin_amdgcn_readlane(mine, __builtin_ctz(todo));
+    todo &= ~static_cast<uint32_t>(__ballot(mine == adapter));
+    use(adapter, number);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// shrink: a workgroup takes 16 rows and one of `splits` parts of the contracted
+// axis; its four waves take a quarter of that each, or, where the rows meet
+// four adapters or more, every fourth adapter.  Partial sums of the parts lie
+// behind each other in `low`, for expand and contract to add in order.
+// ---------------------------------------------------------------------------
+struct ShrinkArgs {
+  Adapters g;
+  const char* x;
+  int64_t ldx, k;
+  float* low;  // splits x rows x 16 chunks
+  int row_tiles, splits;
+};
+
+template <int XE>
+constexpr int kShrinkStep = 4 * 32 / enc_bytes(XE);  // values of the contracted axis that a wave takes at once: 32 bytes a lane
+
+template <int XE, int RC>
+__global__ __launch_bounds__(kAdapterThreads) void adapter_shrink_kernel(ShrinkArgs s) {
+  constexpr int kStep = kShrinkStep<XE>, kLane = kStep / 4, kEights = kLane / 8;
+  __shared__ f32x4 sums[kAdapterWaves][RC][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  const int split = blockIdx.x / s.row_tiles, tile = blockIdx.x - split * s.row_tiles;
+  const int64_t row = static_cast<int64_t>(tile) * 16 + i;
+  const int mine = adapter_of(s.g, row);
+  const char* x = s.x + (row < s.g.rows ? row : s.g.rows - 1) * s.ldx * enc_bytes(XE);
+  int met = 0;
+  for_each_adapter(mine, [&](int, int) { ++met; });
+  const bool many = met >= kAdapterWaves;
+
+  const int64_t steps = (s.k + kStep - 1) / kStep, parts = static_cast<int64_t>(s.splits) * kAdapterWaves, each = (steps + parts - 1) / parts;
+  const int64_t first = (static_cast<int64_t>(split) * kAdapterWaves + (many ? 0 : wave)) * each;
+  const int64_t behind = first + (many ? kAdapterWaves : 1) * each, last = behind < steps ? behind : steps;
+  const int64_t whole = s.k / kStep < last ? s.k / kStep : last;
+
+  f32x4 acc[RC] = {};
+  for_each_adapter(mine, [&](int adapter, int number) {
+    if (many && (number & (kAdapterWaves - 1)) != wave) return;
+    const char* rows[RC];
+#pragma unroll
+    for (int c = 0; c < RC; ++c) {
+      const int rank = c * kRankChunk + i;
+      rows[c] = s.g.a + (static_cast<int64_t>(adapter) * s.g.rank + (rank < s.g.rank ? rank : s.g.rank - 1)) * s.k * enc_bytes(XE);
+    }
+    f32x4 part[RC] = {};
+    // So many steps' loads go out together.
+    constexpr int kTogether = RC == 1 ? 4 : (RC == 2 ? 2 : 1);
+    auto step = [&](int64_t kt, auto together, auto load) {
+      constexpr int kSteps = decltype(together)::value;
+      Eight<XE> v[kSteps][kEights], m[kSteps][RC][kEights];
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+        for (int e = 0; e < kEights; ++e) {
+          const int64_t at = (kt + u) * kStep + q * kLane + 8 * e;
+          v[u][e] = load(x, at);
+#pragma unroll
+          for (int c = 0; c < RC; ++c)
+            if (c < s.g.chunks) m[u][c][e] = load(rows[c], at);
+        }
+#pragma unroll
+      for (int u = 0; u < kSteps; ++u)
+#pragma unroll
+        for (int c = 0; c < RC; ++c) {
+          if (c < s.g.chunks) {
+#pragma unroll
+            for (int e = 0; e < kEights; ++e) mma_eight<XE>(part[c], m[u][c][e], v[u][e]);
+          }
+        }
+    };
+    auto inside = [](const char* p, int64_t c) { return load_eight_whole<XE>(p, c); };
+    int64_t kt = first;
+    for (; kt + kTogether <= whole; kt += kTogether) step(kt, std::integral_constant<int, kTogether>{}, inside);
+    for (; kt < whole; ++kt) step(kt, std::integral_constant<int, 1>{}, inside);
+    if (whole < last && first <= whole)
+      step(whole, std::integral_constant<int, 1>{}, [&](const char* p, int64_t c) { return load_eight_to<XE>(p, c, s.k); });
+#pragma unroll
+    for (int c = 0; c < RC; ++c)
+      if (mine == adapter) acc[c] = part[c];
+  });
+  if (wave > 0) {
+#pragma unroll
+    for (int c = 0; c < RC; ++c) sums[wave][c][lane] = acc[c];
+  }
+  __syncthreads();
+  if (wave > 0 || row >= s.g.rows) return;
+  const float scale = adapter_scale(s.g, mine);
+  const int64_t width = s.g.chunks * kRankChunk;
+#pragma unroll
+  for (int c = 0; c < RC; ++c) {
+    if (c >= s.g.chunks) break;
+#pragma unroll
+    for (int w = 1; w < kAdapterWaves; ++w) acc[c] += sums[w][c][lane];
+    f32x4 out{};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = mine >= 0 && c * kRankChunk + 4 * q + j < s.g.rank ? acc[c][j] * scale : 0.0f;
+    *(SR_GLOBAL floats4*)(s.low + (split * s.g.rows + row) * width + c * kRankChunk + 4 * q) = floats4{out[0], out[1], out[2], out[3]};
+  }
+}
+
+// Sixteen ranks of `low` and of the adapters as the products with FP32 values take them.  With BF16, 32 places of the
+// contracted axis are the sixteen ranks twice, by the truncated parts and by the rests; else four instructions take four
+// ranks each.
+template <int XE>
+struct Sixteen {
+  static constexpr bool kParts = XE == ENC_BF16_RN;
+  uint32_t w[4];  // eight BF16 values, or four FP32 ones
+
+  // The ranks from 16 c on of one row of low, `splits` partial sums `stride` apart.
+  static __device__ __forceinline__ Sixteen of_low(const float* row, int64_t stride, int splits, int c, int q) {
+    Sixteen s;
+    auto four = [&](int at) {
+      const floats4 v = *(const SR_GLOBAL floats4*)(row + at);
+      f32x4 sum{v[0], v[1], v[2], v[3]};
+      for (int p = 1; p < splits; ++p) {
+        const floats4 more = *(const SR_GLOBAL floats4*)(row + p * stride + at);
+        sum += f32x4{more[0], more[1], more[2], more[3]};
+      }
+      return sum;
+    };
+    if constexpr (kParts) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f32x4 v = four(c * kRankChunk + 8 * (q & 1) + 4 * h);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float lo = v[2 * j], hi = v[2 * j + 1];
+          s.w[2 * h + j] = q < 2 ? upper_halves(f32_bits(lo), f32_bits(hi)) : pack_bf16(bf16_rest(lo), bf16_rest(hi));
+        }
+      }
+    } else {
+      const f32x4 v = four(c * kRankChunk + 4 * q);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s.w[j] = f32_bits(v[j]);
+    }
+    return s;
+  }
+
+  // Those of a row of b, of which `rank` are there.
+  static __device__ __forceinline__ Sixteen of_row(const char* row, int rank, int c, int q) {
+    Sixteen s;
+    if constexpr (kParts) {
+      const Eight<XE> e = load_eight_to<XE>(row, c * kRankChunk + 8 * (q & 1), rank);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s.w[j] = e.w[j];
+    } else {
+      const int at = c * kRankChunk + 4 * q;
+      const f32x4 v = load_four<XE>(row + at * enc_bytes(XE), live_four(at, rank));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s.w[j] = f32_bits(v[j]);
+    }
+    return s;
+  }
+
+  __device__ __forceinline__ void mma(f32x4& acc, const Sixteen& second) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+    if constexpr (kParts) {
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, second.w), acc, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bits_f32(w[j]), bits_f32(second.w[j]), acc, 0, 0, 0);
+    }
+#endif
+  }
+};
+
+// ---------------------------------------------------------------------------
+// expand: a wave takes 16 NT columns of `tiles` times 16 rows.  Its instructions
+// take the rows of b in an order that leaves a lane 4 NT neighbouring columns of a
+// row.  The adapter met last stays in registers.
+// ---------------------------------------------------------------------------
+struct ExpandArgs {
+  Adapters g;  // a: count x n x rank
+  const float* low;
+  const char* base;  // or null: zeros
+  char* out;
+  int64_t ldbase, ldout, n;
+  int row_groups, tiles, splits;  // groups of `tiles` times 16 rows
+};
+
+template <int XE, int RC, int NT>
+__global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandArgs s) {
+  constexpr int kSize = enc_bytes(XE);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  const int block = blockIdx.x / s.row_groups, group = blockIdx.x - block * s.row_groups;
+  const int64_t n0 = (static_cast<int64_t>(block) * kAdapterWaves + wave) * 16 * NT;
+  if (n0 >= s.n) return;
+  const int64_t width = s.g.chunks * kRankChunk, stride = s.g.rows * width;
+  const int64_t col = n0 + q * 4 * NT;  // this lane's first
+
+  Sixteen<XE> b[NT][RC];
+  int held = -1;
+  auto hold = [&](int adapter) {
+    if (adapter == held) return;
+    held = adapter;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int64_t at = n0 + (i >> 2) * 4 * NT + 4 * t + (i & 3);
+      const char* row = s.g.a + (static_cast<int64_t>(adapter) * s.n + (at < s.n ? at : s.n - 1)) * s.g.rank * kSize;
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+        if (c < s.g.chunks) b[t][c] = Sixteen<XE>::of_row(row, s.g.rank, c, q);
+    }
+  };
+
+  for (int tile = 0; tile < s.tiles; ++tile) {
+    const int64_t row0 = (static_cast<int64_t>(group) * s.tiles + tile) * 16, row = row0 + i;
+    if (row0 >= s.g.rows) break;
+    const int mine = adapter_of(s.g, row);
+    const int64_t safe = row < s.g.rows ? row : s.g.rows - 1;
+    f32x4 sum[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      sum[t] = s.base ? load_four<XE>(s.base + (safe * s.ldbase + col + 4 * t) * kSize, live_four(col + 4 * t, s.n)) : f32x4{};
+    Sixteen<XE> low[RC];
+#pragma unroll
+    for (int c = 0; c < RC; ++c)
+      if (c < s.g.chunks) low[c] = Sixteen<XE>::of_low(s.low + safe * width, stride, s.splits, c, q);
+    for_each_adapter(mine, [&](int adapter, int) {
+      hold(adapter);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 part = {};
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+          if (c < s.g.chunks) b[t][c].mma(part, low[c]);
+        if (mine == adapter) sum[t] += part;
+      }
+    });
+    if (row < s.g.rows) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) store_four<XE>(s.out + (row * s.ldout + col + 4 * t) * kSize, sum[t], live_four(col + 4 * t, s.n));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// contract: out[i][r][c] = sum over the rows t of adapter i of low[t][r] x[t][c].
+//
+// A workgroup takes an adapter, 16 CJ columns and one part of the rows.  It
+// first lists the part's rows that are the adapter's, in order; its waves then
+// take 32 of them at a time in turn, turned in registers so that rows are the
+// contracted axis, and add their sums in wave order.  Parts leave FP32 sums
+// and whether they had rows at all, for `finish` to add in order.
+// ---------------------------------------------------------------------------
+struct ContractOperand {
+  const float* low;  // splits x rows x 16 chunks
+  int splits;
+  const char* x;
+  int64_t ldx, cols;
+  char* out;         // count x rank x cols, or count x cols x rank where `turned`
+  float* partial;    // parts x count x (16 chunks) x cols
+  int turned;
+  int tiles;         // of 16 CJ columns
+};
+
+struct ContractArgs {
+  Adapters g;
+  ContractOperand op[2];
+  int parts;             // 1: results go straight to out
+  int64_t part_rows;     // a multiple of kListRows
+  int* filled;           // parts x count
+};
+
+constexpr int kListRows = 1024;
+
+// Eight rows of CJ columns at `c` of each, and their transpose: CJ eights of one column each.
+template <int XE, int CJ>
+struct Turned {
+  static constexpr int kWords = CJ * enc_bytes(XE) / 4;
+  uint32_t row[8][kWords];
+
+  __device__ __forceinline__ void load(int e, const char* p, int live) {
+    if (live >= CJ) {
+#pragma unroll
+      for (int h = 0; h < kWords; h += 4) {
+        if constexpr (kWords >= 4) {
+          if constexpr (enc_bytes(XE) == 2) {
+            const halves8 v = *(const SR_GLOBAL halves8*)(p + 4 * h);
+            __builtin_memcpy(row[e] + h, &v, 16);
+          } else {
+            const floats4 v = *(const SR_GLOBAL floats4*)(p + 4 * h);
+            __builtin_memcpy(row[e] + h, &v, 16);
+          }
+        } else {
+          const halves4 v = *(const SR_GLOBAL halves4*)(p);
+          __builtin_memcpy(row[e], &v, 8);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < kWords; ++h) row[e][h] = 0;
+#pragma unroll
+      for (int j = 0; j < CJ; ++j) {
+        if (j < live) {
+          if constexpr (enc_bytes(XE) == 2) row[e][j >> 1] |= static_cast<uint32_t>(gptr<uint16_t>(p)[j]) << (16 * (j & 1));
+          else row[e][j] = gptr<uint32_t>(p)[j];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void clear(int e) {
+#pragma unroll
+    for (int h = 0; h < kWords; ++h) row[e][h] = 0;
+  }
+  // Column j of all eight rows as BF16 pairs.
+  __device__ __forceinline__ void halves(int j, uint32_t (&w)[4]) const {
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      w[p] = j & 1 ? upper_halves(row[2 * p][j >> 1], row[2 * p + 1][j >> 1]) : lower_halves(row[2 * p][j >> 1], row[2 * p + 1][j >> 1]);
+  }
+  // Column j of row e as FP32.
+  __device__ __forceinline__ float value(int j, int e) const {
+    if constexpr (XE == ENC_F32) return bits_f32(row[e][j]);
+    else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(row[e][j >> 1] >> (16 * (j & 1)))));
+  }
+};
+
+template <int XE, int RC, int CJ>
+__global__ __launch_bounds__(kAdapterThreads) void adapter_contract_kernel(ContractArgs s) {
+  constexpr int kSize = enc_bytes(XE);
+  constexpr bool kParts = XE == ENC_BF16_RN;
+  __shared__ uint32_t list[kListRows];
+  __shared__ uint32_t counts[kAdapterWaves];
+  __shared__ f32x4 sums[CJ * RC][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  uint32_t id = blockIdx.x;
+  const uint32_t tiles = s.op[0].tiles + s.op[1].tiles;
+  const uint32_t part = id / (tiles * s.g.count);
+  id -= part * tiles * s.g.count;
+  const int adapter = static_cast<int>(id / tiles);
+  id -= adapter * tiles;
+  const bool second = id >= static_cast<uint32_t>(s.op[0].tiles);
+  const ContractOperand& op = s.op[second];
+  const int64_t c0 = static_cast<int64_t>(second ? id - s.op[0].tiles : id) * 16 * CJ + i * CJ;  // this lane's first column
+  const int live = c0 >= op.cols ? 0 : (op.cols - c0 < CJ ? static_cast<int>(op.cols - c0) : CJ);
+  const int64_t width = s.g.chunks * kRankChunk, stride = s.g.rows * width;
+  const int64_t begin = part * s.part_rows, end = begin + s.part_rows < s.g.rows ? begin + s.part_rows : s.g.rows;
+
+  f32x4 acc[CJ][RC] = {};
+  bool any = false;
+  for (int64_t at = begin; at < end; at += kListRows) {
+    // Each thread looks at four neighbouring rows.
+    constexpr int kOwn = kListRows / kAdapterThreads;
+    uint32_t own = 0;
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      const int64_t row = at + threadIdx.x * kOwn + j;
+      if (row < end && adapter_of(s.g, row) == adapter) own |= 1u << j;
+    }
+    uint32_t before = __builtin_popcount(own);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t up = static_cast<uint32_t>(__shfl_up(static_cast<int>(before), d));
+      if (lane >= d) before += up;
+    }
+    __syncthreads();  // the list of before is done with
+    if (lane == 63) counts[wave] = before;
+    __syncthreads();
+    uint32_t total = 0, place = before - __builtin_popcount(own);
+#pragma unroll
+    for (int w = 0; w < kAdapterWaves; ++w) {
+      if (w < wave) place += counts[w];
+      total += counts[w];
+    }
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j)
+      if (own >> j & 1) list[place++] = threadIdx.x * kOwn + j;
+    __syncthreads();
+    any |= total > 0;
+    for (uint32_t first = wave * 32; first < total; first += 32 * kAdapterWaves) {
+      Turned<XE, CJ> x;
+      float low[RC][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t place_e = first + q * 8 + e;
+        const bool there = place_e < total;
+        const int64_t row = at + list[there ? place_e : 0];
+        x.load(e, op.x + (row * op.ldx + c0) * kSize, live);
+        if (!there) x.clear(e);
+#pragma unroll
+        for (int c = 0; c < RC; ++c) {
+          low[c][e] = 0;
+          if (c < s.g.chunks) {
+            const float* p = op.low + row * width + c * kRankChunk + i;
+            float v = *gptr<float>(p);
+            for (int k = 1; k < op.splits; ++k) v += *gptr<float>(p + k * stride);
+            low[c][e] = there ? v : 0.0f;
+          }
+        }
+      }
+      if constexpr (kParts) {
+        Eight<XE> upper[RC], rest[RC];
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+#pragma unroll
+          for (int p = 0; p < 4; ++p) {
+            upper[c].w[p] = upper_halves(f32_bits(low[c][2 * p]), f32_bits(low[c][2 * p + 1]));
+            rest[c].w[p] = pack_bf16(bf16_rest(low[c][2 * p]), bf16_rest(low[c][2 * p + 1]));
+          }
+#pragma unroll
+        for (int j = 0; j < CJ; ++j) {
+          Eight<XE> column;
+          x.halves(j, column.w);
+#pragma unroll
+          for (int c = 0; c < RC; ++c) {
+            if (c < s.g.chunks) {
+              mma_eight<XE>(acc[j][c], upper[c], column);
+              mma_eight<XE>(acc[j][c], rest[c], column);
+            }
+          }
+        }
+      } else {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+          for (int j = 0; j < CJ; ++j) {
+            const float v = x.value(j, e);
+#pragma unroll
+            for (int c = 0; c < RC; ++c)
+              if (c < s.g.chunks) acc[j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[c][e], v, acc[j][c], 0, 0, 0);
+          }
+#endif
+      }
+    }
+  }
+
+  for (int w = 1; w < kAdapterWaves; ++w) {
+    __syncthreads();
+    if (wave == w) {
+#pragma unroll
+      for (int j = 0; j < CJ; ++j)
+#pragma unroll
+        for (int c = 0; c < RC; ++c) sums[j * RC + c][lane] = acc[j][c];
+    }
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int j = 0; j < CJ; ++j)
+#pragma unroll
+        for (int c = 0; c < RC; ++c) acc[j][c] += sums[j * RC + c][lane];
+    }
+  }
+  if (wave > 0) return;
+  if (s.parts > 1) {
+    if (c0 == 0 && !second && q == 0) s.filled[part * s.g.count + adapter] = any;
+    if (!any) return;
+    float* to = op.partial + (static_cast<int64_t>(part) * s.g.count + adapter) * width * op.cols;
+#pragma unroll
+    for (int c = 0; c < RC; ++c) {
+      if (c >= s.g.chunks) break;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < CJ; j += 4)
+          store_four<ENC_F32>(reinterpret_cast<char*>(to + (c * kRankChunk + 4 * q + e) * op.cols + c0 + j),
+                              f32x4{acc[j][c][e], acc[j + 1][c][e], acc[j + 2][c][e], acc[j + 3][c][e]}, live_four(c0 + j, op.cols));
+    }
+    return;
+  }
+#pragma unroll
+  for (int c = 0; c < RC; ++c) {
+    if (c >= s.g.chunks) break;
+    const int rank = c * kRankChunk + 4 * q;
+    if (op.turned) {
+#pragma unroll
+      for (int j = 0; j < CJ; ++j)
+        if (j < live)
+          store_four<XE>(op.out + ((adapter * op.cols + c0 + j) * s.g.rank + rank) * kSize, acc[j][c], live_four(rank, s.g.rank));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (rank + e < s.g.rank) {
+#pragma unroll
+          for (int j = 0; j < CJ; j += 4)
+            store_four<XE>(op.out + ((static_cast<int64_t>(adapter) * s.g.rank + rank + e) * op.cols + c0 + j) * kSize,
+                           f32x4{acc[j][c][e], acc[j + 1][c][e], acc[j + 2][c][e], acc[j + 3][c][e]}, live_four(c0 + j, op.cols));
+        }
+    }
+  }
+}
+
+// Threads that finish an operand's results.
+inline __host__ __device__ int64_t finish_items(const Adapters& g, const ContractOperand& op) {
+  if (!op.out) return 0;
+  return g.count * (op.turned ? op.cols * ((g.rank + 3) / 4) : (op.cols + 3) / 4 * g.rank);
+}
+
+// Adds the parts' sums: a thread takes four columns of one rank, or of a turned result four ranks of one column.
+template <int XE>
+__global__ __launch_bounds__(256) void adapter_finish_kernel(ContractArgs s) {
+  const int64_t width = s.g.chunks * kRankChunk;
+  int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t firsts = finish_items(s.g, s.op[0]);
+  const bool second = id >= firsts;
+  if (second) id -= firsts;
+  const ContractOperand& op = s.op[second];
+  const int64_t quads = (op.cols + 3) / 4, ranks = (s.g.rank + 3) / 4;
+  int64_t adapter, rank, col;
+  if (op.turned) {
+    // Neighbouring threads take neighbouring columns, whose partial sums lie side by side.
+    col = id % op.cols;
+    rank = id / op.cols % ranks * 4;
+    adapter = id / op.cols / ranks;
+  } else {
+    col = id % quads * 4;
+    rank = id / quads % s.g.rank;
+    adapter = id / quads / s.g.rank;
+  }
+  if (adapter >= s.g.count) return;
+  f32x4 sum{};
+  for (int p = 0; p < s.parts; ++p) {
+    if (!gptr<int>(s.filled)[p * s.g.count + adapter]) continue;
+    const float* from = op.partial + ((p * static_cast<int64_t>(s.g.count) + adapter) * width + rank) * op.cols + col;
+    if (op.turned) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += *gptr<float>(from + e * op.cols);  // ranks up to `width` are there
+    } else {
+      sum += load_four<ENC_F32>(reinterpret_cast<const char*>(from), live_four(col, op.cols));
+    }
+  }
+  if (op.turned)
+    store_four<XE>(op.out + ((adapter * op.cols + col) * s.g.rank + rank) * enc_bytes(XE), sum, live_four(rank, s.g.rank));
+  else
+    store_four<XE>(op.out + ((adapter * s.g.rank + rank) * op.cols + col) * enc_bytes(XE), sum, live_four(col, op.cols));
+}
+
+// ---------------------------------------------------------------------------
+// The adapters turned, for the input's gradient: to[i][c][r] = from[i][r][c], tiles of 64 x 64 through LDS.
+// ---------------------------------------------------------------------------
+struct TurnOperand {
+  const char* from;
+  char* to;
+  int64_t rows, cols;
+  int tiles_n;
+  uint32_t tiles;  // of all matrices
+};
+
+struct TurnArgs {
+  TurnOperand op[2];
+};
+
+template <int SIZE>
+__global__ __launch_bounds__(256) void adapter_turn_kernel(TurnArgs s) {
+  using T = std::conditional_t<SIZE == 4, uint32_t, uint16_t>;
+  __shared__ T tile[64][64 + 4 / SIZE];
+  const bool second = blockIdx.x >= s.op[0].tiles;
+  const TurnOperand& op = s.op[second];
+  const uint32_t id = blockIdx.x - (second ? s.op[0].tiles : 0);
+  const uint32_t tiles_m = static_cast<uint32_t>((op.rows + 63) / 64), each = tiles_m * op.tiles_n;
+  const uint32_t matrix = id / each, within = id - matrix * each;
+  const int64_t r0 = static_cast<int64_t>(within / op.tiles_n) * 64, c0 = static_cast<int64_t>(within % op.tiles_n) * 64;
+  const T* from = reinterpret_cast<const T*>(op.from) + matrix * op.rows * op.cols;
+  T* to = reinterpret_cast<T*>(op.to) + matrix * op.rows * op.cols;
+  const int column = threadIdx.x & 63, first = threadIdx.x >> 6;
+#pragma unroll
+  for (int r = 0; r < 64; r += 4)
+    if (r0 + r + first < op.rows && c0 + column < op.cols) tile[r + first][column] = gptr<T>(from)[(r0 + r + first) * op.cols + c0 + column];
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < 64; c += 4)
+    if (c0 + c + first < op.cols && r0 + column < op.rows) gptr_mut<T>(to)[(c0 + c + first) * op.rows + r0 + column] = tile[column][c + first];
+}
+
+}  // namespace sr

@@ -22,6 +22,7 @@ from .hip import (
     MuonHipRN,
     SGDMHip,
     SGDMHipRN,
+    adapter_add,
     block_cast,
     block_linear,
     block_matmul,
@@ -54,6 +55,7 @@ __all__ = [
     "SGDMReferenceSR",
     "StateFormat",
     "StateOptimizer",
+    "adapter_add",
     "block_cast",
     "block_linear",
     "block_matmul",

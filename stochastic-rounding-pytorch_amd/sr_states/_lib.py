@@ -79,6 +79,7 @@ BLOCK = 128  # values that share a scale along the contracted axis
 SCALE_E8M0, SCALE_F32 = range(2)
 MATRIX_BATCH = 64  # matrices one launch takes
 MATRIX_GROUPS = 4096  # groups one call takes
+MATRIX_ADAPTERS = 65536  # adapters one call takes
 
 
 class BlockMatrix(ctypes.Structure):
@@ -110,6 +111,20 @@ class Groups(ctypes.Structure):
 
 class BlockStack(ctypes.Structure):
     _fields_ = [("out", BlockOutput), ("stride", ctypes.c_int64), ("stride_scale", ctypes.c_int64)]
+
+
+class AdapterSet(ctypes.Structure):
+    _fields_ = [
+        ("a", ctypes.c_void_p),
+        ("b", ctypes.c_void_p),
+        ("index", ctypes.c_void_p),
+        ("scaling", ctypes.c_void_p),
+        ("scale", ctypes.c_float),
+        ("count", ctypes.c_int),
+        ("rank", ctypes.c_int),
+        ("dtype", ctypes.c_int),
+        ("wide", ctypes.c_int),
+    ]
 
 
 class NewtonSchulz(ctypes.Structure):
@@ -217,6 +232,16 @@ MATRIX_SIGNATURES = {
         _int,
         [ctypes.POINTER(BlockMatrix), ctypes.POINTER(BlockMatrix), _i64, ctypes.POINTER(Groups), _vp, _i64, _i64, _int,
          _vp],
+    ),
+    "sr_adapter_low": (_i64, [_i64, _i64, _i64, _int]),
+    "sr_adapter_add": (
+        _int,
+        [ctypes.POINTER(AdapterSet), _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp],
+    ),
+    "sr_adapter_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64, _int]),
+    "sr_adapter_backward": (
+        _int,
+        [ctypes.POINTER(AdapterSet), _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _vp],
     ),
     "sr_orthogonalize_workspace": (_i64, [_i64, _i64, _i64]),
     "sr_orthogonalize": (
@@ -353,7 +378,8 @@ def matrix():
         module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value
                       for name in ("sr_block_cast", "sr_block_matmul", "sr_orthogonalize", "sr_orthogonalize_workspace",
                                    "sr_grouped_columns", "sr_grouped_block_cast", "sr_stacked_block_cast",
-                                   "sr_grouped_block_matmul", "sr_grouped_block_contract")))
+                                   "sr_grouped_block_matmul", "sr_grouped_block_contract", "sr_adapter_low",
+                                   "sr_adapter_workspace", "sr_adapter_add", "sr_adapter_backward")))
         _matrix = module
     return _matrix
 

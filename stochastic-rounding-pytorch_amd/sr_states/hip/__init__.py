@@ -2,6 +2,7 @@
 
 from ._common import is_hip_available
 from .adamw import AdamWHip, AdamWHipRN, hip_adamw_step_
+from .adapter import adapter_add
 from .block import BlockScaled, block_cast, block_linear, block_matmul
 from .cast import cast, rn_cast_bf16, sr_cast_bf16
 from .grouped import grouped_block_cast, grouped_block_linear, grouped_block_matmul
@@ -16,6 +17,7 @@ __all__ = [
     "MuonHipRN",
     "SGDMHip",
     "SGDMHipRN",
+    "adapter_add",
     "block_cast",
     "block_linear",
     "block_matmul",

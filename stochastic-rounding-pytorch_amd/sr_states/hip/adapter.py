@@ -1,0 +1,83 @@
+"""Low-rank adapters of many requests at once, beside a projection that they share.
+
+A batch's rows go through one projection (``block_linear``, or any other), and
+each row adds the low-rank update of its own adapter: ``adapter_add``.  The
+adapters of a batch are stacked, and ``index`` says which one each row uses, in
+any order, or none.  The same call serves single tokens of many requests, a
+prompt batch, and training, with gradients of the input and of the adapters.
+
+The reference package has no counterpart.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from .block import _device_of, _stream
+
+
+class _AdapterAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, base, x, a, b, index, scaling, scale):
+        out = _lib.matrix().adapter_add(base, x, a, b, index, scaling, scale, None, _stream(x.device))
+        if not isinstance(out, tuple):
+            _lib.check("adapter_add", out)
+        ctx.save_for_backward(x, a, b, index, scaling, out[1])
+        ctx.scale = scale
+        return out[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, a, b, index, scaling, low = ctx.saved_tensors
+        need_base, *need = ctx.needs_input_grad[:4]
+        grads = (None, None, None)
+        if any(need):
+            grads = _lib.matrix().adapter_backward(dy, x, a, b, index, scaling, ctx.scale, low, *need, _stream(dy.device))
+            if not isinstance(grads, tuple):
+                _lib.check("adapter_add", grads)
+        return (dy if need_base else None, *grads, None, None, None)
+
+
+def adapter_add(
+    base: torch.Tensor,
+    x: torch.Tensor,
+    a: torch.Tensor,
+    b: torch.Tensor,
+    index: torch.Tensor,
+    *,
+    scaling: float | torch.Tensor = 1.0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """``base + scaling * (x @ a[i].T) @ b[i].T`` with an adapter ``i`` of its own for each row.
+
+    ``x`` is (..., k) and ``base`` (..., n), the result of the projection that the
+    rows share; ``a`` is (adapters, rank, k) and ``b`` (adapters, n, rank), rank 1
+    to 128; all are FP32, BF16 or FP16, alike, on the GPU.  ``index`` (int32 or
+    int64, x's shape without its last size) holds each row's adapter; a row
+    whose number is outside [0, adapters) has none, and its result is ``base``'s.
+    ``scaling`` is a number, or an FP32 tensor with one for each adapter, which
+    gets no gradient.
+
+    Sums are FP32 and rounded once, at the end.  Gradients flow to ``base``, ``x``,
+    ``a`` and ``b``; adapters that no row uses get zeros.  ``out``, which may be
+    ``base`` itself, takes the result without recording gradients: in grad mode
+    neither it nor an operand may require one.
+    """
+    device = _device_of(x, base, a, b, index, out)
+    each = isinstance(scaling, torch.Tensor)
+    if each:
+        if scaling.requires_grad and torch.is_grad_enabled():
+            raise ValueError("scaling gets no gradient: detach it")
+        scale = 1.0
+    else:
+        scale, scaling = float(scaling), None
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, a, b)):
+        if out is not None:
+            raise RuntimeError("a given out records no gradients: call adapter_add under torch.no_grad()")
+        return _AdapterAdd.apply(base, x, a, b, index, scaling, scale)
+    result = _lib.matrix().adapter_add(base, x, a, b, index, scaling, scale, out, _stream(device))
+    if not isinstance(result, tuple):
+        _lib.check("adapter_add", result)
+    return result[0]
