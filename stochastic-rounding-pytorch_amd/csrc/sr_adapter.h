@@ -210,51 +210,60 @@ __device__ __forceinline__ void for_each_adapter(int mine, F&& use) {
 }
 
 // ---------------------------------------------------------------------------
-// shrink: a workgroup takes 16 rows and one of `splits` parts of the contracted
-// axis; its four waves take a quarter of that each, or, where the rows meet
-// four adapters or more, every fourth adapter.  Partial sums of the parts lie
-// behind each other in `low`, for expand and contract to add in order.
+// shrink: a workgroup takes 16 rows, one of `splits` parts of the contracted axis
+// and, of the adapters that the rows meet, every `slots`-th.  Its eight waves
+// share these adapters out as far as they go, and the part's steps beyond that.
+// Partial sums of the parts lie behind each other in `low`, for expand and
+// contract to add in order; a row is written by its adapter's workgroup alone.
 // ---------------------------------------------------------------------------
 struct ShrinkArgs {
   Adapters g;
   const char* x;
   int64_t ldx, k;
   float* low;  // splits x rows x 16 chunks
-  int row_tiles, splits;
+  int row_tiles, splits, slots;
 };
 
+constexpr int kShrinkWaves = 8;
 template <int XE>
 constexpr int kShrinkStep = 4 * 32 / enc_bytes(XE);  // values of the contracted axis that a wave takes at once: 32 bytes a lane
 
 template <int XE, int RC>
-__global__ __launch_bounds__(kAdapterThreads) void adapter_shrink_kernel(ShrinkArgs s) {
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(ShrinkArgs s) {
   constexpr int kStep = kShrinkStep<XE>, kLane = kStep / 4, kEights = kLane / 8;
-  __shared__ f32x4 sums[kAdapterWaves][RC][64];
+  __shared__ f32x4 sums[kShrinkWaves][RC][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
-  const int split = blockIdx.x / s.row_tiles, tile = blockIdx.x - split * s.row_tiles;
+  const int tile = blockIdx.x % s.row_tiles, unit = blockIdx.x / s.row_tiles, slot = unit % s.slots, split = unit / s.slots;
   const int64_t row = static_cast<int64_t>(tile) * 16 + i;
   const int mine = adapter_of(s.g, row);
   const char* x = s.x + (row < s.g.rows ? row : s.g.rows - 1) * s.ldx * enc_bytes(XE);
-  int met = 0;
-  for_each_adapter(mine, [&](int, int) { ++met; });
-  const bool many = met >= kAdapterWaves;
+  int met = 0;          // by this workgroup
+  bool owned = mine < 0 && slot == 0;  // this lane's row is written here
+  for_each_adapter(mine, [&](int adapter, int number) {
+    if (number % s.slots != slot) return;
+    ++met;
+    owned |= mine == adapter;
+  });
+  if (met == 0 && slot > 0) return;
+  const int shares = met >= 8 ? 1 : (met >= 4 ? 2 : (met >= 2 ? 4 : 8));  // waves of one adapter
 
-  const int64_t steps = (s.k + kStep - 1) / kStep, parts = static_cast<int64_t>(s.splits) * kAdapterWaves, each = (steps + parts - 1) / parts;
-  const int64_t first = (static_cast<int64_t>(split) * kAdapterWaves + (many ? 0 : wave)) * each;
-  const int64_t behind = first + (many ? kAdapterWaves : 1) * each, last = behind < steps ? behind : steps;
+  const int64_t steps = (s.k + kStep - 1) / kStep, part = (steps + s.splits - 1) / s.splits;
+  const int64_t begin = split * part, end = begin + part < steps ? begin + part : steps;
+  const int64_t each = (part + shares - 1) / shares, first = begin + wave % shares * each;
+  const int64_t last = first + each < end ? first + each : end;
   const int64_t whole = s.k / kStep < last ? s.k / kStep : last;
 
   f32x4 acc[RC] = {};
   for_each_adapter(mine, [&](int adapter, int number) {
-    if (many && (number & (kAdapterWaves - 1)) != wave) return;
+    if (number % s.slots != slot || number / s.slots % (kShrinkWaves / shares) != wave / shares) return;
     const char* rows[RC];
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
       const int rank = c * kRankChunk + i;
       rows[c] = s.g.a + (static_cast<int64_t>(adapter) * s.g.rank + (rank < s.g.rank ? rank : s.g.rank - 1)) * s.k * enc_bytes(XE);
     }
-    f32x4 part[RC] = {};
+    f32x4 sum[RC] = {};
     // So many steps' loads go out together.
     constexpr int kTogether = RC == 1 ? 4 : (RC == 2 ? 2 : 1);
     auto step = [&](int64_t kt, auto together, auto load) {
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_shrink_kernel(ShrinkA
         for (int c = 0; c < RC; ++c) {
           if (c < s.g.chunks) {
 #pragma unroll
-            for (int e = 0; e < kEights; ++e) mma_eight<XE>(part[c], m[u][c][e], v[u][e]);
+            for (int e = 0; e < kEights; ++e) mma_eight<XE>(sum[c], m[u][c][e], v[u][e]);
           }
         }
     };
@@ -288,26 +297,23 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_shrink_kernel(ShrinkA
       step(whole, std::integral_constant<int, 1>{}, [&](const char* p, int64_t c) { return load_eight_to<XE>(p, c, s.k); });
 #pragma unroll
     for (int c = 0; c < RC; ++c)
-      if (mine == adapter) acc[c] = part[c];
+      if (mine == adapter) acc[c] = sum[c];
   });
-  if (wave > 0) {
 #pragma unroll
-    for (int c = 0; c < RC; ++c) sums[wave][c][lane] = acc[c];
-  }
+  for (int c = 0; c < RC; ++c) sums[wave][c][lane] = acc[c];
   __syncthreads();
-  if (wave > 0 || row >= s.g.rows) return;
+  // Wave c adds chunk c.
+  if (wave >= s.g.chunks || !owned || row >= s.g.rows) return;
+  f32x4 total = sums[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < kShrinkWaves; ++w) total += sums[w][wave][lane];
   const float scale = adapter_scale(s.g, mine);
   const int64_t width = s.g.chunks * kRankChunk;
+  const int rank = wave * kRankChunk + 4 * q;
+  f32x4 out{};
 #pragma unroll
-  for (int c = 0; c < RC; ++c) {
-    if (c >= s.g.chunks) break;
-#pragma unroll
-    for (int w = 1; w < kAdapterWaves; ++w) acc[c] += sums[w][c][lane];
-    f32x4 out{};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = mine >= 0 && c * kRankChunk + 4 * q + j < s.g.rank ? acc[c][j] * scale : 0.0f;
-    *(SR_GLOBAL floats4*)(s.low + (split * s.g.rows + row) * width + c * kRankChunk + 4 * q) = floats4{out[0], out[1], out[2], out[3]};
-  }
+  for (int j = 0; j < 4; ++j) out[j] = mine >= 0 && rank + j < s.g.rank ? total[j] * scale : 0.0f;
+  *(SR_GLOBAL floats4*)(s.low + (split * s.g.rows + row) * width + rank) = floats4{out[0], out[1], out[2], out[3]};
 }
 
 // Sixteen ranks of `low` and of the adapters as the products with FP32 values take them.  With BF16, 32 places of the
@@ -318,34 +324,11 @@ struct Sixteen {
   static constexpr bool kParts = XE == ENC_BF16_RN;
   uint32_t w[4];  // eight BF16 values, or four FP32 ones
 
-  // The ranks from 16 c on of one row of low, `splits` partial sums `stride` apart.
-  static __device__ __forceinline__ Sixteen of_low(const float* row, int64_t stride, int splits, int c, int q) {
-    Sixteen s;
-    auto four = [&](int at) {
-      const floats4 v = *(const SR_GLOBAL floats4*)(row + at);
-      f32x4 sum{v[0], v[1], v[2], v[3]};
-      for (int p = 1; p < splits; ++p) {
-        const floats4 more = *(const SR_GLOBAL floats4*)(row + p * stride + at);
-        sum += f32x4{more[0], more[1], more[2], more[3]};
-      }
-      return sum;
-    };
-    if constexpr (kParts) {
+  // A lane's part of the 64 bytes that expand lays out for a row of low.
+  __device__ __forceinline__ void of_lds(const char* p) {
+    const i32x4 v = read_chunk(p);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const f32x4 v = four(c * kRankChunk + 8 * (q & 1) + 4 * h);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float lo = v[2 * j], hi = v[2 * j + 1];
-          s.w[2 * h + j] = q < 2 ? upper_halves(f32_bits(lo), f32_bits(hi)) : pack_bf16(bf16_rest(lo), bf16_rest(hi));
-        }
-      }
-    } else {
-      const f32x4 v = four(c * kRankChunk + 4 * q);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) s.w[j] = f32_bits(v[j]);
-    }
-    return s;
+    for (int j = 0; j < 4; ++j) w[j] = static_cast<uint32_t>(v[j]);
   }
 
   // Those of a row of b, of which `rank` are there.
@@ -377,9 +360,12 @@ struct Sixteen {
 };
 
 // ---------------------------------------------------------------------------
-// expand: a wave takes 16 NT columns of `tiles` times 16 rows.  Its instructions
-// take the rows of b in an order that leaves a lane 4 NT neighbouring columns of a
-// row.  The adapter met last stays in registers.
+// expand: a workgroup takes TILES times 16 rows, whose `low` it adds up and lays out
+// in LDS once; its waves take 16 NT columns each.  Their instructions take the
+// rows of b in an order that leaves a lane 4 NT neighbouring columns of a row.
+// All of base is on its way before anything waits, and the adapter met last
+// stays in registers.  With `slots` > 1 so many waves take every slots-th of the
+// adapters that 16 rows meet, and write only these rows.
 // ---------------------------------------------------------------------------
 struct ExpandArgs {
   Adapters g;  // a: count x n x rank
@@ -387,19 +373,131 @@ struct ExpandArgs {
   const char* base;  // or null: zeros
   char* out;
   int64_t ldbase, ldout, n;
-  int row_groups, tiles, splits;  // groups of `tiles` times 16 rows
+  int splits, slots;
+  int column_tiles;  // of 16 NT
+  int blocks;        // of kAdapterWaves column tiles and slots
 };
 
-template <int XE, int RC, int NT>
+// N neighbouring values of a row as they lie.
+template <int XE, int N>
+struct Run {
+  static constexpr int kWords = N * enc_bytes(XE) / 4;
+  uint32_t w[kWords];
+
+  __device__ __forceinline__ void load(const char* p) {
+#pragma unroll
+    for (int h = 0; h < kWords; h += 4) {
+      if constexpr (enc_bytes(XE) == 4) {
+        const floats4 v = *(const SR_GLOBAL floats4*)(p + 4 * h);
+        __builtin_memcpy(w + h, &v, 16);
+      } else if constexpr (kWords >= 4) {
+        const halves8 v = *(const SR_GLOBAL halves8*)(p + 4 * h);
+        __builtin_memcpy(w + h, &v, 16);
+      } else {
+        const halves4 v = *(const SR_GLOBAL halves4*)(p);
+        __builtin_memcpy(w, &v, 8);
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const char* p, int live) {
+#pragma unroll
+    for (int h = 0; h < kWords; ++h) w[h] = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < live) {
+        if constexpr (enc_bytes(XE) == 2) w[j >> 1] |= static_cast<uint32_t>(gptr<uint16_t>(p)[j]) << (16 * (j & 1));
+        else w[j] = gptr<uint32_t>(p)[j];
+      }
+    }
+  }
+  __device__ __forceinline__ float value(int j) const {
+    if constexpr (enc_bytes(XE) == 4) return bits_f32(w[j]);
+    else if constexpr (XE == ENC_BF16_RN) return bits_f32(j & 1 ? w[j >> 1] & 0xFFFF0000u : w[j >> 1] << 16);
+    else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)))));
+  }
+  __device__ __forceinline__ void set(int j, float lo, float hi) {  // values j and j + 1, j even
+    if constexpr (enc_bytes(XE) == 4) {
+      w[j] = f32_bits(lo);
+      w[j + 1] = f32_bits(hi);
+    } else if constexpr (XE == ENC_BF16_RN) {
+      w[j >> 1] = pack_bf16(lo, hi);
+    } else {
+      w[j >> 1] = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(lo))) |
+                  static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(hi))) << 16;
+    }
+  }
+  __device__ __forceinline__ void store(char* p) const {
+#pragma unroll
+    for (int h = 0; h < kWords; h += 4) {
+      if constexpr (enc_bytes(XE) == 4)
+        *(SR_GLOBAL floats4*)(p + 4 * h) = floats4{bits_f32(w[h]), bits_f32(w[h + 1]), bits_f32(w[h + 2]), bits_f32(w[h + 3])};
+      else if constexpr (kWords >= 4) *(SR_GLOBAL halves8*)(p + 4 * h) = halves8{w[h], w[h + 1], w[h + 2], w[h + 3]};
+      else *(SR_GLOBAL halves4*)(p) = halves4{w[0], w[1]};
+    }
+  }
+  __device__ __forceinline__ void store(char* p, int live) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (j < live) {
+        if constexpr (enc_bytes(XE) == 2) gptr_mut<uint16_t>(p)[j] = static_cast<uint16_t>(w[j >> 1] >> (16 * (j & 1)));
+        else gptr_mut<uint32_t>(p)[j] = w[j];
+      }
+    }
+  }
+};
+
+template <int XE, int RC, int NT, int TILES>
 __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandArgs s) {
-  constexpr int kSize = enc_bytes(XE);
+  constexpr int kSize = enc_bytes(XE), kRows = 16 * TILES, kChunkBytes = 64;
+  __shared__ __align__(16) char lows[kRows * RC * kChunkBytes];
+  __shared__ int indices[kRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
-  const int block = blockIdx.x / s.row_groups, group = blockIdx.x - block * s.row_groups;
-  const int64_t n0 = (static_cast<int64_t>(block) * kAdapterWaves + wave) * 16 * NT;
-  if (n0 >= s.n) return;
-  const int64_t width = s.g.chunks * kRankChunk, stride = s.g.rows * width;
+  const uint32_t group = blockIdx.x / s.blocks, unit = (blockIdx.x - group * s.blocks) * kAdapterWaves + wave;
+  const uint32_t slot = unit % s.slots;
+  const int64_t n0 = static_cast<int64_t>(unit / s.slots) * 16 * NT, row0 = static_cast<int64_t>(group) * kRows;
   const int64_t col = n0 + q * 4 * NT;  // this lane's first
+  const bool edge = n0 + 16 * NT > s.n;
+  const int live = col >= s.n ? 0 : (s.n - col < 4 * NT ? static_cast<int>(s.n - col) : 4 * NT);
+
+  Run<XE, 4 * NT> base[TILES];
+  if (s.base) {
+#pragma unroll
+    for (int tile = 0; tile < TILES; ++tile) {
+      const int64_t row = row0 + tile * 16 + i;
+      const char* p = s.base + ((row < s.g.rows ? row : s.g.rows - 1) * s.ldbase + col) * kSize;
+      if (edge) base[tile].load(p, live);
+      else base[tile].load(p);
+    }
+  }
+  const int64_t width = s.g.chunks * kRankChunk, stride = s.g.rows * width;
+  if (threadIdx.x < kRows) indices[threadIdx.x] = adapter_of(s.g, row0 + threadIdx.x);
+  // Four values at a time, all of the group's rows side by side.
+  const int64_t fours = (s.g.rows - row0 < kRows ? s.g.rows - row0 : kRows) * width / 4;
+  for (int64_t at = threadIdx.x; at < fours; at += kAdapterThreads) {
+    const float* from = s.low + row0 * width + 4 * at;
+    const floats4 v = *(const SR_GLOBAL floats4*)(from);
+    f32x4 sum{v[0], v[1], v[2], v[3]};
+    for (int p = 1; p < s.splits; ++p) {
+      const floats4 more = *(const SR_GLOBAL floats4*)(from + p * stride);
+      sum += f32x4{more[0], more[1], more[2], more[3]};
+    }
+    const int row = static_cast<int>(4 * at / width), place = static_cast<int>(4 * at - row * width);
+    char* to = lows + (row * RC + place / kRankChunk) * kChunkBytes;
+    const int rank = place % kRankChunk;
+    if constexpr (Sixteen<XE>::kParts) {
+      // Sixteen truncated parts, then the sixteen rests.
+      uint32_t* w = reinterpret_cast<uint32_t*>(to + 2 * rank);
+      w[0] = upper_halves(f32_bits(sum[0]), f32_bits(sum[1]));
+      w[1] = upper_halves(f32_bits(sum[2]), f32_bits(sum[3]));
+      w[8] = pack_bf16(bf16_rest(sum[0]), bf16_rest(sum[1]));
+      w[9] = pack_bf16(bf16_rest(sum[2]), bf16_rest(sum[3]));
+    } else {
+      *reinterpret_cast<f32x4*>(to + 4 * rank) = sum;
+    }
+  }
+  __syncthreads();
+  if (n0 >= s.n) return;
 
   Sixteen<XE> b[NT][RC];
   int held = -1;
@@ -408,42 +506,49 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
     held = adapter;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int64_t at = n0 + (i >> 2) * 4 * NT + 4 * t + (i & 3);
-      const char* row = s.g.a + (static_cast<int64_t>(adapter) * s.n + (at < s.n ? at : s.n - 1)) * s.g.rank * kSize;
+      const int64_t n = n0 + (i >> 2) * 4 * NT + 4 * t + (i & 3);
+      const char* row = s.g.a + (static_cast<int64_t>(adapter) * s.n + (n < s.n ? n : s.n - 1)) * s.g.rank * kSize;
 #pragma unroll
       for (int c = 0; c < RC; ++c)
         if (c < s.g.chunks) b[t][c] = Sixteen<XE>::of_row(row, s.g.rank, c, q);
     }
   };
-
-  for (int tile = 0; tile < s.tiles; ++tile) {
-    const int64_t row0 = (static_cast<int64_t>(group) * s.tiles + tile) * 16, row = row0 + i;
-    if (row0 >= s.g.rows) break;
-    const int mine = adapter_of(s.g, row);
-    const int64_t safe = row < s.g.rows ? row : s.g.rows - 1;
-    f32x4 sum[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-      sum[t] = s.base ? load_four<XE>(s.base + (safe * s.ldbase + col + 4 * t) * kSize, live_four(col + 4 * t, s.n)) : f32x4{};
-    Sixteen<XE> low[RC];
-#pragma unroll
-    for (int c = 0; c < RC; ++c)
-      if (c < s.g.chunks) low[c] = Sixteen<XE>::of_low(s.low + safe * width, stride, s.splits, c, q);
-    for_each_adapter(mine, [&](int adapter, int) {
+  for (int tile = 0; tile < TILES; ++tile) {
+    const int64_t row = row0 + tile * 16 + i;
+    const int mine = indices[tile * 16 + i];
+    f32x4 sum[NT] = {};
+    bool owned = mine < 0 && slot == 0;
+    for_each_adapter(mine, [&](int adapter, int number) {
+      if (number % s.slots != slot) return;
       hold(adapter);
+      owned |= mine == adapter;
+      Sixteen<XE> low[RC];
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+        if (c < s.g.chunks) low[c].of_lds(lows + ((tile * 16 + i) * RC + c) * kChunkBytes + 16 * q);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         f32x4 part = {};
 #pragma unroll
         for (int c = 0; c < RC; ++c)
           if (c < s.g.chunks) b[t][c].mma(part, low[c]);
-        if (mine == adapter) sum[t] += part;
+        if (mine == adapter) sum[t] = part;
       }
     });
-    if (row < s.g.rows) {
+    if (!owned || row >= s.g.rows) continue;
+    Run<XE, 4 * NT> out = base[tile];
+    if (!s.base) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) store_four<XE>(s.out + (row * s.ldout + col + 4 * t) * kSize, sum[t], live_four(col + 4 * t, s.n));
+      for (int j = 0; j < 4 * NT; j += 2) out.set(j, sum[j >> 2][j & 3], sum[j >> 2][(j & 3) + 1]);
+    } else if (mine >= 0) {
+#pragma unroll
+      for (int j = 0; j < 4 * NT; j += 2)
+        out.set(j, base[tile].value(j) + sum[j >> 2][j & 3], base[tile].value(j + 1) + sum[j >> 2][(j & 3) + 1]);
     }
+    char* p = s.out + (row * s.ldout + col) * kSize;
+    if (edge) out.store(p, live);
+    else out.store(p);
   }
 }
 

@@ -16,8 +16,8 @@ void fill(AdapterKernels& k, int at) {
   // A row's eight neighbouring columns where they are 16 bytes and their sums leave registers for the loads.
   constexpr int CJ = enc_bytes(XE) == 4 || RC == 8 ? 4 : 8;
   k.shrink[at] = reinterpret_cast<const void*>(&adapter_shrink_kernel<XE, RC>);
-  k.expand[at][0] = reinterpret_cast<const void*>(&adapter_expand_kernel<XE, RC, 1>);
-  k.expand[at][1] = reinterpret_cast<const void*>(&adapter_expand_kernel<XE, RC, 4>);
+  k.expand[at][0] = reinterpret_cast<const void*>(&adapter_expand_kernel<XE, RC, 1, 1>);
+  k.expand[at][1] = reinterpret_cast<const void*>(&adapter_expand_kernel<XE, RC, 4, kExpandTiles>);
   k.contract[at] = reinterpret_cast<const void*>(&adapter_contract_kernel<XE, RC, CJ>);
   k.contract_columns[at] = 16 * CJ;
 }

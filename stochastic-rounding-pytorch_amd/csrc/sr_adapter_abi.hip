@@ -41,7 +41,7 @@ bool shape_is_good(int64_t rows, int64_t k, int64_t n, int64_t count, int64_t ra
 // Parts of the contracted axis: so many that few rows give every CU work, at least a step for each wave.
 int splits_of(int64_t rows, int64_t k, int dtype) {
   const int64_t tiles = (rows + 15) / 16, steps = (k + kernels(dtype).step - 1) / kernels(dtype).step;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 256 / std::max<int64_t>(tiles, 1), steps / sr::kAdapterWaves})));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({8, 256 / std::max<int64_t>(tiles, 1), steps / sr::kShrinkWaves})));
 }
 
 int64_t low_values(int64_t rows, int64_t k, int rank, int dtype) {
@@ -73,6 +73,9 @@ sr::Adapters adapters_of(const sr_adapters* g, const void* matrices, int64_t row
   return a;
 }
 
+// Workgroups, or waves, that share the adapters of 16 rows: more of them where there are few otherwise.
+int slots_of(int64_t others, int count) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({4, 256 / std::max<int64_t>(others, 1), count}))); }
+
 // low = the scaled products of x with `matrices` (count x rank x k).
 int shrink(const sr_adapters* g, const void* matrices, const void* x, int64_t ldx, int64_t k, int64_t rows, float* low, void* stream) {
   sr::ShrinkArgs s{};
@@ -83,7 +86,9 @@ int shrink(const sr_adapters* g, const void* matrices, const void* x, int64_t ld
   s.low = low;
   s.row_tiles = static_cast<int>((rows + 15) / 16);
   s.splits = splits_of(rows, k, g->dtype);
-  return launch(kernels(g->dtype).shrink[rank_index(s.g.chunks)], static_cast<uint64_t>(s.row_tiles) * s.splits, sr::kAdapterThreads, &s, stream);
+  s.slots = slots_of(static_cast<int64_t>(s.row_tiles) * s.splits, g->count);
+  return launch(kernels(g->dtype).shrink[rank_index(s.g.chunks)], static_cast<uint64_t>(s.row_tiles) * s.splits * s.slots,
+                64 * sr::kShrinkWaves, &s, stream);
 }
 
 // out = base + low by `matrices` (count x n x rank), transposed.
@@ -100,11 +105,12 @@ int expand(const sr_adapters* g, const void* matrices, const float* low, int spl
   s.splits = splits;
   const int64_t row_tiles = (rows + 15) / 16, waves = row_tiles * ((n + 63) / 64);
   const bool wide = waves >= 1024;
-  s.tiles = wide ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(4, waves / 4096))) : 1;
-  s.row_groups = static_cast<int>((row_tiles + s.tiles - 1) / s.tiles);
-  const int64_t columns = (wide ? 64 : 16) * sr::kAdapterWaves;
-  return launch(kernels(g->dtype).expand[rank_index(s.g.chunks)][wide], static_cast<uint64_t>((n + columns - 1) / columns) * s.row_groups,
-                sr::kAdapterThreads, &s, stream);
+  const int64_t groups = wide ? (row_tiles + sr::kExpandTiles - 1) / sr::kExpandTiles : row_tiles;
+  s.slots = wide ? 1 : std::max(1, std::min(4, g->count));
+  s.column_tiles = static_cast<int>((n + (wide ? 63 : 15)) / (wide ? 64 : 16));
+  s.blocks = (s.column_tiles * s.slots + sr::kAdapterWaves - 1) / sr::kAdapterWaves;
+  return launch(kernels(g->dtype).expand[rank_index(s.g.chunks)][wide], static_cast<uint64_t>(groups) * s.blocks, sr::kAdapterThreads, &s,
+                stream);
 }
 
 // How the rows of a gradient are parted.

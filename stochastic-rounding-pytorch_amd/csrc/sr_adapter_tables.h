@@ -4,10 +4,11 @@
 namespace sr {
 
 constexpr int kAdapterRanks = 4;  // up to 16, 32, 64 and 128 ranks
+constexpr int kExpandTiles = 4;   // times 16 rows of a workgroup of expand whose waves take 64 columns; else 1 and 16
 
 struct AdapterKernels {
   const void* shrink[kAdapterRanks];
-  const void* expand[kAdapterRanks][2];  // [.][1]: 64 columns a wave, else 16
+  const void* expand[kAdapterRanks][2];  // [.][1]: 64 columns a wave
   const void* contract[kAdapterRanks];
   int contract_columns[kAdapterRanks];   // of a workgroup
   const void* finish;
