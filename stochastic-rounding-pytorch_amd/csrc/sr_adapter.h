@@ -65,22 +65,27 @@ __device__ __forceinline__ float adapter_scale(const Adapters& g, int adapter) {
   return g.scaling ? gptr<float>(g.scaling)[adapter < 0 ? 0 : adapter] : g.scale;
 }
 
-// Eight consecutive values of the contracted axis, as a matrix instruction takes them.
+// Eight values of the contracted axis, as a matrix instruction takes them.  Which ones share a lane does not matter as
+// long as both operands agree: lane q of a row's four takes 16 bytes at 16 q of each 64, so that an access covers 64
+// neighbouring bytes of a row.
 template <int XE>
 struct Eight {
   uint32_t w[enc_bytes(XE) * 2];
 };
 
+constexpr int kEightSpan = 32;  // values of a row that its four lanes' eights are
+
+// Lane q's of the 32 values from place `at` of a row on.
 template <int XE>
-__device__ __forceinline__ Eight<XE> load_eight_whole(const char* row, int64_t c) {
+__device__ __forceinline__ Eight<XE> load_eight_whole(const char* row, int64_t at, int q) {
   Eight<XE> e;
   if constexpr (enc_bytes(XE) == 2) {
-    const halves8 v = *(const SR_GLOBAL halves8*)(row + 2 * c);
+    const halves8 v = *(const SR_GLOBAL halves8*)(row + 2 * at + 16 * q);
     __builtin_memcpy(e.w, &v, 16);
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const floats4 v = *(const SR_GLOBAL floats4*)(row + 4 * c + 16 * h);
+      const floats4 v = *(const SR_GLOBAL floats4*)(row + 4 * at + 64 * h + 16 * q);
       __builtin_memcpy(e.w + 4 * h, &v, 16);
     }
   }
@@ -89,14 +94,14 @@ __device__ __forceinline__ Eight<XE> load_eight_whole(const char* row, int64_t c
 
 // The same with zeros from place `end` on.
 template <int XE>
-__device__ __forceinline__ Eight<XE> load_eight_to(const char* row, int64_t c, int64_t end) {
-  if (c + 8 <= end) return load_eight_whole<XE>(row, c);
+__device__ __forceinline__ Eight<XE> load_eight_to(const char* row, int64_t at, int q, int64_t end) {
   Eight<XE> e{};
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    if (c + j < end) {
-      if constexpr (enc_bytes(XE) == 2) e.w[j >> 1] |= static_cast<uint32_t>(gptr<uint16_t>(row)[c + j]) << (16 * (j & 1));
-      else e.w[j] = gptr<uint32_t>(row)[c + j];
+    const int64_t c = at + (enc_bytes(XE) == 2 ? 8 * q + j : 16 * (j >> 2) + 4 * q + (j & 3));
+    if (c < end) {
+      if constexpr (enc_bytes(XE) == 2) e.w[j >> 1] |= static_cast<uint32_t>(gptr<uint16_t>(row)[c]) << (16 * (j & 1));
+      else e.w[j] = gptr<uint32_t>(row)[c];
     }
   }
   return e;
@@ -226,11 +231,11 @@ struct ShrinkArgs {
 
 constexpr int kShrinkWaves = 8;
 template <int XE>
-constexpr int kShrinkStep = 4 * 32 / enc_bytes(XE);  // values of the contracted axis that a wave takes at once: 32 bytes a lane
+constexpr int kShrinkStep = 4 * 32 / enc_bytes(XE);  // values of the contracted axis that a wave takes at once: 128 bytes of a row
 
 template <int XE, int RC>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(ShrinkArgs s) {
-  constexpr int kStep = kShrinkStep<XE>, kLane = kStep / 4, kEights = kLane / 8;
+  constexpr int kStep = kShrinkStep<XE>, kEights = kStep / kEightSpan;
   __shared__ f32x4 sums[kShrinkWaves][RC][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
@@ -273,7 +278,7 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Shrin
       for (int u = 0; u < kSteps; ++u)
 #pragma unroll
         for (int e = 0; e < kEights; ++e) {
-          const int64_t at = (kt + u) * kStep + q * kLane + 8 * e;
+          const int64_t at = (kt + u) * kStep + kEightSpan * e;
           v[u][e] = load(x, at);
 #pragma unroll
           for (int c = 0; c < RC; ++c)
@@ -289,12 +294,12 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Shrin
           }
         }
     };
-    auto inside = [](const char* p, int64_t c) { return load_eight_whole<XE>(p, c); };
+    auto inside = [&](const char* p, int64_t c) { return load_eight_whole<XE>(p, c, q); };
     int64_t kt = first;
     for (; kt + kTogether <= whole; kt += kTogether) step(kt, std::integral_constant<int, kTogether>{}, inside);
     for (; kt < whole; ++kt) step(kt, std::integral_constant<int, 1>{}, inside);
     if (whole < last && first <= whole)
-      step(whole, std::integral_constant<int, 1>{}, [&](const char* p, int64_t c) { return load_eight_to<XE>(p, c, s.k); });
+      step(whole, std::integral_constant<int, 1>{}, [&](const char* p, int64_t c) { return load_eight_to<XE>(p, c, q, s.k); });
 #pragma unroll
     for (int c = 0; c < RC; ++c)
       if (mine == adapter) acc[c] = sum[c];
@@ -335,7 +340,8 @@ struct Sixteen {
   static __device__ __forceinline__ Sixteen of_row(const char* row, int rank, int c, int q) {
     Sixteen s;
     if constexpr (kParts) {
-      const Eight<XE> e = load_eight_to<XE>(row, c * kRankChunk + 8 * (q & 1), rank);
+      const int at = c * kRankChunk;
+      const Eight<XE> e = at + 16 <= rank ? load_eight_whole<XE>(row, at, q & 1) : load_eight_to<XE>(row, at, q & 1, rank);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s.w[j] = e.w[j];
     } else {
@@ -362,7 +368,7 @@ struct Sixteen {
 // ---------------------------------------------------------------------------
 // expand: a workgroup takes TILES times 16 rows, whose `low` it adds up and lays out
 // in LDS once; its waves take 16 NT columns each.  Their instructions take the
-// rows of b in an order that leaves a lane 4 NT neighbouring columns of a row.
+// rows of b in an order that leaves a lane runs of 16 bytes, four lanes side by side.
 // All of base is on its way before anything waits, and the adapter met last
 // stays in registers.  With `slots` > 1 so many waves take every slots-th of the
 // adapters that 16 rows meet, and write only these rows.
@@ -456,18 +462,25 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
   const uint32_t group = blockIdx.x / s.blocks, unit = (blockIdx.x - group * s.blocks) * kAdapterWaves + wave;
   const uint32_t slot = unit % s.slots;
   const int64_t n0 = static_cast<int64_t>(unit / s.slots) * 16 * NT, row0 = static_cast<int64_t>(group) * kRows;
-  const int64_t col = n0 + q * 4 * NT;  // this lane's first
+  // This lane's columns are kRuns runs of kRun, each beside those of the row's other three lanes.
+  constexpr int kRun = NT == 1 ? 4 : 16 / kSize, kRuns = 4 * NT / kRun;
+  const int64_t col = n0 + q * kRun;
   const bool edge = n0 + 16 * NT > s.n;
-  const int live = col >= s.n ? 0 : (s.n - col < 4 * NT ? static_cast<int>(s.n - col) : 4 * NT);
+  auto live = [&](int run) { return col + 4 * run * kRun >= s.n ? 0 : (s.n - col - 4 * run * kRun < kRun ? static_cast<int>(s.n - col - 4 * run * kRun) : kRun); };
 
-  Run<XE, 4 * NT> base[TILES];
+  Run<XE, kRun> base[TILES][kRuns];
   if (s.base) {
 #pragma unroll
     for (int tile = 0; tile < TILES; ++tile) {
       const int64_t row = row0 + tile * 16 + i;
       const char* p = s.base + ((row < s.g.rows ? row : s.g.rows - 1) * s.ldbase + col) * kSize;
-      if (edge) base[tile].load(p, live);
-      else base[tile].load(p);
+      if (edge) {
+#pragma unroll
+        for (int run = 0; run < kRuns; ++run) base[tile][run].load(p + 4 * run * kRun * kSize, live(run));
+      } else {
+#pragma unroll
+        for (int run = 0; run < kRuns; ++run) base[tile][run].load(p + 4 * run * kRun * kSize);
+      }
     }
   }
   const int64_t width = s.g.chunks * kRankChunk, stride = s.g.rows * width;
@@ -506,7 +519,9 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
     held = adapter;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const int64_t n = n0 + (i >> 2) * 4 * NT + 4 * t + (i & 3);
+      // Four of the run's columns, as result rows 4 q .. 4 q + 3 of the instruction.
+      constexpr int kFours = kRun / 4;
+      const int64_t n = n0 + t / kFours * 4 * kRun + (i >> 2) * kRun + t % kFours * 4 + (i & 3);
       const char* row = s.g.a + (static_cast<int64_t>(adapter) * s.n + (n < s.n ? n : s.n - 1)) * s.g.rank * kSize;
 #pragma unroll
       for (int c = 0; c < RC; ++c)
@@ -537,18 +552,22 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
       }
     });
     if (!owned || row >= s.g.rows) continue;
-    Run<XE, 4 * NT> out = base[tile];
-    if (!s.base) {
-#pragma unroll
-      for (int j = 0; j < 4 * NT; j += 2) out.set(j, sum[j >> 2][j & 3], sum[j >> 2][(j & 3) + 1]);
-    } else if (mine >= 0) {
-#pragma unroll
-      for (int j = 0; j < 4 * NT; j += 2)
-        out.set(j, base[tile].value(j) + sum[j >> 2][j & 3], base[tile].value(j + 1) + sum[j >> 2][(j & 3) + 1]);
-    }
     char* p = s.out + (row * s.ldout + col) * kSize;
-    if (edge) out.store(p, live);
-    else out.store(p);
+#pragma unroll
+    for (int run = 0; run < kRuns; ++run) {
+      Run<XE, kRun> out = base[tile][run];
+      if (!s.base || mine >= 0) {
+#pragma unroll
+        for (int j = 0; j < kRun; j += 2) {
+          const int at = run * kRun + j;
+          const float lo = sum[at >> 2][at & 3], hi = sum[at >> 2][(at & 3) + 1];
+          if (s.base) out.set(j, base[tile][run].value(j) + lo, base[tile][run].value(j + 1) + hi);
+          else out.set(j, lo, hi);
+        }
+      }
+      if (edge) out.store(p + 4 * run * kRun * kSize, live(run));
+      else out.store(p + 4 * run * kRun * kSize);
+    }
   }
 }
 
@@ -582,63 +601,32 @@ struct ContractArgs {
 
 constexpr int kListRows = 1024;
 
-// Eight rows of CJ columns at `c` of each, and their transpose: CJ eights of one column each.
+// Eight rows of CJ columns, and their transpose: CJ eights of one column each.
 template <int XE, int CJ>
 struct Turned {
   static constexpr int kWords = CJ * enc_bytes(XE) / 4;
-  uint32_t row[8][kWords];
+  Run<XE, CJ> rows[8];
 
-  __device__ __forceinline__ void load(int e, const char* p, int live) {
-    if (live >= CJ) {
-#pragma unroll
-      for (int h = 0; h < kWords; h += 4) {
-        if constexpr (kWords >= 4) {
-          if constexpr (enc_bytes(XE) == 2) {
-            const halves8 v = *(const SR_GLOBAL halves8*)(p + 4 * h);
-            __builtin_memcpy(row[e] + h, &v, 16);
-          } else {
-            const floats4 v = *(const SR_GLOBAL floats4*)(p + 4 * h);
-            __builtin_memcpy(row[e] + h, &v, 16);
-          }
-        } else {
-          const halves4 v = *(const SR_GLOBAL halves4*)(p);
-          __builtin_memcpy(row[e], &v, 8);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int h = 0; h < kWords; ++h) row[e][h] = 0;
-#pragma unroll
-      for (int j = 0; j < CJ; ++j) {
-        if (j < live) {
-          if constexpr (enc_bytes(XE) == 2) row[e][j >> 1] |= static_cast<uint32_t>(gptr<uint16_t>(p)[j]) << (16 * (j & 1));
-          else row[e][j] = gptr<uint32_t>(p)[j];
-        }
-      }
-    }
-  }
+  __device__ __forceinline__ uint32_t word(int e, int h) const { return rows[e].w[h]; }
   __device__ __forceinline__ void clear(int e) {
 #pragma unroll
-    for (int h = 0; h < kWords; ++h) row[e][h] = 0;
+    for (int h = 0; h < kWords; ++h) rows[e].w[h] = 0;
   }
   // Column j of all eight rows as BF16 pairs.
   __device__ __forceinline__ void halves(int j, uint32_t (&w)[4]) const {
 #pragma unroll
     for (int p = 0; p < 4; ++p)
-      w[p] = j & 1 ? upper_halves(row[2 * p][j >> 1], row[2 * p + 1][j >> 1]) : lower_halves(row[2 * p][j >> 1], row[2 * p + 1][j >> 1]);
+      w[p] = j & 1 ? upper_halves(word(2 * p, j >> 1), word(2 * p + 1, j >> 1)) : lower_halves(word(2 * p, j >> 1), word(2 * p + 1, j >> 1));
   }
   // Column j of row e as FP32.
-  __device__ __forceinline__ float value(int j, int e) const {
-    if constexpr (XE == ENC_F32) return bits_f32(row[e][j]);
-    else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(row[e][j >> 1] >> (16 * (j & 1)))));
-  }
+  __device__ __forceinline__ float value(int j, int e) const { return rows[e].value(j); }
 };
 
 template <int XE, int RC, int CJ>
 __global__ __launch_bounds__(kAdapterThreads) void adapter_contract_kernel(ContractArgs s) {
   constexpr int kSize = enc_bytes(XE);
   constexpr bool kParts = XE == ENC_BF16_RN;
-  __shared__ uint32_t list[kListRows];
+  __shared__ __align__(16) uint32_t list[kListRows];  // rows past `at`; behind its end the first row, for loads that nothing uses
   __shared__ uint32_t counts[kAdapterWaves];
   __shared__ f32x4 sums[CJ * RC][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -653,6 +641,7 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_contract_kernel(Contr
   const ContractOperand& op = s.op[second];
   const int64_t c0 = static_cast<int64_t>(second ? id - s.op[0].tiles : id) * 16 * CJ + i * CJ;  // this lane's first column
   const int live = c0 >= op.cols ? 0 : (op.cols - c0 < CJ ? static_cast<int>(op.cols - c0) : CJ);
+  const bool edge = c0 - i * CJ + 16 * CJ > op.cols;
   const int64_t width = s.g.chunks * kRankChunk, stride = s.g.rows * width;
   const int64_t begin = part * s.part_rows, end = begin + s.part_rows < s.g.rows ? begin + s.part_rows : s.g.rows;
 
@@ -685,27 +674,53 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_contract_kernel(Contr
 #pragma unroll
     for (int j = 0; j < kOwn; ++j)
       if (own >> j & 1) list[place++] = threadIdx.x * kOwn + j;
+    for (uint32_t k = total + threadIdx.x; k < (total + 31) / 32 * 32; k += kAdapterThreads) list[k] = 0;
     __syncthreads();
     any |= total > 0;
-    for (uint32_t first = wave * 32; first < total; first += 32 * kAdapterWaves) {
+
+    struct Step {
       Turned<XE, CJ> x;
       float low[RC][8];
+    };
+    auto fetch = [&](uint32_t first, Step& step) {
+      uint32_t places[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t place_e = first + q * 8 + e;
-        const bool there = place_e < total;
-        const int64_t row = at + list[there ? place_e : 0];
-        x.load(e, op.x + (row * op.ldx + c0) * kSize, live);
-        if (!there) x.clear(e);
+      for (int h = 0; h < 2; ++h) {
+        const i32x4 v = read_chunk(reinterpret_cast<const char*>(list + first + q * 8 + 4 * h));
 #pragma unroll
-        for (int c = 0; c < RC; ++c) {
-          low[c][e] = 0;
+        for (int j = 0; j < 4; ++j) places[4 * h + j] = static_cast<uint32_t>(v[j]);
+      }
+      const char* from = op.x + (at * op.ldx + c0) * kSize;
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) step.x.rows[e].load(from + places[e] * op.ldx * kSize, live);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) step.x.rows[e].load(from + places[e] * op.ldx * kSize);
+      }
+      const float* low = op.low + at * width + i;
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+        if (c < s.g.chunks) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) step.low[c][e] = *gptr<float>(low + places[e] * width + c * kRankChunk);
+        }
+      for (int k = 1; k < op.splits; ++k)
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
           if (c < s.g.chunks) {
-            const float* p = op.low + row * width + c * kRankChunk + i;
-            float v = *gptr<float>(p);
-            for (int k = 1; k < op.splits; ++k) v += *gptr<float>(p + k * stride);
-            low[c][e] = there ? v : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) step.low[c][e] += *gptr<float>(low + k * stride + places[e] * width + c * kRankChunk);
           }
+    };
+    auto use = [&](uint32_t first, Step& step) {
+      if (first + 32 > total) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (first + q * 8 + e < total) continue;
+          step.x.clear(e);
+#pragma unroll
+          for (int c = 0; c < RC; ++c) step.low[c][e] = 0;
         }
       }
       if constexpr (kParts) {
@@ -714,13 +729,13 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_contract_kernel(Contr
         for (int c = 0; c < RC; ++c)
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
-            upper[c].w[p] = upper_halves(f32_bits(low[c][2 * p]), f32_bits(low[c][2 * p + 1]));
-            rest[c].w[p] = pack_bf16(bf16_rest(low[c][2 * p]), bf16_rest(low[c][2 * p + 1]));
+            upper[c].w[p] = upper_halves(f32_bits(step.low[c][2 * p]), f32_bits(step.low[c][2 * p + 1]));
+            rest[c].w[p] = pack_bf16(bf16_rest(step.low[c][2 * p]), bf16_rest(step.low[c][2 * p + 1]));
           }
 #pragma unroll
         for (int j = 0; j < CJ; ++j) {
           Eight<XE> column;
-          x.halves(j, column.w);
+          step.x.halves(j, column.w);
 #pragma unroll
           for (int c = 0; c < RC; ++c) {
             if (c < s.g.chunks) {
@@ -735,12 +750,31 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_contract_kernel(Contr
         for (int e = 0; e < 8; ++e)
 #pragma unroll
           for (int j = 0; j < CJ; ++j) {
-            const float v = x.value(j, e);
+            const float v = step.x.value(j, e);
 #pragma unroll
             for (int c = 0; c < RC; ++c)
-              if (c < s.g.chunks) acc[j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(low[c][e], v, acc[j][c], 0, 0, 0);
+              if (c < s.g.chunks) acc[j][c] = __builtin_amdgcn_mfma_f32_16x16x4f32(step.low[c][e], v, acc[j][c], 0, 0, 0);
           }
 #endif
+      }
+    };
+    // A step's loads run under the products of the one before, where the sums leave registers for both.
+    constexpr uint32_t kStride = 32 * kAdapterWaves;
+    uint32_t first = wave * 32;
+    if constexpr (RC <= 2) {
+      Step even, odd;
+      if (first < total) fetch(first, even);
+      for (; first < total; first += 2 * kStride) {
+        if (first + kStride < total) fetch(first + kStride, odd);
+        use(first, even);
+        if (first + 2 * kStride < total) fetch(first + 2 * kStride, even);
+        if (first + kStride < total) use(first + kStride, odd);
+      }
+    } else {
+      for (; first < total; first += kStride) {
+        Step step;
+        fetch(first, step);
+        use(first, step);
       }
     }
   }
