@@ -598,7 +598,7 @@ struct ScaleArea {
   static constexpr int kRow = 36, kFill = 32, kBytes = (S::BM + S::BN) * kRow;
   static constexpr int kPeriod = MODE == kExponents ? kFill : kFill / 4;
 
-  // Row r of the area for blocks [first, first + kPeriod), of which `total` - first are there (values past them mean
+  // Row r of the area for blocks [first, first + kPeriod), of which `total` - first are in memory (values past them mean
   // nothing): rows of A, then of B; rows past the operand's end repeat its last one.
   static __device__ __forceinline__ void row(const BlockProductArgs& g, int row0, int col0, int r, int first, int total,
                                              int (&words)[8]) {
@@ -622,12 +622,14 @@ struct ScaleArea {
     }
   }
 
-  // These blocks of every row.  Sets *far where a factor is not a near one.
-  static __device__ void fill(char* area, int* far, const BlockProductArgs& g, int row0, int col0, int first, int total) {
+  // These blocks of every row, `total` of them in the product and `there` in memory.  Sets *far where a factor of the
+  // product is not a near one.
+  static __device__ void fill(char* area, int* far, const BlockProductArgs& g, int row0, int col0, int first, int total,
+                              int there) {
     ScaleRange range;
     for (int r = threadIdx.x; r < S::BM + S::BN; r += S::kThreads) {
       int words[8];
-      row(g, row0, col0, r, first, total, words);
+      row(g, row0, col0, r, first, there, words);
       int* to = reinterpret_cast<int*>(area + r * kRow);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -770,7 +772,7 @@ __device__ __forceinline__ void sum_far_scales(const BlockProductArgs& g, char* 
 #pragma unroll
     for (int ni = 0; ni < S::NI; ++ni) acc[mi][ni] = f32x4{};
   for (int kt = 0; kt < stages; ++kt) {
-    if (kt % Area::kPeriod == 0) Area::fill(area, far, g, row0, col0, kt, stages);
+    if (kt % Area::kPeriod == 0) Area::fill(area, far, g, row0, col0, kt, stages, stages);
     if (group == 0) stager.load_through(lds, static_cast<int64_t>(kt) * kStageBytes, g.k, wave, lane);
     lds_barrier();
     if (group == 0) {
@@ -809,9 +811,10 @@ constexpr int product_lds() {
   return kLds;
 }
 
-// The results from (row0, col0) on.
+// The results from (row0, col0) on.  `scales`: how many of every row are in memory, where that is more than the product
+// has blocks (an access of 16 bytes beats one of each byte).
 template <int MODE, int FA, int FB, class S, bool ASYNC>
-__device__ __forceinline__ void product_tile(const BlockProductArgs& g, char* lds, int row0, int col0) {
+__device__ __forceinline__ void product_tile(const BlockProductArgs& g, char* lds, int row0, int col0, int scales = 0) {
   static_assert(ASYNC || S::kGroups == 1, "groups take aligned rows");
   using Area = ScaleArea<MODE, S>;
   constexpr int kLds = product_lds<MODE, S>();
@@ -851,7 +854,7 @@ __device__ __forceinline__ void product_tile(const BlockProductArgs& g, char* ld
 
   auto refill = [&](int kt) {
     if ((kt & (Area::kPeriod - 1)) == 0) {
-      Area::fill(area, far, g, row0, col0, kt, stages);
+      Area::fill(area, far, g, row0, col0, kt, stages, scales > stages ? scales : stages);
       lds_barrier();
     }
   };

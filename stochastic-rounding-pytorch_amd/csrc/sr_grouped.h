@@ -213,11 +213,12 @@ __global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void grouped_contrac
   p.b.base += start;
   p.scale_a += start / SR_BLOCK * size;
   p.scale_b += start / SR_BLOCK * size;
+  const int scales = static_cast<int>((p.k - start) / SR_BLOCK);  // up to the matrix's end
   p.k = columns;
   p.out += output_bytes(p, group * g.stride_out);
   uint32_t tile_m, tile_n;
   band_tile(id - group * each, p.tiles_m, p.tiles_n, tile_m, tile_n);
-  product_tile<MODE, FA, FB, S, ASYNC>(p, lds, tile_m * S::BM, tile_n * S::BN);
+  product_tile<MODE, FA, FB, S, ASYNC>(p, lds, tile_m * S::BM, tile_n * S::BN, scales);
 }
 
 // ---------------------------------------------------------------------------
