@@ -42,6 +42,7 @@ struct GroupedProductKernels {
   const void* rows;                  // tiles of 16 rows
   const void* tile[kBlockTiles][2];  // as above
   const void* contract[kBlockTiles];
+  const void* lean[2];               // rows and contract: kExponents only
 };
 using GroupedProductTable = GroupedProductKernels[2][2][3];
 enum GroupedCastKind { kGroupedParts, kGroupedWhole, kStackedParts, kStackedWhole, kStackedSquare, kGroupedCastKinds };

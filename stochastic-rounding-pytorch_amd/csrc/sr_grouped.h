@@ -109,19 +109,22 @@ struct GroupTable {
   }
 };
 
-// Rows [start, start + rows) of group `group` where every group's rows are padded to whole blocks.
-__device__ __forceinline__ void padded_group(const Groups& g, int group, uint32_t limit, uint32_t& start, uint32_t& rows) {
-  GroupChunk<SR_BLOCK, true> c;
-  uint32_t before = 0;
-  int at = 0;
-  for (;; at += 64) {
-    c.load(g, at, before, 0, limit);
-    if (group < at + 64) break;
-    before = c.rows_end;
+// The groups where every group's rows are padded to whole blocks.
+struct PaddedGroups {
+  GroupChunk<SR_BLOCK, true> chunk;  // the first 64
+
+  __device__ __forceinline__ void load(const Groups& g, uint32_t limit) { chunk.load(g, 0, 0, 0, limit); }
+  __device__ __forceinline__ void find(const Groups& g, int group, uint32_t limit, uint32_t& start, uint32_t& rows) const {
+    GroupChunk<SR_BLOCK, true> c = chunk;
+    int at = 0;
+    while (group >= at + 64) {
+      at += 64;
+      c.load(g, at, c.rows_end, 0, limit);
+    }
+    start = lane_value(c.start, group - at);
+    rows = lane_value(c.rows, group - at);
   }
-  start = lane_value(c.start, group - at);
-  rows = lane_value(c.rows, group - at);
-}
+};
 
 // ---------------------------------------------------------------------------
 // Products.
@@ -207,7 +210,9 @@ __global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void grouped_contrac
   const uint32_t each = p.tiles_m * p.tiles_n, id = xcd_run(blockIdx.x, each * static_cast<uint32_t>(g.groups.count));
   const uint32_t group = id / each;
   uint32_t start, columns;
-  padded_group(g.groups, static_cast<int>(group), static_cast<uint32_t>(p.k), start, columns);
+  PaddedGroups table;
+  table.load(g.groups, static_cast<uint32_t>(p.k));
+  table.find(g.groups, static_cast<int>(group), static_cast<uint32_t>(p.k), start, columns);
   const int64_t size = p.scale_f32 ? 4 : 1;
   p.a.base += start;
   p.b.base += start;
@@ -219,6 +224,149 @@ __global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void grouped_contrac
   uint32_t tile_m, tile_n;
   band_tile(id - group * each, p.tiles_m, p.tiles_n, tile_m, tile_n);
   product_tile<MODE, FA, FB, S, ASYNC>(p, lds, tile_m * S::BM, tile_n * S::BN, scales);
+}
+
+// ---------------------------------------------------------------------------
+// The same products in 128 x 128 tiles with E8M0 scales, over whole blocks of the
+// contracted axis.
+//
+// One stage in LDS, so that three workgroups share a CU: each waits for its loads,
+// and what it spends outside its products (its group, its stages' way from
+// memory, its results' way out) runs under the others'.  With two stages in LDS
+// and two workgroups, a contraction of 16 groups of 512 rows to 2048 x 2048 took 85 us
+// and takes 69 so, of 2048 rows 161 and 150; where a CU has one tile at a time it
+// loses (one group of 8192 rows: 49 and 67).
+// ---------------------------------------------------------------------------
+// The chip holds 512 tiles of two workgroups a CU: where there are more of them, this one takes less time (rows of 16
+// groups, 2048 x 2048: 624 tiles 28.5 us and 33.8, 1152 55.9 and 59.7, 4672 of 8192 x 2048 202 and 212; contractions of 640
+// tiles 34 and 41), up to there more (416 tiles 23.6 and 21.0, contractions of 512 20.1 and 18.0).
+constexpr int64_t kLeanTiles = 512;
+constexpr int kLeanStages = 16;    // whose scales are in LDS at a time
+constexpr int kLeanScaleRow = 20;  // bytes of a row of them: 32 rows' same bytes lie in different banks
+
+template <int FA, int FB, bool CONTRACT>
+__global__ __launch_bounds__(256, 3) void grouped_lean_kernel(GroupedProductArgs g) {
+  using S = TileShape<128, 128, 2, 2>;
+  __shared__ __align__(1024) char lds[S::kStage + (S::BM + S::BN) * kLeanScaleRow];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave_m = wave / S::WN * S::kRowsM, wave_n = wave % S::WN * S::kRowsN;
+
+  // This workgroup's group and tile, and the scales that a row has in memory.
+  BlockProductArgs p = g.p;
+  uint32_t tile_m, tile_n;
+  int scales;
+  if constexpr (CONTRACT) {
+    const uint32_t each = p.tiles_m * p.tiles_n, id = xcd_run(blockIdx.x, each * static_cast<uint32_t>(g.groups.count));
+    const uint32_t group = id / each, limit = static_cast<uint32_t>(p.k);
+    uint32_t start, columns;
+    PaddedGroups table;
+    table.load(g.groups, limit);
+    table.find(g.groups, static_cast<int>(group), limit, start, columns);
+    p.a.base += start;
+    p.b.base += start;
+    p.scale_a += start / SR_BLOCK;
+    p.scale_b += start / SR_BLOCK;
+    p.k = columns;
+    p.out += output_bytes(p, group * g.stride_out);
+    scales = static_cast<int>((limit - start) / SR_BLOCK);
+    band_tile(id - group * each, p.tiles_m, p.tiles_n, tile_m, tile_n);
+  } else {
+    GroupTable<S::BM> table;
+    const uint32_t limit = static_cast<uint32_t>(p.m);
+    table.load(g.groups, limit);
+    const uint32_t total = (table.tiles + (g.zero_behind ? (limit - table.rows + S::BM - 1) / S::BM : 0)) * p.tiles_n;
+    if (blockIdx.x >= total) return;
+    const uint32_t id = xcd_run(blockIdx.x, total);
+    const GroupTile in = table.find(g.groups, id / p.tiles_n, limit);
+    p = rows_product<S::BM>(g, in);
+    scales = static_cast<int>(p.k / SR_BLOCK);
+    band_tile(id - in.first * p.tiles_n, p.tiles_m, p.tiles_n, tile_m, tile_n);
+  }
+  const int row0 = tile_m * S::BM, col0 = tile_n * S::BN, stages = static_cast<int>(p.k / SR_BLOCK);
+  // Sixteen-row fragments of this wave that the group has.
+  const int left = p.m - row0 - wave_m, live = left <= 0 ? 0 : (left >= S::kRowsM ? S::MI : (left + 15) / 16);
+
+  Stager<S> stager;
+  stager.init(p.a, p.b, row0, col0, wave, lane);
+  // The scales of stages [first, first + kLeanStages), a row for each thread.
+  char* marks = lds + S::kStage;
+  auto fill = [&](int first) {
+    const int r = threadIdx.x;
+    const bool of_a = r < S::BM;
+    const int row = of_a ? row0 + r : col0 + r - S::BM, rows = of_a ? p.m : p.n;
+    const char* from = (of_a ? p.scale_a : p.scale_b) +
+                       ((row < rows ? row : rows - 1) >> (of_a ? p.shift_a : p.shift_b)) * (of_a ? p.ld_scale_a : p.ld_scale_b) + first;
+    const int there = scales - first;
+    char* to = marks + r * kLeanScaleRow;
+    if (there >= kLeanStages) {
+      const i32x4 v = load_whole_chunk(from, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) reinterpret_cast<int*>(to)[j] = v[j];
+    } else {
+#pragma unroll 1
+      for (int j = 0; j < there; ++j) to[j] = static_cast<char>(gptr<uint8_t>(from)[j]);
+    }
+  };
+
+  f32x4 acc[S::MI][S::NI] = {};
+  const uint32_t fragment = fragment_offset(lane);
+  if (stages) {
+    stager.load_async(lds, 0, wave);
+    fill(0);
+  }
+  for (int kt = 0; kt < stages; ++kt) {
+    stage_barrier();
+    if (live > 0) {
+      Fragment<kExponents, FB> b[S::NI];
+      Scales<kExponents, S::MI, S::NI> marked;
+      const char* at = marks + kt % kLeanStages;
+#pragma unroll
+      for (int i = 0; i < S::MI; ++i)
+        marked.a[i] = *reinterpret_cast<const uint8_t*>(at + (wave_m + 16 * i + (lane & 15)) * kLeanScaleRow);
+#pragma unroll
+      for (int i = 0; i < S::NI; ++i)
+        marked.b[i][0] = *reinterpret_cast<const uint8_t*>(at + (S::BM + wave_n + 16 * i + (lane & 15)) * kLeanScaleRow);
+      const char* sa = lds + wave_m * kStageBytes;
+      const char* sb = lds + (S::BM + wave_n) * kStageBytes;
+#pragma unroll
+      for (int i = 0; i < S::NI; ++i)
+        b[i].set(read_chunk(sb + fragment + i * 16 * kStageBytes), read_chunk(sb + (fragment ^ 64) + i * 16 * kStageBytes));
+      auto row = [&](int mi) {
+        Fragment<kExponents, FA> a;
+        a.set(read_chunk(sa + fragment + mi * 16 * kStageBytes), read_chunk(sa + (fragment ^ 64) + mi * 16 * kStageBytes));
+#pragma unroll
+        for (int ni = 0; ni < S::NI; ++ni) block_mma<false>(acc[mi][ni], a, b[ni], marked, mi, ni);
+      };
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) row(mi);
+    }
+    lds_barrier();  // every wave is done with the stage
+    if (kt + 1 < stages) {
+      stager.load_async(lds, (kt + 1) * kStageBytes, wave);
+      if ((kt + 1) % kLeanStages == 0) fill(kt + 1);
+    }
+  }
+
+  // The results pass the stage's LDS, 32 rows of a wave at a time: four values of a row at place (place ^ row) of its
+  // sixteen, so that neither side's accesses meet in the same banks.
+  char* turned = lds + wave * (S::kStage / 4);
+  auto place = [&](int row, int four) { return reinterpret_cast<f32x4*>(turned + row * 256 + ((four ^ row) & 15) * 16); };
+  with_output(p, row0, col0, S::BM, S::BN, [&](auto out, auto edge) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (half * 2 >= live) break;
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+        for (int ni = 0; ni < S::NI; ++ni) *place(16 * mi + (lane & 15), 4 * ni + (lane >> 4)) = acc[2 * half + mi][ni];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int row = 4 * k + (lane >> 4);
+        store_results<decltype(out)::value, decltype(edge)::value>(p, row0 + wave_m + 32 * half + row, col0 + wave_n + 4 * (lane & 15),
+                                                                   *place(row, lane & 15));
+      }
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------

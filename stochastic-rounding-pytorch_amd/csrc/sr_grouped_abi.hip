@@ -220,6 +220,10 @@ int sr_grouped_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, 
   const bool async = aligned_rows(a) && aligned_rows(b) && b_stride % 16 == 0;
   auto tiles = [&](int64_t side) { return (rows / side + (full + 1) / 2) * ((g.p.n + side - 1) / side); };
   const sr::BlockTile tile = sr::tile_by_count(tiles);
+  if (fn.lean[0] && async && k % SR_BLOCK == 0 && tiles(128) > sr::kLeanTiles) {
+    g.p.tiles_n = (g.p.n + 127) / 128;
+    return launch(fn.lean[0], room(128) * g.p.tiles_n, 256, &g, stream);
+  }
   return with_tile(async || tile == sr::kTile128 ? tile : sr::kTile64, [&](sr::BlockTile index, auto shape) {
     using S = decltype(shape);
     g.p.tiles_n = (g.p.n + S::BN - 1) / S::BN;
@@ -242,6 +246,11 @@ int sr_grouped_block_contract(const sr_block_matrix* a, const sr_block_matrix* b
   g.stride_out = out_stride;
   const sr::GroupedProductKernels& fn = kernels(a, b, out_dtype);
   auto tiles = [&](int64_t side) { return groups->count * ((g.p.m + side - 1) / side) * ((g.p.n + side - 1) / side); };
+  if (fn.lean[1] && tiles(128) > sr::kLeanTiles) {
+    g.p.tiles_m = (g.p.m + 127) / 128;
+    g.p.tiles_n = (g.p.n + 127) / 128;
+    return launch(fn.lean[1], static_cast<uint64_t>(g.p.tiles_m) * g.p.tiles_n * groups->count, 256, &g, stream);
+  }
   return with_tile(sr::tile_by_count(tiles), [&](sr::BlockTile index, auto shape) {
     using S = decltype(shape);
     g.p.tiles_m = (g.p.m + S::BM - 1) / S::BM;

@@ -30,6 +30,8 @@ void fill(GroupedProductKernels& k) {
 template <int FB>
 void fill_modes(GroupedProductKernels (&k)[kProductModes]) {
   fill<FB, kExponents>(k[kExponents]);
+  k[kExponents].lean[0] = reinterpret_cast<const void*>(&grouped_lean_kernel<FA, FB, false>);
+  k[kExponents].lean[1] = reinterpret_cast<const void*>(&grouped_lean_kernel<FA, FB, true>);
   fill<FB, kFactors>(k[kFactors]);
   fill<FB, kWide>(k[kWide]);
 }

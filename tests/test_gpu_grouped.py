@@ -44,6 +44,12 @@ def _assert_near(got, want, magnitude, k):
     if got.dtype == torch.float16:
         limit = limit + 2.0**-25
     assert got.shape == want.shape and not got.isnan().any()
+    # Results of 65520 = 2^16 - 2^4 or more round to FP16's infinities: half a step of 2^5 above its largest number.
+    top = 65520.0 if got.dtype == torch.float16 else float("inf")
+    high = want.abs() >= top
+    assert not (got.isinf() & (want.abs() + limit < top)).any()
+    got = torch.where(got.isinf() & (want.abs() + limit >= top) & (got.sign() == want.sign()), want, got.double())
+    assert not (high & (want.abs() - limit >= top) & (got != want)).any()
     if got.numel():
         assert float(((got.double() - want).abs() - limit).max()) <= 0
 
@@ -204,6 +210,32 @@ def test_contraction_equals_the_definition(cuda, tokens, counts, m, n, scale, ou
     sr_states.grouped_block_matmul(a, b, _sizes(counts, cuda), out=kept[:, :m, :n])
     assert torch.equal(kept[:, :m, :n], got)
     assert (kept[:, m:] == 7).all() and (kept[:, :, n:] == 7).all()
+
+
+@pytest.mark.parametrize("a_dtype, b_dtype", [(E4M3, E4M3), (E5M2, E4M3), (E4M3, E5M2)])
+@pytest.mark.parametrize("k", [128, 640, 2048 + 384])
+@pytest.mark.parametrize("counts", [[1500, 0, 129, 1, 900, 60], [0, 3000], [1] * 80 + [2500], [0, 0]])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float16])
+def test_products_of_more_tiles_than_the_chip_holds(cuda, a_dtype, b_dtype, k, counts, out):
+    rows, n = 3100, 3001
+    counts = counts if k == 128 else counts[-6:]
+    a = _operand((rows, k), a_dtype, "e8m0", False, cuda, 1)
+    b = _operand((len(counts), n, k), b_dtype, "e8m0", True, cuda, 2)
+    got = sr_states.grouped_block_matmul(a, b, _sizes(counts, cuda), out_dtype=out)
+    _assert_near(got, *grouped.product(a, b, counts), k)
+    kept = torch.full((rows, n), 7.0, device=cuda, dtype=out)
+    sr_states.grouped_block_matmul(a, b, _sizes(counts, cuda), out=kept)
+    assert torch.equal(kept[:sum(counts)], got[:sum(counts)]) and (kept[sum(counts):] == 7).all()
+
+
+@pytest.mark.parametrize("tokens, counts", [(3000, [300, 0, 129, 1, 2300, 60]), (100, [1] * 90)])
+@pytest.mark.parametrize("a_dtype, b_dtype", [(E4M3, E4M3), (E4M3, E5M2), (E5M2, E5M2)])
+def test_contractions_of_more_tiles_than_the_chip_holds(cuda, tokens, counts, a_dtype, b_dtype):
+    m, n = (1300, 1281) if len(counts) < 10 else (130, 500)
+    width = grouped.columns(tokens, len(counts))
+    a, b = _padded(m, counts, width, a_dtype, "e8m0", cuda, 1), _padded(n, counts, width, b_dtype, "e8m0", cuda, 2)
+    got = sr_states.grouped_block_matmul(a, b, _sizes(counts, cuda))
+    _assert_near(got, *grouped.contract(a, b, counts), max(counts))
 
 
 def test_sizes_that_lead_beyond_the_columns_end_there(cuda):
