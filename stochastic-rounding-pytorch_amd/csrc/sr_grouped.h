@@ -111,11 +111,24 @@ struct GroupTable {
 
 // The groups where every group's rows are padded to whole blocks.
 struct PaddedGroups {
-  GroupChunk<SR_BLOCK, true> chunk;  // the first 64
+  int group;
+  uint32_t start, rows;
 
-  __device__ __forceinline__ void load(const Groups& g, uint32_t limit) { chunk.load(g, 0, 0, 0, limit); }
-  __device__ __forceinline__ void find(const Groups& g, int group, uint32_t limit, uint32_t& start, uint32_t& rows) const {
-    GroupChunk<SR_BLOCK, true> c = chunk;
+  // Group number `number`, the largest ones first where a wave holds them all.
+  __device__ __forceinline__ void find(const Groups& g, int number, uint32_t limit) {
+    GroupChunk<SR_BLOCK, true> c;
+    c.load(g, 0, 0, 0, limit);
+    if (g.count <= 64) {
+      const int lane = threadIdx.x & 63;
+      int larger = 0;
+      for (int j = 0; j < g.count; ++j) {
+        const uint32_t other = lane_value(c.rows, j);
+        larger += other > c.rows || (other == c.rows && j < lane);
+      }
+      group = __builtin_ctzll(__ballot(lane < g.count && larger == number));
+    } else {
+      group = number;
+    }
     int at = 0;
     while (group >= at + 64) {
       at += 64;
@@ -131,7 +144,10 @@ struct PaddedGroups {
 //
 //   rows      out[t] = a[t] b[g]^T for the rows t of group g, b a stack of matrices
 //   contract  out[g] = a[:, g] b[:, g]^T over the columns of group g, which start
-//             on multiples of 128 and end in zeros
+//             on multiples of 128 and end in zeros.  Every XCD takes an eighth of each
+//             result, large groups first: their tiles cost as much as they have
+//             rows, and with whole groups to an XCD the unluckiest one set the time
+//             (16 groups of 60 to 2000 rows to 2048 x 2048: 99 us and 72)
 //
 // Both find their group and go on as a plain product does, on the part of the
 // operands that the group has: what a plain product measured holds for them
@@ -203,26 +219,38 @@ __global__ __launch_bounds__(64 * kRowWaves) void grouped_product_rows_kernel(Gr
   product_rows<MODE, FA, FB>(rows_product<16>(g, at), sums, static_cast<int>(tile_n) * 16);
 }
 
+// Workgroups of one result, an eighth of them on each XCD.
+inline __host__ __device__ uint32_t contract_groups(uint32_t tiles) { return (tiles + 7) / 8 * 8; }
+
+// The product of this workgroup's result and its tile in it; false where there is none.  `scales`: of a row, up to the
+// matrix's end.
+__device__ __forceinline__ bool contract_product(const GroupedProductArgs& g, BlockProductArgs& p, uint32_t& tile_m, uint32_t& tile_n,
+                                                 int& scales) {
+  p = g.p;
+  const uint32_t tiles = p.tiles_m * p.tiles_n, each = contract_groups(tiles), number = blockIdx.x / each;
+  const uint32_t id = xcd_run(blockIdx.x - number * each, each);
+  if (id >= tiles) return false;
+  PaddedGroups in;
+  in.find(g.groups, static_cast<int>(number), static_cast<uint32_t>(p.k));
+  const int64_t size = p.scale_f32 ? 4 : 1;
+  scales = static_cast<int>((p.k - in.start) / SR_BLOCK);
+  p.a.base += in.start;
+  p.b.base += in.start;
+  p.scale_a += in.start / SR_BLOCK * size;
+  p.scale_b += in.start / SR_BLOCK * size;
+  p.k = in.rows;
+  p.out += output_bytes(p, in.group * g.stride_out);
+  band_tile(id, p.tiles_m, p.tiles_n, tile_m, tile_n);
+  return true;
+}
+
 template <int MODE, int FA, int FB, class S, bool ASYNC>
 __global__ __launch_bounds__(S::kThreads, kProductWaves<S>) void grouped_contract_kernel(GroupedProductArgs g) {
   __shared__ __align__(1024) char lds[product_lds<MODE, S>() + 16];
-  BlockProductArgs p = g.p;
-  const uint32_t each = p.tiles_m * p.tiles_n, id = xcd_run(blockIdx.x, each * static_cast<uint32_t>(g.groups.count));
-  const uint32_t group = id / each;
-  uint32_t start, columns;
-  PaddedGroups table;
-  table.load(g.groups, static_cast<uint32_t>(p.k));
-  table.find(g.groups, static_cast<int>(group), static_cast<uint32_t>(p.k), start, columns);
-  const int64_t size = p.scale_f32 ? 4 : 1;
-  p.a.base += start;
-  p.b.base += start;
-  p.scale_a += start / SR_BLOCK * size;
-  p.scale_b += start / SR_BLOCK * size;
-  const int scales = static_cast<int>((p.k - start) / SR_BLOCK);  // up to the matrix's end
-  p.k = columns;
-  p.out += output_bytes(p, group * g.stride_out);
+  BlockProductArgs p;
   uint32_t tile_m, tile_n;
-  band_tile(id - group * each, p.tiles_m, p.tiles_n, tile_m, tile_n);
+  int scales;
+  if (!contract_product(g, p, tile_m, tile_n, scales)) return;
   product_tile<MODE, FA, FB, S, ASYNC>(p, lds, tile_m * S::BM, tile_n * S::BN, scales);
 }
 
@@ -256,20 +284,7 @@ __global__ __launch_bounds__(256, 3) void grouped_lean_kernel(GroupedProductArgs
   uint32_t tile_m, tile_n;
   int scales;
   if constexpr (CONTRACT) {
-    const uint32_t each = p.tiles_m * p.tiles_n, id = xcd_run(blockIdx.x, each * static_cast<uint32_t>(g.groups.count));
-    const uint32_t group = id / each, limit = static_cast<uint32_t>(p.k);
-    uint32_t start, columns;
-    PaddedGroups table;
-    table.load(g.groups, limit);
-    table.find(g.groups, static_cast<int>(group), limit, start, columns);
-    p.a.base += start;
-    p.b.base += start;
-    p.scale_a += start / SR_BLOCK;
-    p.scale_b += start / SR_BLOCK;
-    p.k = columns;
-    p.out += output_bytes(p, group * g.stride_out);
-    scales = static_cast<int>((limit - start) / SR_BLOCK);
-    band_tile(id - group * each, p.tiles_m, p.tiles_n, tile_m, tile_n);
+    if (!contract_product(g, p, tile_m, tile_n, scales)) return;
   } else {
     GroupTable<S::BM> table;
     const uint32_t limit = static_cast<uint32_t>(p.m);
@@ -359,11 +374,31 @@ __global__ __launch_bounds__(256, 3) void grouped_lean_kernel(GroupedProductArgs
       for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
         for (int ni = 0; ni < S::NI; ++ni) *place(16 * mi + (lane & 15), 4 * ni + (lane >> 4)) = acc[2 * half + mi][ni];
+      constexpr int kOut = decltype(out)::value;
+      if constexpr (kOut != SR_F32 && !decltype(edge)::value) {
+        // Eight values a lane, eight lanes a row.  The result is not read again here: its stores pass the caches by.
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int row = 8 * k + (lane >> 3);
+          uint32_t w[4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const f32x4 v = *place(row, 2 * (lane & 7) + h);
+            const float x[4] = {v[0], v[1], v[2], v[3]};
+            uint32_t pair[2];
+            encode_group<kOut == SR_BF16 ? ENC_BF16_RN : ENC_F16_RN>(x, 0u, pair);
+            w[2 * h] = pair[0];
+            w[2 * h + 1] = pair[1];
+          }
+          uint16_t* to = reinterpret_cast<uint16_t*>(p.out) + (row0 + wave_m + 32 * half + row) * p.ldo + col0 + wave_n + 8 * (lane & 7);
+          __builtin_nontemporal_store(eight_halves{w[0], w[1], w[2], w[3]}, (SR_GLOBAL eight_halves*)(to));
+        }
+        continue;
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int row = 4 * k + (lane >> 4);
-        store_results<decltype(out)::value, decltype(edge)::value>(p, row0 + wave_m + 32 * half + row, col0 + wave_n + 4 * (lane & 15),
-                                                                   *place(row, lane & 15));
+        store_results<kOut, decltype(edge)::value>(p, row0 + wave_m + 32 * half + row, col0 + wave_n + 4 * (lane & 15), *place(row, lane & 15));
       }
     }
   });

@@ -249,13 +249,13 @@ int sr_grouped_block_contract(const sr_block_matrix* a, const sr_block_matrix* b
   if (fn.lean[1] && tiles(128) > sr::kLeanTiles) {
     g.p.tiles_m = (g.p.m + 127) / 128;
     g.p.tiles_n = (g.p.n + 127) / 128;
-    return launch(fn.lean[1], static_cast<uint64_t>(g.p.tiles_m) * g.p.tiles_n * groups->count, 256, &g, stream);
+    return launch(fn.lean[1], static_cast<uint64_t>(sr::contract_groups(g.p.tiles_m * g.p.tiles_n)) * groups->count, 256, &g, stream);
   }
   return with_tile(sr::tile_by_count(tiles), [&](sr::BlockTile index, auto shape) {
     using S = decltype(shape);
     g.p.tiles_m = (g.p.m + S::BM - 1) / S::BM;
     g.p.tiles_n = (g.p.n + S::BN - 1) / S::BN;
-    return launch(fn.contract[index], static_cast<uint64_t>(g.p.tiles_m) * g.p.tiles_n * groups->count, S::kThreads, &g, stream);
+    return launch(fn.contract[index], static_cast<uint64_t>(sr::contract_groups(g.p.tiles_m * g.p.tiles_n)) * groups->count, S::kThreads, &g, stream);
   });
 }
 
