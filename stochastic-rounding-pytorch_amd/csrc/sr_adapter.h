@@ -226,7 +226,7 @@ struct ShrinkArgs {
   const char* x;
   int64_t ldx, k;
   float* low;  // splits x rows x 16 chunks
-  int row_tiles, splits, slots;
+  int row_tiles, splits, slot_bits;  // 2^slot_bits slots
 };
 
 constexpr int kShrinkWaves = 8;
@@ -239,29 +239,30 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Shrin
   __shared__ f32x4 sums[kShrinkWaves][RC][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
-  const int tile = blockIdx.x % s.row_tiles, unit = blockIdx.x / s.row_tiles, slot = unit % s.slots, split = unit / s.slots;
+  const int tile = blockIdx.x % s.row_tiles, unit = blockIdx.x / s.row_tiles;
+  const int slots = 1 << s.slot_bits, slot = unit & (slots - 1), split = unit >> s.slot_bits;
   const int64_t row = static_cast<int64_t>(tile) * 16 + i;
   const int mine = adapter_of(s.g, row);
   const char* x = s.x + (row < s.g.rows ? row : s.g.rows - 1) * s.ldx * enc_bytes(XE);
   int met = 0;          // by this workgroup
   bool owned = mine < 0 && slot == 0;  // this lane's row is written here
   for_each_adapter(mine, [&](int adapter, int number) {
-    if (number % s.slots != slot) return;
+    if ((number & (slots - 1)) != slot) return;
     ++met;
     owned |= mine == adapter;
   });
   if (met == 0 && slot > 0) return;
-  const int shares = met >= 8 ? 1 : (met >= 4 ? 2 : (met >= 2 ? 4 : 8));  // waves of one adapter
+  const int share_bits = met >= 8 ? 0 : (met >= 4 ? 1 : (met >= 2 ? 2 : 3)), shares = 1 << share_bits;  // waves of one adapter
 
   const int64_t steps = (s.k + kStep - 1) / kStep, part = (steps + s.splits - 1) / s.splits;
   const int64_t begin = split * part, end = begin + part < steps ? begin + part : steps;
-  const int64_t each = (part + shares - 1) / shares, first = begin + wave % shares * each;
+  const int64_t each = (part + shares - 1) >> share_bits, first = begin + (wave & (shares - 1)) * each;
   const int64_t last = first + each < end ? first + each : end;
   const int64_t whole = s.k / kStep < last ? s.k / kStep : last;
 
   f32x4 acc[RC] = {};
   for_each_adapter(mine, [&](int adapter, int number) {
-    if (number % s.slots != slot || number / s.slots % (kShrinkWaves / shares) != wave / shares) return;
+    if ((number & (slots - 1)) != slot || ((number >> s.slot_bits) & ((kShrinkWaves >> share_bits) - 1)) != wave >> share_bits) return;
     const char* rows[RC];
 #pragma unroll
     for (int c = 0; c < RC; ++c) {
@@ -370,7 +371,7 @@ struct Sixteen {
 // in LDS once; its waves take 16 NT columns each.  Their instructions take the
 // rows of b in an order that leaves a lane runs of 16 bytes, four lanes side by side.
 // All of base is on its way before anything waits, and the adapter met last
-// stays in registers.  With `slots` > 1 so many waves take every slots-th of the
+// stays in registers.  With slots so many waves take every slots-th of the
 // adapters that 16 rows meet, and write only these rows.
 // ---------------------------------------------------------------------------
 struct ExpandArgs {
@@ -379,7 +380,7 @@ struct ExpandArgs {
   const char* base;  // or null: zeros
   char* out;
   int64_t ldbase, ldout, n;
-  int splits, slots;
+  int splits, slot_bits;
   int column_tiles;  // of 16 NT
   int blocks;        // of kAdapterWaves column tiles and slots
 };
@@ -460,8 +461,8 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
   const uint32_t group = blockIdx.x / s.blocks, unit = (blockIdx.x - group * s.blocks) * kAdapterWaves + wave;
-  const uint32_t slot = unit % s.slots;
-  const int64_t n0 = static_cast<int64_t>(unit / s.slots) * 16 * NT, row0 = static_cast<int64_t>(group) * kRows;
+  const uint32_t slots = 1u << s.slot_bits, slot = unit & (slots - 1);
+  const int64_t n0 = static_cast<int64_t>(unit >> s.slot_bits) * 16 * NT, row0 = static_cast<int64_t>(group) * kRows;
   // This lane's columns are kRuns runs of kRun, each beside those of the row's other three lanes.
   constexpr int kRun = NT == 1 ? 4 : 16 / kSize, kRuns = 4 * NT / kRun;
   const int64_t col = n0 + q * kRun;
@@ -535,7 +536,7 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
     f32x4 sum[NT] = {};
     bool owned = mine < 0 && slot == 0;
     for_each_adapter(mine, [&](int adapter, int number) {
-      if (number % s.slots != slot) return;
+      if ((number & (slots - 1)) != slot) return;
       hold(adapter);
       owned |= mine == adapter;
       Sixteen<XE> low[RC];

@@ -73,8 +73,11 @@ sr::Adapters adapters_of(const sr_adapters* g, const void* matrices, int64_t row
   return a;
 }
 
-// Workgroups, or waves, that share the adapters of 16 rows: more of them where there are few otherwise.
-int slots_of(int64_t others, int count) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({4, 256 / std::max<int64_t>(others, 1), count}))); }
+// Workgroups, or waves, that share the adapters of 16 rows, as a power of two: more of them where there are few otherwise.
+int slot_bits_of(int64_t others, int count) {
+  const int64_t wanted = std::min<int64_t>(256 / std::max<int64_t>(others, 1), count);
+  return wanted >= 4 ? 2 : (wanted >= 2 ? 1 : 0);
+}
 
 // low = the scaled products of x with `matrices` (count x rank x k).
 int shrink(const sr_adapters* g, const void* matrices, const void* x, int64_t ldx, int64_t k, int64_t rows, float* low, void* stream) {
@@ -86,8 +89,8 @@ int shrink(const sr_adapters* g, const void* matrices, const void* x, int64_t ld
   s.low = low;
   s.row_tiles = static_cast<int>((rows + 15) / 16);
   s.splits = splits_of(rows, k, g->dtype);
-  s.slots = slots_of(static_cast<int64_t>(s.row_tiles) * s.splits, g->count);
-  return launch(kernels(g->dtype).shrink[rank_index(s.g.chunks)], static_cast<uint64_t>(s.row_tiles) * s.splits * s.slots,
+  s.slot_bits = slot_bits_of(static_cast<int64_t>(s.row_tiles) * s.splits, g->count);
+  return launch(kernels(g->dtype).shrink[rank_index(s.g.chunks)], (static_cast<uint64_t>(s.row_tiles) * s.splits) << s.slot_bits,
                 64 * sr::kShrinkWaves, &s, stream);
 }
 
@@ -106,9 +109,9 @@ int expand(const sr_adapters* g, const void* matrices, const float* low, int spl
   const int64_t row_tiles = (rows + 15) / 16, waves = row_tiles * ((n + 63) / 64);
   const bool wide = waves >= 1024;
   const int64_t groups = wide ? (row_tiles + sr::kExpandTiles - 1) / sr::kExpandTiles : row_tiles;
-  s.slots = wide ? 1 : std::max(1, std::min(4, g->count));
+  s.slot_bits = wide ? 0 : slot_bits_of(1, g->count);
   s.column_tiles = static_cast<int>((n + (wide ? 63 : 15)) / (wide ? 64 : 16));
-  s.blocks = (s.column_tiles * s.slots + sr::kAdapterWaves - 1) / sr::kAdapterWaves;
+  s.blocks = ((s.column_tiles << s.slot_bits) + sr::kAdapterWaves - 1) / sr::kAdapterWaves;
   return launch(kernels(g->dtype).expand[rank_index(s.g.chunks)][wide], static_cast<uint64_t>(groups) * s.blocks, sr::kAdapterThreads, &s,
                 stream);
 }

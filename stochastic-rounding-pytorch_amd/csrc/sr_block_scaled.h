@@ -223,8 +223,9 @@ __device__ __forceinline__ int live_of(T at, T end, int width) {
 
 // The tile of 128 rows and 8 LANES columns from (row0, col0), by a workgroup
 // of 32 LANES threads, of which LANES share four neighbouring rows.  The columns
-// are stored up to row `stored`, zeros behind the matrix's last row.
-template <int XE, int QE, bool SQUARE, int LANES>
+// are stored up to row `stored`, zeros behind the matrix's last row, which with
+// RAGGED may leave whole waves without rows to encode.
+template <int XE, int QE, bool SQUARE, int LANES, bool RAGGED = false>
 __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, int64_t col0, bool want_rows, bool want_cols,
                                           int64_t stored) {
   constexpr int kGroups = 32, kThreads = kGroups * LANES, kCols = 8 * LANES;
@@ -291,9 +292,10 @@ __device__ __forceinline__ void cast_tile(const BlockCastArgs& a, int64_t row0, 
     }
   }
 
-  uint32_t by_col[2][4];
+  uint32_t by_col[2][4] = {};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    if (RAGGED && r0 >= a.rows) break;
     const int64_t r = r0 + i;
     uint32_t hash[2][4], words[2];
     hash_eight<QE>(a.counter_base + static_cast<uint32_t>(r) * static_cast<uint32_t>(a.cols) + static_cast<uint32_t>(c), hash);

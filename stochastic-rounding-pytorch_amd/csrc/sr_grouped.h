@@ -465,7 +465,7 @@ __global__ __launch_bounds__(kTileThreads, 4) void grouped_cast_tile_kernel(Grou
     return;
   }
   const BlockCastArgs p = cast_of_group(g.c, at, enc_bytes(XE));
-  cast_tile<XE, QE, false, 16>(p, static_cast<int64_t>(within) * kCastTile, col0, true, true,
+  cast_tile<XE, QE, false, 16, true>(p, static_cast<int64_t>(within) * kCastTile, col0, true, true,
                                static_cast<int64_t>(within + 1) * kCastTile);
 }
 
@@ -492,7 +492,7 @@ __global__ __launch_bounds__(kPartThreads, enc_stochastic(QE) ? 5 : 6) void grou
   const GroupTile at = table.find(g.groups, tile, limit);
   const uint32_t within = tile - at.first;
   const BlockCastArgs p = cast_of_group(g.c, at, enc_bytes(XE));
-  cast_tile<XE, QE, false, kPartLanes>(p, static_cast<int64_t>(within) * kCastTile, col0, false, true,
+  cast_tile<XE, QE, false, kPartLanes, true>(p, static_cast<int64_t>(within) * kCastTile, col0, false, true,
                                        static_cast<int64_t>(within + 1) * kCastTile);
 }
 
