@@ -453,37 +453,127 @@ struct Run {
   }
 };
 
+constexpr int kLowBytes = 64;  // of 16 ranks of a row in LDS
+
+// Lays four values of a row's `low`, from rank `rank` of their chunk on, out for Sixteen::of_lds.
+template <int XE>
+__device__ __forceinline__ void put_low(char* chunk, int rank, const f32x4& v) {
+  if constexpr (Sixteen<XE>::kParts) {
+    // Sixteen truncated parts, then the sixteen rests.
+    uint32_t* w = reinterpret_cast<uint32_t*>(chunk + 2 * rank);
+    w[0] = upper_halves(f32_bits(v[0]), f32_bits(v[1]));
+    w[1] = upper_halves(f32_bits(v[2]), f32_bits(v[3]));
+    w[8] = pack_bf16(bf16_rest(v[0]), bf16_rest(v[1]));
+    w[9] = pack_bf16(bf16_rest(v[2]), bf16_rest(v[3]));
+  } else {
+    *reinterpret_cast<f32x4*>(chunk + 4 * rank) = v;
+  }
+}
+
+// 16 NT columns of a wave: a lane's are kRuns runs of kRun, each beside those of its row's other three lanes.
+template <int XE, int RC, int NT>
+struct Columns {
+  static constexpr int kSize = enc_bytes(XE), kRun = NT == 1 ? 4 : 16 / kSize, kRuns = 4 * NT / kRun;
+  using Base = Run<XE, kRun>[kRuns];
+  int64_t n0, col;
+  bool edge;
+  int held;
+  Sixteen<XE> b[NT][RC];
+
+  __device__ __forceinline__ void start(const ExpandArgs& s, int64_t first, int q) {
+    n0 = first;
+    col = n0 + q * kRun;
+    edge = n0 + 16 * NT > s.n;
+    held = -1;
+  }
+  __device__ __forceinline__ int live(const ExpandArgs& s, int run) const {
+    const int64_t at = col + 4 * run * kRun;
+    return at >= s.n ? 0 : (s.n - at < kRun ? static_cast<int>(s.n - at) : kRun);
+  }
+  __device__ __forceinline__ void load(const ExpandArgs& s, int64_t row, Base& base) const {
+    if (!s.base) return;
+    const char* p = s.base + ((row < s.g.rows ? row : s.g.rows - 1) * s.ldbase + col) * kSize;
+    if (edge) {
+#pragma unroll
+      for (int run = 0; run < kRuns; ++run) base[run].load(p + 4 * run * kRun * kSize, live(s, run));
+    } else {
+#pragma unroll
+      for (int run = 0; run < kRuns; ++run) base[run].load(p + 4 * run * kRun * kSize);
+    }
+  }
+  __device__ __forceinline__ void hold(const ExpandArgs& s, int adapter, int i, int q) {
+    if (adapter == held) return;
+    held = adapter;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      // Four of the run's columns, as result rows 4 q .. 4 q + 3 of the instruction.
+      constexpr int kFours = kRun / 4;
+      const int64_t n = n0 + t / kFours * 4 * kRun + (i >> 2) * kRun + t % kFours * 4 + (i & 3);
+      const char* row = s.g.a + (static_cast<int64_t>(adapter) * s.n + (n < s.n ? n : s.n - 1)) * s.g.rank * kSize;
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+        if (c < s.g.chunks) b[t][c] = Sixteen<XE>::of_row(row, s.g.rank, c, q);
+    }
+  }
+  // The results of 16 rows; `low`: this lane's row in LDS.
+  __device__ __forceinline__ void results(const ExpandArgs& s, int64_t row, int mine, const char* low_row, const Base& base,
+                                          uint32_t slot, int i, int q) {
+    const uint32_t slots = 1u << s.slot_bits;
+    f32x4 sum[NT] = {};
+    bool owned = mine < 0 && slot == 0;
+    for_each_adapter(mine, [&](int adapter, int number) {
+      if ((number & (slots - 1)) != slot) return;
+      hold(s, adapter, i, q);
+      owned |= mine == adapter;
+      Sixteen<XE> low[RC];
+#pragma unroll
+      for (int c = 0; c < RC; ++c)
+        if (c < s.g.chunks) low[c].of_lds(low_row + c * kLowBytes + 16 * q);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        f32x4 part = {};
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+          if (c < s.g.chunks) b[t][c].mma(part, low[c]);
+        if (mine == adapter) sum[t] = part;
+      }
+    });
+    if (!owned || row >= s.g.rows) return;
+    char* p = s.out + (row * s.ldout + col) * kSize;
+#pragma unroll
+    for (int run = 0; run < kRuns; ++run) {
+      Run<XE, kRun> out = base[run];
+      if (!s.base || mine >= 0) {
+#pragma unroll
+        for (int j = 0; j < kRun; j += 2) {
+          const int at = run * kRun + j;
+          const float lo = sum[at >> 2][at & 3], hi = sum[at >> 2][(at & 3) + 1];
+          if (s.base) out.set(j, base[run].value(j) + lo, base[run].value(j + 1) + hi);
+          else out.set(j, lo, hi);
+        }
+      }
+      if (edge) out.store(p + 4 * run * kRun * kSize, live(s, run));
+      else out.store(p + 4 * run * kRun * kSize);
+    }
+  }
+};
+
 template <int XE, int RC, int NT, int TILES>
 __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandArgs s) {
-  constexpr int kSize = enc_bytes(XE), kRows = 16 * TILES, kChunkBytes = 64;
-  __shared__ __align__(16) char lows[kRows * RC * kChunkBytes];
+  constexpr int kRows = 16 * TILES;
+  __shared__ __align__(16) char lows[kRows * RC * kLowBytes];
   __shared__ int indices[kRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
   const uint32_t group = blockIdx.x / s.blocks, unit = (blockIdx.x - group * s.blocks) * kAdapterWaves + wave;
-  const uint32_t slots = 1u << s.slot_bits, slot = unit & (slots - 1);
-  const int64_t n0 = static_cast<int64_t>(unit >> s.slot_bits) * 16 * NT, row0 = static_cast<int64_t>(group) * kRows;
-  // This lane's columns are kRuns runs of kRun, each beside those of the row's other three lanes.
-  constexpr int kRun = NT == 1 ? 4 : 16 / kSize, kRuns = 4 * NT / kRun;
-  const int64_t col = n0 + q * kRun;
-  const bool edge = n0 + 16 * NT > s.n;
-  auto live = [&](int run) { return col + 4 * run * kRun >= s.n ? 0 : (s.n - col - 4 * run * kRun < kRun ? static_cast<int>(s.n - col - 4 * run * kRun) : kRun); };
+  const uint32_t slot = unit & ((1u << s.slot_bits) - 1);
+  const int64_t row0 = static_cast<int64_t>(group) * kRows;
+  Columns<XE, RC, NT> columns;
+  columns.start(s, static_cast<int64_t>(unit >> s.slot_bits) * 16 * NT, q);
 
-  Run<XE, kRun> base[TILES][kRuns];
-  if (s.base) {
+  typename Columns<XE, RC, NT>::Base base[TILES];
 #pragma unroll
-    for (int tile = 0; tile < TILES; ++tile) {
-      const int64_t row = row0 + tile * 16 + i;
-      const char* p = s.base + ((row < s.g.rows ? row : s.g.rows - 1) * s.ldbase + col) * kSize;
-      if (edge) {
-#pragma unroll
-        for (int run = 0; run < kRuns; ++run) base[tile][run].load(p + 4 * run * kRun * kSize, live(run));
-      } else {
-#pragma unroll
-        for (int run = 0; run < kRuns; ++run) base[tile][run].load(p + 4 * run * kRun * kSize);
-      }
-    }
-  }
+  for (int tile = 0; tile < TILES; ++tile) columns.load(s, row0 + tile * 16 + i, base[tile]);
   const int64_t width = s.g.chunks * kRankChunk, stride = s.g.rows * width;
   if (threadIdx.x < kRows) indices[threadIdx.x] = adapter_of(s.g, row0 + threadIdx.x);
   // Four values at a time, all of the group's rows side by side.
@@ -497,79 +587,13 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
       sum += f32x4{more[0], more[1], more[2], more[3]};
     }
     const int row = static_cast<int>(4 * at / width), place = static_cast<int>(4 * at - row * width);
-    char* to = lows + (row * RC + place / kRankChunk) * kChunkBytes;
-    const int rank = place % kRankChunk;
-    if constexpr (Sixteen<XE>::kParts) {
-      // Sixteen truncated parts, then the sixteen rests.
-      uint32_t* w = reinterpret_cast<uint32_t*>(to + 2 * rank);
-      w[0] = upper_halves(f32_bits(sum[0]), f32_bits(sum[1]));
-      w[1] = upper_halves(f32_bits(sum[2]), f32_bits(sum[3]));
-      w[8] = pack_bf16(bf16_rest(sum[0]), bf16_rest(sum[1]));
-      w[9] = pack_bf16(bf16_rest(sum[2]), bf16_rest(sum[3]));
-    } else {
-      *reinterpret_cast<f32x4*>(to + 4 * rank) = sum;
-    }
+    put_low<XE>(lows + (row * RC + place / kRankChunk) * kLowBytes, place % kRankChunk, sum);
   }
   __syncthreads();
-  if (n0 >= s.n) return;
-
-  Sixteen<XE> b[NT][RC];
-  int held = -1;
-  auto hold = [&](int adapter) {
-    if (adapter == held) return;
-    held = adapter;
+  if (columns.n0 >= s.n) return;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      // Four of the run's columns, as result rows 4 q .. 4 q + 3 of the instruction.
-      constexpr int kFours = kRun / 4;
-      const int64_t n = n0 + t / kFours * 4 * kRun + (i >> 2) * kRun + t % kFours * 4 + (i & 3);
-      const char* row = s.g.a + (static_cast<int64_t>(adapter) * s.n + (n < s.n ? n : s.n - 1)) * s.g.rank * kSize;
-#pragma unroll
-      for (int c = 0; c < RC; ++c)
-        if (c < s.g.chunks) b[t][c] = Sixteen<XE>::of_row(row, s.g.rank, c, q);
-    }
-  };
-#pragma unroll
-  for (int tile = 0; tile < TILES; ++tile) {
-    const int64_t row = row0 + tile * 16 + i;
-    const int mine = indices[tile * 16 + i];
-    f32x4 sum[NT] = {};
-    bool owned = mine < 0 && slot == 0;
-    for_each_adapter(mine, [&](int adapter, int number) {
-      if ((number & (slots - 1)) != slot) return;
-      hold(adapter);
-      owned |= mine == adapter;
-      Sixteen<XE> low[RC];
-#pragma unroll
-      for (int c = 0; c < RC; ++c)
-        if (c < s.g.chunks) low[c].of_lds(lows + ((tile * 16 + i) * RC + c) * kChunkBytes + 16 * q);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        f32x4 part = {};
-#pragma unroll
-        for (int c = 0; c < RC; ++c)
-          if (c < s.g.chunks) b[t][c].mma(part, low[c]);
-        if (mine == adapter) sum[t] = part;
-      }
-    });
-    if (!owned || row >= s.g.rows) continue;
-    char* p = s.out + (row * s.ldout + col) * kSize;
-#pragma unroll
-    for (int run = 0; run < kRuns; ++run) {
-      Run<XE, kRun> out = base[tile][run];
-      if (!s.base || mine >= 0) {
-#pragma unroll
-        for (int j = 0; j < kRun; j += 2) {
-          const int at = run * kRun + j;
-          const float lo = sum[at >> 2][at & 3], hi = sum[at >> 2][(at & 3) + 1];
-          if (s.base) out.set(j, base[tile][run].value(j) + lo, base[tile][run].value(j + 1) + hi);
-          else out.set(j, lo, hi);
-        }
-      }
-      if (edge) out.store(p + 4 * run * kRun * kSize, live(run));
-      else out.store(p + 4 * run * kRun * kSize);
-    }
-  }
+  for (int tile = 0; tile < TILES; ++tile)
+    columns.results(s, row0 + tile * 16 + i, indices[tile * 16 + i], lows + (tile * 16 + i) * RC * kLowBytes, base[tile], slot, i, q);
 }
 
 // ---------------------------------------------------------------------------
