@@ -372,6 +372,11 @@ at::Tensor grouped_product(const Scaled& a, const Scaled& b, const at::Tensor& s
     value_error("b has " + std::to_string(b.data.size(0)) + " matrices for " + std::to_string(groups.count) + " groups");
   const int64_t m = left.rows, n = b.data.size(-2), count = groups.count;
   const bool given = out.defined();
+  if (given) {
+    const auto [start, end] = span(out);
+    const auto [first, last] = span(sizes);
+    if (start < last && first < end) value_error("out must not overlap the sizes");
+  }
   if (stacked) {
     const int64_t stride = result_of(out, {m, n}, out_code, a, b, "grouped_block_matmul");
     if (!m || !n) return out;

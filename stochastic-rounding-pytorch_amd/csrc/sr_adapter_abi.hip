@@ -210,6 +210,8 @@ int sr_adapter_backward(const sr_adapters* g, const void* x, int64_t ldx, int64_
 
   if (live && (want_x || want_a)) {
     sr::TurnArgs t{};
+    if (int64_t{g->count} * ((n + 63) / 64 + (k + 63) / 64) * ((g->rank + 63) / 64) > 0x7FFFFF)
+      return fail(SR_ERR_ARGUMENT, "%d adapters of %lld to %lld exceed a launch", g->count, (long long)k, (long long)n);
     auto turn = [&](const void* from, int64_t to, int64_t r, int64_t c) {
       const int64_t tiles_n = (c + 63) / 64;
       return sr::TurnOperand{static_cast<const char*>(from), work + to, r, c, static_cast<int>(tiles_n),
