@@ -8,7 +8,7 @@
 //
 // bind(block_cast, block_matmul, orthogonalize, orthogonalize_workspace, grouped_columns, grouped_block_cast,
 //      stacked_block_cast, grouped_block_matmul, grouped_block_contract, adapter_low, adapter_workspace, adapter_add,
-//      adapter_backward)
+//      adapter_backward, last_error)
 //   Keep the addresses of these sr_ entry points, taken from the loaded library.
 //
 // block_cast(x, code, rule, square, axes, seed, offset, stream) -> tuple or int
@@ -32,13 +32,13 @@
 //   As block_cast, of a matrix whose rows are in groups of `sizes`, or (None) of a stack of matrices.
 // grouped_matmul(a_data, a_scale, b_data, b_scale, sizes, out_code, out, stream) -> tensor or int
 //   Each group's rows of a by its matrix of b, or its columns of a by its columns of b where b is a matrix.
-// grouped_linear_forward(x, weight, sizes, formats, seed, need_x, need_weight, stream)
-// grouped_linear_backward(dy, sizes, x_t data, x_t scale, w_t data, w_t scale, formats, seed, dx_code, dw_code, stream)
-//   As linear_forward and linear_backward.
+// grouped_linear(x, weight, sizes, formats, seed, stream) -> tensor or int
+//   The grouped layer, recorded for autograd in grad mode.
+// adapter_add(base, x, a, b, index, scaling, scale, out, stream) -> tensor or int
+//   base plus each row's low-rank update, into `out` where it is not None; else recorded for autograd in grad mode.
 //
-// adapter_add(base, x, a, b, index, scaling, scale, out, stream) -> (tensor, low) or int
-//   base plus each row's low-rank update, into `out` where it is not None, and what the gradients need of it.
-// adapter_backward(dy, x, a, b, index, scaling, scale, low, need_x, need_a, need_b, stream) -> (dx, da, db) or int
+// The last two are nodes of the autograd graph themselves: through a Python function a training step of a small layer
+// took 119 us, of which its kernels are 58, and one of small adapters 101.
 //
 // Errors of the tensors raise TypeError or ValueError before anything is
 // launched.  Every entry runs with the first tensor's device current and the
@@ -51,11 +51,15 @@
 #include <ATen/ops/empty_strided.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
 #include <cstdint>
 #include <exception>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <type_traits>
@@ -81,6 +85,7 @@ decltype(&sr_adapter_low) g_adapter_low = nullptr;
 decltype(&sr_adapter_workspace) g_adapter_workspace = nullptr;
 decltype(&sr_adapter_add) g_adapter_add = nullptr;
 decltype(&sr_adapter_backward) g_adapter_backward = nullptr;
+decltype(&sr_last_error) g_last_error = nullptr;
 PyObject* g_out_of_memory = nullptr;  // torch.OutOfMemoryError
 
 // A refusal, raised as `type`.
@@ -489,9 +494,120 @@ at::Tensor add_adapters(const at::Tensor& base, const at::Tensor& x, const Adapt
   return out;
 }
 
+// ---- nodes of the autograd graph ----
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Runs a node's gradients: a failed launch becomes an error here, where the message of this thread's last one is, and
+// the gradients cannot be differentiated again.
+template <class Body>
+variable_list gradients(const char* name, Body&& body) {
+  const bool recorded = c10::GradMode::is_enabled();
+  variable_list out;
+  try {
+    const at::AutoGradMode off(false);
+    out = body();
+  } catch (const Status& status) {
+    throw std::runtime_error(std::string(name) + " failed (" + std::to_string(status.code) + "): " + g_last_error());
+  }
+  if (!recorded) return out;
+  for (at::Tensor& t : out)
+    if (t.defined()) t = t.detach().set_requires_grad(true);
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string("trying to differentiate twice: the gradients of ") + name + " have none", static_cast<int64_t>(out.size()));
+  return (*error)(std::move(out));
+}
+
+struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
+  struct Options {
+    int format[6];
+    uint32_t seed[3];
+    void* stream;
+  };
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& sizes, bool need_x,
+                            bool need_w, const Options& o) {
+    Scaled qx, qx_t, qw, qw_t;
+    const at::Tensor rows = as_rows(x.detach()), weight = as_stack(w.detach());
+    cast_groups_into(rows, sizes, o.format[0], o.format[1], o.seed[0], 0, &qx, need_w ? &qx_t : nullptr, o.stream);
+    cast_stack_into(weight, o.format[2], o.format[3], true, o.seed[1], 0, &qw, need_x ? &qw_t : nullptr, o.stream);
+    if (need_x || need_w) {
+      ctx->save_for_backward({sizes, qx_t.data, qx_t.scale, qw_t.data, qw_t.scale});
+      ctx->saved_data["rule"] = std::vector<int64_t>{o.format[4], o.format[5], o.seed[2], dtype_code(x.scalar_type()), dtype_code(w.scalar_type()),
+                                                     static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.stream))};
+    }
+    return grouped_product(qx, qw, sizes, dtype_code(x.scalar_type()), at::Tensor(), o.stream);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return gradients("grouped_block_linear", [&] {
+      const variable_list saved = ctx->get_saved_variables();
+      const std::vector<int64_t> rule = ctx->saved_data["rule"].toIntVector();
+      void* stream = address(static_cast<unsigned long long>(rule[5]));  // the engine runs a node on its forward pass's stream
+      const at::Tensor& dy = grads[0];
+      at::Tensor dx, dw;
+      if (dy.defined()) {
+        const c10::DeviceGuard guard(dy.device());
+        const Scaled x{saved[1], saved[2]}, w{saved[3], saved[4]};
+        const bool need_x = w.data.defined() && ctx->needs_input_grad(0), need_w = x.data.defined() && ctx->needs_input_grad(1);
+        Scaled by_rows, by_cols;
+        cast_groups_into(as_rows(dy.detach()), saved[0], static_cast<int>(rule[0]), static_cast<int>(rule[1]),
+                         static_cast<uint32_t>(rule[2]), 0, need_x ? &by_rows : nullptr, need_w ? &by_cols : nullptr, stream);
+        if (need_x) dx = grouped_product(by_rows, w, saved[0], static_cast<int>(rule[3]), at::Tensor(), stream);
+        if (need_w) dw = grouped_product(by_cols, x, saved[0], static_cast<int>(rule[4]), at::Tensor(), stream);
+      }
+      return variable_list{dx, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    });
+  }
+};
+
+struct AdapterAdd : torch::autograd::Function<AdapterAdd> {
+  struct Options {
+    at::Tensor scaling;  // or undefined: `scale` for all
+    double scale;
+    void* stream;
+  };
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& base, const at::Tensor& x, const at::Tensor& a, const at::Tensor& b,
+                            const at::Tensor& index, const Options& o) {
+    at::Tensor low;
+    const at::Tensor y = add_adapters(base, x, AdapterSet(x, a, b, index, o.scaling, o.scale), at::Tensor(), low, o.stream);
+    ctx->save_for_backward({x, a, b, index, o.scaling, low});
+    ctx->saved_data["scale"] = o.scale;
+    ctx->saved_data["stream"] = static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.stream));
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    return gradients("adapter_add", [&] {
+      const variable_list saved = ctx->get_saved_variables();
+      const at::Tensor &x = saved[0], &a = saved[1], &b = saved[2], &dy = grads[0];
+      void* stream = address(static_cast<unsigned long long>(ctx->saved_data["stream"].toInt()));
+      at::Tensor dbase, dx, da, db;
+      const bool need_x = ctx->needs_input_grad(1), need_a = ctx->needs_input_grad(2), need_b = ctx->needs_input_grad(3);
+      if (dy.defined()) {
+        const c10::DeviceGuard guard(dy.device());
+        if (ctx->needs_input_grad(0)) dbase = dy;
+        if (need_x || need_a || need_b) {
+          const AdapterSet set(x, a, b, saved[3], saved[4], ctx->saved_data["scale"].toDouble());
+          const at::Tensor rows = as_rows(x.detach().resolve_neg()), from = as_rows(dy.detach().resolve_neg());
+          if (need_x) dx = at::empty(x.sizes(), x.options());
+          if (need_a) da = at::empty(a.sizes(), a.options());
+          if (need_b) db = at::empty(b.sizes(), b.options());
+          const at::Tensor workspace = at::empty({g_adapter_workspace(set.rows, set.k, set.n, set.g.count, set.g.rank, set.g.dtype)},
+                                                 x.options().dtype(c10::ScalarType::Byte));
+          auto place = [](const at::Tensor& t) { return t.defined() ? memory(t) : nullptr; };
+          checked(g_adapter_backward(&set.g, memory(rows), row_stride(rows, "x"), set.k, memory(from), row_stride(from, "dy"), set.n,
+                                     set.rows, static_cast<const float*>(memory(saved[5])), place(dx), set.k, place(da), place(db),
+                                     memory(workspace), stream));
+        }
+      }
+      return variable_list{dbase, dx, da, db, at::Tensor(), at::Tensor()};
+    });
+  }
+};
+
 bool bound() {
   return g_cast && g_matmul && g_orthogonalize && g_workspace && g_columns && g_grouped_cast && g_stacked_cast &&
-         g_grouped_matmul && g_grouped_contract && g_adapter_low && g_adapter_workspace && g_adapter_add && g_adapter_backward;
+         g_grouped_matmul && g_grouped_contract && g_adapter_low && g_adapter_workspace && g_adapter_add && g_adapter_backward &&
+         g_last_error;
 }
 
 // Runs `body` as the entries promise; nullptr with an exception set, the
@@ -505,6 +621,7 @@ PyObject* run(const at::Device& device, Body body, Result result) {
   int status = 0;
   std::string message;
   PyObject* type = nullptr;
+  std::optional<python_error> raised;  // by a hook of saved tensors, in Python
   Py_BEGIN_ALLOW_THREADS
   try {
     const c10::OptionalDeviceGuard guard(device.is_cuda() ? c10::optional<at::Device>(device) : c10::nullopt);
@@ -514,6 +631,8 @@ PyObject* run(const at::Device& device, Body body, Result result) {
     message = refusal.what();
   } catch (const Status& s) {
     status = s.code;
+  } catch (python_error& error) {
+    raised.emplace(std::move(error));
   } catch (const c10::OutOfMemoryError& error) {
     type = g_out_of_memory;
     message = error.what_without_backtrace();
@@ -525,6 +644,10 @@ PyObject* run(const at::Device& device, Body body, Result result) {
     message = "unknown C++ exception in a native entry";
   }
   Py_END_ALLOW_THREADS
+  if (raised) {
+    raised->restore();
+    return nullptr;
+  }
   if (type) {
     PyErr_SetString(type, message.c_str());
     return nullptr;
@@ -562,9 +685,9 @@ PyObject* wrap_casts(const std::string& wanted, const Scaled& by_rows, const Sca
 }
 
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long at[13];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKK", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6], &at[7], &at[8], &at[9],
-                        &at[10], &at[11], &at[12]))
+  unsigned long long at[14];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKKK", &at[0], &at[1], &at[2], &at[3], &at[4], &at[5], &at[6], &at[7], &at[8], &at[9],
+                        &at[10], &at[11], &at[12], &at[13]))
     return nullptr;
   auto keep = [](auto& function, unsigned long long value) {
     function = reinterpret_cast<std::remove_reference_t<decltype(function)>>(address(value));
@@ -582,6 +705,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   keep(g_adapter_workspace, at[10]);
   keep(g_adapter_add, at[11]);
   keep(g_adapter_backward, at[12]);
+  keep(g_last_error, at[13]);
   if (!bound()) {
     PyErr_SetString(PyExc_ValueError, "null entry point address");
     return nullptr;
@@ -742,50 +866,24 @@ PyObject* grouped_matmul(PyObject*, PyObject* args) {
       });
 }
 
-PyObject* grouped_linear_forward(PyObject*, PyObject* args) {
+PyObject* grouped_linear(PyObject*, PyObject* args) {
   PyObject *x_object, *w_object, *sizes_object;
-  int format[6], need_x, need_w;
+  GroupedLinear::Options o;
   unsigned long long seed[3], stream;
-  if (!PyArg_ParseTuple(args, "OOO(iiiiii)(KKK)ppK", &x_object, &w_object, &sizes_object, &format[0], &format[1], &format[2],
-                        &format[3], &format[4], &format[5], &seed[0], &seed[1], &seed[2], &need_x, &need_w, &stream))
+  if (!PyArg_ParseTuple(args, "OOO(iiiiii)(KKK)K", &x_object, &w_object, &sizes_object, &o.format[0], &o.format[1], &o.format[2],
+                        &o.format[3], &o.format[4], &o.format[5], &seed[0], &seed[1], &seed[2], &stream))
     return nullptr;
+  for (int k = 0; k < 3; ++k) o.seed[k] = static_cast<uint32_t>(seed[k]);
+  o.stream = address(stream);
   const at::Tensor &x = tensor(x_object), &w = tensor(w_object), &sizes = tensor(sizes_object);
-  Scaled qx, qx_t, qw, qw_t;
   at::Tensor y;
   return run(
       x.device(),
       [&] {
-        const at::Tensor rows = as_rows(x.detach()), weight = as_stack(w.detach());
-        cast_groups_into(rows, sizes, format[0], format[1], static_cast<uint32_t>(seed[0]), 0, &qx, need_w ? &qx_t : nullptr, address(stream));
-        cast_stack_into(weight, format[2], format[3], true, static_cast<uint32_t>(seed[1]), 0, &qw, need_x ? &qw_t : nullptr, address(stream));
-        y = grouped_product(qx, qw, sizes, dtype_code(x.scalar_type()), at::Tensor(), address(stream));
+        const bool recorded = c10::GradMode::is_enabled();
+        y = GroupedLinear::apply(x, w, sizes, recorded && x.requires_grad(), recorded && w.requires_grad(), o);
       },
-      [&] { return wrap_all({&y, &qx_t.data, &qx_t.scale, &qw_t.data, &qw_t.scale}); });
-}
-
-PyObject* grouped_linear_backward(PyObject*, PyObject* args) {
-  PyObject *dy_object, *sizes_object, *x_data, *x_scale, *w_data, *w_scale;
-  int code, rule, dx_code, dw_code;
-  unsigned long long seed, stream;
-  if (!PyArg_ParseTuple(args, "OOOOOOiiKiiK", &dy_object, &sizes_object, &x_data, &x_scale, &w_data, &w_scale, &code, &rule, &seed,
-                        &dx_code, &dw_code, &stream))
-    return nullptr;
-  const at::Tensor &dy = tensor(dy_object), &sizes = tensor(sizes_object);
-  const bool need_w = x_data != Py_None, need_x = w_data != Py_None;
-  Scaled x, w, by_rows, by_cols;
-  if (need_w) x = {tensor(x_data), tensor(x_scale)};
-  if (need_x) w = {tensor(w_data), tensor(w_scale)};
-  at::Tensor dx, dw;
-  return run(
-      dy.device(),
-      [&] {
-        const at::Tensor rows = as_rows(dy.detach());
-        cast_groups_into(rows, sizes, code, rule, static_cast<uint32_t>(seed), 0, need_x ? &by_rows : nullptr,
-                         need_w ? &by_cols : nullptr, address(stream));
-        if (need_x) dx = grouped_product(by_rows, w, sizes, dx_code, at::Tensor(), address(stream));
-        if (need_w) dw = grouped_product(by_cols, x, sizes, dw_code, at::Tensor(), address(stream));
-      },
-      [&] { return wrap_all({&dx, &dw}); });
+      [&] { return wrap(y); });
 }
 
 PyObject* adapter_add(PyObject*, PyObject* args) {
@@ -802,41 +900,20 @@ PyObject* adapter_add(PyObject*, PyObject* args) {
   if (out_object != Py_None) out = tensor(out_object);
   const bool given = out.defined();
   return run(
-      x.device(), [&] { result = add_adapters(base, x, AdapterSet(x, a, b, index, scaling, scale), out, low, address(stream)); },
-      [&]() -> PyObject* {
-        if (!given) return wrap_all({&result, &low});
-        return Py_BuildValue("(ON)", out_object, wrap(low));
-      });
-}
-
-PyObject* adapter_backward(PyObject*, PyObject* args) {
-  PyObject *dy_object, *x_object, *a_object, *b_object, *index_object, *scaling_object, *low_object;
-  double scale;
-  int need_x, need_a, need_b;
-  unsigned long long stream;
-  if (!PyArg_ParseTuple(args, "OOOOOOdOpppK", &dy_object, &x_object, &a_object, &b_object, &index_object, &scaling_object, &scale,
-                        &low_object, &need_x, &need_a, &need_b, &stream))
-    return nullptr;
-  const at::Tensor &dy = tensor(dy_object), &x = tensor(x_object), &a = tensor(a_object), &b = tensor(b_object),
-                   &index = tensor(index_object), &low = tensor(low_object);
-  at::Tensor scaling, dx, da, db;
-  if (scaling_object != Py_None) scaling = tensor(scaling_object);
-  return run(
       x.device(),
       [&] {
-        const AdapterSet set(x, a, b, index, scaling, scale);
-        const at::Tensor rows = as_rows(x.detach().resolve_neg()), from = as_rows(dy.detach().resolve_neg());
-        if (need_x) dx = at::empty(x.sizes(), x.options());
-        if (need_a) da = at::empty(a.sizes(), a.options());
-        if (need_b) db = at::empty(b.sizes(), b.options());
-        const at::Tensor workspace = at::empty({g_adapter_workspace(set.rows, set.k, set.n, set.g.count, set.g.rank, set.g.dtype)},
-                                               x.options().dtype(c10::ScalarType::Byte));
-        auto place = [](const at::Tensor& t) { return t.defined() ? memory(t) : nullptr; };
-        checked(g_adapter_backward(&set.g, memory(rows), row_stride(rows, "x"), set.k, memory(from), row_stride(from, "dy"), set.n,
-                                   set.rows, static_cast<const float*>(memory(low)), place(dx), set.k, place(da), place(db),
-                                   memory(workspace), address(stream)));
+        const bool recorded = c10::GradMode::is_enabled() &&
+                              (base.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad());
+        if (recorded && given)
+          throw Refusal(PyExc_RuntimeError, "a given out records no gradients: call adapter_add under torch.no_grad()");
+        if (recorded) result = AdapterAdd::apply(base, x, a, b, index, AdapterAdd::Options{scaling, scale, address(stream)});
+        else result = add_adapters(base, x, AdapterSet(x, a, b, index, scaling, scale), out, low, address(stream));
       },
-      [&] { return wrap_all({&dx, &da, &db}); });
+      [&]() -> PyObject* {
+        if (!given) return wrap(result);
+        Py_INCREF(out_object);
+        return out_object;
+      });
 }
 
 PyObject* orthogonalize(PyObject*, PyObject* args) {
@@ -894,10 +971,8 @@ PyMethodDef methods[] = {
     {"linear_backward", guarded<linear_backward>, METH_VARARGS, "Gradients of the block-scaled linear layer."},
     {"grouped_cast", guarded<grouped_cast>, METH_VARARGS, "Cast rows in groups, or a stack of matrices, to FP8 with block scales."},
     {"grouped_matmul", guarded<grouped_matmul>, METH_VARARGS, "Multiply each group's rows by its matrix, or contract its columns."},
-    {"grouped_linear_forward", guarded<grouped_linear_forward>, METH_VARARGS, "Forward pass of the grouped linear layer."},
-    {"grouped_linear_backward", guarded<grouped_linear_backward>, METH_VARARGS, "Gradients of the grouped linear layer."},
+    {"grouped_linear", guarded<grouped_linear>, METH_VARARGS, "The grouped linear layer."},
     {"adapter_add", guarded<adapter_add>, METH_VARARGS, "Add each row's low-rank update."},
-    {"adapter_backward", guarded<adapter_backward>, METH_VARARGS, "Gradients of the low-rank updates."},
     {"orthogonalize", guarded<orthogonalize>, METH_VARARGS, "Orthogonalise matrices."},
     {nullptr, nullptr, 0, nullptr},
 };

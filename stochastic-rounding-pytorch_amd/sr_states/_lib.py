@@ -379,7 +379,7 @@ def matrix():
                       for name in ("sr_block_cast", "sr_block_matmul", "sr_orthogonalize", "sr_orthogonalize_workspace",
                                    "sr_grouped_columns", "sr_grouped_block_cast", "sr_stacked_block_cast",
                                    "sr_grouped_block_matmul", "sr_grouped_block_contract", "sr_adapter_low",
-                                   "sr_adapter_workspace", "sr_adapter_add", "sr_adapter_backward")))
+                                   "sr_adapter_workspace", "sr_adapter_add", "sr_adapter_backward", "sr_last_error")))
         _matrix = module
     return _matrix
 

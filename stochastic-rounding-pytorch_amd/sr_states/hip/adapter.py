@@ -17,29 +17,6 @@ from .. import _lib
 from .block import _device_of, _stream
 
 
-class _AdapterAdd(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, base, x, a, b, index, scaling, scale):
-        out = _lib.matrix().adapter_add(base, x, a, b, index, scaling, scale, None, _stream(x.device))
-        if not isinstance(out, tuple):
-            _lib.check("adapter_add", out)
-        ctx.save_for_backward(x, a, b, index, scaling, out[1])
-        ctx.scale = scale
-        return out[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, a, b, index, scaling, low = ctx.saved_tensors
-        need_base, *need = ctx.needs_input_grad[:4]
-        grads = (None, None, None)
-        if any(need):
-            grads = _lib.matrix().adapter_backward(dy, x, a, b, index, scaling, ctx.scale, low, *need, _stream(dy.device))
-            if not isinstance(grads, tuple):
-                _lib.check("adapter_add", grads)
-        return (dy if need_base else None, *grads, None, None, None)
-
-
 def adapter_add(
     base: torch.Tensor,
     x: torch.Tensor,
@@ -73,11 +50,7 @@ def adapter_add(
         scale = 1.0
     else:
         scale, scaling = float(scaling), None
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (base, x, a, b)):
-        if out is not None:
-            raise RuntimeError("a given out records no gradients: call adapter_add under torch.no_grad()")
-        return _AdapterAdd.apply(base, x, a, b, index, scaling, scale)
     result = _lib.matrix().adapter_add(base, x, a, b, index, scaling, scale, out, _stream(device))
-    if not isinstance(result, tuple):
+    if not isinstance(result, torch.Tensor):
         _lib.check("adapter_add", result)
-    return result[0]
+    return result

@@ -100,28 +100,6 @@ def grouped_block_matmul(
     return result
 
 
-class _GroupedBlockLinear(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, sizes, codes, seed, recorded):
-        # As in block_linear: the grad mode is the caller's.
-        need_x, need_w = (recorded and need for need in ctx.needs_input_grad[:2])
-        seeds = tuple(state_key(seed, k) for k in range(3))
-        out = _lib.matrix().grouped_linear_forward(x, weight, sizes, codes, seeds, need_x, need_w, _stream(x.device))
-        if not isinstance(out, tuple):
-            _lib.check("grouped_block_linear", out)
-        ctx.save_for_backward(sizes, *out[1:])
-        ctx.options = (*codes[4:], seeds[2], _lib.DTYPE_CODES[x.dtype], _lib.DTYPE_CODES[weight.dtype])
-        return out[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        out = _lib.matrix().grouped_linear_backward(dy, *ctx.saved_tensors, *ctx.options, _stream(dy.device))
-        if not isinstance(out, tuple):
-            _lib.check("grouped_block_linear", out)
-        return *out, None, None, None, None
-
-
 def grouped_block_linear(
     x: torch.Tensor,
     weight: torch.Tensor,
@@ -153,5 +131,9 @@ def grouped_block_linear(
         raise ValueError("x, weight and sizes must be on the same GPU device")
     if sizes.shape != weight.shape[:1]:
         raise ValueError(f"{weight.shape[0]} weights take as many sizes, not {tuple(sizes.shape)}")
-    _device_of(x, weight, sizes)
-    return _GroupedBlockLinear.apply(x, weight, sizes, codes, _lib.low32(seed), torch.is_grad_enabled())
+    device = _device_of(x, weight, sizes)
+    key = _lib.low32(seed)
+    y = _lib.matrix().grouped_linear(x, weight, sizes, codes, tuple(state_key(key, k) for k in range(3)), _stream(device))
+    if not isinstance(y, torch.Tensor):
+        _lib.check("grouped_block_linear", y)
+    return y

@@ -154,3 +154,32 @@ def test_optimizers_update_what_the_layer_learns(cuda):
         optimizer.step()
     for name, p in parameters.items():
         assert p.isfinite().all() and not torch.equal(p, before[name]), name
+
+
+def test_gradients_are_not_differentiated_again(cuda):
+    tensors, sizes, index, dy = _inputs(cuda)
+    x = tensors["x"].clone().requires_grad_()
+    up = tensors["up"].clone().requires_grad_()
+    a = tensors["a"].clone().requires_grad_()
+    for y, leaves in ((sr_states.grouped_block_linear(x, up, sizes), (x, up)),
+                      (sr_states.adapter_add(x * 1.0, x, a, tensors["b"], index), (x, a))):
+        scale = torch.ones_like(y).requires_grad_()
+        plain = torch.autograd.grad(y, leaves, torch.ones_like(y), retain_graph=True)
+        again = torch.autograd.grad(y, leaves, scale, create_graph=True)
+        for got, want in zip(again, plain):
+            assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            again[1].sum().backward()
+
+
+def test_gradients_through_saved_tensor_hooks(cuda):
+    """Saved tensors that move to the host and back, as activation offloading has it."""
+    tensors, sizes, index, dy = _inputs(cuda)
+    want = _gradients(_layer, tensors, sizes, index, dy)
+
+    def offloaded(**arguments):
+        with torch.autograd.graph.save_on_cpu():
+            return _layer(**arguments)
+
+    for got, expected in zip(_gradients(offloaded, tensors, sizes, index, dy), want):
+        assert torch.equal(got, expected)
