@@ -1,7 +1,7 @@
 /*
  * sr_matrix_hip.h -- C ABI of the matrix operators of libsr_states_hip.so:
- * FP8 products with a scale for each block of 128, and orthogonalised
- * (Muon) updates.
+ * FP8 products with a scale for each block of 128, also of rows in groups with
+ * a matrix each, low-rank adapters, and orthogonalised (Muon) updates.
  *
  * The conventions are those of sr_states_hip.h: 0 or an SR_ERR_* code is
  * returned, sr_last_error() holds the message, `stream` is a hipStream_t on

@@ -7,8 +7,11 @@ launch for the groups it takes, one parameter at a time otherwise) at the
 top level, the functional updates in ``sr_states.reference``, and the
 fused multi-tensor optimizers and casts in ``sr_states.hip`` (the
 counterpart of ``sr_states.triton``).  Beyond the reference: FP8 matrices with block scales
-and their products (``block_cast``, ``block_matmul``, ``block_linear``), and
-orthogonalised updates (``orthogonalize``, ``MuonHip``).  All arithmetic runs in the HIP
+and their products (``block_cast``, ``block_matmul``, ``block_linear``), the same
+for rows that are sorted into groups with a weight each (``grouped_block_cast``,
+``grouped_block_matmul``, ``grouped_block_linear``), low-rank adapters of many
+requests at once (``adapter_add``), and orthogonalised updates
+(``orthogonalize``, ``MuonHip``).  All arithmetic runs in the HIP
 library ``libsr_states_hip.so``; there is no CPU execution path.
 """
 

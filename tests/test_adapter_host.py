@@ -80,7 +80,7 @@ def test_invalid_arguments_fail_before_any_device_work():
 def test_workspaces_cover_the_shapes_that_are_taken():
     low, workspace = _lib.library().sr_adapter_low, _lib.library().sr_adapter_workspace
     assert low(8192, 2048, 16, _lib.SR_BF16) == 8192 * 16  # rows enough for every CU
-    assert low(1, 2048, 8, _lib.SR_BF16) == 8 * 16  # eight parts of one row
+    assert low(1, 2048, 8, _lib.SR_BF16) == 4 * 16  # four parts of one row, eight waves and a step each
     assert low(1, 1, 17, _lib.SR_F32) == 32
     assert low(4, 64, 129, _lib.SR_F32) == low(-1, 64, 8, _lib.SR_F32) == low(4, 64, 8, _lib.SR_E4M3) == 0
     turned = 4 * 8 * (2048 + 512) * 2
