@@ -214,12 +214,35 @@ __device__ __forceinline__ void for_each_adapter(int mine, F&& use) {
   }
 }
 
+// Whether the adapters of 64 rows, one a lane, do not come in runs in ascending order: `order` then receives the rows in
+// the order of their adapters, between which they keep their own.  For a whole workgroup, whose waves hold the same.
+__device__ __forceinline__ bool order_rows(int mine, int* order) {
+  const int lane = threadIdx.x & 63, above = __shfl_up(mine, 1);
+  if (__ballot(lane > 0 && mine < above) == 0) return false;
+  if (threadIdx.x < 64) {
+    int place = 0;
+    for (int j = 0; j < 64; ++j) {
+      const int other = __builtin_amdgcn_readlane(mine, j);
+      place += other < mine || (other == mine && j < lane);
+    }
+    order[place] = lane;
+  }
+  __syncthreads();
+  return true;
+}
+
 // ---------------------------------------------------------------------------
 // shrink: a workgroup takes 16 rows, one of `splits` parts of the contracted axis
 // and, of the adapters that the rows meet, every `slots`-th.  Its eight waves
 // share these adapters out as far as they go, and the part's steps beyond that.
 // Partial sums of the parts lie behind each other in `low`, for expand and
 // contract to add in order; a row is written by its adapter's workgroup alone.
+//
+// 8192 x 2048 BF16, rank 16: 16 us, 6.5 of them bytes; the rest is the chain of
+// index, rows, sums and launch (twice as many values of x take 7 us more).  Loads of
+// x ahead of the index, and more of them together, are level.  One row of 2048:
+// 3.8 us; 64 rows with 32 adapters: 8.4, in one part for the whole axis 10 to 15%
+// more, without slots 40%.
 // ---------------------------------------------------------------------------
 struct ShrinkArgs {
   Adapters g;
@@ -237,12 +260,18 @@ template <int XE, int RC>
 __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(ShrinkArgs s) {
   constexpr int kStep = kShrinkStep<XE>, kEights = kStep / kEightSpan;
   __shared__ f32x4 sums[kShrinkWaves][RC][64];
+  __shared__ int order[64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
   const int tile = blockIdx.x % s.row_tiles, unit = blockIdx.x / s.row_tiles;
   const int slots = 1 << s.slot_bits, slot = unit & (slots - 1), split = unit >> s.slot_bits;
-  const int64_t row = static_cast<int64_t>(tile) * 16 + i;
-  const int mine = adapter_of(s.g, row);
+  // A quarter of 64 rows, which are taken in the order of their adapters where that is another.
+  const int64_t row0 = static_cast<int64_t>(tile >> 2) * 64;
+  const int all = adapter_of(s.g, row0 + lane);
+  int place = (tile & 3) * 16 + i;
+  if (row0 + 64 <= s.g.rows && order_rows(all, order)) place = order[place];
+  const int64_t row = row0 + place;
+  const int mine = __shfl(all, place);
   const char* x = s.x + (row < s.g.rows ? row : s.g.rows - 1) * s.ldx * enc_bytes(XE);
   int met = 0;          // by this workgroup
   bool owned = mine < 0 && slot == 0;  // this lane's row is written here
@@ -371,8 +400,15 @@ struct Sixteen {
 // in LDS once; its waves take 16 NT columns each.  Their instructions take the
 // rows of b in an order that leaves a lane runs of 16 bytes, four lanes side by side.
 // All of base is on its way before anything waits, and the adapter met last
-// stays in registers.  With slots so many waves take every slots-th of the
+// stays in registers.  Where 64 rows do not come in runs of one adapter they are
+// taken in the order of their adapters, so that each adapter is read about once,
+// here and in shrink (8192 rows of 8 adapters in any order, 2048 to 2048, rank 16: 96
+// us and 58 in all; in runs 27).  With slots so many waves take every slots-th of the
 // adapters that 16 rows meet, and write only these rows.
+//
+// 8192 rows to 8192 columns, rank 16: 58 us, at the rate of a large copy 52.  With
+// `low` read by every wave instead of once a workgroup it took 70, and with tiles
+// one after the other, each waiting for its own loads, 108.
 // ---------------------------------------------------------------------------
 struct ExpandArgs {
   Adapters g;  // a: count x n x rank
@@ -562,7 +598,7 @@ template <int XE, int RC, int NT, int TILES>
 __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandArgs s) {
   constexpr int kRows = 16 * TILES;
   __shared__ __align__(16) char lows[kRows * RC * kLowBytes];
-  __shared__ int indices[kRows];
+  __shared__ int indices[kRows], order[kRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
   const uint32_t group = blockIdx.x / s.blocks, unit = (blockIdx.x - group * s.blocks) * kAdapterWaves + wave;
@@ -590,10 +626,18 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
     put_low<XE>(lows + (row * RC + place / kRankChunk) * kLowBytes, place % kRankChunk, sum);
   }
   __syncthreads();
+  bool mixed = false;
+  if constexpr (kRows == 64) mixed = order_rows(indices[lane], order);
   if (columns.n0 >= s.n) return;
+  int rows[TILES];
+#pragma unroll
+  for (int tile = 0; tile < TILES; ++tile) {
+    rows[tile] = mixed ? order[tile * 16 + i] : tile * 16 + i;
+    if (mixed) columns.load(s, row0 + rows[tile], base[tile]);
+  }
 #pragma unroll
   for (int tile = 0; tile < TILES; ++tile)
-    columns.results(s, row0 + tile * 16 + i, indices[tile * 16 + i], lows + (tile * 16 + i) * RC * kLowBytes, base[tile], slot, i, q);
+    columns.results(s, row0 + rows[tile], indices[rows[tile]], lows + rows[tile] * RC * kLowBytes, base[tile], slot, i, q);
 }
 
 // ---------------------------------------------------------------------------
@@ -604,6 +648,10 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
 // take 32 of them at a time in turn, turned in registers so that rows are the
 // contracted axis, and add their sums in wave order.  Parts leave FP32 sums
 // and whether they had rows at all, for `finish` to add in order.
+//
+// 8191 rows by 2048 and 2304 columns, rank 32, 4 adapters: 30 us for 71 MB (14 at a copy's
+// rate); 50 without the next rows' loads under this step's products.  Without
+// parts one adapter of all rows takes 113 us a backward pass and not 59.
 // ---------------------------------------------------------------------------
 struct ContractOperand {
   const float* low;  // splits x rows x 16 chunks

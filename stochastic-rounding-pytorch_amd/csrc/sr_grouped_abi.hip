@@ -213,12 +213,16 @@ int sr_grouped_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, 
   const int64_t rows = a->rows, full = std::min<int64_t>(groups->count, rows);  // groups that can have rows
   // Room for any sizes: every group, and the rows behind them, may end inside a tile.
   auto room = [&](int64_t side) { return static_cast<uint64_t>((rows + (side - 1) * (full + g.zero_behind)) / side); };
-  if (rows <= 16 * full) {
+  const bool async = aligned_rows(a) && aligned_rows(b) && b_stride % 16 == 0;
+  // Tiles to expect: one a group where groups are small, and half a tile more than its rows fill where they are large.
+  auto tiles = [&](int64_t side) { return std::max(full, rows / side + (full + 1) / 2) * ((g.p.n + side - 1) / side); };
+  // Few rows a group to few columns: a wave's own loads have less to wait for than a tile's stages (4 groups by 2048 x 2048: 4
+  // rows each 6.9 us and 7.9, 8 rows 7.3 and 7.9, 12 rows 10.4 and 8.0; 16 groups, 8 rows in all, 256 tiles 6.9 and 7.9; 64
+  // groups, 12 rows in all, 384 tiles 14.0 and 11.1).
+  if (rows <= 8 * full && tiles(64) <= 256) {
     g.p.tiles_n = (g.p.n + 15) / 16;
     return launch(fn.rows, room(16) * g.p.tiles_n, 64 * sr::kRowWaves, &g, stream);
   }
-  const bool async = aligned_rows(a) && aligned_rows(b) && b_stride % 16 == 0;
-  auto tiles = [&](int64_t side) { return (rows / side + (full + 1) / 2) * ((g.p.n + side - 1) / side); };
   const sr::BlockTile tile = sr::tile_by_count(tiles);
   if (fn.lean[0] && async && k % SR_BLOCK == 0 && tiles(128) > sr::kLeanTiles) {
     g.p.tiles_n = (g.p.n + 127) / 128;
