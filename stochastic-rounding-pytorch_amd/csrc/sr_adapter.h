@@ -935,16 +935,30 @@ __global__ __launch_bounds__(256) void adapter_finish_kernel(ContractArgs s) {
     adapter = id / quads / s.g.rank;
   }
   if (adapter >= s.g.count) return;
+  // Eight parts' loads go out together; what a part without rows holds means nothing.
+  constexpr int kTogether = 8;
   f32x4 sum{};
-  for (int p = 0; p < s.parts; ++p) {
-    if (!gptr<int>(s.filled)[p * s.g.count + adapter]) continue;
-    const float* from = op.partial + ((p * static_cast<int64_t>(s.g.count) + adapter) * width + rank) * op.cols + col;
-    if (op.turned) {
+  const int live = live_four(col, op.cols);
+  for (int first = 0; first < s.parts; first += kTogether) {
+    f32x4 values[kTogether];
+    int filled[kTogether];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sum[e] += *gptr<float>(from + e * op.cols);  // ranks up to `width` are there
-    } else {
-      sum += load_four<ENC_F32>(reinterpret_cast<const char*>(from), live_four(col, op.cols));
+    for (int j = 0; j < kTogether; ++j) {
+      const int64_t p = first + j < s.parts ? first + j : s.parts - 1;
+      filled[j] = gptr<int>(s.filled)[p * s.g.count + adapter];
+      const float* from = op.partial + ((p * s.g.count + adapter) * width + rank) * op.cols + col;
+      if (op.turned) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) values[j][e] = *gptr<float>(from + e * op.cols);  // ranks up to `width` are there
+      } else {
+        // The places of the last column stand in for those behind it.
+#pragma unroll
+        for (int e = 0; e < 4; ++e) values[j][e] = *gptr<float>(from + (e < live ? e : live - 1));
+      }
     }
+#pragma unroll
+    for (int j = 0; j < kTogether; ++j)
+      if (first + j < s.parts && filled[j]) sum += values[j];
   }
   if (op.turned)
     store_four<XE>(op.out + ((adapter * op.cols + col) * s.g.rank + rank) * enc_bytes(XE), sum, live_four(rank, s.g.rank));
@@ -980,9 +994,16 @@ __global__ __launch_bounds__(256) void adapter_turn_kernel(TurnArgs s) {
   const T* from = reinterpret_cast<const T*>(op.from) + matrix * op.rows * op.cols;
   T* to = reinterpret_cast<T*>(op.to) + matrix * op.rows * op.cols;
   const int column = threadIdx.x & 63, first = threadIdx.x >> 6;
+  // Places past the matrix's edges repeat its last ones, so that no load waits for a condition.
+  const int64_t col = c0 + column < op.cols ? c0 + column : op.cols - 1;
+  T values[16];
 #pragma unroll
-  for (int r = 0; r < 64; r += 4)
-    if (r0 + r + first < op.rows && c0 + column < op.cols) tile[r + first][column] = gptr<T>(from)[(r0 + r + first) * op.cols + c0 + column];
+  for (int r = 0; r < 16; ++r) {
+    const int64_t row = r0 + 4 * r + first;
+    values[r] = gptr<T>(from)[(row < op.rows ? row : op.rows - 1) * op.cols + col];
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) tile[4 * r + first][column] = values[r];
   __syncthreads();
 #pragma unroll
   for (int c = 0; c < 64; c += 4)
