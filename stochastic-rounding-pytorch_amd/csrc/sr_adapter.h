@@ -256,15 +256,15 @@ constexpr int kShrinkWaves = 8;
 template <int XE>
 constexpr int kShrinkStep = 4 * 32 / enc_bytes(XE);  // values of the contracted axis that a wave takes at once: 128 bytes of a row
 
-template <int XE, int RC>
-__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(ShrinkArgs s) {
+// Wave c ends with chunk c's sums of the rows that this workgroup writes: use(row, c, the four of this lane's row from
+// rank 4 (lane / 16) of the chunk on).
+template <int XE, int RC, class F>
+__device__ __forceinline__ void shrink_tile(const ShrinkArgs& s, f32x4 (&sums)[kShrinkWaves][RC][64], int (&order)[64], int tile,
+                                            int split, int slot, F&& use) {
   constexpr int kStep = kShrinkStep<XE>, kEights = kStep / kEightSpan;
-  __shared__ f32x4 sums[kShrinkWaves][RC][64];
-  __shared__ int order[64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, q = lane >> 4;
-  const int tile = blockIdx.x % s.row_tiles, unit = blockIdx.x / s.row_tiles;
-  const int slots = 1 << s.slot_bits, slot = unit & (slots - 1), split = unit >> s.slot_bits;
+  const int slots = 1 << s.slot_bits;
   // A quarter of 64 rows, which are taken in the order of their adapters where that is another.
   const int64_t row0 = static_cast<int64_t>(tile >> 2) * 64;
   const int all = adapter_of(s.g, row0 + lane);
@@ -343,12 +343,27 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(Shrin
 #pragma unroll
   for (int w = 1; w < kShrinkWaves; ++w) total += sums[w][wave][lane];
   const float scale = adapter_scale(s.g, mine);
-  const int64_t width = s.g.chunks * kRankChunk;
   const int rank = wave * kRankChunk + 4 * q;
   f32x4 out{};
 #pragma unroll
   for (int j = 0; j < 4; ++j) out[j] = mine >= 0 && rank + j < s.g.rank ? total[j] * scale : 0.0f;
-  *(SR_GLOBAL floats4*)(s.low + (split * s.g.rows + row) * width + rank) = floats4{out[0], out[1], out[2], out[3]};
+  use(row, wave, out);
+}
+
+// Part `split` of a row's chunk.
+__device__ __forceinline__ void store_low(const ShrinkArgs& s, int64_t row, int split, int chunk, int q, const f32x4& v) {
+  *(SR_GLOBAL floats4*)(s.low + (split * s.g.rows + row) * s.g.chunks * kRankChunk + chunk * kRankChunk + 4 * q) =
+      floats4{v[0], v[1], v[2], v[3]};
+}
+
+template <int XE, int RC>
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_shrink_kernel(ShrinkArgs s) {
+  __shared__ f32x4 sums[kShrinkWaves][RC][64];
+  __shared__ int order[64];
+  const int tile = blockIdx.x % s.row_tiles, unit = blockIdx.x / s.row_tiles;
+  const int slot = unit & ((1 << s.slot_bits) - 1), split = unit >> s.slot_bits, q = (threadIdx.x & 63) >> 4;
+  shrink_tile<XE, RC>(s, sums, order, tile, split, slot,
+                      [&](int64_t row, int chunk, const f32x4& v) { store_low(s, row, split, chunk, q, v); });
 }
 
 // Sixteen ranks of `low` and of the adapters as the products with FP32 values take them.  With BF16, 32 places of the
@@ -638,6 +653,39 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_expand_kernel(ExpandA
 #pragma unroll
   for (int tile = 0; tile < TILES; ++tile)
     columns.results(s, row0 + rows[tile], indices[rows[tile]], lows + rows[tile] * RC * kLowBytes, base[tile], slot, i, q);
+}
+
+// ---------------------------------------------------------------------------
+// Both in one, for a few rows: every workgroup goes through the rows' adapters by
+// itself, and on to 16 columns a wave.  One launch; the adapters' a comes from the
+// caches after the first (one row of 2048 to 2048, rank 8: 7.4 us a call, 9.6 in two).
+// ---------------------------------------------------------------------------
+struct FewArgs {
+  ShrinkArgs down;  // in one part
+  ExpandArgs up;
+  int parts;        // of `low` as a backward pass adds them up: all but the first become zeros
+};
+
+template <int XE, int RC>
+__global__ __launch_bounds__(64 * kShrinkWaves) void adapter_few_kernel(FewArgs s) {
+  __shared__ f32x4 sums[kShrinkWaves][RC][64];
+  __shared__ int order[64];
+  __shared__ __align__(16) char lows[16 * RC * kLowBytes];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = lane & 15, q = lane >> 4;
+  Columns<XE, RC, 1> columns;
+  typename Columns<XE, RC, 1>::Base base;
+  columns.start(s.up, (static_cast<int64_t>(blockIdx.x) * kShrinkWaves + wave) * 16, q);
+  columns.load(s.up, i, base);
+  shrink_tile<XE, RC>(s.down, sums, order, 0, 0, 0, [&](int64_t row, int chunk, const f32x4& v) {
+    put_low<XE>(lows + (row * RC + chunk) * kLowBytes, 4 * q, v);
+    if (blockIdx.x == 0) {
+      store_low(s.down, row, 0, chunk, q, v);
+      for (int part = 1; part < s.parts; ++part) store_low(s.down, row, part, chunk, q, f32x4{});
+    }
+  });
+  __syncthreads();
+  if (columns.n0 < s.up.n) columns.results(s.up, i, adapter_of(s.up.g, i), lows + i * RC * kLowBytes, base, 0, i, q);
 }
 
 // ---------------------------------------------------------------------------

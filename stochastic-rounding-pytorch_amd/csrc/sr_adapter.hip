@@ -18,6 +18,7 @@ void fill(AdapterKernels& k, int at) {
   k.shrink[at] = reinterpret_cast<const void*>(&adapter_shrink_kernel<XE, RC>);
   k.expand[at][0] = reinterpret_cast<const void*>(&adapter_expand_kernel<XE, RC, 1, 1>);
   k.expand[at][1] = reinterpret_cast<const void*>(&adapter_expand_kernel<XE, RC, 4, kExpandTiles>);
+  k.few[at] = reinterpret_cast<const void*>(&adapter_few_kernel<XE, RC>);
   k.contract[at] = reinterpret_cast<const void*>(&adapter_contract_kernel<XE, RC, CJ>);
   k.contract_columns[at] = 16 * CJ;
 }

@@ -131,6 +131,17 @@ int expand(const sr_adapters* g, const sr::ExpandArgs& args, void* stream) {
 // The one and then the other.  (In one kernel, 16 rows a workgroup, all of b passes each of them: 8192 rows of 2048 to 8192
 // took 114 us, and take 73 in two.)
 int shrink_and_expand(const sr_adapters* g, const sr::ShrinkArgs& down, const sr::ExpandArgs& up, void* stream) {
+  // Bytes of the adapters' a that every workgroup of the one launch would read by itself, a chunk of ranks at a time: one row of
+  // 2048 to 2048 takes 7.8 us and 10.1, of 4096 8.5 and 10.2, two of 2048 8.9 and 9.5; one of 8192 12.7 and 10.3, four of 2048
+  // 15.1 and 9.6.  More rows can meet more adapters, one after the other (eight rows of 512 12.0 us).
+  if (down.g.rows <= 2 && up.n && down.g.rows * down.g.chunks * down.k * element(g->dtype) <= 8192) {
+    sr::FewArgs s{down, up, down.splits};
+    s.down.splits = 1;
+    s.down.slot_bits = s.up.slot_bits = 0;
+    constexpr int64_t kColumns = 16 * sr::kShrinkWaves;
+    return launch(kernels(g->dtype).few[rank_index(s.down.g.chunks)], static_cast<uint64_t>((up.n + kColumns - 1) / kColumns),
+                  64 * sr::kShrinkWaves, &s, stream);
+  }
   if (int rc = shrink(g, down, stream)) return rc;
   return up.n ? expand(g, up, stream) : SR_OK;
 }

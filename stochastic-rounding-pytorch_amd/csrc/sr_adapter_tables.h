@@ -9,6 +9,7 @@ constexpr int kExpandTiles = 4;   // times 16 rows of a workgroup of expand whos
 struct AdapterKernels {
   const void* shrink[kAdapterRanks];
   const void* expand[kAdapterRanks][2];  // [.][1]: 64 columns a wave
+  const void* few[kAdapterRanks];        // shrink and expand in one, for few rows
   const void* contract[kAdapterRanks];
   int contract_columns[kAdapterRanks];   // of a workgroup
   const void* finish;

@@ -91,6 +91,28 @@ def test_equals_the_definition(cuda, rows, k, n, count, rank, dtype, index):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows, k, n, rank", [(1, 2048, 2048, 8), (1, 100, 37, 16), (2, 1000, 300, 16), (2, 2048, 130, 20),
+                                              (1, 4096, 64, 3), (3, 512, 64, 16), (1, 64, 64, 128)])
+def test_single_tokens(cuda, dtype, rows, k, n, rank):
+    """One launch or two, whichever the rows and ranks take, and the gradients that follow."""
+    base, x, a, b, _, scaling = _inputs(cuda, rows, k, n, 3, rank, dtype, "none")
+    dy = torch.randn(rows, n, device=cuda).to(dtype)
+    for t in (x, a, b):
+        t.requires_grad_()
+    for index in ([0, 2, 1], [1, 1, 1], [2, -1, 0], [-1, 0, 2], [-1, -1, -1]):
+        index = torch.tensor(index[:rows], device=cuda)
+        y = sr_states.adapter_add(base, x, a, b, index, scaling=scaling)
+        _assert_near(y.detach(), oracle.add(base, x, a, b, index, scaling), k + rank)
+        got = torch.autograd.grad(y, (x, a, b), dy)
+        for g, want, terms in zip(got, oracle.gradients(dy, x, a, b, index, scaling), (n + rank, n + rows, k + rows)):
+            _assert_near(g, want, terms)
+        with torch.no_grad():
+            into = base.clone()
+            sr_states.adapter_add(into, x, a, b, index, scaling=scaling, out=into)
+            assert torch.equal(into, y)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("order", ["mixed", "runs"])
 @pytest.mark.parametrize("rank", [8, 32])
 def test_many_rows(cuda, dtype, order, rank):
