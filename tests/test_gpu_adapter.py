@@ -158,6 +158,23 @@ def test_nothing_of_an_adapter_reaches_other_rows(cuda, dtype):
     assert torch.equal(clean[0][3], base[3]) and clean[0][4, 0].isnan() and torch.equal(clean[0][4, 1:], base[4, 1:])
 
 
+@pytest.mark.parametrize("rows", [1, 64, 4096])
+@pytest.mark.parametrize("dtype, x, a, b", [
+    (torch.float16, -20, 5, 10), (torch.float16, 0, -20, 10), (torch.float16, 0, 8, -20),
+    (torch.bfloat16, -130, 100, 20), (torch.bfloat16, 100, -130, 20), (torch.bfloat16, 50, 60, -130), (torch.bfloat16, -60, -70, 100),
+    (torch.float32, -140, 100, 20), (torch.float32, 60, 50, -140), (torch.float32, -60, -75, 100),
+])
+def test_subnormal_values_count(cuda, rows, dtype, x, a, b):
+    """Powers of two, so that every product and sum is exact; each case has an operand or a value between below the normal range."""
+    def full(shape, log):
+        return torch.full(shape, 2.0**log, device=cuda, dtype=dtype)
+
+    index = torch.zeros(rows, dtype=torch.int32, device=cuda)
+    y = sr_states.adapter_add(torch.zeros(rows, 80, device=cuda, dtype=dtype), full((rows, 64), x), full((1, 16, 64), a),
+                              full((1, 80, 16), b), index)
+    assert (y.double() == 2.0 ** (6 + 4 + x + a + b)).all()
+
+
 def test_indices_outside_the_adapters_are_none(cuda):
     base, x, a, b, _, scaling = _inputs(cuda, 6, 64, 64, 3, 8, torch.bfloat16, "none")
     index = torch.tensor([0, 3, -1, 1 << 40, -(1 << 40), 2], device=cuda)
