@@ -967,6 +967,7 @@ __global__ __launch_bounds__(256) void adapter_finish_kernel(ContractArgs s) {
   const int64_t width = s.g.chunks * kRankChunk;
   int64_t id = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   const int64_t firsts = finish_items(s.g, s.op[0]);
+  if (id >= firsts + finish_items(s.g, s.op[1])) return;  // an operand that is not there has no sizes to divide by
   const bool second = id >= firsts;
   if (second) id -= firsts;
   const ContractOperand& op = s.op[second];
@@ -982,7 +983,6 @@ __global__ __launch_bounds__(256) void adapter_finish_kernel(ContractArgs s) {
     rank = id / quads % s.g.rank;
     adapter = id / quads / s.g.rank;
   }
-  if (adapter >= s.g.count) return;
   // Eight parts' loads go out together; what a part without rows holds means nothing.
   constexpr int kTogether = 8;
   f32x4 sum{};

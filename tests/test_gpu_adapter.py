@@ -259,6 +259,24 @@ def test_gradients_that_are_not_wanted_are_not_made(cuda):
     assert torch.equal(leaf.grad, dy)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k, n, rank, count", [(201, 333, 20, 3), (7, 2, 1, 1)])
+def test_some_gradients_of_rows_in_parts(cuda, dtype, k, n, rank, count):
+    """The parts' sums are joined by 256 threads at a time, more than either gradient alone has use for."""
+    base, x, a, b, index, scaling = _inputs(cuda, 2500, k, n, count, rank, dtype, "mixed")
+    assert (count * -(-k // 4) * rank) % 256 and (count * n * -(-rank // 4)) % 256
+    dy = torch.randn(2500, n, device=cuda).to(dtype)
+    leaves = [t.clone().requires_grad_() for t in (x, a, b)]
+    whole = torch.autograd.grad(sr_states.adapter_add(base, *leaves, index, scaling=scaling), leaves, dy)
+    for got, want, terms in zip(whole, oracle.gradients(dy, x, a, b, index, scaling), (n + rank, n + 2500, k + 2500)):
+        _assert_near(got, want, terms)
+    for wanted in range(1, 7):
+        leaves = [t.clone().requires_grad_(bool(wanted >> j & 1)) for j, t in enumerate((x, a, b))]
+        sr_states.adapter_add(base, *leaves, index, scaling=scaling).backward(dy)
+        for j, leaf in enumerate(leaves):
+            assert leaf.grad is None if not wanted >> j & 1 else torch.equal(leaf.grad, whole[j])
+
+
 def test_without_rows_adapters_or_values(cuda):
     for rows, k, n, count in ((0, 20, 30, 3), (7, 20, 30, 0), (7, 0, 30, 3), (7, 20, 0, 3)):
         base, x, a, b, index, scaling = _inputs(cuda, rows, k, n, count, 4, torch.float32, "none")
