@@ -443,6 +443,7 @@ struct BlockProductArgs {
   const char* scale_b;
   int64_t ld_scale_a, ld_scale_b;
   int shift_a, shift_b;  // log2 of the rows that share a scale: 0 or 7
+  int first_a;           // of the rows of a in the matrix that its scales are those of: they may share one with rows before
   int64_t k;
   char* out;
   int64_t ldo;
@@ -607,8 +608,9 @@ struct ScaleArea {
     const int size = g.scale_f32 ? 4 : 1;
     const bool of_a = r < S::BM;
     const int at = of_a ? row0 + r : col0 + r - S::BM, rows = of_a ? g.m : g.n;
+    const int row_at = (of_a ? g.first_a : 0) + (at < rows ? at : rows - 1);
     const char* from = (of_a ? g.scale_a : g.scale_b) +
-                       (((at < rows ? at : rows - 1) >> (of_a ? g.shift_a : g.shift_b)) * (of_a ? g.ld_scale_a : g.ld_scale_b) + first) * size;
+                       ((row_at >> (of_a ? g.shift_a : g.shift_b)) * (of_a ? g.ld_scale_a : g.ld_scale_b) + first) * size;
     const int64_t end = static_cast<int64_t>(total - first) * size;
     const i32x4 lo = load_chunk(from, 0, end);
     if (MODE == kWide && !g.scale_f32) {
@@ -933,7 +935,7 @@ __device__ __forceinline__ void product_rows(const BlockProductArgs& g, f32x4 (&
   const char* pa = g.a.base + row_a * g.a.ld;
   const char* pb = g.b.base + row_b * g.b.ld;
   const int size = g.scale_f32 ? 4 : 1;
-  const char* scale_a = g.scale_a + (row_a >> g.shift_a) * g.ld_scale_a * size;
+  const char* scale_a = g.scale_a + ((g.first_a + row_a) >> g.shift_a) * g.ld_scale_a * size;
   const char* scale_b[Scales<MODE, 1, 1>::kPerB];
 #pragma unroll
   for (int j = 0; j < Scales<MODE, 1, 1>::kPerB; ++j) {

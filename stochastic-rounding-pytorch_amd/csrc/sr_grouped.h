@@ -169,10 +169,9 @@ __device__ __forceinline__ int64_t output_bytes(const BlockProductArgs& p, int64
 template <int TILE>
 __device__ __forceinline__ BlockProductArgs rows_product(const GroupedProductArgs& g, const GroupTile& at) {
   BlockProductArgs p = g.p;
-  const int64_t size = p.scale_f32 ? 4 : 1;
   p.a.base += at.start * p.a.ld;
   p.a.rows = p.m = static_cast<int>(at.rows);
-  p.scale_a += at.start * p.ld_scale_a * size;
+  p.first_a = static_cast<int>(at.start);  // a group may start inside a block of 128 rows
   p.out += output_bytes(p, at.start * p.ldo);
   p.tiles_m = at.tiles;
   if (at.group == g.groups.count) {
@@ -309,8 +308,9 @@ __global__ __launch_bounds__(256, 3) void grouped_lean_kernel(GroupedProductArgs
     const int r = threadIdx.x;
     const bool of_a = r < S::BM;
     const int row = of_a ? row0 + r : col0 + r - S::BM, rows = of_a ? p.m : p.n;
+    const int row_at = (of_a ? p.first_a : 0) + (row < rows ? row : rows - 1);
     const char* from = (of_a ? p.scale_a : p.scale_b) +
-                       ((row < rows ? row : rows - 1) >> (of_a ? p.shift_a : p.shift_b)) * (of_a ? p.ld_scale_a : p.ld_scale_b) + first;
+                       (row_at >> (of_a ? p.shift_a : p.shift_b)) * (of_a ? p.ld_scale_a : p.ld_scale_b) + first;
     const int there = scales - first;
     char* to = marks + r * kLeanScaleRow;
     if (there >= kLeanStages) {

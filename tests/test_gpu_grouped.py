@@ -182,6 +182,49 @@ def test_product_of_every_format(cuda, a_dtype, b_dtype, a_square, b_square, sca
         _assert_near(got, *grouped.product(a, b, counts), 272)
 
 
+# The 16-row kernel, 64 x 64 tiles in one, two and four groups of waves, aligned and not, 128 x 128 tiles, and those of one
+# stage: groups start inside blocks of 128 rows, at their ends, and behind an empty group.
+@pytest.mark.parametrize("rows, counts, n, k, pad", [
+    (20, [3, 9, 8], 140, 272, 0), (300, [40] * 7, 33, 130, 3), (330, [1, 127, 0, 128, 44], 140, 272, 0),
+    (700, [300, 0, 17, 250], 200, 384, 3), (700, [300, 0, 17, 250], 70, 1408, 16), (2600, [1300, 1, 1200], 1000, 256, 0),
+    (3100, [1500, 0, 129, 1, 900, 60], 3001, 384, 0), (2600, [130] * 20, 2000, 200, 1),
+])
+@pytest.mark.parametrize("a_dtype, scale, out", [
+    (E4M3, "e8m0", torch.bfloat16), (E5M2, "fp32", torch.float16), (E4M3, "e8m0", torch.float32), (E4M3, "fp32", torch.float32),
+])
+def test_groups_of_rows_that_share_scales(cuda, rows, counts, n, k, pad, a_dtype, scale, out):
+    a = _operand((rows, k), a_dtype, scale, True, cuda, 5, pad)
+    assert a.scale.shape[0] == -(-rows // 128)
+    b = _operand((len(counts), n, k), E4M3, scale, True, cuda, 6, pad)
+    got = sr_states.grouped_block_matmul(a, b, _sizes(counts, cuda), out_dtype=out)
+    _assert_near(got, *grouped.product(a, b, grouped.counts_of(counts, rows)), k)
+    shared = a.scale.view(torch.uint8 if scale == "e8m0" else torch.float32).repeat_interleave(128, 0)[:rows].view(a.scale.dtype)
+    same = sr_states.grouped_block_matmul(BlockScaled(a.data, shared), b, _sizes(counts, cuda), out_dtype=out)
+    assert torch.equal(got, same)  # a scale for each row: the same values
+
+
+@pytest.mark.parametrize("counts", [[100, 7, 93], [0, 200]])
+def test_groups_of_a_cast_in_square_blocks(cuda, counts):
+    x, w = _spread((200, 300), cuda, 1, torch.bfloat16), _spread((2, 90, 300), cuda, 2)
+    w = torch.cat((w, w[:1] * 3))[:len(counts)]
+    a = sr_states.block_cast(x, block=(128, 128), rounding="nearest")
+    b = sr_states.grouped_block_cast(w, block=(128, 128), rounding="nearest")
+    got = sr_states.grouped_block_matmul(a, b, _sizes(counts, cuda), out_dtype=torch.float32)
+    _assert_near(got, *grouped.product(a, b, counts), 300)
+
+
+def test_shared_scales_that_are_far_from_one(cuda):
+    """Factors whose products leave FP32's normal range on the way to a result: a tile's sums are taken once more."""
+    counts = [100, 0, 300, 112]
+    a = _operand((512, 512), E4M3, "fp32", True, cuda, 7)
+    b = _operand((4, 200, 512), E4M3, "fp32", False, cuda, 8)
+    a.scale[1:3] = 2.0**100
+    b.scale[:] = b.scale.clamp(0.25, 1) * 2.0**-120
+    for out in (torch.bfloat16, torch.float32):
+        got = sr_states.grouped_block_matmul(a, b, _sizes(counts, cuda), out_dtype=out)
+        _assert_near(got, *grouped.product(a, b, counts), 512)
+
+
 def _padded(rows, counts, width, dtype, scale, device, seed):
     """An operand of a contraction: random values in the groups' columns, zeros in the others."""
     q = _operand((rows, width), dtype, scale, False, device, seed)
