@@ -17,8 +17,8 @@
 // Numbers.  Products of x and the adapters run on their type's matrix
 // instructions; what follows takes `low` as FP32.  With BF16 operands a value
 // of it enters as two BF16 parts, truncated and rest, which keep 15 bits: far
-// below the result's rounding.  FP16 has no exponents for that, so FP16 operands
-// widen to FP32 there.
+// below the result's rounding unless the ranks cancel.  FP16 has no exponents for
+// that, so FP16 operands widen to FP32 there.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -130,11 +130,18 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ uint32_t upper_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 __device__ __forceinline__ uint32_t lower_halves(uint32_t lo, uint32_t hi) { return __builtin_amdgcn_perm(hi, lo, 0x05040100u); }
 
-// What truncation to BF16 leaves of x; nothing of infinities and NaN.
-__device__ __forceinline__ float bf16_rest(float x) {
-  const uint32_t b = f32_bits(x);
-  return (b & 0x7F800000u) == 0x7F800000u ? 0.0f : x - bits_f32(b & 0xFFFF0000u);
-}
+// x as two BF16 values of its sign, of which neither is zero unless x is: beside an infinite factor a zero would turn an
+// infinite sum into NaN.  The upper half of `upper` is x cut off below its magnitude, one step less where x is a BF16 value itself,
+// and `rest` what that leaves (infinite with x).  A rest below 2^-134 rounds to zero, which a magnitude of x below 2^-110
+// can leave.
+struct TwoParts {
+  uint32_t upper;
+  float rest;
+  __device__ __forceinline__ explicit TwoParts(float x) {
+    upper = f32_bits(x) - (x != 0.0f);
+    rest = x - bits_f32(upper & 0xFFFF0000u);
+  }
+};
 
 // Four values in T at `p`, of which `live` are there.
 template <int XE>
@@ -512,10 +519,12 @@ __device__ __forceinline__ void put_low(char* chunk, int rank, const f32x4& v) {
   if constexpr (Sixteen<XE>::kParts) {
     // Sixteen truncated parts, then the sixteen rests.
     uint32_t* w = reinterpret_cast<uint32_t*>(chunk + 2 * rank);
-    w[0] = upper_halves(f32_bits(v[0]), f32_bits(v[1]));
-    w[1] = upper_halves(f32_bits(v[2]), f32_bits(v[3]));
-    w[8] = pack_bf16(bf16_rest(v[0]), bf16_rest(v[1]));
-    w[9] = pack_bf16(bf16_rest(v[2]), bf16_rest(v[3]));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const TwoParts lo(v[2 * h]), hi(v[2 * h + 1]);
+      w[h] = upper_halves(lo.upper, hi.upper);
+      w[8 + h] = pack_bf16(lo.rest, hi.rest);
+    }
   } else {
     *reinterpret_cast<f32x4*>(chunk + 4 * rank) = v;
   }
@@ -850,8 +859,9 @@ __global__ __launch_bounds__(kAdapterThreads) void adapter_contract_kernel(Contr
         for (int c = 0; c < RC; ++c)
 #pragma unroll
           for (int p = 0; p < 4; ++p) {
-            upper[c].w[p] = upper_halves(f32_bits(step.low[c][2 * p]), f32_bits(step.low[c][2 * p + 1]));
-            rest[c].w[p] = pack_bf16(bf16_rest(step.low[c][2 * p]), bf16_rest(step.low[c][2 * p + 1]));
+            const TwoParts lo(step.low[c][2 * p]), hi(step.low[c][2 * p + 1]);
+            upper[c].w[p] = upper_halves(lo.upper, hi.upper);
+            rest[c].w[p] = pack_bf16(lo.rest, hi.rest);
           }
 #pragma unroll
         for (int j = 0; j < CJ; ++j) {

@@ -175,6 +175,49 @@ def test_subnormal_values_count(cuda, rows, dtype, x, a, b):
     assert (y.double() == 2.0 ** (6 + 4 + x + a + b)).all()
 
 
+# One launch for a row, 16 columns a wave, 64 columns a wave and rows in parts.
+@pytest.mark.parametrize("rows, n, rank", [(1, 40, 16), (60, 80, 1), (60, 80, 40), (300, 70, 128), (2500, 900, 20)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("infinite", ["base", "x", "a", "b", "dy", "scaling"])
+def test_infinities_are_the_definitions(cuda, rows, n, rank, dtype, infinite):
+    """Where the definition multiplies an infinity by zero or adds two of them, NaN, and nowhere else: not where BF16
+    holds a sum between the products, as it does those of x and a here, small multiples of a power of two."""
+    gen = torch.Generator().manual_seed(5)
+
+    def powers(shape, log, signed=False):
+        t = 2.0 ** torch.randint(log, log + 2, shape, generator=gen)
+        return (t * (1 - 2 * torch.randint(0, 2, shape, generator=gen)) if signed else t).to(dtype)
+
+    k, count = 8, 3
+    base, x, dy = powers((rows, n), 0, True), powers((rows, k), 0), powers((rows, n), -9)
+    a, b = powers((count, rank, k), -1), powers((count, n, rank), -4)
+    b[2] *= 1 - 2 * torch.randint(0, 2, (n, rank), generator=gen).to(dtype)
+    index = torch.arange(rows) % (count + 1)  # the last has no adapter
+    scaling = torch.tensor([1.0, -2.0, 0.5])
+    if rows > 1:
+        x[1::7] = 0
+    operands = {"base": base, "x": x, "a": a, "b": b, "dy": dy}
+    if infinite == "scaling":
+        scaling[0] = float("inf")
+    else:
+        t = operands[infinite]
+        flat = t.view(-1)
+        flat[::max(flat.numel() // 5, 7)] = float("inf")
+        flat[3::max(flat.numel() // 3, 11)] = -float("inf")
+    want = [oracle.add(base, x, a, b, index, scaling), *oracle.gradients(dy, x, a, b, index, scaling)]
+    assert any(value.isinf().any() for value, _ in want)
+    leaves = [t.to(cuda).requires_grad_() for t in (x, a, b)]
+    y = sr_states.adapter_add(base.to(cuda), *leaves, index.to(cuda), scaling=scaling.to(cuda))
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy.to(cuda))]
+    for result, (value, size), terms in zip(got, want, (k + rank, n + rank, n + rows, k + rows)):
+        result, value = result.cpu(), value.reshape(result.shape)
+        special = ~value.isfinite()
+        assert torch.equal(result.isnan(), value.isnan())
+        assert torch.equal(result[value.isinf()].double(), value[value.isinf()])
+        clean = [torch.where(special, 0, t.reshape(result.shape)) for t in (value, size)]
+        _assert_near(torch.where(special, 0, result), clean, terms)
+
+
 def test_indices_outside_the_adapters_are_none(cuda):
     base, x, a, b, _, scaling = _inputs(cuda, 6, 64, 64, 3, 8, torch.bfloat16, "none")
     index = torch.tensor([0, 3, -1, 1 << 40, -(1 << 40), 2], device=cuda)
