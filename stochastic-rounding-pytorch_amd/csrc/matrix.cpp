@@ -49,6 +49,7 @@
 #include <Python.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_strided.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <torch/csrc/Exceptions.h>
@@ -866,6 +867,14 @@ PyObject* grouped_matmul(PyObject*, PyObject* args) {
       });
 }
 
+// No operand may carry a tangent of forward-mode differentiation: the result would lose it without a word.
+void refuse_tangents(std::initializer_list<const at::Tensor*> operands, const char* name) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor* t : operands)
+    if (t->defined() && t->_fw_grad(0).defined())
+      throw Refusal(PyExc_NotImplementedError, std::string(name) + " has no forward-mode derivatives, and an operand has a tangent");
+}
+
 PyObject* grouped_linear(PyObject*, PyObject* args) {
   PyObject *x_object, *w_object, *sizes_object;
   GroupedLinear::Options o;
@@ -880,6 +889,7 @@ PyObject* grouped_linear(PyObject*, PyObject* args) {
   return run(
       x.device(),
       [&] {
+        refuse_tangents({&x, &w}, "grouped_block_linear");
         const bool recorded = c10::GradMode::is_enabled();
         y = GroupedLinear::apply(x, w, sizes, recorded && x.requires_grad(), recorded && w.requires_grad(), o);
       },
@@ -902,6 +912,7 @@ PyObject* adapter_add(PyObject*, PyObject* args) {
   return run(
       x.device(),
       [&] {
+        refuse_tangents({&base, &x, &a, &b, &scaling, &out}, "adapter_add");
         const bool recorded = c10::GradMode::is_enabled() &&
                               (base.requires_grad() || x.requires_grad() || a.requires_grad() || b.requires_grad());
         if (recorded && given)

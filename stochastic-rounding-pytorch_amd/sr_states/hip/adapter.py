@@ -38,7 +38,8 @@ def adapter_add(
     gets no gradient.
 
     Sums are FP32 and rounded once, at the end.  Gradients flow to ``base``, ``x``,
-    ``a`` and ``b``; adapters that no row uses get zeros.  ``out``, which may be
+    ``a`` and ``b``; adapters that no row uses get zeros.  There are no forward-mode
+    derivatives: an operand with a tangent is refused.  ``out``, which may be
     ``base`` itself, takes the result without recording gradients: in grad mode
     neither it nor an operand may require one.
     """

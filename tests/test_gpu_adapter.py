@@ -15,6 +15,7 @@ import _adapter_oracle as oracle
 import pytest
 import sr_states
 import torch
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 HALF_ULP = {torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11, torch.float32: 2.0**-24}
@@ -383,6 +384,24 @@ def test_an_operand_changed_before_the_backward_pass_is_noticed(cuda):
         t.add_(1)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+def test_tangents_are_refused(cuda):
+    """Forward-mode differentiation, in every grad mode; a tangent would be lost without a word."""
+    base, x, a, b, index, scaling = _inputs(cuda, 20, 80, 90, 4, 10, torch.float32, "mixed")
+    want = sr_states.adapter_add(base, x, a, b, index, scaling=scaling)
+    operands = {"base": base, "x": x, "a": a, "b": b, "scaling": scaling, "out": base.clone()}
+    with forward_ad.dual_level():
+        for name, t in operands.items():
+            dual = {**operands, name: forward_ad.make_dual(t, torch.ones_like(t))}
+            if name != "out":
+                dual.pop("out")
+            for mode in (True, False):
+                with torch.set_grad_enabled(mode), pytest.raises(NotImplementedError, match="forward-mode"):
+                    sr_states.adapter_add(index=index, **dual)
+            with forward_ad._set_fwd_grad_enabled(False):  # nothing is lost where nothing is differentiated
+                assert torch.equal(sr_states.adapter_add(index=index, **dual), want)
+        assert torch.equal(sr_states.adapter_add(base, x, a, b, index, scaling=scaling), want)
 
 
 def test_refusals(cuda):

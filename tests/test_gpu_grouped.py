@@ -14,6 +14,7 @@ import pytest
 import sr_states
 import torch
 from sr_states import BlockScaled
+from torch.autograd import forward_ad
 
 pytestmark = pytest.mark.gpu
 E4M3, E5M2 = torch.float8_e4m3fn, torch.float8_e5m2
@@ -431,6 +432,15 @@ def test_calls_on_two_streams_at_once(cuda):
     torch.cuda.synchronize()
     for k in range(2):
         assert all(torch.equal(y, want[k]) for y in got[k])
+
+
+def test_tangents_are_refused(cuda):
+    x, w, sizes = torch.randn(8, 256, device=cuda), torch.randn(2, 16, 256, device=cuda), _sizes([3, 5], cuda)
+    with forward_ad.dual_level():
+        for operands in ((forward_ad.make_dual(x, torch.ones_like(x)), w), (x, forward_ad.make_dual(w, torch.ones_like(w)))):
+            for mode in (True, False):
+                with torch.set_grad_enabled(mode), pytest.raises(NotImplementedError, match="forward-mode"):
+                    sr_states.grouped_block_linear(*operands, sizes)
 
 
 def test_refusals(cuda):
