@@ -73,8 +73,11 @@ def units() -> list[tuple[Path, list[str], Path]]:
     return jobs
 
 
-def walk_command(output: Path, source: Path = CSRC / "group_walk.cpp") -> list[str]:
-    """g++ line for a CPython extension against the running torch (the group walk by default)."""
+def walk_command(output: Path, source: Path = CSRC / "group_walk.cpp", streams: bool = False) -> list[str]:
+    """g++ line for a CPython extension against the running torch (the group walk by default).
+
+    ``streams``: it asks torch for its current stream of a device.
+    """
     import torch.utils.cpp_extension as ext
 
     torch_lib = ext.library_paths()[0]
@@ -88,11 +91,13 @@ def walk_command(output: Path, source: Path = CSRC / "group_walk.cpp") -> list[s
         f"-D_GLIBCXX_USE_CXX11_ABI={int(__import__('torch')._C._GLIBCXX_USE_CXX11_ABI)}",
         f"-I{sysconfig.get_paths()['include']}",
         *(f"-I{path}" for path in ext.include_paths()),
+        *((f"-I{Path(shutil.which(HIPCC) or HIPCC).parent.parent / 'include'}", "-D__HIP_PLATFORM_AMD__") if streams else ()),
         str(source),
         "-o",
         str(output),
         f"-L{torch_lib}",
         "-lc10",
+        *(("-lc10_hip",) if streams else ()),
         "-ltorch",
         "-ltorch_cpu",
         "-ltorch_python",
@@ -124,7 +129,7 @@ def build(jobs: int | None = None, verbose: bool = False) -> Path:
     launch_tmp = LAUNCH_OUTPUT.with_name(LAUNCH_OUTPUT.name + ".tmp")
     commands.append(walk_command(launch_tmp, CSRC / "launch.cpp"))
     matrix_tmp = MATRIX_OUTPUT.with_name(MATRIX_OUTPUT.name + ".tmp")
-    commands.append(walk_command(matrix_tmp, CSRC / "matrix.cpp"))
+    commands.append(walk_command(matrix_tmp, CSRC / "matrix.cpp", streams=True))
     workers = jobs or min(len(commands), max(1, min(16, os.cpu_count() or 1)))
     with ThreadPoolExecutor(workers) as pool:
         for cmd, _ in zip(commands, pool.map(_run, commands)):

@@ -52,6 +52,7 @@
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -500,6 +501,10 @@ at::Tensor add_adapters(const at::Tensor& base, const at::Tensor& x, const Adapt
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The engine runs a node on the stream of its forward pass; who calls one directly has it run on the caller's, where its
+// workspace and results belong too.
+void* current_stream(const at::Device& device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
+
 // Runs a node's gradients: a failed launch becomes an error here, where the message of this thread's last one is, and
 // the gradients cannot be differentiated again.
 template <class Body>
@@ -534,8 +539,7 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     cast_stack_into(weight, o.format[2], o.format[3], true, o.seed[1], 0, &qw, need_x ? &qw_t : nullptr, o.stream);
     if (need_x || need_w) {
       ctx->save_for_backward({sizes, qx_t.data, qx_t.scale, qw_t.data, qw_t.scale});
-      ctx->saved_data["rule"] = std::vector<int64_t>{o.format[4], o.format[5], o.seed[2], dtype_code(x.scalar_type()), dtype_code(w.scalar_type()),
-                                                     static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.stream))};
+      ctx->saved_data["rule"] = std::vector<int64_t>{o.format[4], o.format[5], o.seed[2], dtype_code(x.scalar_type()), dtype_code(w.scalar_type())};
     }
     return grouped_product(qx, qw, sizes, dtype_code(x.scalar_type()), at::Tensor(), o.stream);
   }
@@ -543,11 +547,11 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     return gradients("grouped_block_linear", [&] {
       const variable_list saved = ctx->get_saved_variables();
       const std::vector<int64_t> rule = ctx->saved_data["rule"].toIntVector();
-      void* stream = address(static_cast<unsigned long long>(rule[5]));  // the engine runs a node on its forward pass's stream
       const at::Tensor& dy = grads[0];
       at::Tensor dx, dw;
       if (dy.defined()) {
         const c10::DeviceGuard guard(dy.device());
+        void* stream = current_stream(dy.device());
         const Scaled x{saved[1], saved[2]}, w{saved[3], saved[4]};
         const bool need_x = w.data.defined() && ctx->needs_input_grad(0), need_w = x.data.defined() && ctx->needs_input_grad(1);
         Scaled by_rows, by_cols;
@@ -573,18 +577,17 @@ struct AdapterAdd : torch::autograd::Function<AdapterAdd> {
     const at::Tensor y = add_adapters(base, x, AdapterSet(x, a, b, index, o.scaling, o.scale), at::Tensor(), low, o.stream);
     ctx->save_for_backward({x, a, b, index, o.scaling, low});
     ctx->saved_data["scale"] = o.scale;
-    ctx->saved_data["stream"] = static_cast<int64_t>(reinterpret_cast<uintptr_t>(o.stream));
     return y;
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
     return gradients("adapter_add", [&] {
       const variable_list saved = ctx->get_saved_variables();
       const at::Tensor &x = saved[0], &a = saved[1], &b = saved[2], &dy = grads[0];
-      void* stream = address(static_cast<unsigned long long>(ctx->saved_data["stream"].toInt()));
       at::Tensor dbase, dx, da, db;
       const bool need_x = ctx->needs_input_grad(1), need_a = ctx->needs_input_grad(2), need_b = ctx->needs_input_grad(3);
       if (dy.defined()) {
         const c10::DeviceGuard guard(dy.device());
+        void* stream = current_stream(dy.device());
         if (ctx->needs_input_grad(0)) dbase = dy;
         if (need_x || need_a || need_b) {
           const AdapterSet set(x, a, b, saved[3], saved[4], ctx->saved_data["scale"].toDouble());

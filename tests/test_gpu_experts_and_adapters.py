@@ -183,3 +183,46 @@ def test_gradients_through_saved_tensor_hooks(cuda):
 
     for got, expected in zip(_gradients(offloaded, tensors, sizes, index, dy), want):
         assert torch.equal(got, expected)
+
+
+@pytest.mark.parametrize("operator", ["adapters", "experts"])
+def test_a_node_called_by_itself_runs_on_the_callers_stream(cuda, operator):
+    """Beside the engine, which sets the stream of the forward pass: a call from another one, and a captured call."""
+    tensors, sizes, index, dy = _inputs(cuda)
+    names = ("x", "a", "b") if operator == "adapters" else ("x", "up")
+    x, *weights = (tensors[name].requires_grad_() for name in names)
+    if operator == "adapters":
+        y = sr_states.adapter_add(tensors["shared"][:1].expand(300, -1), x, *weights, index)
+    else:
+        y, dy = sr_states.grouped_block_linear(x, *weights, sizes), dy.repeat(1, 2)[:, :384].contiguous()
+
+    def node():
+        with torch.no_grad():
+            return [g for g in y.grad_fn(dy) if g is not None]
+
+    def engine():
+        return torch.autograd.grad(y, (x, *weights), dy, retain_graph=True)
+
+    first = engine()
+    torch.cuda.synchronize()
+    side, work = torch.cuda.Stream(), torch.randn(4096, 4096, device=cuda)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            work = work @ work * 1e-2
+        dy.mul_(2)
+        got = node()
+    torch.cuda.synchronize()
+    want = engine()
+    assert len(got) == len(want) and not torch.equal(want[0], first[0])
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = node()
+    for factor in (0.25, 4.0, -1.0):
+        dy.mul_(factor)
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, w in zip(captured, engine()):
+            assert torch.equal(g, w)
+        torch.cuda.synchronize()
