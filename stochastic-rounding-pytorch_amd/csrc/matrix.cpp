@@ -385,11 +385,14 @@ at::Tensor grouped_product(const Scaled& a, const Scaled& b, const at::Tensor& s
     if (start < last && first < end) value_error("out must not overlap the sizes");
   }
   if (stacked) {
-    const int64_t stride = result_of(out, {m, n}, out_code, a, b, "grouped_block_matmul");
+    sr_block_matrix right{};
+    if (count) {
+      right = operand(matrix_of(b.data), matrix_of(b.scale), "b");
+      if (left.scale_type != right.scale_type) type_error("a and b must have scales of one type");
+    }
+    const int64_t stride = result_of(out, {m, n}, out_code, a, b, "grouped_block_matmul");  // after every refusal
     if (!m || !n) return out;
     if (!count) return given ? out : out.zero_();
-    const sr_block_matrix right = operand(matrix_of(b.data), matrix_of(b.scale), "b");
-    if (left.scale_type != right.scale_type) type_error("a and b must have scales of one type");
     checked(g_grouped_matmul(&left, &right, stack_stride(b.data), stack_stride(b.scale), k, &groups, memory(out), stride, out_code,
                              !given, stream));
     return out;

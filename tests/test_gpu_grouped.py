@@ -434,6 +434,22 @@ def test_calls_on_two_streams_at_once(cuda):
         assert all(torch.equal(y, want[k]) for y in got[k])
 
 
+def test_a_refused_call_leaves_its_result_alone(cuda):
+    x, sizes = torch.ones(8, 256, device=cuda), _sizes([3, 5], cuda)
+    q, w = sr_states.block_cast(x), sr_states.grouped_block_cast(torch.ones(2, 16, 256, device=cuda))
+    out = torch.full((8, 16), 7.0, device=cuda)
+    version = out._version
+    for error, a, b in ((ValueError, q, BlockScaled(w.data, w.scale[:, :, :1])), (ValueError, q, BlockScaled(w.data, w.scale[:, :15])),
+                        (TypeError, q, BlockScaled(w.data, w.scale.view(torch.uint8))), (TypeError, q, BlockScaled(w.data.float(), w.scale)),
+                        (TypeError, BlockScaled(q.data, q.scale.float()), w)):
+        with pytest.raises(error):
+            sr_states.grouped_block_matmul(a, b, sizes, out=out)
+        assert out._version == version
+    assert (out == 7).all()
+    sr_states.grouped_block_matmul(q, w, sizes, out=out)
+    assert out._version > version and (out == 256).all()
+
+
 def test_tangents_are_refused(cuda):
     x, w, sizes = torch.randn(8, 256, device=cuda), torch.randn(2, 16, 256, device=cuda), _sizes([3, 5], cuda)
     with forward_ad.dual_level():
