@@ -508,6 +508,12 @@ using torch::autograd::variable_list;
 // workspace and results belong too.
 void* current_stream(const at::Device& device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
+// The engine checks the gradients that it passes; a node that is called directly may get any tensor.
+void check_gradient(const at::Tensor& dy, at::IntArrayRef shape, int dtype, const at::Device& device) {
+  if (dtype_code(dy.scalar_type()) != dtype || dy.sizes() != shape || dy.device() != device)
+    value_error("the gradient must be a " + shape_of(shape) + " tensor of " + name_of(scalar_type(dtype)) + " on " + device.str());
+}
+
 // Runs a node's gradients: a failed launch becomes an error here, where the message of this thread's last one is, and
 // the gradients cannot be differentiated again.
 template <class Body>
@@ -542,7 +548,8 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
     cast_stack_into(weight, o.format[2], o.format[3], true, o.seed[1], 0, &qw, need_x ? &qw_t : nullptr, o.stream);
     if (need_x || need_w) {
       ctx->save_for_backward({sizes, qx_t.data, qx_t.scale, qw_t.data, qw_t.scale});
-      ctx->saved_data["rule"] = std::vector<int64_t>{o.format[4], o.format[5], o.seed[2], dtype_code(x.scalar_type()), dtype_code(w.scalar_type())};
+      ctx->saved_data["rule"] = std::vector<int64_t>{o.format[4], o.format[5], o.seed[2], dtype_code(x.scalar_type()), dtype_code(w.scalar_type()),
+                                                     x.size(0), w.size(1)};
     }
     return grouped_product(qx, qw, sizes, dtype_code(x.scalar_type()), at::Tensor(), o.stream);
   }
@@ -555,6 +562,7 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
       if (dy.defined()) {
         const c10::DeviceGuard guard(dy.device());
         void* stream = current_stream(dy.device());
+        check_gradient(dy, {rule[5], rule[6]}, static_cast<int>(rule[3]), saved[0].device());
         const Scaled x{saved[1], saved[2]}, w{saved[3], saved[4]};
         const bool need_x = w.data.defined() && ctx->needs_input_grad(0), need_w = x.data.defined() && ctx->needs_input_grad(1);
         Scaled by_rows, by_cols;
@@ -594,6 +602,13 @@ struct AdapterAdd : torch::autograd::Function<AdapterAdd> {
         if (ctx->needs_input_grad(0)) dbase = dy;
         if (need_x || need_a || need_b) {
           const AdapterSet set(x, a, b, saved[3], saved[4], ctx->saved_data["scale"].toDouble());
+          auto shape = x.sizes().vec();
+          shape.back() = set.n;
+          check_gradient(dy, shape, set.g.dtype, x.device());
+          const at::Tensor low = saved[5].contiguous();  // a hook of saved tensors may have put another in its place
+          if (low.scalar_type() != c10::ScalarType::Float || low.device() != x.device() ||
+              low.numel() != g_adapter_low(set.rows, set.k, set.g.rank, set.g.dtype))
+            value_error("the tensors kept for the backward pass have changed their types or sizes");
           const at::Tensor rows = as_rows(x.detach().resolve_neg()), from = as_rows(dy.detach().resolve_neg());
           if (need_x) dx = at::empty(x.sizes(), x.options());
           if (need_a) da = at::empty(a.sizes(), a.options());
@@ -602,7 +617,7 @@ struct AdapterAdd : torch::autograd::Function<AdapterAdd> {
                                                  x.options().dtype(c10::ScalarType::Byte));
           auto place = [](const at::Tensor& t) { return t.defined() ? memory(t) : nullptr; };
           checked(g_adapter_backward(&set.g, memory(rows), row_stride(rows, "x"), set.k, memory(from), row_stride(from, "dy"), set.n,
-                                     set.rows, static_cast<const float*>(memory(saved[5])), place(dx), set.k, place(da), place(db),
+                                     set.rows, static_cast<const float*>(memory(low)), place(dx), set.k, place(da), place(db),
                                      memory(workspace), stream));
         }
       }

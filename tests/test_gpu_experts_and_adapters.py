@@ -226,3 +226,23 @@ def test_a_node_called_by_itself_runs_on_the_callers_stream(cuda, operator):
         for g, w in zip(captured, engine()):
             assert torch.equal(g, w)
         torch.cuda.synchronize()
+
+
+def test_nodes_refuse_gradients_and_kept_tensors_of_other_shapes(cuda):
+    """What the engine would not pass: a node called by itself, and a hook that puts other tensors in place of saved ones."""
+    tensors, sizes, index, dy = _inputs(cuda)
+    x, a, up = (tensors[name].requires_grad_() for name in ("x", "a", "up"))
+
+    def calls():
+        return ((sr_states.adapter_add(x * 1.0, x, a, tensors["b"], index), dy),
+                (sr_states.grouped_block_linear(x, up, sizes), dy.repeat(1, 2)[:, :384].contiguous()))
+
+    for y, grad in calls():
+        for other in (grad[:1], grad[:, :128], grad.float(), grad.cpu(), grad[None]):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="the gradient must be"):
+                y.grad_fn(other)
+    for change in (lambda t: t[:1], lambda t: t.double(), lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: change(t) if t.dtype == torch.float32 else t):
+            y = sr_states.adapter_add(tensors["shared"][:1].expand(300, -1), x, a, tensors["b"], index)
+        with pytest.raises(RuntimeError, match="kept for the backward pass"):
+            torch.autograd.grad(y, a, dy)
