@@ -129,7 +129,8 @@ int sr_stacked_block_cast(const void* x, int64_t x_stride, int64_t ldx, int64_t 
 
 /* out[t] = a[t] b[i]^T for the rows t of every group i, where b is
  * groups->count matrices, `b_stride` bytes and `b_stride_scale` scales apart;
- * otherwise as sr_block_matmul.  Rows behind the last group become zeros with
+ * otherwise as sr_block_matmul.  Where 128 rows of a share a scale, they are
+ * counted from a's first row, wherever groups start.  Rows behind the last group become zeros with
  * `zero_behind`, and keep what they hold without it. */
 int sr_grouped_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t b_stride, int64_t b_stride_scale,
                             int64_t k, const sr_groups* groups, void* out, int64_t ldo, int out_dtype, int zero_behind,
@@ -172,7 +173,8 @@ int64_t sr_adapter_low(int64_t rows, int64_t k, int64_t rank, int dtype);
 /* out[t] = base[t] + s_i (x[t] a_i^T) b_i^T for i = index[t], and base[t] for
  * rows without an adapter.  x (rows x k), base and out (rows x n; out may be
  * base itself) have the adapters' dtype.  `low` receives s_i x[t] a_i^T, in
- * parts, for sr_adapter_backward. */
+ * parts, for sr_adapter_backward; with BF16 the second product takes it to
+ * 2^-15 of itself, as the gradients' second products take theirs. */
 int sr_adapter_add(const sr_adapters* g, const void* x, int64_t ldx, int64_t k, const void* base, int64_t ldbase, int64_t n,
                    int64_t rows, void* out, int64_t ldo, float* low, void* stream);
 

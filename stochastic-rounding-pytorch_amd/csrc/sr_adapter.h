@@ -223,6 +223,8 @@ __device__ __forceinline__ void for_each_adapter(int mine, F&& use) {
 
 // Whether the adapters of 64 rows, one a lane, do not come in runs in ascending order: `order` then receives the rows in
 // the order of their adapters, between which they keep their own.  For a whole workgroup, whose waves hold the same.
+// (8192 rows of 2048 to 2048 in ascending or descending runs 26.5 us without a look and 26.9 with it; in runs of 100 rows in any
+// order, whose ends are put in order though they need none, 34.2 and 37.9; mixed row by row 96 and 58.)
 __device__ __forceinline__ bool order_rows(int mine, int* order) {
   const int lane = threadIdx.x & 63, above = __shfl_up(mine, 1);
   if (__ballot(lane > 0 && mine < above) == 0) return false;

@@ -37,11 +37,18 @@ def adapter_add(
     ``scaling`` is a number, or an FP32 tensor with one for each adapter, which
     gets no gradient.
 
-    Sums are FP32 and rounded once, at the end.  Gradients flow to ``base``, ``x``,
-    ``a`` and ``b``; adapters that no row uses get zeros.  There are no forward-mode
-    derivatives: an operand with a tangent is refused.  ``out``, which may be
-    ``base`` itself, takes the result without recording gradients: in grad mode
-    neither it nor an operand may require one.
+    Sums are FP32 and the result is rounded once, at the end.  In BF16 calls a sum
+    between two products (of x and a, and in the gradients of dy and b) enters
+    the second to 2**-15 of itself, below the result's rounding unless the ranks
+    cancel; infinities and NaN come out as the formula has them, for sums of
+    2**-110 and more.
+
+    Gradients flow to ``base``, ``x``, ``a`` and ``b``; adapters that no row uses get
+    zeros.  ``x``, ``a``, ``b``, ``index`` and ``scaling`` are kept for the backward pass
+    and must not change before it.  There are no forward-mode derivatives: an
+    operand with a tangent is refused.  ``out``, which may be ``base`` itself, takes
+    the result without recording gradients: in grad mode neither it nor an
+    operand may require one.
     """
     device = _device_of(x, base, a, b, index, out)
     each = isinstance(scaling, torch.Tensor)

@@ -84,7 +84,8 @@ def grouped_block_matmul(
     behind its rows.
 
     Types, scales, ``out_dtype`` and ``out`` are those of :func:`block_matmul`;
-    ``sizes`` is that of :func:`grouped_block_cast`.
+    ``sizes`` is that of :func:`grouped_block_cast`.  Where 128 rows of ``a`` share a
+    scale, they are counted from its first row, wherever groups start.
     """
     (a_data, a_scale), (b_data, b_scale) = a, b
     if out_dtype is None:
