@@ -130,8 +130,8 @@ int sr_stacked_block_cast(const void* x, int64_t x_stride, int64_t ldx, int64_t 
 /* out[t] = a[t] b[i]^T for the rows t of every group i, where b is
  * groups->count matrices, `b_stride` bytes and `b_stride_scale` scales apart;
  * otherwise as sr_block_matmul.  Where 128 rows of a share a scale, they are
- * counted from a's first row, wherever groups start.  Rows behind the last group become zeros with
- * `zero_behind`, and keep what they hold without it. */
+ * counted from a's first row, wherever groups start.  Rows behind the last
+ * group become zeros with `zero_behind`, and keep what they hold without it. */
 int sr_grouped_block_matmul(const sr_block_matrix* a, const sr_block_matrix* b, int64_t b_stride, int64_t b_stride_scale,
                             int64_t k, const sr_groups* groups, void* out, int64_t ldo, int out_dtype, int zero_behind,
                             void* stream);
